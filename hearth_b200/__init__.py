@@ -6,6 +6,8 @@
   handle with an HBM-resident expert store.
 * ``Model`` — the whole decoder of a container (embedding, GQA attention with its KV cache, MoE and
   dense FFN layers, LM head) on the GPU, evaluated like hearth_eval.
+* ``rope``, ``kv_write``, ``kv_read``, ``decode_attention``, ``latent_attention`` — rotary positions, a
+  paged (optionally quantised) key-value cache and decode attention over it, on torch CUDA tensors.
 
 Everything runs through the C ABI of include/hearth_b200.h in ``libhearth_b200.so``; there is no
 CPU fallback.
@@ -15,5 +17,8 @@ from ._lib import (BF16, F16, F32, POLICY_LFU, POLICY_LRU, Q4, Q8, SCORE_SIGMOID
 from . import native  # noqa: F401
 from .moe import MoeBackend, container_probe  # noqa: F401
 from .model import Model  # noqa: F401
+from .attention import (decode_attention, kv_read, kv_write, latent_attention, rope, rope_freqs,  # noqa: F401
+                        rope_table)
 
-__all__ = ["lib", "last_error", "native", "MoeBackend", "Model", "container_probe", "F32", "F16", "BF16", "Q8", "Q4"]
+__all__ = ["lib", "last_error", "native", "MoeBackend", "Model", "container_probe", "rope_freqs", "rope_table", "rope",
+           "kv_write", "kv_read", "decode_attention", "latent_attention", "F32", "F16", "BF16", "Q8", "Q4"]

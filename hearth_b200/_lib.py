@@ -31,6 +31,8 @@ EXPORTS = [
     "hxb_moe_share_expert", "hxb_model_default_options", "hxb_model_open", "hxb_model_close", "hxb_model_info",
     "hxb_model_forward", "hxb_model_last_routes", "hxb_model_set_replay", "hxb_model_moe", "hxb_model_synthesize",
     "hxb_model_forward_dev", "hxb_model_sync", "hxb_moe_get_expert",
+    "hxb_rope_freqs", "hxb_rope_table_dev", "hxb_rope_dev", "hxb_kv_write_dev", "hxb_kv_read_dev",
+    "hxb_attn_decode_workspace", "hxb_attn_decode_dev", "hxb_latent_decode_workspace", "hxb_latent_decode_dev",
 ]
 
 
@@ -61,6 +63,17 @@ class ContainerInfo(C.Structure):
                 ("slab_bytes", C.c_uint64)]
 
 
+class Rope(C.Structure):
+    _fields_ = [("cs", C.c_void_p), ("n_pos", C.c_int64), ("rope_dim", C.c_int), ("offset", C.c_int), ("style", C.c_int)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int),
+                ("n_pages", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int),
+                ("n_seqs", C.c_int)]
+
+
 class MoeStats(C.Structure):
     _fields_ = [("tokens", C.c_uint64), ("forward_calls", C.c_uint64), ("expert_uses", C.c_uint64),
                 ("expert_loads_unique", C.c_uint64), ("hits", C.c_uint64), ("misses", C.c_uint64),
@@ -85,7 +98,7 @@ def lib() -> C.CDLL:
         from . import build as _b
         _b.build()
     L = C.CDLL(LIB_PATH)
-    vp, i, i64, sz, f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
+    vp, i, i64, sz, f, d = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float, C.c_double
     sig = {
         "hxb_version": (C.c_char_p, []), "hxb_last_error": (C.c_char_p, []), "hxb_device_count": (i, []),
         "hxb_row_bytes": (sz, [i, i64]),
@@ -138,6 +151,15 @@ def lib() -> C.CDLL:
         "hxb_model_forward_dev": (i, [vp, vp, i, i, vp, i, vp]),
         "hxb_model_sync": (i, [vp, vp]),
         "hxb_moe_get_expert": (i, [vp, i, i, vp, sz]),
+        "hxb_rope_freqs": (i, [i, d, i, d, i, d, d, vp, vp]),
+        "hxb_rope_table_dev": (i, [vp, i, d, i64, i64, vp, vp]),
+        "hxb_rope_dev": (i, [vp, vp, i64, i, i, vp, i, i64, i64, vp, i, i64, i64, vp]),
+        "hxb_kv_write_dev": (i, [vp, vp, vp, i64, vp, i64, i64, vp, i64, i64, i, vp, vp]),
+        "hxb_kv_read_dev": (i, [vp, vp, vp, i64, vp, i64, i64, vp, i64, i64, i, vp]),
+        "hxb_attn_decode_workspace": (sz, [vp, i]),
+        "hxb_attn_decode_dev": (i, [vp, vp, vp, i64, i64, i, i, f, vp, i64, i64, vp, vp, sz, vp]),
+        "hxb_latent_decode_workspace": (sz, [vp, i, i]),
+        "hxb_latent_decode_dev": (i, [vp, vp, vp, i64, i64, vp, i, i, i, i, i, f, vp, i64, i64, vp, sz, vp]),
         "hxb_model_synthesize": (vp, [C.POINTER(ModelArch), C.POINTER(ModelOptions), C.c_uint64, C.c_char_p, sz]),
     }
     for name, (res, args) in sig.items():

@@ -1,0 +1,540 @@
+// hx_attention.cu — rotary positions and the paged key-value cache on device buffers (hxb_rope_*,
+// hxb_kv_*): the reference's rope_tables / rope_apply (engine/src/model.c:386-411) and its cache rows
+// (model.c:484-517), with pages, element types and Q8 blocks of their own.
+#include "hx_paged.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+namespace hx {
+
+void set_last_error(const char *msg);
+
+int attn_fail(int code, const char *fmt, ...) {
+    char buf[320];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    set_last_error(buf);
+    return code;
+}
+
+bool attn_launched(const char *who) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return true;
+    attn_fail(HXB_E_DEVICE, "%s: %s", who, cudaGetErrorString(e));
+    return false;
+}
+
+static bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+static size_t elem_size(int dtype) { return dtype == F32 ? 4 : 2; }
+static bool io_dtype(int dtype) { return dtype == F32 || dtype == F16 || dtype == BF16; }
+
+int kv_view(const hxb_kv_cache *c, const char *who, bool latent, KvView *o) {
+    if (!c) return attn_fail(HXB_E_ARG, "%s: null cache", who);
+    if (c->dtype != F16 && c->dtype != BF16 && c->dtype != Q8)
+        return attn_fail(HXB_E_UNSUPPORTED, "%s: cache dtype %d (F16, BF16 or Q8)", who, c->dtype);
+    const bool q8 = c->dtype == Q8;
+    if (c->n_kv_heads < 1 || c->n_kv_heads > 65535 || c->head_dim < 8 || c->head_dim > 1024 || c->head_dim % 8 ||
+        (q8 && c->head_dim % KV_BLOCK))
+        return attn_fail(HXB_E_ARG, "%s: %d heads of %d (head_dim a multiple of %d up to 1024)", who, c->n_kv_heads,
+                         c->head_dim, q8 ? KV_BLOCK : 8);
+    if (c->page_tokens < 1 || c->page_tokens > 1024 || (c->page_tokens & (c->page_tokens - 1)))
+        return attn_fail(HXB_E_ARG, "%s: page_tokens %d (a power of two up to 1024)", who, c->page_tokens);
+    if (c->n_pages < 0 || c->n_pages > 0x7fffffff || c->table_pages < 0 || c->n_seqs < 0 || c->table_stride < 0 ||
+        (int64_t)c->table_pages * c->page_tokens > 0x7fffffff)
+        return attn_fail(HXB_E_ARG, "%s: bad page counts", who);
+    if (c->table_stride && c->table_stride < c->table_pages)
+        return attn_fail(HXB_E_ARG, "%s: table rows overlap (stride %lld, %d pages)", who, (long long)c->table_stride,
+                         c->table_pages);
+    if (latent && (c->n_kv_heads != 1 || c->v || c->v_scale))
+        return attn_fail(HXB_E_ARG, "%s: a latent cache has one row a token and no v", who);
+    if (c->n_pages && (!c->k || (!latent && !c->v) || (q8 && (!c->k_scale || (!latent && !c->v_scale)))))
+        return attn_fail(HXB_E_ARG, "%s: null pool", who);
+    if (!q8 && (c->k_scale || c->v_scale)) return attn_fail(HXB_E_ARG, "%s: scales with a cache that is not Q8", who);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) ||
+        !aligned(c->table, 4))
+        return attn_fail(HXB_E_ARG, "%s: pool or table not aligned", who);
+    if (c->n_seqs && c->table_pages && !c->table) return attn_fail(HXB_E_ARG, "%s: null page table", who);
+    o->k = c->k, o->v = c->v, o->ks = c->k_scale, o->vs = c->v_scale;
+    o->table = c->table, o->table_stride = c->table_stride, o->n_pages = c->n_pages;
+    o->table_pages = c->table_pages, o->n_seqs = c->n_seqs, o->Hkv = c->n_kv_heads, o->hd = c->head_dim;
+    o->pt_log2 = 0;
+    while ((1 << o->pt_log2) < c->page_tokens) o->pt_log2++;
+    return HXB_OK;
+}
+
+namespace {
+
+constexpr int ROW_THREADS = 256;
+// Eight-element items a CTA of the row kernels (rotation, cache write and read) takes: a few per thread, so
+// that each has several loads in flight, while single tokens still spread over many CTAs.
+constexpr int ROW_ITEMS = 1024;
+
+// ------------------------------------------------------------------------------------------- rotary tables
+
+struct FreqArg {
+    double turns[512];   // inv_freq / (2 pi)
+};
+
+// cs[i][j] = factor * (cos, sin)(2 pi frac(p * turns_j)). The product and its fractional part are formed in 64
+// bits (far positions keep their phase); the f32 part of the fraction goes through sincospif and the rest, below
+// 2^-25 of a turn, enters to first order. 16 bytes written a thread.
+__global__ void __launch_bounds__(256) k_rope_table(const __grid_constant__ FreqArg f, int half, double factor,
+                                                    int64_t pos0, int64_t n_pos, float2 *__restrict__ cs) {
+    const int64_t n = n_pos * half;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t p = i / half;
+        const int j = (int)(i - p * half);
+        const double t = (double)(pos0 + p) * f.turns[j];
+        const double r = 2.0 * (t - rint(t));      // half turns, in [-1, 1], exact after the product
+        const float hi = (float)r, lo = (float)(r - (double)hi) * 3.14159265358979f;
+        float s, c;
+        sincospif(hi, &s, &c);
+        cs[i] = make_float2((float)(factor * (double)__fmaf_rn(-lo, s, c)), (float)(factor * (double)__fmaf_rn(lo, c, s)));
+    }
+}
+
+// ------------------------------------------------------------------------------------------- rotation
+
+struct RopeView {
+    const float *cs;
+    int64_t n_pos;
+    int half, off, style;
+};
+
+__device__ __forceinline__ void rotate(float &a, float &b, float c, float s) {
+    const float na = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+    b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+    a = na;
+}
+
+struct RopeArgs {
+    RopeView r;
+    const int32_t *pos;
+    const void *x;
+    void *y;
+    int64_t T, xs, xh, ys, yh;
+    int H, hd, units, tpc, in_place, vec;
+    FastDiv per_tok, per_head;
+};
+
+// Items own what they read and write, so y may be x. vec: an item is a chunk of eight (halves: the pair of
+// chunks j, j + half; then the chunks that are not rotated); otherwise one pair or one copied value.
+template <class TX, class TY>
+__global__ void __launch_bounds__(ROW_THREADS) k_rope(const __grid_constant__ RopeArgs a) {
+    const int64_t t0 = (int64_t)blockIdx.x * a.tpc;
+    const int nt = (int)min((int64_t)a.tpc, a.T - t0);
+    const int per = a.H * a.units, rot = 2 * a.r.half;
+    for (int i = threadIdx.x; i < nt * per; i += ROW_THREADS) {
+        const int tl = (int)a.per_tok.div(i), u0 = i - tl * per;
+        const int h = (int)a.per_head.div(u0), u = u0 - h * a.units;
+        const int64_t t = t0 + tl;
+        const TX *x = static_cast<const TX *>(a.x) + t * a.xs + h * a.xh;
+        TY *y = static_cast<TY *>(a.y) + t * a.ys + h * a.yh;
+        const int n_rot = a.vec ? (a.r.style == 0 ? a.r.half / 8 : rot / 8) : a.r.half;
+        if (u >= n_rot) {   // not rotated
+            if (a.in_place) continue;
+            int e = (u - n_rot) * (a.vec ? 8 : 1);
+            if (e >= a.r.off) e += rot;
+            if (a.vec) {
+                float v[8];
+                load8(x + e, v, true);
+                store8(y + e, v, true);
+            } else {
+                y[e] = from_f32<TY>(to_f32(x[e]));
+            }
+            continue;
+        }
+        const int p = a.pos[t];
+        const bool ok = p >= 0 && p < a.r.n_pos;
+        const float *cs = a.r.cs + (ok ? (int64_t)p : 0) * rot;
+        if (!a.vec) {
+            const int ia = a.r.off + (a.r.style == 0 ? u : 2 * u), ib = a.r.style == 0 ? ia + a.r.half : ia + 1;
+            float va = to_f32(x[ia]), vb = to_f32(x[ib]);
+            rotate(va, vb, ok ? cs[2 * u] : kv_nan(), ok ? cs[2 * u + 1] : kv_nan());
+            y[ia] = from_f32<TY>(va);
+            y[ib] = from_f32<TY>(vb);
+        } else if (a.r.style == 0) {
+            float va[8], vb[8], c[16];
+            load8(x + a.r.off + 8 * u, va, true);
+            load8(x + a.r.off + a.r.half + 8 * u, vb, true);
+            load8(cs + 16 * u, c, ok);
+            load8(cs + 16 * u + 8, c + 8, ok);
+#pragma unroll
+            for (int j = 0; j < 8; j++) rotate(va[j], vb[j], ok ? c[2 * j] : kv_nan(), ok ? c[2 * j + 1] : kv_nan());
+            store8(y + a.r.off + 8 * u, va, true);
+            store8(y + a.r.off + a.r.half + 8 * u, vb, true);
+        } else {
+            float v[8], c[8];
+            load8(x + a.r.off + 8 * u, v, true);
+            load8(cs + 8 * u, c, true);
+#pragma unroll
+            for (int j = 0; j < 4; j++) rotate(v[2 * j], v[2 * j + 1], ok ? c[2 * j] : kv_nan(), ok ? c[2 * j + 1] : kv_nan());
+            store8(y + a.r.off + 8 * u, v, true);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------- cache rows
+
+struct RowArgs {
+    KvView c;
+    RopeView r;              // half 0: no rotation
+    const int32_t *start, *pos0;
+    void *x[2];              // k, v: rows read by a write, written by a read
+    int64_t T, xs[2], xh[2];
+    int sides, tpc, vec, rvec;
+    FastDiv per_tok, per_side, per_head;
+};
+
+// Sequence of row t and its position; false for padding rows.
+__device__ __forceinline__ bool row_place(const RowArgs &a, int64_t t, int &b, int &pos) {
+    int lo = 0, hi = a.c.n_seqs;   // the last b with start[b] <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.start[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    const int s0 = a.start[lo];
+    if (t < s0 || t >= a.start[lo + 1]) return false;
+    b = lo;
+    const int64_t p = (int64_t)a.pos0[lo] + (t - s0);
+    pos = p < 0 || p > 0x7fffffff ? -1 : (int)p;
+    return true;
+}
+
+// The rotated values of elements e .. e + 7 of a key row (its pairs may lie in another chunk, so they are read
+// again there; the cache never overlaps the row).
+template <class TX>
+__device__ __forceinline__ void rotated8(const RowArgs &a, const TX *row, int e, int pos, float v[8]) {
+    const int rot = 2 * a.r.half, r0 = e - a.r.off;
+    if (r0 + 8 <= 0 || r0 >= rot) return;
+    const bool ok = pos >= 0 && pos < a.r.n_pos;
+    const float *cs = a.r.cs + (ok ? (int64_t)pos : 0) * rot;
+    if (a.rvec && a.r.style == 0) {
+        const bool first = r0 < a.r.half;
+        const int j0 = first ? r0 : r0 - a.r.half;
+        float w[8], c[16];
+        load8(row + (first ? e + a.r.half : e - a.r.half), w, a.vec);
+        load8(cs + 2 * j0, c, true);
+        load8(cs + 2 * j0 + 8, c + 8, true);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float x = first ? v[j] : w[j], y = first ? w[j] : v[j];
+            rotate(x, y, ok ? c[2 * j] : kv_nan(), ok ? c[2 * j + 1] : kv_nan());
+            v[j] = first ? x : y;
+        }
+        return;
+    }
+    if (a.rvec) {
+        float c[8];
+        load8(cs + r0, c, true);
+#pragma unroll
+        for (int j = 0; j < 4; j++) rotate(v[2 * j], v[2 * j + 1], ok ? c[2 * j] : kv_nan(), ok ? c[2 * j + 1] : kv_nan());
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int q = r0 + i;
+        if (q < 0 || q >= rot) continue;
+        const bool first = a.r.style == 0 ? q < a.r.half : !(q & 1);
+        const int j = a.r.style == 0 ? (first ? q : q - a.r.half) : q >> 1;
+        const int mate = a.r.style == 0 ? (first ? q + a.r.half : q - a.r.half) : q ^ 1;
+        const float self = to_f32(row[a.r.off + q]), other = to_f32(row[a.r.off + mate]);
+        float x = first ? self : other, y = first ? other : self;
+        rotate(x, y, ok ? cs[2 * j] : kv_nan(), ok ? cs[2 * j + 1] : kv_nan());
+        v[i] = first ? x : y;
+    }
+}
+
+template <class TX, int CACHE>
+__global__ void __launch_bounds__(ROW_THREADS) k_kv_write(const __grid_constant__ RowArgs a) {
+    const int64_t t0 = (int64_t)blockIdx.x * a.tpc;
+    const int nt = (int)min((int64_t)a.tpc, a.T - t0);
+    const int per = (int)a.per_tok.d, side_n = (int)a.per_side.d, head_n = (int)a.per_head.d;
+    for (int i = threadIdx.x; i < nt * per; i += ROW_THREADS) {
+        const int tl = (int)a.per_tok.div(i);
+        int u = i - tl * per;
+        const int side = (int)a.per_side.div(u);
+        u -= side * side_n;
+        const int h = (int)a.per_head.div(u), e = (u - h * head_n) * 8;
+        const int64_t t = t0 + tl;
+        int b, pos;
+        if (!row_place(a, t, b, pos)) continue;
+        const int64_t row0 = kv_row(a.c, b, pos);
+        if (row0 < 0) continue;
+        const int64_t row = row0 + ((int64_t)h << a.c.pt_log2);
+        const TX *x = static_cast<const TX *>(a.x[side]) + t * a.xs[side] + h * a.xh[side];
+        float v[8];
+        load8(x + e, v, a.vec);
+        if (side == 0 && a.r.half) rotated8(a, x, e, pos, v);
+        if constexpr (CACHE == Q8) {
+            // eight lanes hold a block: a CTA's items of one head are a multiple of eight, in lane order
+            const uint32_t grp = 0xffu << (threadIdx.x & 24);
+            float amax = 0.0f;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                amax = fmaxf(amax, fabsf(v[j]));
+                bad = bad || !(fabsf(v[j]) < kv_inf());
+            }
+#pragma unroll
+            for (int s = 4; s >= 1; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(grp, amax, s));
+            bad = (__ballot_sync(grp, bad) & grp) != 0;
+            const float d = __fdiv_rn(amax, 127.0f);
+            const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            uint32_t q[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float s = __fmul_rn(v[j], id);
+                if (s != s) s = 0.0f;
+                s = fminf(fmaxf(s, -127.0f), 127.0f);
+                q[j >> 2] |= ((uint32_t)__float2int_rn(s) & 0xffu) << (8 * (j & 3));
+            }
+            int8_t *pool = static_cast<int8_t *>(side ? a.c.v : a.c.k);
+            *reinterpret_cast<uint2 *>(pool + row * a.c.hd + e) = make_uint2(q[0], q[1]);
+            if (e % KV_BLOCK == 0) (side ? a.c.vs : a.c.ks)[row * (a.c.hd / KV_BLOCK) + e / KV_BLOCK] = bad ? kv_nan() : d;
+        } else if constexpr (CACHE == F16) {
+            store8(static_cast<__half *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
+        } else {
+            store8(static_cast<__nv_bfloat16 *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
+        }
+    }
+}
+
+template <class TY, int CACHE>
+__global__ void __launch_bounds__(ROW_THREADS) k_kv_read(const __grid_constant__ RowArgs a) {
+    const int64_t t0 = (int64_t)blockIdx.x * a.tpc;
+    const int nt = (int)min((int64_t)a.tpc, a.T - t0);
+    const int per = (int)a.per_tok.d, side_n = (int)a.per_side.d, head_n = (int)a.per_head.d;
+    for (int i = threadIdx.x; i < nt * per; i += ROW_THREADS) {
+        const int tl = (int)a.per_tok.div(i);
+        int u = i - tl * per;
+        const int side = (int)a.per_side.div(u);
+        u -= side * side_n;
+        const int h = (int)a.per_head.div(u), e = (u - h * head_n) * 8;
+        const int64_t t = t0 + tl;
+        int b, pos;
+        if (!row_place(a, t, b, pos)) continue;
+        const int64_t row0 = kv_row(a.c, b, pos);
+        const int64_t row = row0 + ((int64_t)h << a.c.pt_log2);
+        TY *y = static_cast<TY *>(a.x[side]) + t * a.xs[side] + h * a.xh[side];
+        float v[8];
+        if (row0 < 0) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = kv_nan();
+        } else if constexpr (CACHE == Q8) {
+            const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(side ? a.c.v : a.c.k) + row * a.c.hd + e);
+            const float d = (side ? a.c.vs : a.c.ks)[row * (a.c.hd / KV_BLOCK) + e / KV_BLOCK];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                v[j] = __fmul_rn((float)(int8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3))), d);
+        } else if constexpr (CACHE == F16) {
+            load8(static_cast<const __half *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
+        } else {
+            load8(static_cast<const __nv_bfloat16 *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
+        }
+        store8(y + e, v, a.vec);
+    }
+}
+
+bool rope_view(const hxb_rope *r, int head_dim, const char *who, RopeView *o, int *rc) {
+    if (r->rope_dim < 2 || r->rope_dim % 2 || r->rope_dim > head_dim || r->offset < 0 ||
+        r->offset > head_dim - r->rope_dim || (r->style != 0 && r->style != 1)) {
+        *rc = attn_fail(HXB_E_ARG, "%s: rotation of %d values at %d (style %d) in a head of %d", who, r->rope_dim,
+                        r->offset, r->style, head_dim);
+        return false;
+    }
+    if (r->n_pos < 1 || !r->cs || !aligned(r->cs, 4)) {
+        *rc = attn_fail(HXB_E_ARG, "%s: bad rotary table", who);
+        return false;
+    }
+    o->cs = r->cs, o->n_pos = r->n_pos, o->half = r->rope_dim / 2, o->off = r->offset, o->style = r->style;
+    return true;
+}
+
+// Eight-element access needs 16-byte aligned rows: the base and every stride that is used.
+bool vec_rows(const void *p, int dtype, int64_t T, int64_t ts, int H, int64_t hs) {
+    const int64_t n = 16 / (int64_t)elem_size(dtype);
+    return aligned(p, 16) && (T < 2 || ts % n == 0) && (H < 2 || hs % n == 0);
+}
+
+bool rope_vec(const RopeView &r) {
+    return aligned(r.cs, 16) && r.off % 8 == 0 && (r.style == 0 ? r.half % 8 == 0 : r.half % 4 == 0);
+}
+
+// Whether rows [T][H][n] by these strides may overlap themselves; used for outputs.
+bool rows_overlap(int64_t T, int64_t ts, int H, int64_t hs, int n) {
+    if (T > 1 && ts < 1) return true;
+    if (H > 1 && hs < 1) return true;
+    if (H > 1 && hs < n) return true;
+    if (T <= 1) return false;
+    if (H <= 1) return ts < n;
+    return !(ts >= (H - 1) * hs + n || (hs >= (T - 1) * ts + n && ts >= n));
+}
+
+template <class TX>
+cudaError_t rope_to(const RopeArgs &a, int y_dtype, int grid, cudaStream_t s) {
+    if (y_dtype == F32) k_rope<TX, float><<<grid, ROW_THREADS, 0, s>>>(a);
+    else if (y_dtype == F16) k_rope<TX, __half><<<grid, ROW_THREADS, 0, s>>>(a);
+    else k_rope<TX, __nv_bfloat16><<<grid, ROW_THREADS, 0, s>>>(a);
+    return cudaSuccess;
+}
+
+template <class T>
+void rows_launch(const RowArgs &a, int cache, bool write, int grid, cudaStream_t s) {
+    if (write) {
+        if (cache == F16) k_kv_write<T, F16><<<grid, ROW_THREADS, 0, s>>>(a);
+        else if (cache == BF16) k_kv_write<T, BF16><<<grid, ROW_THREADS, 0, s>>>(a);
+        else k_kv_write<T, Q8><<<grid, ROW_THREADS, 0, s>>>(a);
+    } else {
+        if (cache == F16) k_kv_read<T, F16><<<grid, ROW_THREADS, 0, s>>>(a);
+        else if (cache == BF16) k_kv_read<T, BF16><<<grid, ROW_THREADS, 0, s>>>(a);
+        else k_kv_read<T, Q8><<<grid, ROW_THREADS, 0, s>>>(a);
+    }
+}
+
+int kv_rows(const char *who, const hxb_kv_cache *c, const int32_t *start, const int32_t *pos0, int64_t T, void *k,
+            int64_t ks, int64_t kh, void *v, int64_t vs, int64_t vh, int dtype, const hxb_rope *rope, bool write,
+            void *stream) {
+    RowArgs a = {};
+    const bool latent = c && !c->v;
+    int rc = kv_view(c, who, latent, &a.c);
+    if (rc != HXB_OK) return rc;
+    if (T < 0 || T > 0x7fffffff || !io_dtype(dtype)) return attn_fail(HXB_E_ARG, "%s: bad row count or dtype", who);
+    if (rope && !rope_view(rope, c->head_dim, who, &a.r, &rc)) return rc;
+    if (T == 0 || c->n_seqs == 0) return HXB_OK;
+    if (!start || !pos0 || !k || (!latent && !v)) return attn_fail(HXB_E_ARG, "%s: null pointer", who);
+    if (latent && v) return attn_fail(HXB_E_ARG, "%s: v rows for a cache without v", who);
+    if (!aligned(start, 4) || !aligned(pos0, 4) || !aligned(k, elem_size(dtype)) || !aligned(v, elem_size(dtype)))
+        return attn_fail(HXB_E_ARG, "%s: pointer not aligned to its elements", who);
+    if (ks < 0 || kh < 0 || (!latent && (vs < 0 || vh < 0)) ||
+        (!write && (rows_overlap(T, ks, c->n_kv_heads, kh, c->head_dim) ||
+                    (!latent && rows_overlap(T, vs, c->n_kv_heads, vh, c->head_dim)))))
+        return attn_fail(HXB_E_ARG, "%s: bad strides", who);
+    a.start = start, a.pos0 = pos0, a.T = T;
+    a.x[0] = k, a.xs[0] = ks, a.xh[0] = kh;
+    a.x[1] = v, a.xs[1] = vs, a.xh[1] = vh;
+    a.sides = latent ? 1 : 2;
+    a.vec = vec_rows(k, dtype, T, ks, c->n_kv_heads, kh) && (latent || vec_rows(v, dtype, T, vs, c->n_kv_heads, vh));
+    a.rvec = rope && rope_vec(a.r);
+    const int per_head = c->head_dim / 8, per_side = per_head * c->n_kv_heads, per = per_side * a.sides;
+    a.per_head = FastDiv(per_head), a.per_side = FastDiv(per_side), a.per_tok = FastDiv(per);
+    a.tpc = std::max(1, ROW_ITEMS / per);
+    const int64_t grid = (T + a.tpc - 1) / a.tpc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == F32) rows_launch<float>(a, c->dtype, write, (int)grid, s);
+    else if (dtype == F16) rows_launch<__half>(a, c->dtype, write, (int)grid, s);
+    else rows_launch<__nv_bfloat16>(a, c->dtype, write, (int)grid, s);
+    return attn_launched(who) ? HXB_OK : HXB_E_DEVICE;
+}
+
+}  // namespace
+}  // namespace hx
+
+using namespace hx;
+
+extern "C" HXB_API int hxb_rope_freqs(int rope_dim, double theta, int scaling, double factor, int original,
+                                      double beta_fast, double beta_slow, double *inv_freq, double *attn_factor) {
+    if (rope_dim < 2 || rope_dim % 2 || rope_dim > 1024 || !(theta > 1.0) || !std::isfinite(theta) || !inv_freq || !attn_factor)
+        return attn_fail(HXB_E_ARG, "rope_freqs: bad rope_dim, theta or pointer");
+    if (scaling < HXB_ROPE_NONE || scaling > HXB_ROPE_YARN)
+        return attn_fail(HXB_E_ARG, "rope_freqs: unknown scaling %d", scaling);
+    if (scaling != HXB_ROPE_NONE && (!(factor >= 1.0) || !std::isfinite(factor)))
+        return attn_fail(HXB_E_ARG, "rope_freqs: factor %g (at least 1)", factor);
+    if (scaling == HXB_ROPE_NTK && rope_dim == 2) return attn_fail(HXB_E_ARG, "rope_freqs: base scaling needs rope_dim over 2");
+    const double pi = 3.14159265358979323846;
+    double lo = 0, hi = 0;
+    if (scaling == HXB_ROPE_YARN) {
+        if (original < 1 || !(beta_fast > beta_slow) || !(beta_slow > 0) || !std::isfinite(beta_fast))
+            return attn_fail(HXB_E_ARG, "rope_freqs: bad original, beta_fast or beta_slow");
+        // the j at which a frequency makes beta turns over the original positions
+        lo = std::floor(rope_dim * std::log(original / (beta_fast * 2 * pi)) / (2 * std::log(theta)));
+        hi = std::ceil(rope_dim * std::log(original / (beta_slow * 2 * pi)) / (2 * std::log(theta)));
+        lo = std::max(lo, 0.0);
+        hi = std::min(hi, (double)rope_dim - 1);
+    }
+    const double base = scaling == HXB_ROPE_NTK ? theta * std::pow(factor, (double)rope_dim / (rope_dim - 2)) : theta;
+    for (int j = 0; j < rope_dim / 2; j++) {
+        const double f = std::pow(base, -2.0 * j / rope_dim);
+        double keep = 1.0;
+        if (scaling == HXB_ROPE_LINEAR) keep = 0.0;
+        if (scaling == HXB_ROPE_YARN) keep = 1.0 - std::min(std::max((j - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+        inv_freq[j] = f * keep + (scaling == HXB_ROPE_NONE || scaling == HXB_ROPE_NTK ? 0.0 : f / factor * (1.0 - keep));
+    }
+    *attn_factor = scaling == HXB_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    return HXB_OK;
+}
+
+extern "C" HXB_API int hxb_rope_table_dev(const double *inv_freq, int rope_dim, double attn_factor, int64_t pos0,
+                                          int64_t n_pos, float *cs, void *stream) {
+    if (rope_dim < 2 || rope_dim % 2 || rope_dim > 1024 || !inv_freq || n_pos < 0 || pos0 <= -(1ll << 31) ||
+        pos0 >= (1ll << 31) || n_pos > (1ll << 31) - std::max<int64_t>(pos0, 0))
+        return attn_fail(HXB_E_ARG, "rope_table: bad rope_dim, positions or frequencies");
+    if (n_pos == 0) return HXB_OK;
+    if (!cs || !aligned(cs, 8)) return attn_fail(HXB_E_ARG, "rope_table: the table must be 8-byte aligned");
+    FreqArg f;
+    for (int j = 0; j < rope_dim / 2; j++) {
+        if (!std::isfinite(inv_freq[j])) return attn_fail(HXB_E_ARG, "rope_table: frequency %d is not finite", j);
+        f.turns[j] = inv_freq[j] / (2 * 3.14159265358979323846);
+    }
+    const int64_t n = n_pos * (rope_dim / 2);
+    const int grid = (int)std::min<int64_t>((n + 255) / 256, 148 * 16);
+    k_rope_table<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(f, rope_dim / 2, attn_factor, pos0, n_pos,
+                                                                      reinterpret_cast<float2 *>(cs));
+    return attn_launched("rope_table") ? HXB_OK : HXB_E_DEVICE;
+}
+
+extern "C" HXB_API int hxb_rope_dev(const hxb_rope *r, const int32_t *pos, int64_t T, int n_heads, int head_dim,
+                                    const void *x, int x_dtype, int64_t x_stride, int64_t x_head_stride, void *y,
+                                    int y_dtype, int64_t y_stride, int64_t y_head_stride, void *stream) {
+    RopeArgs a = {};
+    int rc = HXB_OK;
+    if (!r) return attn_fail(HXB_E_ARG, "rope: null rotation");
+    if (T < 0 || T > 0x7fffffff || n_heads < 1 || n_heads > 65535 || head_dim < 2 || head_dim > 1024)
+        return attn_fail(HXB_E_ARG, "rope: bad shape (%lld tokens, %d heads of %d)", (long long)T, n_heads, head_dim);
+    if (!io_dtype(x_dtype) || !io_dtype(y_dtype)) return attn_fail(HXB_E_ARG, "rope: bad dtype");
+    if (!rope_view(r, head_dim, "rope", &a.r, &rc)) return rc;
+    if (T == 0) return HXB_OK;
+    if (!pos || !x || !y) return attn_fail(HXB_E_ARG, "rope: null pointer");
+    if (!aligned(pos, 4) || !aligned(x, elem_size(x_dtype)) || !aligned(y, elem_size(y_dtype)))
+        return attn_fail(HXB_E_ARG, "rope: pointer not aligned to its elements");
+    if (x_stride < 0 || x_head_stride < 0 || rows_overlap(T, y_stride, n_heads, y_head_stride, head_dim))
+        return attn_fail(HXB_E_ARG, "rope: bad strides");
+    a.in_place = x == y;
+    if (a.in_place && (x_dtype != y_dtype || (T > 1 && x_stride != y_stride) || (n_heads > 1 && x_head_stride != y_head_stride)))
+        return attn_fail(HXB_E_ARG, "rope: in place needs one type and one set of strides");
+    a.pos = pos, a.x = x, a.y = y, a.T = T, a.xs = x_stride, a.xh = x_head_stride, a.ys = y_stride, a.yh = y_head_stride;
+    a.H = n_heads, a.hd = head_dim;
+    a.vec = head_dim % 8 == 0 && rope_vec(a.r) && (2 * a.r.half) % 8 == 0 && vec_rows(x, x_dtype, T, x_stride, n_heads, x_head_stride) &&
+            vec_rows(y, y_dtype, T, y_stride, n_heads, y_head_stride);
+    const int rot = 2 * a.r.half;
+    a.units = a.vec ? (a.r.style == 0 ? a.r.half / 8 : rot / 8) + (head_dim - rot) / 8 : a.r.half + head_dim - rot;
+    a.per_head = FastDiv(a.units), a.per_tok = FastDiv(a.units * n_heads);
+    a.tpc = std::max(1, ROW_ITEMS / (a.units * n_heads));
+    const int grid = (int)((T + a.tpc - 1) / a.tpc);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (x_dtype == F32) rope_to<float>(a, y_dtype, grid, s);
+    else if (x_dtype == F16) rope_to<__half>(a, y_dtype, grid, s);
+    else rope_to<__nv_bfloat16>(a, y_dtype, grid, s);
+    return attn_launched("rope") ? HXB_OK : HXB_E_DEVICE;
+}
+
+extern "C" HXB_API int hxb_kv_write_dev(const hxb_kv_cache *c, const int32_t *start, const int32_t *pos0, int64_t T,
+                                        const void *k, int64_t k_stride, int64_t k_head_stride, const void *v,
+                                        int64_t v_stride, int64_t v_head_stride, int dtype, const hxb_rope *rope,
+                                        void *stream) {
+    return kv_rows("kv_write", c, start, pos0, T, const_cast<void *>(k), k_stride, k_head_stride, const_cast<void *>(v),
+                   v_stride, v_head_stride, dtype, rope, true, stream);
+}
+
+extern "C" HXB_API int hxb_kv_read_dev(const hxb_kv_cache *c, const int32_t *start, const int32_t *pos0, int64_t T,
+                                       void *k_out, int64_t k_stride, int64_t k_head_stride, void *v_out,
+                                       int64_t v_stride, int64_t v_head_stride, int dtype, void *stream) {
+    return kv_rows("kv_read", c, start, pos0, T, k_out, k_stride, k_head_stride, v_out, v_stride, v_head_stride, dtype,
+                   nullptr, false, stream);
+}

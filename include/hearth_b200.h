@@ -5,7 +5,8 @@
  * passed as void* / float*, CUDA streams as void* (cudaStream_t). A NULL stream means, for the
  * hxb_moe_* calls on a handle, the handle's own non-blocking stream; for the handle-less
  * device-pointer calls (hxb_act_quantize_dev, hxb_matmul_dev, hxb_dequantize_dev, hxb_expf_dev,
- * hxb_matmul_noalloc), which have no stream of their own, CUDA's legacy default stream.
+ * hxb_matmul_noalloc, hxb_rope_*, hxb_kv_*, hxb_attn_*, hxb_latent_*), which have no stream of their
+ * own, CUDA's legacy default stream.
  *
  * The entry points replace these reference interfaces (pierce-lonergan/hearth):
  *   hxb_matmul          hearth_matmul       engine/include/hearth.h:157-158, engine/src/quant.c:574-600
@@ -86,6 +87,114 @@ HXB_API int hxb_expf_dev(uint32_t x0, int64_t n, float *out, void *stream);
 #define HXB_NOALLOC_SCRATCH_BYTES ((size_t)4 << 20)
 HXB_API int hxb_matmul_noalloc(int dtype, const void *W, int64_t n_rows, int64_t n_cols, const float *X, int T,
                                float *Y, void *stream);
+
+/* ---- attention operators on device buffers ----------------------------------------------------
+ * Rotary positions, a paged key-value cache and decode attention for programs that keep their own
+ * decoder around these kernels (the whole decoder below keeps an f32 cache and the reference's
+ * canonical order; these calls have a smaller cache and their own order of summation, stated per
+ * call, so their results are close to it, not bit-identical). The reference's counterparts are
+ * rope_tables / rope_apply (engine/src/model.c:386-411), the KV cache rows (model.c:484-517), its
+ * GQA attention (model.c:519-629) and its absorbed latent attention (model.c:739-787).
+ *
+ * Common rules. Every pointer is a buffer of the current CUDA device. Calls are asynchronous on
+ * `stream` (NULL: the legacy default stream), allocate nothing, keep no state and may be captured
+ * into a CUDA graph; lengths, positions and page tables are read on the device when the work runs.
+ * Element types F32 (0), F16 (1), BF16 (2); strides count elements, the innermost one is 1. Outputs
+ * may not overlap inputs unless a call says so. Arguments that break a rule return HXB_E_ARG or
+ * HXB_E_UNSUPPORTED (a shape the kernels do not take) with a message, before anything is enqueued.
+ * Values on the device that break one (a page id outside the pool, a position outside a table)
+ * never cause an access: what they would have given reads as NaN, what they would have written is
+ * left out. */
+
+/* Rotary frequencies (host arithmetic in 64 bits): inv_freq[j], j < rope_dim / 2, and the factor for
+ * the table's values. scaling: HXB_ROPE_NONE theta^(-2j / rope_dim); HXB_ROPE_LINEAR the same / factor;
+ * HXB_ROPE_NTK with theta * factor^(rope_dim / (rope_dim - 2)); HXB_ROPE_YARN per frequency between
+ * none and linear by the number of turns it makes over `original` positions (beta_fast and more: none,
+ * beta_slow and fewer: linear, a ramp over j between), attn_factor 0.1 ln(factor) + 1. */
+enum { HXB_ROPE_NONE = 0, HXB_ROPE_LINEAR = 1, HXB_ROPE_NTK = 2, HXB_ROPE_YARN = 3 };
+HXB_API int hxb_rope_freqs(int rope_dim, double theta, int scaling, double factor, int original, double beta_fast,
+                           double beta_slow, double *inv_freq, double *attn_factor);
+/* cs [n_pos][rope_dim / 2][2] = attn_factor * (cos, sin)(p * inv_freq[j]) for p = pos0 + i, |p| < 2^31. inv_freq
+ * is a host array. The angle is reduced in 64 bits, so far positions lose nothing (within 2 ulp of f32). */
+HXB_API int hxb_rope_table_dev(const double *inv_freq, int rope_dim, double attn_factor, int64_t pos0, int64_t n_pos,
+                               float *cs, void *stream);
+
+/* The rotation of a call: values [offset, offset + rope_dim) of every head, pairs (j, j + rope_dim / 2)
+ * (style 0) or (2j, 2j + 1) (style 1): a' = a cos - b sin, b' = b cos + a sin in f32, each product and
+ * sum rounded (rope_apply's order). */
+typedef struct hxb_rope {
+    const float *cs;       /* [n_pos][rope_dim / 2][2] */
+    int64_t n_pos;
+    int rope_dim, offset, style;
+} hxb_rope;
+/* y[t][h] = x[t][h] with the rotation of position pos[t] (device, [T]); the other values are copied. x and y
+ * [T][n_heads][head_dim] by token and head strides, any two element types, rounded to nearest. y may be x
+ * itself (same pointer, type and strides). A position outside [0, n_pos) gives NaN. */
+HXB_API int hxb_rope_dev(const hxb_rope *r, const int32_t *pos, int64_t T, int n_heads, int head_dim, const void *x,
+                         int x_dtype, int64_t x_stride, int64_t x_head_stride, void *y, int y_dtype, int64_t y_stride,
+                         int64_t y_head_stride, void *stream);
+
+/* One layer's cache as pages, with the page tables of a batch of sequences. Position p of sequence b is slot
+ * p % page_tokens of page table[b][p / page_tokens]. dtype F16, BF16 or Q8 (3): int8 codes with one f32 scale for
+ * each 64 values, the rule of hxb_act_quantize_dev (scale = max|x| / 127, code = round(x * (1 / scale)); a
+ * block that holds a NaN or an infinity reads back as NaN; under a maximum of 2^-121, where 1 / scale is infinite, codes
+ * are 0 or +-127). A latent cache (one row a token for keys and
+ * values) has n_kv_heads 1 and v, v_scale NULL. Table entries past a sequence's end are not read. */
+typedef struct hxb_kv_cache {
+    int dtype;
+    int n_kv_heads, head_dim;        /* head_dim: a multiple of 8 up to 1024 (Q8: of 64) */
+    int page_tokens;                 /* a power of two up to 1024 */
+    int64_t n_pages;
+    void *k, *v;                     /* [n_pages][n_kv_heads][page_tokens][head_dim], 16-byte aligned */
+    float *k_scale, *v_scale;        /* Q8: [n_pages][n_kv_heads][page_tokens][head_dim / 64], 4-byte aligned */
+    const int32_t *table;            /* [n_seqs][table_pages], rows table_stride apart (0: one row for all) */
+    int64_t table_stride;
+    int table_pages, n_seqs;
+} hxb_kv_cache;
+/* T rows of keys and values [T][n_kv_heads][head_dim] into the cache: rows start[b] .. start[b+1] - 1 are
+ * positions pos0[b], pos0[b] + 1, ... of sequence b (start [n_seqs + 1] ascending, pos0 [n_seqs], device). Rows
+ * before start[0] and from start[n_seqs] on are padding: nothing is written for them. rope (may be NULL)
+ * rotates the keys by their positions first. Slots of other positions keep their bytes. Two sequences of one
+ * call may share pages that neither of them writes; a slot that two rows of one call write is left undefined. */
+HXB_API int hxb_kv_write_dev(const hxb_kv_cache *c, const int32_t *start, const int32_t *pos0, int64_t T, const void *k,
+                             int64_t k_stride, int64_t k_head_stride, const void *v, int64_t v_stride,
+                             int64_t v_head_stride, int dtype, const hxb_rope *rope, void *stream);
+/* The same rows back: k_out, v_out (v_out NULL for a latent cache) in any element type, rounded to nearest;
+ * padding rows keep what they hold. */
+HXB_API int hxb_kv_read_dev(const hxb_kv_cache *c, const int32_t *start, const int32_t *pos0, int64_t T, void *k_out,
+                            int64_t k_stride, int64_t k_head_stride, void *v_out, int64_t v_stride,
+                            int64_t v_head_stride, int dtype, void *stream);
+
+/* Attention of one new token a sequence over its cached positions 0 .. lens[b] - 1 (lens [n_seqs], device; the new
+ * token's own row is in the cache): out[b][h] = sum_r p_r v_r, p = softmax(scale * q[b][h] . k_r), kv head
+ * h / (n_heads / n_kv_heads); lse[b][h] (may be NULL) = ln sum_r exp(scale * q . k_r). A length of 0 or less
+ * gives zeros and -inf. q and out [n_seqs][n_heads][head_dim] of one element type; head_dim a multiple of 16 up
+ * to 256. Several tokens of one sequence are several rows with a shared table row (table_stride 0, or equal
+ * rows) and their own lengths. Scores, maxima, sums and outputs are f32 until the last rounding. The work is split over the
+ * positions whatever the lengths are and joined in a fixed order: the same inputs give the same bits.
+ * ws: device scratch of at least hxb_attn_decode_workspace(c, n_heads) bytes, 16-byte aligned, contents free
+ * before and after; calls that may overlap on the GPU need one each. */
+HXB_API size_t hxb_attn_decode_workspace(const hxb_kv_cache *c, int n_heads);
+HXB_API int hxb_attn_decode_dev(const hxb_kv_cache *c, const int32_t *lens, const void *q, int64_t q_stride,
+                                int64_t q_head_stride, int n_heads, int dtype, float scale, void *out,
+                                int64_t out_stride, int64_t out_head_stride, float *lse, void *ws, size_t ws_bytes,
+                                void *stream);
+
+/* Latent attention in its absorbed form, one new token a sequence, over a latent cache whose rows are
+ * [latent (rank) | rotated key part (head_dim - rank)]: with w [n_heads][nope + v_dim][rank] (rows 0 .. nope-1
+ * expand a latent to the head's key, the others to its value) and q [n_seqs][n_heads][nope + head_dim - rank]
+ * (rotated part already rotated),
+ *   qa = sum_d q[d] w[h][d], p = softmax(scale * (qa . latent_r + q_rot . key_r)), o = sum_r p_r latent_r,
+ *   out[b][h][j] = o . w[h][nope + j].
+ * Lengths, empty sequences and ws as for hxb_attn_decode_dev. q, w and out share an element type F16 or BF16;
+ * the cache has it too, or is Q8. rank a multiple of 128 up to 512, head_dim - rank a multiple of 16 from 16
+ * to 64, nope and v_dim multiples of 16 up to 256, n_heads up to 256; w contiguous, 16-byte aligned. qa is rounded to the
+ * element type (Q8: bf16) for the matrix instructions; scores, sums and o stay f32. */
+HXB_API size_t hxb_latent_decode_workspace(const hxb_kv_cache *c, int n_heads, int rank);
+HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_t *lens, const void *q, int64_t q_stride,
+                                  int64_t q_head_stride, const void *w, int n_heads, int rank, int nope, int v_dim,
+                                  int dtype, float scale, void *out, int64_t out_stride, int64_t out_head_stride,
+                                  void *ws, size_t ws_bytes, void *stream);
 
 /* ---- MoE backend handle ---------------------------------------------------------------------- */
 typedef struct hxb_moe hxb_moe;

@@ -1,0 +1,630 @@
+"""The attention operators on the GPU against plain 64-bit forms on the CPU.
+
+Tolerances. u(t) is half a step of an element type (tests/attn_util.half_step), w = 2^-24 that of f32. Stored
+values are one rounding of a value known to 64 bits: u(t), plus what the f32 steps before it lose. An attention
+output is off by at most u(out) |o| + (2 ds + up + 2^-21 + n w) sum_r p_r |v_r|: each weight exp(s_r) / sum is off by twice
+the largest score error ds, by the rounding up of a weight as an operand of the matrix instructions (none where
+operands carry f32's bits) and by the f32 exponential and rescalings (2^-21 together), and a sum of n terms by n w."""
+import itertools
+import math
+
+import pytest
+import torch
+
+import hearth_b200 as hb
+from tests.attn_util import F, attend, dequant, gen, half_step, pool, put, quant, randn, rotate, table_of
+
+pytestmark = pytest.mark.gpu
+W = 2.0 ** -24
+r32 = lambda v: v.float().double()  # noqa: E731
+
+
+def cu(x):
+    return None if x is None else x.cuda()
+
+
+def table64(dim, n_pos, theta=1e4):
+    f = theta ** (-torch.arange(dim // 2, dtype=torch.float64) * 2 / dim)
+    a = torch.arange(n_pos, dtype=torch.float64)[:, None] * f
+    return a.cos(), a.sin()
+
+
+def cs_of(cos, sin):
+    return torch.stack([cos, sin], -1).float()
+
+
+# ----------------------------------------------------------------------------------------- rotary positions
+
+@pytest.mark.parametrize("dim,first,n,scaling", [(2, 0, 7, "none"), (64, 0, 1000, "none"), (128, 999_983, 517, "linear"),
+                                                 (80, 2_147_483_000, 600, "none"), (64, -300, 400, "yarn"),
+                                                 (1024, 12345, 33, "ntk")])
+def test_rope_table(gpu, dim, first, n, scaling):
+    f, a = hb.rope_freqs(dim, 1e6, scaling=scaling, factor=1.0 if scaling == "none" else 8.0)
+    got = hb.rope_table(f, n, first=first, factor=a).cpu().double()
+    ang = torch.arange(first, first + n, dtype=torch.float64)[:, None] * torch.from_numpy(f)
+    want = torch.stack([ang.cos(), ang.sin()], -1) * a
+    # 2 ulp of the value (4 half steps), and the 64-bit phase: angle * 2^-52
+    tol = 4 * W * want.abs() + a * (ang.abs() * 2.0 ** -51)[..., None] + 2.0 ** -40
+    assert (got - want).abs().le(tol).all(), ((got - want).abs() / tol).max()
+
+
+def test_rope_table_empty(gpu):
+    assert hb.rope_table([1.0], 0).shape == (0, 1, 2)
+
+
+ROPES = [dict(T=1, H=1, D=64, rot=64, off=0), dict(T=5, H=3, D=80, rot=40, off=40), dict(T=7, H=2, D=192, rot=64, off=128),
+         dict(T=3, H=4, D=50, rot=18, off=3), dict(T=130, H=5, D=128, rot=128, off=0), dict(T=9, H=64, D=576, rot=64, off=512),
+         dict(T=4, H=2, D=10, rot=2, off=8), dict(T=2, H=3, D=256, rot=24, off=8)]
+
+
+@pytest.mark.parametrize("shape", ROPES, ids=str)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("x,y", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f16", "bf16")])
+def test_rope(gpu, shape, inter, x, y):
+    T, H, D, rot, off = (shape[k] for k in ("T", "H", "D", "rot", "off"))
+    g = gen(1)
+    cos, sin = table64(rot, 300)
+    pos = torch.randint(0, 300, (T,), generator=g, dtype=torch.int32)
+    xs = randn(g, T, H, D, dtype=F[x])
+    cs = cs_of(cos, sin)
+    want = rotate(xs.double(), cs[pos.long(), :, 0].double(), cs[pos.long(), :, 1].double(), inter, off, r32).to(F[y])
+    wide = torch.zeros(T, H + 1, D + 5, dtype=F[x])        # odd strides: the element path
+    wide[:, :H, :D] = xs
+    out = torch.full((T, H, D), 7.0, dtype=F[y]).cuda()
+    for src in (xs.cuda(), wide.cuda()[:, :H, :D]):
+        got = hb.rope(src, pos.cuda(), cs.cuda(), interleaved=inter, offset=off, out=out.fill_(7.0))
+        assert torch.equal(got.cpu(), want)                 # the f32 steps are defined: equal bits
+    if x == y:
+        buf = xs.cuda()
+        assert torch.equal(hb.rope(buf, pos.cuda(), cs.cuda(), interleaved=inter, offset=off, out=buf).cpu(), want)
+        buf = wide.cuda()
+        hb.rope(buf[:, :H, :D], pos.cuda(), cs.cuda(), interleaved=inter, offset=off, out=buf[:, :H, :D])
+        assert torch.equal(buf[:, :H, :D].cpu(), want)
+        assert (buf[:, H:] == 0).all() and (buf[:, :, D:] == 0).all()
+
+
+def test_rope_positions_outside_the_table_and_no_tokens(gpu):
+    cs = cs_of(*table64(64, 50)).cuda()
+    x = randn(gen(2), 4, 2, 96, dtype=torch.bfloat16).cuda()
+    for inter in (False, True):
+        y = hb.rope(x, torch.tensor([0, -1, 50, 49], dtype=torch.int32).cuda(), cs, interleaved=inter)
+        bad = torch.isnan(y).all(-1).cpu(), torch.isnan(y[..., :64]).all(-1).cpu()
+        assert bad[1].tolist() == [[False] * 2, [True] * 2, [True] * 2, [False] * 2] and not bad[0].any()
+        assert torch.equal(y[..., 64:], x[..., 64:])
+    assert hb.rope(x[:0], torch.zeros(0, dtype=torch.int32).cuda(), cs).shape == (0, 2, 96)
+
+
+# ----------------------------------------------------------------------------------------- cache rows
+
+KV = [dict(news=[1], past=[0], Hkv=1, D=64, pt=16), dict(news=[3, 0, 40, 1], past=[5, 9, 30, 0], Hkv=2, D=128, pt=16),
+      dict(news=[17, 5], past=[3, 1], Hkv=3, D=64, pt=1), dict(news=[70, 9, 33], past=[0, 63, 64], Hkv=1, D=576, pt=32, latent=True),
+      dict(news=[9, 2], past=[2, 2], Hkv=5, D=256, pt=8), dict(news=[6, 130], past=[1, 250], Hkv=2, D=64, pt=128)]
+
+
+def kv_case(g, c, cache, x):
+    B, lens = len(c["news"]), [a + b for a, b in zip(c["news"], c["past"])]
+    table, total = table_of(g, lens, c["pt"])
+    start = torch.tensor([0] + list(itertools.accumulate(c["news"])), dtype=torch.int32) + 2    # two padding rows in front
+    T = int(start[-1]) + 3                                                                      # three behind
+    k, v = (randn(g, T, c["Hkv"], c["D"], dtype=F[x]) for _ in range(2))
+    pools = [pool(g, total, c["Hkv"], c["pt"], c["D"], cache, fill=3.0) for _ in range(2)]
+    return B, lens, table, start, torch.tensor(c["past"], dtype=torch.int32), T, k, v, pools
+
+
+def bits(t):
+    return t.contiguous().view(torch.uint8)
+
+
+@pytest.mark.parametrize("c", KV, ids=str)
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("x", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rope", [None, "half", "inter"])
+def test_kv_write_and_read(gpu, c, cache, x, rope):
+    g = gen(3)
+    latent = c.get("latent", False)
+    B, lens, table, start, pos0, T, k, v, ((kp, ks), (vp, vs)) = kv_case(g, c, cache, x)
+    rot, off = (64, 512) if latent else (c["D"] // 2, 0)
+    cs = cs_of(*table64(rot, max(lens)))
+    rows = [(b, t, int(pos0[b]) + t - int(start[b])) for b in range(B) for t in range(int(start[b]), int(start[b + 1]))]
+    kd = k.double()
+    if rope:
+        for b, t, p in rows:
+            kd[t] = rotate(kd[t:t + 1], cs[p:p + 1, :, 0].double(), cs[p:p + 1, :, 1].double(), rope == "inter", off, r32)[0]
+    dev = [cu(t) for t in (kp, None if latent else vp, ks, None if latent else vs)]
+    wide = torch.zeros(T, c["Hkv"] + 1, c["D"] + 4, dtype=F[x])
+    wide[:, :c["Hkv"], :c["D"]] = k
+    for src in (k.cuda(), wide.cuda()[:, :c["Hkv"], :c["D"]]):
+        hb.kv_write(src, None if latent else v.cuda(), dev[0], dev[1], table.cuda(), start.cuda(), pos0.cuda(), k_scale=dev[2], v_scale=dev[3],
+                    cs=cu(cs) if rope else None, interleaved=rope == "inter", offset=off)
+    want = {}
+    for b, t, p in rows:
+        want[t] = put(kp, ks, table, b, p, c["pt"], kd[t]), None if latent else put(vp, vs, table, b, p, c["pt"], v[t].double())
+    for got, ref in zip(dev, (kp, vp, ks, vs)):     # what was written, and every other byte
+        assert got is None or torch.equal(bits(got.cpu()), bits(ref))
+    for y in ("f32", "f16", "bf16"):
+        outs = [torch.full((T, c["Hkv"], c["D"]), 9.0, dtype=F[y]).cuda() for _ in range(1 if latent else 2)]
+        hb.kv_read(dev[0], dev[1], table.cuda(), start.cuda(), pos0.cuda(), outs[0], None if latent else outs[1], k_scale=dev[2], v_scale=dev[3])
+        for i, o in enumerate(outs):
+            o = o.cpu()
+            for t in range(T):
+                ref = want[t][i].float().to(F[y]) if t in want else torch.full((c["Hkv"], c["D"]), 9.0, dtype=F[y])
+                assert torch.equal(o[t], ref), (y, i, t)
+
+
+def test_kv_bad_pages_and_positions(gpu):
+    """Ids outside the pool, positions outside the table or negative: nothing written, NaN read; the rest works."""
+    kp, vp = torch.zeros(4, 1, 8, 64, dtype=torch.bfloat16).cuda(), torch.zeros(4, 1, 8, 64, dtype=torch.bfloat16).cuda()
+    table = torch.tensor([[2, 4], [-7, 1], [3, 2_000_000_000]], dtype=torch.int32).cuda()
+    start = torch.tensor([0, 17, 33, 43], dtype=torch.int32).cuda()
+    pos0 = torch.tensor([0, 0, -2], dtype=torch.int32).cuda()
+    k = randn(gen(4), 43, 1, 64, dtype=torch.bfloat16).cuda()
+    hb.kv_write(k, k, kp, vp, table, start, pos0)
+    assert torch.equal(kp[2, 0], k[:8, 0]) and torch.equal(kp[1, 0], k[25:33, 0]) and torch.equal(kp[3, 0], k[35:43, 0])
+    assert (kp[0] == 0).all()
+    ko, vo = torch.zeros_like(k), torch.zeros_like(k)
+    hb.kv_read(kp, vp, table, start, pos0, ko, vo)
+    good = torch.zeros(43, dtype=torch.bool)
+    good[:8] = good[25:33] = good[35:43] = True
+    assert torch.equal(ko[good.cuda()], k[good.cuda()]) and torch.isnan(ko[~good.cuda()]).all() and torch.isnan(vo[~good.cuda()]).all()
+
+
+def test_kv_q8_values_at_the_edges(gpu):
+    """Zero blocks, blocks of subnormal and of the largest values, ties, and blocks that hold NaN or infinities."""
+    x = randn(gen(5), 12, 1, 128)
+    x[0] = 0
+    x[1, 0, :64] *= 1e-42
+    x[2, 0, :64] *= 1e38
+    x[3, 0, 5] = float("nan")
+    x[4, 0, 70] = float("inf")
+    x[5, 0, 3] = -float("inf")
+    x[6, 0, :64] = torch.arange(64) - 31.5
+    x[6, 0, 0] = 127.0
+    x[7] = -0.0
+    kp, ks = torch.zeros(1, 1, 16, 128, dtype=torch.int8), torch.zeros(1, 1, 16, 2)
+    dev = [t.cuda() for t in (kp, ks)]
+    tab, start, p0 = torch.zeros(1, 1, dtype=torch.int32), torch.tensor([0, 12], dtype=torch.int32), torch.tensor([0], dtype=torch.int32)
+    hb.kv_write(x.cuda(), None, dev[0], None, tab.cuda(), start.cuda(), p0.cuda(), k_scale=dev[1])
+    code, d = quant(x)
+    fin = torch.isfinite(d)
+    assert torch.equal(torch.isfinite(dev[1][0, 0, :12].cpu()), fin[:, 0])
+    assert torch.equal(dev[1][0, 0, :12].cpu()[fin[:, 0]], d[:, 0][fin[:, 0]])
+    got = dev[0][0, 0, :12].cpu().view(12, 2, 64)
+    assert torch.equal(got[fin[:, 0]], code.view(12, 2, 64)[fin[:, 0]])
+    out = torch.zeros(12, 1, 128).cuda()
+    hb.kv_read(dev[0], None, tab.cuda(), start.cuda(), p0.cuda(), out, None, k_scale=dev[1])
+    assert torch.equal(torch.isnan(out.cpu()).view(12, 2, 64).all(-1), ~fin[:, 0])
+    blk = (out.cpu().double() - x.double()).abs().view(12, 2, 64)[fin[:, 0]]
+    dd = d[:, 0][fin[:, 0]].double()[:, None]
+    # half a code and the f32 steps (the scale's own rounding is at most half of 2^-149, 127 times over); where
+    # 1 / scale passes f32's range (scales under 2^-128) every code is 0 or +-127: off by less than the block's maximum
+    assert (blk <= torch.where(dd < 2.0 ** -128, 127 * dd, (0.5 + 127 * 3 * W) * dd) + 2.0 ** -149 * 64).all()
+
+
+# ----------------------------------------------------------------------------------------- decode attention
+
+def filled(g, lens, Hkv, pt, D, cache, width=None, scale=1.0, sides=2):
+    """A cache with its sequences' rows: pools, scales, table, and the f64 rows [n, Hkv, D] of each sequence."""
+    table, total = table_of(g, lens, pt, width=width)
+    pools, rows = [], []
+    for _ in range(sides):
+        p, s = pool(g, total, Hkv, pt, D, cache)
+        seqs = []
+        for b, n in enumerate(lens):
+            x = randn(g, max(n, 0), Hkv, D, scale=scale).double()
+            seqs.append(torch.stack([put(p, s, table, b, i, pt, x[i]) for i in range(n)]) if n > 0 else x)
+        pools.append((p, s))
+        rows.append(seqs)
+    return pools, table, rows
+
+
+def operand(cache, x):
+    """Half a step of a softmax weight as an operand: none for f32 queries."""
+    if x == "f32":
+        return 0.0
+    return half_step(torch.float16 if cache == "f16" else torch.bfloat16)
+
+
+def check_out(got, want, vabs, big, n, x, up, D):
+    ds = (D + 16) * W * big[:, None]
+    tol = half_step(F[x]) * want.abs() + (2 * ds + up + 2.0 ** -21 + n * W) * vabs + 1e-30
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), (err / tol).max()
+
+
+def check_attn(lens, H, Hkv, D, pt, cache, x, seed=6, width=None, qscale=1.0, **kw):
+    g = gen(seed)
+    pools, table, (krows, vrows) = filled(g, lens, Hkv, pt, D, cache, width)
+    q = randn(g, len(lens), H, D, dtype=F[x], scale=qscale)
+    (kp, ks), (vp, vs) = pools
+    scale = D ** -0.5
+    out, lse = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scale=scale,
+                                   k_scale=cu(ks), v_scale=cu(vs), return_lse=True, **kw)
+    out, lse = out.cpu(), lse.cpu()
+    for b, n in enumerate(lens):
+        want, wl, vabs, big = attend(q[b].double(), krows[b], vrows[b], scale)
+        if n <= 0:
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all()
+            continue
+        check_out(out[b], want, vabs, big, n, x, operand(cache, x), D)
+        assert ((lse[b].double() - wl).abs() <= (D + 16) * W * big + 2.0 ** -20 + n * W + 2 * W * wl.abs()).all()
+
+
+LENS = [[1], [0], [2, 1, 0, 15, 16, 17], [31, 33, 63, 64, 65, 127, 129, 0, 255, 257], [700, 3], [1100]]
+
+
+@pytest.mark.parametrize("lens", LENS, ids=str)
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("x", ["f32", "f16", "bf16"])
+def test_decode_attention_lengths(gpu, lens, cache, x):
+    check_attn(lens, 8, 2, 128, 16, cache, x)
+
+
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (3, 3), (4, 1), (7, 1), (8, 1), (9, 1), (24, 2), (32, 2), (40, 1), (64, 1), (33, 11)])
+@pytest.mark.parametrize("cache,x", [("bf16", "bf16"), ("q8", "f32"), ("f16", "f16")])
+def test_decode_attention_heads(gpu, H, Hkv, cache, x):
+    check_attn([37, 5, 130], H, Hkv, 64, 16, cache, x)
+
+
+@pytest.mark.parametrize("D", [16, 32, 48, 64, 80, 96, 112, 128, 144, 160, 192, 240, 256])
+@pytest.mark.parametrize("cache,x", [("f16", "f32"), ("bf16", "bf16"), ("q8", "bf16")])
+def test_decode_attention_dims(gpu, D, cache, x):
+    if cache == "q8" and D % 64:
+        pytest.skip("Q8 rows come in blocks of 64")
+    check_attn([50, 129, 1], 6, 2, D, 32, cache, x)
+
+
+@pytest.mark.parametrize("pt", [1, 2, 4, 8, 16, 32, 64, 128, 1024])
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+def test_decode_attention_pages(gpu, pt, cache):
+    check_attn([73, 0, 200, 6], 8, 2, 64, pt, cache, "bf16")
+
+
+def test_decode_attention_large_scores(gpu):
+    for x in ("f32", "bf16", "f16"):
+        check_attn([300, 40], 8, 2, 128, 16, "f16", x, qscale=30.0)
+        check_attn([300, 40], 8, 2, 128, 16, "bf16", x, qscale=30.0)
+
+
+def test_decode_attention_query_ranges(gpu):
+    """Queries whose size is far from one, in both directions, against every cache: nothing overflows or is flushed."""
+    for cache, s in itertools.product(("f16", "bf16", "q8"), (1e-6, 3e4)):
+        g = gen(7)
+        pools, table, (krows, vrows) = filled(g, [90], 1, 16, 64, cache)
+        q = randn(g, 1, 4, 64, dtype=torch.bfloat16, scale=s)
+        scale = 1.0 / (8.0 * s)
+        (kp, ks), (vp, vs) = pools
+        out = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.tensor([90], dtype=torch.int32).cuda(), scale=scale,
+                                  k_scale=cu(ks), v_scale=cu(vs)).cpu()
+        want, _, vabs, big = attend(q[0].double(), krows[0], vrows[0], scale)
+        check_out(out[0], want, vabs, big, 90, "bf16", operand(cache, "bf16"), 64)
+
+
+def test_decode_attention_one_heavy_among_many_light(gpu):
+    """One position takes nearly all the weight; the others' small weights still add up."""
+    n, D = 3000, 64
+    for cache, x in itertools.product(("f16", "bf16", "q8"), ("f32", "bf16", "f16")):
+        g = gen(8)
+        pools, table, (krows, vrows) = filled(g, [n], 1, 64, D, cache, scale=0.25)
+        (kp, ks), (vp, vs) = pools
+        q = randn(g, 1, 2, D, dtype=F[x], scale=0.1)
+        q[..., 0] = 12.0
+        heavy = torch.zeros(1, D, dtype=torch.float64)
+        heavy[0, 0] = 8.0
+        krows[0][1234] = put(kp, ks, table, 0, 1234, 64, heavy)
+        scale = 0.15
+        out = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), scale=scale,
+                                  k_scale=cu(ks), v_scale=cu(vs)).cpu()
+        want, _, vabs, big = attend(q[0].double(), krows[0], vrows[0], scale)
+        check_out(out[0], want, vabs, big, n, x, operand(cache, x), D)
+
+
+def test_decode_attention_bad_pages_and_infinities(gpu):
+    g = gen(9)
+    pools, table, (krows, vrows) = filled(g, [40, 40, 40, 40, 40], 1, 16, 64, "bf16")
+    (kp, _), (vp, _) = pools
+    q = randn(g, 5, 8, 64, dtype=torch.bfloat16)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    table[1, 1] = 99                                          # no such page
+    lens = torch.tensor([40, 40, 40, 40, 1000], dtype=torch.int32)   # the last is longer than its table
+    kp[int(table[2, 0]), 0, 3, 0] = float("inf")              # a score of +inf: the formula gives NaN
+    kp[int(table[3, 0]), 0, 3, 0] = -float("inf")             # -inf: no weight
+    krows[3][3, 0, 0] = -float("inf")
+    out, lse = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), lens.cuda(), scale=0.125, return_lse=True)
+    out, lse = out.cpu(), lse.cpu()
+    assert torch.isnan(out[[1, 2, 4]]).all() and torch.isnan(lse[[1, 4]]).all()
+    for b in (0, 3):
+        keep = [i for i in range(40) if not (b == 3 and i == 3)]
+        want, wl, vabs, big = attend(q[b].double(), krows[b][keep], vrows[b][keep], 0.125)
+        check_out(out[b], want, vabs, big, 40, "bf16", operand("bf16", "bf16"), 64)
+
+
+def test_decode_attention_all_scores_minus_infinity(gpu):
+    """A row whose scores leave nothing gives zeros and -inf, like an empty one."""
+    kp = torch.full((2, 1, 16, 64), -float("inf"), dtype=torch.bfloat16)
+    vp = torch.ones_like(kp)
+    q = torch.ones(1, 4, 64, dtype=torch.bfloat16)
+    out, lse = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), torch.tensor([[0, 1]], dtype=torch.int32).cuda(),
+                                   torch.tensor([20], dtype=torch.int32).cuda(), scale=1.0, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_decode_attention_strides_shared_table_and_scratch(gpu):
+    """Padded query and output rows, one table row for several tokens of a sequence, a scratch of the caller's full
+    of NaN, and the same bits again."""
+    g = gen(10)
+    (kp, _), (vp, _) = (p := filled(g, [200], 2, 16, 128, "bf16"))[0]
+    table, (krows, vrows) = p[1], p[2]
+    lens = [197, 198, 199, 200, 1, 0]
+    wide = randn(g, 6, 9, 136, dtype=torch.bfloat16).cuda()
+    q = wide[:, :8, 3:131]
+    out = torch.full((6, 9, 136), 5.0, dtype=torch.bfloat16).cuda()
+    shared = table.cuda().expand(6, -1)
+    ws = torch.full((1 << 24,), 255, dtype=torch.uint8).cuda()
+    args = (q, kp.cuda(), vp.cuda(), shared, torch.tensor(lens, dtype=torch.int32).cuda())
+    hb.decode_attention(*args, scale=0.1, out=out[:, :8, 3:131], workspace=ws)
+    again = hb.decode_attention(*args, scale=0.1)
+    assert torch.equal(again, out[:, :8, 3:131])
+    rest = out.clone()
+    rest[:, :8, 3:131] = 5.0
+    assert (rest == 5.0).all()
+    for b, n in enumerate(lens):
+        want, _, vabs, big = attend(q[b].cpu().double(), krows[0][:n], vrows[0][:n], 0.1)
+        check_out(again[b].cpu(), want, vabs, big, n, "bf16", operand("bf16", "bf16"), 128)
+    with pytest.raises(ValueError, match="workspace"):
+        hb.decode_attention(*args, scale=0.1, workspace=ws[:8])
+
+
+def test_decode_attention_many_sequences(gpu):
+    """More sequences than CTAs, lengths from nothing to a few pages."""
+    g = gen(11)
+    lens = [int(v) for v in torch.randint(0, 40, (701,), generator=g)]
+    check_attn(lens, 4, 2, 64, 8, "bf16", "bf16", seed=12)
+
+
+def test_decode_attention_long_split_over_the_cache(gpu):
+    """A context long enough that every CTA has a share of one sequence, beside short ones."""
+    g = gen(13)
+    n, D = 70_001, 64
+    k = torch.randn((2, 1100, 1, 64, D), generator=g, dtype=torch.float32).to(torch.bfloat16)
+    perm = torch.randperm(1100, generator=g)[:1094].to(torch.int32)
+    table = torch.stack([perm, perm])
+    table[1, 0] = perm[5]
+    q = randn(g, 2, 8, D, dtype=torch.float32)
+    out = hb.decode_attention(q.cuda(), k[0].cuda(), k[1].cuda(), table.cuda(), torch.tensor([n, 7], dtype=torch.int32).cuda(), scale=0.125).cpu()
+    for b, m in ((0, n), (1, 7)):
+        kr, vr = (k[i][table[b].long()].transpose(1, 2).reshape(-1, 1, D)[:m].double() for i in (0, 1))
+        want, _, vabs, big = attend(q[b].double(), kr, vr, 0.125)
+        check_out(out[b], want, vabs, big, m, "f32", 0.0, D)
+
+
+# ----------------------------------------------------------------------------------------- latent attention
+
+def check_latent(lens, H, R, dr, dn, dv, pt, cache, x, seed=20, c_rows=None, **kw):
+    g = gen(seed)
+    pools, table, (rows,) = filled(g, lens, 1, pt, R + dr, cache, sides=1)
+    cp, cs = pools[0]
+    q = randn(g, len(lens), H, dn + dr, dtype=F[x])
+    w = randn(g, H, dn + dv, R, dtype=F[x], scale=R ** -0.5)
+    scale = (dn + dr) ** -0.5
+    out = hb.latent_attention(q.cuda(), w.cuda(), cp.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scale=scale,
+                              c_scale=cu(cs), **kw).cpu()
+    mma = torch.bfloat16 if cache == "q8" else F[x]
+    up = half_step(mma)
+    for b, n in enumerate(lens):
+        if n <= 0:
+            assert (out[b] == 0).all()
+            continue
+        qa = torch.einsum("hd,hdr->hr", q[b, :, :dn].double(), w[:, :dn].double())
+        qf = torch.cat([qa, q[b, :, dn:].double()], -1)
+        o, _, vabs, big = attend(qf, rows[b], rows[b][..., :R], scale)
+        wv = w[:, dn:].double()
+        want = torch.einsum("hr,hvr->hv", o, wv)
+        wabs = torch.einsum("hr,hvr->hv", vabs, wv.abs())
+        # scores: qa rounded to an operand, and f32 sums; weights rounded to an operand; o split in two operands
+        # (its rest is below 2^-15); f32 sums over n and R terms
+        ds = (up + (R + dr + dn + 32) * W) * big[:, None]
+        tol = half_step(F[x]) * want.abs() + (2 * ds + up + 2.0 ** -15 + (n + R + 16) * W) * wabs
+        err = (out[b].double() - want).abs()
+        assert (err <= tol).all(), (b, (err / tol).max())
+        # the roundings are independent: in the 2-norm at most the three operands' and the output's half steps together
+        assert err.norm() <= 4 * max(up, half_step(F[x])) * want.norm(), (b, err.norm() / want.norm())
+
+
+@pytest.mark.parametrize("lens", [[1], [0], [3, 0, 15, 16, 17], [63, 64, 65, 127, 128, 129, 0, 200], [1000, 2]], ids=str)
+@pytest.mark.parametrize("cache,x", [("bf16", "bf16"), ("f16", "f16"), ("q8", "bf16"), ("q8", "f16")])
+def test_latent_attention_lengths(gpu, lens, cache, x):
+    check_latent(lens, 16, 512, 64, 128, 128, 64, cache, x)
+
+
+@pytest.mark.parametrize("H", [1, 2, 7, 8, 16, 24, 40, 64, 65, 128, 200])
+def test_latent_attention_heads(gpu, H):
+    check_latent([70, 1, 130], H, 512, 64, 64, 64, 32, "bf16", "bf16")
+    check_latent([70, 1, 130], H, 512, 64, 64, 64, 32, "q8", "bf16")
+
+
+@pytest.mark.parametrize("R,dr,dn,dv", [(128, 16, 16, 16), (256, 64, 64, 128), (384, 32, 128, 64), (512, 48, 48, 256), (512, 64, 256, 16)])
+@pytest.mark.parametrize("cache,x", [("bf16", "bf16"), ("f16", "f16"), ("q8", "bf16")])
+def test_latent_attention_dims(gpu, R, dr, dn, dv, cache, x):
+    if cache == "q8" and dr % 64:
+        pytest.skip("Q8 rows come in blocks of 64")
+    check_latent([90, 33], 12, R, dr, dn, dv, 16, cache, x)
+
+
+@pytest.mark.parametrize("pt", [1, 2, 8, 16, 32, 64, 128, 1024])
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+def test_latent_attention_pages(gpu, pt, cache):
+    check_latent([73, 0, 150], 16, 512, 64, 64, 64, pt, cache, "bf16")
+
+
+def test_latent_attention_many_sequences(gpu):
+    g = gen(21)
+    check_latent([int(v) for v in torch.randint(0, 30, (331,), generator=g)], 8, 128, 64, 16, 16, 8, "bf16", "bf16")
+
+
+def test_latent_attention_bad_pages_strides_and_scratch(gpu):
+    g = gen(22)
+    pools, table, (rows,) = filled(g, [100, 100, 100], 1, 16, 576, "bf16", sides=1)
+    cp = pools[0][0].cuda()
+    wide = randn(g, 3, 17, 200, dtype=torch.bfloat16).cuda()
+    q, w = wide[:, :16, 8:200], randn(g, 16, 256, 512, dtype=torch.bfloat16, scale=0.05).cuda()
+    lens = torch.tensor([100, 100, 100], dtype=torch.int32).cuda()
+    good = hb.latent_attention(q, w, cp, table.cuda(), lens, scale=0.07)
+    out = torch.full((3, 17, 131), 5.0, dtype=torch.bfloat16).cuda()
+    ws = torch.full((1 << 25,), 255, dtype=torch.uint8).cuda()
+    hb.latent_attention(q, w, cp, table.cuda(), lens, scale=0.07, out=out[:, :16, 2:130], workspace=ws)
+    assert torch.equal(out[:, :16, 2:130], good)
+    rest = out.clone()
+    rest[:, :16, 2:130] = 5.0
+    assert (rest == 5.0).all()
+    assert torch.equal(hb.latent_attention(q.contiguous(), w, cp, table.cuda(), lens, scale=0.07), good)
+    table[1, 2] = -5
+    lens[2] = 10_000
+    got = hb.latent_attention(q, w, cp, table.cuda(), lens, scale=0.07)
+    assert torch.equal(got[0], good[0]) and torch.isnan(got[1:]).all()
+
+
+# ----------------------------------------------------------------------------------------- together
+
+def run_decode(dec, steps, graph):
+    """Steps of a decoder's attention: queries rotated, keys rotated into the cache, attention; `graph`: the first step
+    captured, the others replayed with new inputs in the same buffers."""
+    outs = []
+    if graph:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            dec.load(0)
+            dec.step()
+        torch.cuda.current_stream().wait_stream(side)
+        G = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(G):
+            dec.step()
+    for i in range(steps):
+        dec.load(i)
+        if graph:
+            G.replay()
+        else:
+            dec.step()
+        outs.append(dec.out.cpu().clone())
+    return outs
+
+
+class _Gqa:
+    def __init__(self, cache, B=3, H=8, Hkv=2, D=128, pt=16, steps=20):
+        g = gen(30)
+        self.B, self.H, self.Hkv, self.D, self.steps = B, H, Hkv, D, steps
+        self.q, self.k, self.v = (randn(g, steps, B, n, D) for n in (H, Hkv, Hkv))
+        self.past = [0, 13, 30]
+        table, total = table_of(g, [p + steps for p in self.past], pt)
+        (kp, ks), (vp, vs) = (pool(g, total, Hkv, pt, D, cache) for _ in range(2))
+        self.dev = [cu(t) for t in (kp, vp, ks, vs, table)]
+        freqs, a = hb.rope_freqs(D, 1e4)
+        self.cs = hb.rope_table(freqs, 64, factor=a)
+        self.start = torch.arange(B + 1, dtype=torch.int32).cuda()
+        self.bq, self.bk, self.bv = (torch.zeros(B, n, D).cuda() for n in (H, Hkv, Hkv))
+        self.pos, self.lens = torch.zeros(B, dtype=torch.int32).cuda(), torch.zeros(B, dtype=torch.int32).cuda()
+        self.qr, self.out = torch.zeros(B, H, D).cuda(), torch.zeros(B, H, D).cuda()
+        # the past of each sequence
+        pk, pv = (randn(g, sum(self.past), Hkv, D) for _ in range(2))
+        st = torch.tensor([0] + list(itertools.accumulate(self.past)), dtype=torch.int32)
+        hb.kv_write(pk.cuda(), pv.cuda(), self.dev[0], self.dev[1], self.dev[4], st.cuda(), torch.zeros(B, dtype=torch.int32).cuda(),
+                    k_scale=self.dev[2], v_scale=self.dev[3], cs=self.cs)
+        self.seqs = [([pk[st[b]:st[b + 1]]], [pv[st[b]:st[b + 1]]]) for b in range(B)]
+
+    def load(self, i):
+        for buf, x in ((self.bq, self.q[i]), (self.bk, self.k[i]), (self.bv, self.v[i])):
+            buf.copy_(x)
+        self.pos.copy_(torch.tensor([p + i for p in self.past], dtype=torch.int32))
+        self.lens.copy_(torch.tensor([p + i + 1 for p in self.past], dtype=torch.int32))
+
+    def step(self):
+        kp, vp, ks, vs, table = self.dev
+        hb.rope(self.bq, self.pos, self.cs, out=self.qr)
+        hb.kv_write(self.bk, self.bv, kp, vp, table, self.start, self.pos, k_scale=ks, v_scale=vs, cs=self.cs)
+        hb.decode_attention(self.qr, kp, vp, table, self.lens, scale=self.D ** -0.5, k_scale=ks, v_scale=vs, out=self.out)
+
+    def want(self, i, b, cache):
+        cos, sin = (t.float().double() for t in table64(self.D, 64))
+        n = self.past[b] + i + 1
+        k = torch.cat([self.seqs[b][0][0], self.k[:i + 1, b]]).double()
+        v = torch.cat([self.seqs[b][1][0], self.v[:i + 1, b]]).double()
+        k = rotate(k, cos[:n], sin[:n], False, 0, r32)
+        store = (lambda t: dequant(*quant(t.float()))) if cache == "q8" else (lambda t: t.to(F[cache]).double())
+        p = n - 1
+        q = rotate(self.q[i, b:b + 1].double(), cos[p:p + 1], sin[p:p + 1], False, 0, r32)[0]
+        return (*attend(q, store(k), store(v), self.D ** -0.5), n)
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("graph", [False, True])
+def test_decoder_steps(gpu, cache, graph):
+    """Twenty steps of three sequences with pages filling up, eager and replayed from one captured graph. The table
+    is within 2 ulp of the oracle's, which moves a rotated key by 4 w and now and then a stored value by one step."""
+    d = _Gqa(cache)
+    for i, out in enumerate(run_decode(d, d.steps, graph)):
+        for b in range(d.B):
+            want, _, vabs, big, n = d.want(i, b, cache)
+            step = {"f16": 2.0 ** -10, "bf16": 2.0 ** -7, "q8": 1 / 100}[cache]
+            err = (out[b].double() - want).abs()
+            assert (err <= (2 * (step / 8 + 160 * W) * big[:, None] + 2.0 ** -20) * vabs).all(), (i, b)
+            assert err.norm() <= 1e-3 * want.norm()
+
+
+def test_latent_decoder_steps_with_rotation_and_prompt(gpu):
+    """A latent prompt written in one call, then single tokens; several query tokens of one sequence by a shared table."""
+    g = gen(31)
+    H, R, dr, dn, dv, pt, n0, steps = 8, 512, 64, 64, 64, 16, 37, 5
+    freqs, a = hb.rope_freqs(dr, 1e4, scaling="yarn", factor=4.0)
+    cs = hb.rope_table(freqs, 64, factor=a)
+    table, total = table_of(g, [n0 + steps], pt)
+    cp = pool(g, total, 1, pt, R + dr, "bf16")[0].cuda()
+    rows = randn(g, n0 + steps, 1, R + dr)
+    w, q = randn(g, H, dn + dv, R, scale=0.05, dtype=torch.bfloat16), randn(g, n0 + steps, H, dn + dr, dtype=torch.bfloat16)
+    td = table.cuda()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    hb.kv_write(rows[:n0].cuda(), None, cp, None, td, i32(0, n0), i32(0), cs=cs, interleaved=True, offset=R)
+    for i in range(steps):
+        hb.kv_write(rows[n0 + i:n0 + i + 1].cuda(), None, cp, None, td, i32(0, 1), i32(n0 + i), cs=cs, interleaved=True, offset=R)
+    n = n0 + steps
+    pos = torch.arange(n, dtype=torch.int32).cuda()
+    qr = hb.rope(q.cuda(), pos, cs, interleaved=True, offset=dn)
+    out = hb.latent_attention(qr, w.cuda(), cp, td.expand(n, -1), pos + 1, scale=0.1).cpu()
+    cos, sin = cs[..., 0].cpu().double(), cs[..., 1].cpu().double()
+    c = rotate(rows.double(), cos[:n], sin[:n], True, R, r32).to(torch.bfloat16).double()
+    qq = rotate(q.double(), cos[:n], sin[:n], True, dn, r32).to(torch.bfloat16).double()
+    for t in range(n):
+        qa = torch.einsum("hd,hdr->hr", qq[t, :, :dn], w[:, :dn].double())
+        o, _, _, _ = attend(torch.cat([qa, qq[t, :, dn:]], -1), c[:t + 1], c[:t + 1, :, :R], 0.1)
+        want = torch.einsum("hr,hvr->hv", o, w[:, dn:].double())
+        assert (out[t].double() - want).norm() <= 4 * half_step(torch.bfloat16) * want.norm(), t
+
+
+def test_two_streams_and_two_graphs_at_once(gpu):
+    """Calls on two streams at once, and two captured graphs replayed side by side, each with its own scratch."""
+    cases = []
+    for seed in (40, 41):
+        g = gen(seed)
+        (kp, _), (vp, _) = (f := filled(g, [3000, 10], 2, 64, 64, "bf16"))[0]
+        q = randn(g, 2, 8, 64, dtype=torch.bfloat16).cuda()
+        cases.append((q, kp.cuda(), vp.cuda(), f[1].cuda(), torch.tensor([3000, 10], dtype=torch.int32).cuda()))
+    want = [hb.decode_attention(*c, scale=0.1) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(20):
+        got = []
+        for c, s in zip(cases, streams):
+            got.append(hb.decode_attention(*c, scale=0.1, stream=s, out=torch.empty_like(c[0])))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for c in cases:
+        G = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(G):
+            outs.append(hb.decode_attention(*c, scale=0.1))
+        graphs.append(G)
+    for _ in range(20):
+        for G, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                G.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
