@@ -17,9 +17,10 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhearth_b200.so")
 SOURCES = ["hx_kernels.cu", "hx_decode.cu", "hx_prefill_tc.cu", "hx_capi.cu", "hx_store.cpp", "hx_noalloc.cu", "hx_container.cpp", "hx_model.cu",
-           "hx_attention.cu", "hx_attn_decode.cu"]
+           "hx_attention.cu", "hx_attn_decode.cu", "hx_latent.cu"]
 HEADERS = ["hx_common.cuh", "hx_device.cuh", "hx_kernels.h", "hx_store.h", "hx_route.cuh", "hx_moe_job.cuh", "hx_container.h",
-           "hx_moe_internal.h", "hx_paged.cuh"]
+           "hx_moe_internal.h", "hx_paged.cuh",
+           "hx_attn.cuh"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-fmad=false", "-lineinfo",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-Xcompiler", "-ffp-contract=off",
               "-shared"]

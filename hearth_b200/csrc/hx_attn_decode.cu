@@ -1,221 +1,627 @@
-// hx_attn_decode.cu — attention of one new token a sequence over its pages (hxb_attn_decode_dev) and
-// absorbed latent attention (hxb_latent_decode_dev): softmax(scale q K^T) V with a running maximum and
-// sum in f32 (the reference's engine/src/model.c:519-629 and 739-787, in another order of summation).
-#include "hx_paged.cuh"
+// hx_attn_decode.cu — attention of one new token a sequence over its pages (hxb_attn_decode_dev; the
+// reference's engine/src/model.c:519-629 in another order of summation).
+//
+// o = sum_r p_r v_r, p = softmax(scale q . k_r). Each key and value is read once: a kv head's bytes
+// are shared by the query heads of its group, so the work is n * 2 * row bytes of reading against
+// 4 n H D operations, 1 to 16 a byte: HBM bounds it as long as the products ride on the matrix
+// instructions (mma.sync m16n8k16; at 8 heads a kv head its rate is far above the reads', and the
+// fifth-generation unit's 128-row tiles would be 1/16 full).
+//
+// Split. A unit is 64 (Q8: 128) positions of one kv head of one sequence. The grid is as many CTAs as fit
+// the GPU at once, and CTA c takes units [c N / G, (c + 1) N / G) of all N, in the order (sequence, kv head,
+// position), with N summed from the lengths on the device: the shares are equal whatever the lengths are, and a
+// captured graph follows them. A CTA that does all of a (sequence, kv head) writes its output; otherwise it
+// leaves (maximum, sum, output) in the scratch and the join kernel adds the pieces in order.
+//
+// A warp takes 16 (Q8: 32) positions of a unit. Keys and values go from HBM to registers in the order the
+// matrix instructions want, without a stop in shared memory: S^T = K Q^T takes a 16-byte piece of a key row
+// per lane as two steps' operands (the same permutation of the head's dims on both sides leaves the
+// dot as it is); P^T is the accumulator transposed by movmatrix; O^T = V^T P^T takes 16-byte pieces of four
+// value rows per lane, paired by byte permutes. With heads as the 8 columns nothing is padded for groups
+// of 8. The next tile's keys are on their way while the softmax and the values are worked on, and so on in turn:
+// 8 KB a warp, 12 warps an SM.
+//
+// Bits. Matrix operands have the cache's type (Q8: bf16, which holds the codes exactly, with the scales
+// applied in f32). Queries of more bits are split into terms (bf16: 3 for f32, 2 for f16; f16: 2 for f32,
+// after a power of two that puts the head's largest value at 2^13), and weights into 2 terms (bf16 for f32
+// outputs: 3), since one rounding of each weight to the operand's type would be as large as the output's own.
+// f16 weights carry 2^14, so that those down to 2^-38 of the largest count.
+#include "hx_attn.cuh"
 
 #include <algorithm>
 
 namespace hx {
 namespace {
 
-constexpr int AD_THREADS = 128;
+constexpr int AD_WARPS = 4, AD_THREADS = 32 * AD_WARPS;
 
-__device__ __forceinline__ float io_load(const void *p, int dtype, int64_t i) {
-    if (dtype == F32) return static_cast<const float *>(p)[i];
-    if (dtype == F16) return to_f32(static_cast<const __half *>(p)[i]);
-    return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
-__device__ __forceinline__ void io_store(void *p, int dtype, int64_t i, float x) {
-    if (dtype == F32) static_cast<float *>(p)[i] = x;
-    else if (dtype == F16) static_cast<__half *>(p)[i] = from_f32<__half>(x);
-    else static_cast<__nv_bfloat16 *>(p)[i] = from_f32<__nv_bfloat16>(x);
-}
-__device__ __forceinline__ float pool_load(const void *pool, const float *scale, int dtype, int hd, int64_t row, int e) {
-    if (dtype == Q8) return (float)static_cast<const int8_t *>(pool)[row * hd + e] * scale[row * (hd / KV_BLOCK) + e / KV_BLOCK];
-    return io_load(pool, dtype, row * hd + e);
-}
+constexpr int ad_nj(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : 4; }   // blocks of 64 dims, padded
+// Resident CTAs an SM by registers: at 128 dims and one column tile 12 warps with 168 registers each.
+constexpr int ad_ctas(int nj, int nht) { return nj * nht <= 2 ? 3 : 2; }
 
-struct CoreArgs {
+struct SplitArgs {
     KvView c;
     const int32_t *lens;
     const void *q;
     void *out;
     float *lse;
     int64_t qs, qh, os, oh;
-    int H, dtype_c, dtype_q, dtype_o, vd, latent;
-    float scale;
+    int H, group, passes, dtype, D;
+    float sc2;              // scale * log2(e)
+    int4 *desc;             // [n_seqs][kv heads * passes]: {first CTA, its slot, last CTA, 1 if split}
+    float2 *ml;             // [CTAs][2][columns]: maximum (log2 domain), sum
+    float *o;               // [CTAs][2][columns][D]
 };
 
-// One CTA a (head, sequence): tiles of AD_THREADS positions, a thread a score, then a thread an output value.
-__global__ void __launch_bounds__(AD_THREADS) k_attn_core(const __grid_constant__ CoreArgs a) {
-    __shared__ float q[1024], p[AD_THREADS], red[AD_THREADS / 32];
-    __shared__ int64_t rows[AD_THREADS];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const int g = h / (a.H / a.c.Hkv);
-    for (int i = tid; i < a.c.hd; i += AD_THREADS) q[i] = io_load(a.q, a.dtype_q, b * a.qs + h * a.qh + i);
-    const int n = a.lens[b];
-    float m = -kv_inf(), l = 0.0f, o[8] = {};
-    for (int r0 = 0; r0 < n; r0 += AD_THREADS) {
-        __syncthreads();
-        float s = -kv_inf();
-        int64_t row = -1;
-        if (r0 + tid < n) {
-            row = kv_row(a.c, b, r0 + tid);
-            if (row >= 0) row += (int64_t)g << a.c.pt_log2;
-            float d = 0.0f;
-            for (int i = 0; row >= 0 && i < a.c.hd; i++) d = __fmaf_rn(q[i], pool_load(a.c.k, a.c.ks, a.dtype_c, a.c.hd, row, i), d);
-            s = row < 0 ? kv_nan() : d * a.scale;
-        }
-        rows[tid] = row;
-        float mx = s;
-        for (int k = 16; k >= 1; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-        if (tid % 32 == 0) red[tid / 32] = mx;
-        __syncthreads();
-        float m2 = m;
-        for (int k = 0; k < AD_THREADS / 32; k++) m2 = fmaxf(m2, red[k]);
-        const float base = m2 == -kv_inf() ? 0.0f : m2;
-        const float fade = expf(m - base);
-        p[tid] = expf(s - base);
-        __syncthreads();
-        l *= fade;
-        for (int k = 0; k < AD_THREADS; k++) l += p[k];
-        const int lim = min(AD_THREADS, n - r0);
-        for (int j = 0; j < 8; j++) {
-            const int e = tid + j * AD_THREADS;
-            if (e >= a.vd) break;
-            float x = o[j] * fade;
-            for (int k = 0; k < lim; k++)
-                if (rows[k] >= 0)
-                    x = __fmaf_rn(p[k], a.latent ? pool_load(a.c.k, a.c.ks, a.dtype_c, a.c.hd, rows[k], e)
-                                                 : pool_load(a.c.v, a.c.vs, a.dtype_c, a.c.hd, rows[k], e), x);
-                else x = kv_nan();
-            o[j] = x;
-        }
-        m = m2;
-    }
-    for (int j = 0; j < 8; j++) {
-        const int e = tid + j * AD_THREADS;
-        if (e < a.vd) io_store(a.out, a.dtype_o, b * a.os + h * a.oh + e, l == 0.0f ? 0.0f : o[j] / l);
-    }
-    if (a.lse && tid == 0) a.lse[(int64_t)b * a.H + h] = l == 0.0f ? -kv_inf() : (m == -kv_inf() ? 0.0f : m) + logf(l);
+// ------------------------------------------------------------------------------------------- the split kernel
+
+template <int CACHE>
+__device__ __forceinline__ void mma16(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (CACHE == F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-struct SideArgs {
-    const void *q, *w;
-    float *qa, *o;
-    void *out;
-    int64_t qs, qh, os, oh;
-    int H, R, dr, dn, dv, dtype;
+__device__ __forceinline__ uint32_t trans8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Two f32 as a pair of 16-bit operands (x in the low half); their rest is left in x, y.
+template <int CACHE>
+__device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
+    if constexpr (CACHE == F16) {
+        const __half2 h = __floats2half2_rn(x, y);
+        x = __fsub_rn(x, __low2float(h)), y = __fsub_rn(y, __high2float(h));
+        return reinterpret_cast<const uint32_t &>(h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        x = __fsub_rn(x, __low2float(h)), y = __fsub_rn(y, __high2float(h));
+        return reinterpret_cast<const uint32_t &>(h);
+    }
+}
+
+// Signed bytes 0, 1 (HI: 2, 3) of w as a bf16 pair, exactly: byte b is (128 + (b & 127)) - (128 + (b & 128)), and
+// 0x43 over a byte below 128 is the bf16 of 128 + it, over 0x80 of 256.
+template <bool HI>
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+    const uint32_t x = __byte_perm(w, 0x43434343u, HI ? 0x4342 : 0x4140);
+    const uint32_t a = x & 0xff7fff7fu, b = x & 0xff80ff80u;
+    const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a), reinterpret_cast<const __nv_bfloat162 &>(b));
+    return reinterpret_cast<const uint32_t &>(r);
+}
+
+template <int CACHE, int NTQ, int NTP, int NJ, int NHT>
+struct SplitShape {
+    static constexpr int NS = CACHE == Q8 && NJ <= 2 ? 2 : 1;      // 16-position tiles a warp takes at once
+    static constexpr int UNIT = AD_WARPS * 16 * NS;
+    static constexpr int COLS = 8 * NHT;
+    static constexpr int OROW = 64 * NJ + 4;                       // floats between heads in the merge buffer
+    static constexpr size_t Q_BYTES = (size_t)NTQ * NHT * 2 * NJ * 32 * 16;
+    static constexpr size_t SMEM = Q_BYTES + (size_t)AD_WARPS * COLS * OROW * 4;
 };
 
-// qa[b][h] = [sum_d q[d] w[h][d] | q's rotated part] in f32.
-__global__ void k_latent_absorb(const __grid_constant__ SideArgs a) {
-    const int h = blockIdx.x, b = blockIdx.y;
-    float *qa = a.qa + ((int64_t)b * a.H + h) * (a.R + a.dr);
-    const int64_t q0 = b * a.qs + h * a.qh, w0 = (int64_t)h * (a.dn + a.dv) * a.R;
-    for (int r = threadIdx.x; r < a.R + a.dr; r += blockDim.x) {
-        float x = 0.0f;
-        if (r < a.R)
-            for (int d = 0; d < a.dn; d++) x = __fmaf_rn(io_load(a.q, a.dtype, q0 + d), io_load(a.w, a.dtype, w0 + (int64_t)d * a.R + r), x);
-        else x = io_load(a.q, a.dtype, q0 + a.dn + r - a.R);
-        qa[r] = x;
+template <int CACHE, int NTQ, int NTP, int NJ, int NHT>
+__global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(const __grid_constant__ SplitArgs a) {
+    using Sh = SplitShape<CACHE, NTQ, NTP, NJ, NHT>;
+    constexpr int NS = Sh::NS, UNIT = Sh::UNIT, COLS = Sh::COLS;
+    constexpr float POFF = CACHE == F16 ? 14.0f : 0.0f;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint4 *qs = reinterpret_cast<uint4 *>(smem);                    // [term][column tile][32-dim step][lane]
+    float *mrg = reinterpret_cast<float *>(smem + Sh::Q_BYTES);     // [warp][column][OROW]
+    __shared__ int64_t scan[AD_WARPS];
+    __shared__ float wm[AD_WARPS][COLS], wl[AD_WARPS][COLS], qfac[COLS];
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int D = a.D, chunks = D / 8, n_pairs = a.c.Hkv * a.passes;
+    pdl_trigger();
+
+    // my share of the units
+    int b;
+    int64_t cur, end, acc, total;
+    int ctas;
+    if (!my_units<AD_THREADS>(a.c, a.lens, UNIT, n_pairs, scan, b, acc, cur, end, total, ctas)) return;
+    const int64_t first_unit = cur;
+    int nu = units_of(a.c, a.lens, b, UNIT);
+    int pi = (int)((cur - acc * n_pairs) / nu), u = (int)((cur - acc * n_pairs) % nu);
+
+    while (cur < end) {
+        const int n = a.lens[b];
+        const int nseg = (int)min((int64_t)(nu - u), end - cur);
+        const int kvh = pi / a.passes, h0 = kvh * a.group + (pi - kvh * a.passes) * COLS;
+        const int nh = min(COLS, (kvh + 1) * a.group - h0);
+
+        // pages of the warp's tiles, one tile ahead of their rows
+        auto page_of = [&](int i) {
+            const int tok = (u + i) * UNIT + warp * 16 * NS + (a.c.pt_log2 >= 4 ? 0 : (lane & 15));
+            return i < nseg && tok < n ? a.c.table[(int64_t)b * a.c.table_stride + (tok >> a.c.pt_log2)] : -1;
+        };
+        // Second tile of a pair (NS 2): its own page where pages are smaller than 32 or tiles of 16 differ.
+        auto page2_of = [&](int i) {
+            if constexpr (NS == 1) return -1;
+            const int tok = (u + i) * UNIT + warp * 16 * NS + 16 + (a.c.pt_log2 >= 4 ? 0 : (lane & 15));
+            return i < nseg && tok < n ? a.c.table[(int64_t)b * a.c.table_stride + (tok >> a.c.pt_log2)] : -1;
+        };
+        // row of position tok (relative to the pool's first row of this head), -1: none
+        auto row_at = [&](int page, int tok, int rel) -> int64_t {
+            int pg = page;
+            if (a.c.pt_log2 < 4) pg = __shfl_sync(0xffffffffu, page, rel);
+            if (tok + rel >= n || (uint32_t)pg >= (uint64_t)a.c.n_pages) return -1;
+            return (((int64_t)pg * a.c.Hkv + kvh) << a.c.pt_log2) + ((tok + rel) & ((1 << a.c.pt_log2) - 1));
+        };
+
+        constexpr int KW = CACHE == Q8 ? NJ : 2 * NJ;
+        uint4 kr[NS][2][KW];
+        float ks[NS][2][CACHE == Q8 ? NJ : 1], vs[NS][2][CACHE == Q8 ? NJ : 1];
+        uint32_t vr[NS][4][NJ][CACHE == Q8 ? 2 : 4];
+        bool dead[NS][2];     // a position in range without a row
+
+        auto load_k = [&](const int *pg, int i) {
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const int tok = (u + i) * UNIT + (warp * NS + s) * 16;
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const int64_t row = row_at(pg[s], tok, g + 8 * r);
+                    dead[s][r] = row < 0 && tok + g + 8 * r < n;
+                    const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * D * (CACHE == Q8 ? 1 : 2);
+#pragma unroll
+                    for (int j = 0; j < KW; j++) {
+                        const bool on = row >= 0 && (CACHE == Q8 ? 64 * j < D : 4 * j + t < chunks);
+                        kr[s][r][j] = on ? __ldg(reinterpret_cast<const uint4 *>(p) + 4 * j + t) : make_uint4(0, 0, 0, 0);
+                    }
+                    if constexpr (CACHE == Q8) {
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) {
+                            const bool on = row >= 0 && 64 * j < D;
+                            ks[s][r][j] = on ? __ldg(a.c.ks + row * (D / KV_BLOCK) + j) : 0.0f;
+                            vs[s][r][j] = on ? __ldg(a.c.vs + row * (D / KV_BLOCK) + j) : 0.0f;
+                        }
+                    }
+                }
+            }
+        };
+        auto load_v = [&](const int *pg, int i) {
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const int tok = (u + i) * UNIT + (warp * NS + s) * 16;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int64_t row = row_at(pg[s], tok, 2 * t + (r & 1) + 8 * (r >> 1));
+                    const uint8_t *p = static_cast<const uint8_t *>(a.c.v) + row * D * (CACHE == Q8 ? 1 : 2);
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) {
+                        const bool on = row >= 0 && g + 8 * j < chunks;
+                        if constexpr (CACHE == Q8) {
+                            const uint2 x = on ? __ldg(reinterpret_cast<const uint2 *>(p) + g + 8 * j) : make_uint2(0, 0);
+                            vr[s][r][j][0] = x.x, vr[s][r][j][1] = x.y;
+                        } else {
+                            const uint4 x = on ? __ldg(reinterpret_cast<const uint4 *>(p) + g + 8 * j) : make_uint4(0, 0, 0, 0);
+                            vr[s][r][j][0] = x.x, vr[s][r][j][1] = x.y, vr[s][r][j][2] = x.z, vr[s][r][j][3] = x.w;
+                        }
+                    }
+                }
+            }
+        };
+
+        int pg[2] = {page_of(0), page2_of(0)}, pg_next[2];
+        load_k(pg, 0);
+        load_v(pg, 0);
+        pg_next[0] = page_of(1), pg_next[1] = page2_of(1);
+
+        // queries into shared memory as the products' column operands: a warp a head, a lane eight dims
+        for (int h = warp; h < COLS; h += AD_WARPS) {
+            float x[8] = {};
+            if (h < nh && lane < chunks) {
+                const int64_t at = b * a.qs + (int64_t)(h0 + h) * a.qh + lane * 8;
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = io_load(a.q, a.dtype, at + i);
+            }
+            float fac = a.sc2;
+            if constexpr (CACHE == F16) {
+                float m = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                // 2^k with k = 13 - floor(log2 max), kept where both it and its inverse are normal
+                int k = 140 - (int)(__float_as_uint(m) >> 23);
+                if (m == 0.0f || !(m < kv_inf())) k = 0;
+                k = min(k, 120);
+                const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = __fmul_rn(x[i], up);
+                fac = __fmul_rn(fac, __uint_as_float((uint32_t)(127 - k) << 23));
+            }
+            if (lane == 0) qfac[h] = fac;
+            if (lane < 8 * NJ) {
+                const int step = CACHE == Q8 ? 2 * (lane >> 3) + (lane & 1) : lane >> 2, tt = CACHE == Q8 ? (lane & 7) >> 1 : lane & 3;
+#pragma unroll
+                for (int k = 0; k < NTQ; k++) {
+                    uint4 w;
+                    w.x = take_pair<CACHE>(x[0], x[1]), w.y = take_pair<CACHE>(x[2], x[3]);
+                    w.z = take_pair<CACHE>(x[4], x[5]), w.w = take_pair<CACHE>(x[6], x[7]);
+                    qs[((k * NHT + (h >> 3)) * 2 * NJ + step) * 32 + (h & 7) * 4 + tt] = w;
+                }
+            }
+        }
+        __syncthreads();
+        float fac[NHT][2];
+#pragma unroll
+        for (int c = 0; c < NHT; c++) fac[c][0] = qfac[8 * c + 2 * t], fac[c][1] = qfac[8 * c + 2 * t + 1];
+
+        float o[NHT][NJ][4][4] = {};
+        float m[NHT][2], l[NHT][2];
+#pragma unroll
+        for (int c = 0; c < NHT; c++) m[c][0] = m[c][1] = -kv_inf(), l[c][0] = l[c][1] = 0.0f;
+
+        for (int i = 0; i < nseg; i++) {
+            const int tok = (u + i) * UNIT + warp * 16 * NS;
+            float s[NS][NHT][4];
+            // S^T = K Q^T
+#pragma unroll
+            for (int z = 0; z < NS; z++)
+#pragma unroll
+                for (int c = 0; c < NHT; c++) {
+                    s[z][c][0] = s[z][c][1] = s[z][c][2] = s[z][c][3] = 0.0f;
+                    if constexpr (CACHE == Q8) {
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) {
+                            float p[4] = {};
+                            const uint32_t w0[4] = {kr[z][0][j].x, kr[z][0][j].y, kr[z][0][j].z, kr[z][0][j].w};
+                            const uint32_t w1[4] = {kr[z][1][j].x, kr[z][1][j].y, kr[z][1][j].z, kr[z][1][j].w};
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const uint32_t a0 = codes2<false>(w0[e]), a1 = codes2<false>(w1[e]);
+                                const uint32_t a2 = codes2<true>(w0[e]), a3 = codes2<true>(w1[e]);
+#pragma unroll
+                                for (int k = NTQ - 1; k >= 0; k--) {
+                                    const uint4 q = qs[((k * NHT + c) * 2 * NJ + 2 * j + (e >> 1)) * 32 + lane];
+                                    mma16<CACHE>(p, a0, a1, a2, a3, e & 1 ? q.z : q.x, e & 1 ? q.w : q.y);
+                                }
+                            }
+                            s[z][c][0] = __fmaf_rn(p[0], ks[z][0][j], s[z][c][0]);
+                            s[z][c][1] = __fmaf_rn(p[1], ks[z][0][j], s[z][c][1]);
+                            s[z][c][2] = __fmaf_rn(p[2], ks[z][1][j], s[z][c][2]);
+                            s[z][c][3] = __fmaf_rn(p[3], ks[z][1][j], s[z][c][3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2 * NJ; j++)
+#pragma unroll
+                            for (int k = NTQ - 1; k >= 0; k--) {
+                                const uint4 q = qs[((k * NHT + c) * 2 * NJ + j) * 32 + lane];
+                                mma16<CACHE>(s[z][c], kr[z][0][j].x, kr[z][1][j].x, kr[z][0][j].y, kr[z][1][j].y, q.x, q.y);
+                                mma16<CACHE>(s[z][c], kr[z][0][j].z, kr[z][1][j].z, kr[z][0][j].w, kr[z][1][j].w, q.z, q.w);
+                            }
+                    }
+                }
+            // scores in the log2 domain; positions past the end have no weight, one without a row has no value
+#pragma unroll
+            for (int z = 0; z < NS; z++)
+#pragma unroll
+                for (int c = 0; c < NHT; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float x = __fmul_rn(s[z][c][e], fac[c][e & 1]);
+                        s[z][c][e] = dead[z][e >> 1] ? kv_nan() : tok + 16 * z + g + 8 * (e >> 1) < n ? x : -kv_inf();
+                    }
+            float pv[NS][2][CACHE == Q8 ? NJ : 1];   // the values' scales of this tile
+            if constexpr (CACHE == Q8) {
+#pragma unroll
+                for (int z = 0; z < NS; z++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) pv[z][r][j] = vs[z][r][j];
+            }
+            const int pgv[2] = {pg_next[0], pg_next[1]};
+            if (i + 1 < nseg) load_k(pg_next, i + 1);
+            pg_next[0] = page_of(i + 2), pg_next[1] = page2_of(i + 2);
+
+            // running maximum and sum
+#pragma unroll
+            for (int c = 0; c < NHT; c++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float x = m[c][e];
+#pragma unroll
+                    for (int z = 0; z < NS; z++) x = fmaxf(x, fmaxf(s[z][c][e], s[z][c][e + 2]));
+#pragma unroll
+                    for (int w = 4; w <= 16; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+                    const float base = x == -kv_inf() ? 0.0f : x;
+                    const float fade = exp2_fast(__fsub_rn(m[c][e], base));
+                    l[c][e] = __fmul_rn(l[c][e], fade);
+#pragma unroll
+                    for (int z = 0; z < NS; z++) {
+                        s[z][c][e] = exp2_fast(__fadd_rn(__fsub_rn(s[z][c][e], base), POFF));
+                        s[z][c][e + 2] = exp2_fast(__fadd_rn(__fsub_rn(s[z][c][e + 2], base), POFF));
+                        l[c][e] = __fadd_rn(l[c][e], __fadd_rn(s[z][c][e], s[z][c][e + 2]));
+                    }
+                    m[c][e] = x;
+                    if (!__all_sync(0xffffffffu, fade == 1.0f)) {
+#pragma unroll
+                        for (int j = 0; j < NJ; j++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) o[c][j][k][e] = __fmul_rn(o[c][j][k][e], fade), o[c][j][k][e + 2] = __fmul_rn(o[c][j][k][e + 2], fade);
+                    }
+                }
+
+            // O^T += V^T P^T
+#pragma unroll
+            for (int z = 0; z < NS; z++) {
+                uint32_t bp[NHT][CACHE == Q8 ? NJ : 1][NTP][2];
+#pragma unroll
+                for (int c = 0; c < NHT; c++)
+#pragma unroll
+                    for (int j = 0; j < (CACHE == Q8 ? NJ : 1); j++) {
+                        float x[4] = {s[z][c][0], s[z][c][1], s[z][c][2], s[z][c][3]};
+                        if constexpr (CACHE == Q8) {
+                            x[0] = __fmul_rn(x[0], pv[z][0][j]), x[1] = __fmul_rn(x[1], pv[z][0][j]);
+                            x[2] = __fmul_rn(x[2], pv[z][1][j]), x[3] = __fmul_rn(x[3], pv[z][1][j]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < NTP; k++) {
+                            bp[c][j][k][0] = trans8x8(take_pair<CACHE>(x[0], x[1]));
+                            bp[c][j][k][1] = trans8x8(take_pair<CACHE>(x[2], x[3]));
+                        }
+                    }
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t a0, a1, a2, a3;
+                        if constexpr (CACHE == Q8) {
+                            const uint32_t w0 = __byte_perm(vr[z][0][j][k >> 1], vr[z][1][j][k >> 1], k & 1 ? 0x7362 : 0x5140);
+                            const uint32_t w1 = __byte_perm(vr[z][2][j][k >> 1], vr[z][3][j][k >> 1], k & 1 ? 0x7362 : 0x5140);
+                            a0 = codes2<false>(w0), a1 = codes2<true>(w0), a2 = codes2<false>(w1), a3 = codes2<true>(w1);
+                        } else {
+                            a0 = __byte_perm(vr[z][0][j][k], vr[z][1][j][k], 0x5410), a1 = __byte_perm(vr[z][0][j][k], vr[z][1][j][k], 0x7632);
+                            a2 = __byte_perm(vr[z][2][j][k], vr[z][3][j][k], 0x5410), a3 = __byte_perm(vr[z][2][j][k], vr[z][3][j][k], 0x7632);
+                        }
+#pragma unroll
+                        for (int c = 0; c < NHT; c++)
+#pragma unroll
+                            for (int x = NTP - 1; x >= 0; x--)
+                                mma16<CACHE>(o[c][j][k], a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
+                    }
+            }
+            if (i + 1 < nseg) load_v(pgv, i + 1);
+        }
+
+        // the warps' pieces into one
+#pragma unroll
+        for (int c = 0; c < NHT; c++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int w = 4; w <= 16; w <<= 1) l[c][e] = __fadd_rn(l[c][e], __shfl_xor_sync(0xffffffffu, l[c][e], w));
+                if (g == 0) wm[warp][8 * c + 2 * t + e] = m[c][e], wl[warp][8 * c + 2 * t + e] = l[c][e];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NHT; c++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int h = 8 * c + 2 * t + e;
+                float x = wm[0][h];
+#pragma unroll
+                for (int w = 1; w < AD_WARPS; w++) x = fmaxf(x, wm[w][h]);
+                const float fade = exp2_fast(__fsub_rn(m[c][e], x == -kv_inf() ? 0.0f : x));
+                float *dst = mrg + (warp * COLS + h) * Sh::OROW;
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        *reinterpret_cast<float2 *>(dst + 64 * j + 8 * g + 2 * k) =
+                            make_float2(__fmul_rn(o[c][j][k][e], fade), __fmul_rn(o[c][j][k][e + 2], fade));
+            }
+        __syncthreads();
+        const bool whole = nseg == nu;
+        const int slot = cur == first_unit ? 0 : 1;
+        const int64_t piece = (int64_t)blockIdx.x * 2 + slot;
+        for (int h = warp; h < nh; h += AD_WARPS) {
+            float x = wm[0][h], sum = 0.0f;
+#pragma unroll
+            for (int w = 1; w < AD_WARPS; w++) x = fmaxf(x, wm[w][h]);
+#pragma unroll
+            for (int w = 0; w < AD_WARPS; w++) sum = __fmaf_rn(wl[w][h], exp2_fast(__fsub_rn(wm[w][h], x == -kv_inf() ? 0.0f : x)), sum);
+            for (int d = lane; d < D; d += 32) {
+                float v = mrg[h * Sh::OROW + d];
+#pragma unroll
+                for (int w = 1; w < AD_WARPS; w++) v = __fadd_rn(v, mrg[(w * COLS + h) * Sh::OROW + d]);
+                if (whole) io_store(a.out, a.dtype, b * a.os + (int64_t)(h0 + h) * a.oh + d, sum == 0.0f ? 0.0f : __fdiv_rn(v, sum));
+                else a.o[(piece * COLS + h) * D + d] = v;
+            }
+            if (lane == 0) {
+                if (!whole) a.ml[piece * COLS + h] = make_float2(x, sum);
+                else if (a.lse) a.lse[(int64_t)b * a.H + h0 + h] = lse_of(x, sum, POFF);
+            }
+        }
+        if (u == 0 && tid == 0) {
+            const int64_t upto = cur + nu;   // its last unit is in the CTA c with c total / ctas < upto <= (c + 1) total / ctas
+            a.desc[(int64_t)b * n_pairs + pi] = make_int4(blockIdx.x, slot, (int)((upto * ctas - 1) / total), whole ? 0 : 1);
+        }
+        __syncthreads();
+
+        cur += nseg, u = 0, pi++;
+        if (pi == n_pairs && cur < end) {
+            pi = 0;
+            do nu = units_of(a.c, a.lens, ++b, UNIT);
+            while (nu == 0);
+        }
     }
 }
 
-// out[b][h][j] = o[b][h] . w[h][dn + j]
-__global__ void k_latent_expand(const __grid_constant__ SideArgs a) {
-    const int h = blockIdx.x, b = blockIdx.y;
-    const float *o = a.o + ((int64_t)b * a.H + h) * a.R;
-    for (int j = threadIdx.x; j < a.dv; j += blockDim.x) {
-        const int64_t w0 = ((int64_t)h * (a.dn + a.dv) + a.dn + j) * a.R;
-        float x = 0.0f;
-        for (int r = 0; r < a.R; r++) x = __fmaf_rn(o[r], io_load(a.w, a.dtype, w0 + r), x);
-        io_store(a.out, a.dtype, b * a.os + h * a.oh + j, x);
+// ------------------------------------------------------------------------------------------- the join
+
+constexpr int JOIN_THREADS = 256;
+
+// A CTA a (head, sequence): 256 / (D / 4) groups of threads take every such piece in turn, four dims a thread.
+__global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constant__ SplitArgs a, const __grid_constant__ JoinArgs j,
+                                                            float off) {
+    __shared__ float w[ATTN_SMS * 4], red[2][JOIN_THREADS / 32];
+    __shared__ float4 part[JOIN_THREADS];
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = j.D;
+    const int kvh = h / a.group, hg = h - kvh * a.group, pass = hg / j.cols, col = hg - pass * j.cols;
+    pdl_wait();
+    const int n = j.lens[b];
+    if (n <= 0 || n > j.capacity) {
+        for (int d = tid; d < D; d += JOIN_THREADS) io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + d, n <= 0 ? 0.0f : kv_nan());
+        if (tid == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = n <= 0 ? -kv_inf() : kv_nan();
+        return;
     }
+    const int4 ds = j.desc[(int64_t)b * j.n_pairs + kvh * a.passes + pass];
+    if (!ds.w) return;
+    const int count = ds.z - ds.x + 1;
+    auto piece = [&](int i) { return ((int64_t)(ds.x + i) * 2 + (i == 0 ? ds.y : 0)) * j.cols + col; };
+    float m = -kv_inf(), l[2] = {};
+    float2 mine[2];
+    for (int k = 0; k < 2; k++) {
+        const int i = tid + k * JOIN_THREADS;
+        mine[k] = i < count ? j.ml[piece(i)] : make_float2(-kv_inf(), 0.0f);
+        m = fmaxf(m, mine[k].x);
+    }
+    for (int s = 16; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+    if (tid % 32 == 0) red[0][tid / 32] = m;
+    __syncthreads();
+    for (int k = 0; k < JOIN_THREADS / 32; k++) m = fmaxf(m, red[0][k]);
+    for (int k = 0; k < 2; k++) {
+        const int i = tid + k * JOIN_THREADS;
+        const float x = exp2_fast(__fsub_rn(mine[k].x, m == -kv_inf() ? 0.0f : m));
+        if (i < count) w[i] = x;
+        l[0] = __fmaf_rn(x, mine[k].y, l[0]);
+    }
+    for (int s = 16; s >= 1; s >>= 1) l[0] = __fadd_rn(l[0], __shfl_xor_sync(0xffffffffu, l[0], s));
+    if (tid % 32 == 0) red[1][tid / 32] = l[0];
+    __syncthreads();
+    float sum = 0.0f;
+    for (int k = 0; k < JOIN_THREADS / 32; k++) sum = __fadd_rn(sum, red[1][k]);
+    const int quads = D / 4, groups = JOIN_THREADS / quads, gr = tid / quads, qd = tid - gr * quads;
+    float4 o = make_float4(0, 0, 0, 0);
+    if (gr < groups)
+#pragma unroll 4
+        for (int i = gr; i < count; i += groups) {
+            const float4 x = *reinterpret_cast<const float4 *>(j.o + piece(i) * D + 4 * qd);
+            o.x = __fmaf_rn(w[i], x.x, o.x), o.y = __fmaf_rn(w[i], x.y, o.y), o.z = __fmaf_rn(w[i], x.z, o.z), o.w = __fmaf_rn(w[i], x.w, o.w);
+        }
+    part[tid] = o;
+    __syncthreads();
+    if (gr == 0) {
+        for (int k = 1; k < groups; k++) {
+            const float4 x = part[k * quads + qd];
+            o.x = __fadd_rn(o.x, x.x), o.y = __fadd_rn(o.y, x.y), o.z = __fadd_rn(o.z, x.z), o.w = __fadd_rn(o.w, x.w);
+        }
+        const float v[4] = {o.x, o.y, o.z, o.w};
+        for (int k = 0; k < 4; k++)
+            io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + 4 * qd + k, sum == 0.0f ? 0.0f : __fdiv_rn(v[k], sum));
+    }
+    if (tid == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = lse_of(m, sum, off);
 }
 
-size_t elem(int dtype) { return dtype == F32 ? 4 : 2; }
-bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// ------------------------------------------------------------------------------------------- host side
 
-// Checks of a call's rows and strides that both entry points make.
-int check_io(const char *who, int B, int H, const void *q, int64_t qs, int64_t qh, int qd, void *out, int64_t os,
-             int64_t oh, int od, int dtype, const int32_t *lens, float scale) {
+struct Plan {
+    int nj, nht, passes, ctas;
+    size_t desc, ml, o, bytes;
+};
+
+Plan plan_of(const hxb_kv_cache *c, int H) {
+    Plan p = {};
+    const int group = H / c->n_kv_heads;
+    p.nj = ad_nj(c->head_dim);
+    // 16 columns halve the reads of groups over 8; at 256 dims their sums do not fit the registers
+    p.nht = group > 8 && p.nj <= 2 ? 2 : 1;
+    p.passes = (group + 8 * p.nht - 1) / (8 * p.nht);
+    p.ctas = ATTN_SMS * ad_ctas(p.nj, p.nht);
+    p.desc = (size_t)c->n_seqs * c->n_kv_heads * p.passes * sizeof(int4);
+    p.ml = (size_t)p.ctas * 2 * 8 * p.nht * sizeof(float2);
+    p.o = (size_t)p.ctas * 2 * 8 * p.nht * c->head_dim * sizeof(float);
+    p.bytes = p.desc + p.ml + p.o;
+    return p;
+}
+
+template <int CACHE, int NTQ, int NTP, int NJ, int NHT>
+cudaError_t split(const SplitArgs &a, const JoinArgs &j, int ctas, cudaStream_t s) {
+    using Sh = SplitShape<CACHE, NTQ, NTP, NJ, NHT>;
+    auto k = k_attn_split<CACHE, NTQ, NTP, NJ, NHT>;
+    if (Sh::SMEM > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM);
+        if (e != cudaSuccess) return e;
+    }
+    const cudaError_t e = launch_pdl(false, k, dim3(ctas), dim3(AD_THREADS), Sh::SMEM, s, a);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(true, k_attn_join, dim3(a.H, a.c.n_seqs), dim3(JOIN_THREADS), 0, s, a, j, CACHE == F16 ? 14.0f : 0.0f);
+}
+
+template <int CACHE, int NTQ, int NTP>
+cudaError_t split_shape(const SplitArgs &a, const JoinArgs &j, const Plan &p, cudaStream_t s) {
+    if (p.nj == 1) return p.nht == 1 ? split<CACHE, NTQ, NTP, 1, 1>(a, j, p.ctas, s) : split<CACHE, NTQ, NTP, 1, 2>(a, j, p.ctas, s);
+    if (p.nj == 2) return p.nht == 1 ? split<CACHE, NTQ, NTP, 2, 1>(a, j, p.ctas, s) : split<CACHE, NTQ, NTP, 2, 2>(a, j, p.ctas, s);
+    return split<CACHE, NTQ, NTP, 4, 1>(a, j, p.ctas, s);
+}
+
+}  // namespace
+
+int attn_check_io(const char *who, int B, int H, const void *q, int64_t qs, int64_t qh, void *out, int64_t os, int64_t oh,
+                  int od, int dtype, const int32_t *lens, float scale) {
+    const size_t size = dtype == F32 ? 4 : 2;
+    auto off = [](const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
     if (!q || !out || !lens) return attn_fail(HXB_E_ARG, "%s: null pointer", who);
-    if (!aligned(q, elem(dtype)) || !aligned(out, elem(dtype)) || !aligned(lens, 4))
-        return attn_fail(HXB_E_ARG, "%s: pointer not aligned to its elements", who);
+    if (off(q, size) || off(out, size) || off(lens, 4)) return attn_fail(HXB_E_ARG, "%s: pointer not aligned to its elements", who);
     if (qs < 0 || qh < 0 || os < 0 || (H > 1 && oh < od) || (B > 1 && os < (int64_t)(H - 1) * oh + od))
         return attn_fail(HXB_E_ARG, "%s: bad strides", who);
     if (!(fabsf(scale) < INFINITY)) return attn_fail(HXB_E_ARG, "%s: scale is not finite", who);
     return HXB_OK;
 }
 
-}  // namespace
 }  // namespace hx
 
 using namespace hx;
 
 extern "C" HXB_API size_t hxb_attn_decode_workspace(const hxb_kv_cache *c, int n_heads) {
-    (void)c, (void)n_heads;
-    return 16;
+    if (!c || c->n_seqs < 0 || c->n_kv_heads < 1 || n_heads < 1 || n_heads % c->n_kv_heads || c->head_dim < 1) return 0;
+    return plan_of(c, n_heads).bytes;
 }
 
 extern "C" HXB_API int hxb_attn_decode_dev(const hxb_kv_cache *c, const int32_t *lens, const void *q, int64_t q_stride,
                                            int64_t q_head_stride, int n_heads, int dtype, float scale, void *out,
                                            int64_t out_stride, int64_t out_head_stride, float *lse, void *ws,
                                            size_t ws_bytes, void *stream) {
-    CoreArgs a = {};
-    int rc = kv_view(c, "attn_decode", false, &a.c);
+    const char *who = "attn_decode";
+    SplitArgs a = {};
+    int rc = kv_view(c, who, false, &a.c);
     if (rc != HXB_OK) return rc;
     if (c->head_dim % 16 || c->head_dim > 256)
-        return attn_fail(HXB_E_UNSUPPORTED, "attn_decode: head_dim %d (a multiple of 16 up to 256)", c->head_dim);
-    if (n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv_heads)
-        return attn_fail(HXB_E_ARG, "attn_decode: %d heads over %d kv heads", n_heads, c->n_kv_heads);
-    if (dtype != F32 && dtype != F16 && dtype != BF16) return attn_fail(HXB_E_ARG, "attn_decode: bad dtype");
+        return attn_fail(HXB_E_UNSUPPORTED, "%s: head_dim %d (a multiple of 16 up to 256)", who, c->head_dim);
+    if (n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv_heads || c->n_seqs > 65535)
+        return attn_fail(HXB_E_ARG, "%s: %d heads over %d kv heads, %d sequences (up to 65535)", who, n_heads, c->n_kv_heads, c->n_seqs);
+    if (dtype != F32 && dtype != F16 && dtype != BF16) return attn_fail(HXB_E_ARG, "%s: bad dtype", who);
     if (c->n_seqs == 0) return HXB_OK;
-    rc = check_io("attn_decode", c->n_seqs, n_heads, q, q_stride, q_head_stride, c->head_dim, out, out_stride,
-                  out_head_stride, c->head_dim, dtype, lens, scale);
+    rc = attn_check_io(who, c->n_seqs, n_heads, q, q_stride, q_head_stride, out, out_stride, out_head_stride, c->head_dim, dtype, lens, scale);
     if (rc != HXB_OK) return rc;
-    if (!aligned(lse, 4)) return attn_fail(HXB_E_ARG, "attn_decode: pointer not aligned to its elements");
-    if (!ws || !aligned(ws, 16) || ws_bytes < hxb_attn_decode_workspace(c, n_heads))
-        return attn_fail(HXB_E_ARG, "attn_decode: workspace of %zu bytes, 16-byte aligned, needed",
-                         hxb_attn_decode_workspace(c, n_heads));
+    if (reinterpret_cast<uintptr_t>(lse) % 4) return attn_fail(HXB_E_ARG, "%s: pointer not aligned to its elements", who);
+    const Plan p = plan_of(c, n_heads);
+    if (!ws || reinterpret_cast<uintptr_t>(ws) % 16 || ws_bytes < p.bytes)
+        return attn_fail(HXB_E_ARG, "%s: workspace of %zu bytes, 16-byte aligned, needed", who, p.bytes);
     a.lens = lens, a.q = q, a.out = out, a.lse = lse, a.qs = q_stride, a.qh = q_head_stride, a.os = out_stride, a.oh = out_head_stride;
-    a.H = n_heads, a.dtype_c = c->dtype, a.dtype_q = a.dtype_o = dtype, a.vd = c->head_dim, a.scale = scale;
-    k_attn_core<<<dim3(n_heads, c->n_seqs), AD_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return attn_launched("attn_decode") ? HXB_OK : HXB_E_DEVICE;
-}
-
-extern "C" HXB_API size_t hxb_latent_decode_workspace(const hxb_kv_cache *c, int n_heads, int rank) {
-    if (!c || n_heads < 1 || rank < 1 || c->n_seqs < 0) return 0;
-    return ((size_t)c->n_seqs * n_heads * ((size_t)c->head_dim + rank)) * 4 + 16;
-}
-
-extern "C" HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_t *lens, const void *q, int64_t q_stride,
-                                             int64_t q_head_stride, const void *w, int n_heads, int rank, int nope,
-                                             int v_dim, int dtype, float scale, void *out, int64_t out_stride,
-                                             int64_t out_head_stride, void *ws, size_t ws_bytes, void *stream) {
-    CoreArgs a = {};
-    int rc = kv_view(c, "latent_decode", true, &a.c);
-    if (rc != HXB_OK) return rc;
-    if (dtype != F16 && dtype != BF16) return attn_fail(HXB_E_ARG, "latent_decode: dtype %d (F16 or BF16)", dtype);
-    if (c->dtype != Q8 && c->dtype != dtype)
-        return attn_fail(HXB_E_ARG, "latent_decode: the cache is Q8 or has the type of q");
-    const int dr = c->head_dim - rank;
-    if (rank < 128 || rank > 512 || rank % 128 || dr < 16 || dr > 64 || dr % 16)
-        return attn_fail(HXB_E_UNSUPPORTED, "latent_decode: rank %d in rows of %d (rank a multiple of 128 up to 512, 16 to 64 more)",
-                         rank, c->head_dim);
-    if (nope < 16 || nope > 256 || nope % 16 || v_dim < 16 || v_dim > 256 || v_dim % 16)
-        return attn_fail(HXB_E_UNSUPPORTED, "latent_decode: nope %d, v_dim %d (multiples of 16 up to 256)", nope, v_dim);
-    if (n_heads < 1 || n_heads > 256) return attn_fail(HXB_E_ARG, "latent_decode: %d heads (up to 256)", n_heads);
-    if (c->n_seqs == 0) return HXB_OK;
-    rc = check_io("latent_decode", c->n_seqs, n_heads, q, q_stride, q_head_stride, nope + dr, out, out_stride, out_head_stride,
-                  v_dim, dtype, lens, scale);
-    if (rc != HXB_OK) return rc;
-    if (!w || !aligned(w, 16)) return attn_fail(HXB_E_ARG, "latent_decode: w must be 16-byte aligned");
-    if (!ws || !aligned(ws, 16) || ws_bytes < hxb_latent_decode_workspace(c, n_heads, rank))
-        return attn_fail(HXB_E_ARG, "latent_decode: workspace of %zu bytes, 16-byte aligned, needed",
-                         hxb_latent_decode_workspace(c, n_heads, rank));
+    a.H = n_heads, a.group = n_heads / c->n_kv_heads, a.passes = p.passes, a.dtype = dtype, a.D = c->head_dim;
+    a.sc2 = scale * 1.44269504088896f;
+    uint8_t *w = static_cast<uint8_t *>(ws);
+    a.desc = reinterpret_cast<int4 *>(w), a.ml = reinterpret_cast<float2 *>(w + p.desc), a.o = reinterpret_cast<float *>(w + p.desc + p.ml);
+    JoinArgs j = {lens, a.desc, a.ml, a.o, (int64_t)c->table_pages * c->page_tokens, c->n_kv_heads * p.passes, 8 * p.nht, c->head_dim, p.ctas};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    SideArgs e = {};
-    e.q = q, e.w = w, e.qa = static_cast<float *>(ws), e.o = e.qa + (size_t)c->n_seqs * n_heads * c->head_dim, e.out = out;
-    e.qs = q_stride, e.qh = q_head_stride, e.os = out_stride, e.oh = out_head_stride;
-    e.H = n_heads, e.R = rank, e.dr = dr, e.dn = nope, e.dv = v_dim, e.dtype = dtype;
-    a.lens = lens, a.q = e.qa, a.qs = (int64_t)n_heads * c->head_dim, a.qh = c->head_dim, a.out = e.o;
-    a.os = (int64_t)n_heads * rank, a.oh = rank, a.H = n_heads, a.dtype_c = c->dtype, a.dtype_q = a.dtype_o = F32;
-    a.vd = rank, a.latent = 1, a.scale = scale;
-    const dim3 grid(n_heads, c->n_seqs);
-    k_latent_absorb<<<grid, 128, 0, s>>>(e);
-    k_attn_core<<<grid, AD_THREADS, 0, s>>>(a);
-    k_latent_expand<<<grid, 128, 0, s>>>(e);
-    return attn_launched("latent_decode") ? HXB_OK : HXB_E_DEVICE;
+    cudaError_t e;
+    if (c->dtype == F16) e = dtype == F32 ? split_shape<F16, 2, 2>(a, j, p, s) : split_shape<F16, 1, 2>(a, j, p, s);
+    else if (c->dtype == BF16)
+        e = dtype == F32 ? split_shape<BF16, 3, 3>(a, j, p, s) : dtype == F16 ? split_shape<BF16, 2, 2>(a, j, p, s) : split_shape<BF16, 1, 2>(a, j, p, s);
+    else e = dtype == F32 ? split_shape<Q8, 3, 3>(a, j, p, s) : dtype == F16 ? split_shape<Q8, 2, 2>(a, j, p, s) : split_shape<Q8, 1, 2>(a, j, p, s);
+    if (e != cudaSuccess) return attn_fail(HXB_E_DEVICE, "%s: %s", who, cudaGetErrorString(e));
+    return HXB_OK;
 }
