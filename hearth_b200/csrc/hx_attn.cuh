@@ -39,12 +39,14 @@ __device__ __forceinline__ int units_of(const KvView &c, const int32_t *lens, in
     return n <= 0 || n > table_capacity(c) ? 0 : (int)(((int64_t)n + unit - 1) / unit);
 }
 
-// The calling CTA's share [cur, end) of the N = n_pairs * sum_b units_of(b) units, laid out sequence by sequence,
-// pair by pair: the sequence of unit cur and the sum of the units of the sequences before it. False without a
-// share. Every thread of the CTA calls it; scan: one word a warp.
+// The share [cur, end) of CTA `cta` of `grid` in the N = n_pairs * sum_b units_of(b) units, laid out sequence by
+// sequence, pair by pair: the sequence of unit cur and the sum of the units of the sequences before it. False
+// without a share. ctas: the CTAs that have one (the first min(grid, N)). Every thread of the CTA calls it;
+// scan: one word a warp.
 template <int THREADS>
-__device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, int unit, int n_pairs, int64_t *scan, int &b,
-                                         int64_t &before, int64_t &cur, int64_t &end, int64_t &total, int &ctas) {
+__device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, int unit, int n_pairs, int cta, int grid,
+                                         int64_t *scan, int &b, int64_t &before, int64_t &cur, int64_t &end,
+                                         int64_t &total, int &ctas) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = c.n_seqs;
     const int per = (B + THREADS - 1) / THREADS;
     int64_t mine = 0;
@@ -64,11 +66,11 @@ __device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, i
         sum += scan[w];
     }
     total = sum * n_pairs;
-    ctas = (int)min((int64_t)gridDim.x, total);
+    ctas = (int)min((int64_t)grid, total);
     const int64_t start = base + upto - mine;             // units of the sequences before my chunk
     cur = end = 0;
-    if (total) cur = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
-    const bool none = blockIdx.x >= ctas;
+    if (total) cur = cta * total / ctas, end = (cta + 1) * total / ctas;
+    const bool none = cta >= ctas;
     // the chunk that holds unit cur: the last one that starts at or before it
     const int chunk = __syncthreads_count(start * n_pairs <= cur) - 1;
     if (tid == chunk) scan[0] = start;
@@ -83,16 +85,39 @@ __device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, i
     return true;
 }
 
-// One launch after the split kernel: pieces of each (sequence, head) whose work several CTAs did are joined in CTA
-// order (weights 2^(m_i - max m)); empty sequences get zeros and -inf, ones longer than their table NaN.
-struct JoinArgs {
-    const int32_t *lens;
-    const int4 *desc;       // [n_seqs][n_pairs]: first CTA, its slot, last CTA, 1 if split
-    const float2 *ml;       // [CTAs][2][cols]
-    const float *o;         // [CTAs][2][cols][D]
-    int64_t capacity;
-    int n_pairs, cols, D, max_ctas;
-};
+// Two f32 as a pair of 16-bit matrix operands of TYPE F16 or BF16 (x in the low half); what they leave stays in x, y.
+template <int TYPE>
+__device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
+    if constexpr (TYPE == F16) {
+        const __half2 h = __floats2half2_rn(x, y);
+        x = __fsub_rn(x, __low2float(h)), y = __fsub_rn(y, __high2float(h));
+        return reinterpret_cast<const uint32_t &>(h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        x = __fsub_rn(x, __low2float(h)), y = __fsub_rn(y, __high2float(h));
+        return reinterpret_cast<const uint32_t &>(h);
+    }
+}
+
+// d += A B, m16n8k16 on operands of TYPE F16 or BF16.
+template <int TYPE>
+__device__ __forceinline__ void mma16(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (TYPE == F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The power of two 2^k, as its exponent k, that brings a largest magnitude m to [2^13, 2^14), the upper part of f16's
+// range; k <= 120, so that 2^k and 2^-k are normal, and 0 for m = 0 or not finite.
+__device__ __forceinline__ int f16_lift(float m) {
+    return m == 0.0f || !(m < kv_inf()) ? 0 : min(140 - (int)(__float_as_uint(m) >> 23), 120);
+}
+__device__ __forceinline__ float pow2i(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
 
 int attn_check_io(const char *who, int B, int H, const void *q, int64_t qs, int64_t qh, void *out, int64_t os, int64_t oh,
                   int od, int dtype, const int32_t *lens, float scale);

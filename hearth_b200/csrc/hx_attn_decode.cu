@@ -39,6 +39,12 @@ constexpr int ad_nj(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : 4; }   // block
 // Resident CTAs an SM by registers: at 128 dims and one column tile 12 warps with 168 registers each.
 constexpr int ad_ctas(int nj, int nht) { return nj * nht <= 2 ? 3 : 2; }
 
+// What the join needs beside SplitArgs.
+struct JoinArgs {
+    int64_t capacity;       // positions a table row can name
+    int cols;               // heads of a pair's piece
+};
+
 struct SplitArgs {
     KvView c;
     const int32_t *lens;
@@ -55,36 +61,10 @@ struct SplitArgs {
 
 // ------------------------------------------------------------------------------------------- the split kernel
 
-template <int CACHE>
-__device__ __forceinline__ void mma16(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (CACHE == F16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 __device__ __forceinline__ uint32_t trans8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-// Two f32 as a pair of 16-bit operands (x in the low half); their rest is left in x, y.
-template <int CACHE>
-__device__ __forceinline__ uint32_t take_pair(float &x, float &y) {
-    if constexpr (CACHE == F16) {
-        const __half2 h = __floats2half2_rn(x, y);
-        x = __fsub_rn(x, __low2float(h)), y = __fsub_rn(y, __high2float(h));
-        return reinterpret_cast<const uint32_t &>(h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        x = __fsub_rn(x, __low2float(h)), y = __fsub_rn(y, __high2float(h));
-        return reinterpret_cast<const uint32_t &>(h);
-    }
 }
 
 // Signed bytes 0, 1 (HI: 2, 3) of w as a bf16 pair, exactly: byte b is (128 + (b & 127)) - (128 + (b & 128)), and
@@ -112,6 +92,7 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
     using Sh = SplitShape<CACHE, NTQ, NTP, NJ, NHT>;
     constexpr int NS = Sh::NS, UNIT = Sh::UNIT, COLS = Sh::COLS;
     constexpr float POFF = CACHE == F16 ? 14.0f : 0.0f;
+    constexpr int OT = CACHE == F16 ? F16 : BF16;   // the operands' type
     extern __shared__ __align__(16) uint8_t smem[];
     uint4 *qs = reinterpret_cast<uint4 *>(smem);                    // [term][column tile][32-dim step][lane]
     float *mrg = reinterpret_cast<float *>(smem + Sh::Q_BYTES);     // [warp][column][OROW]
@@ -126,7 +107,7 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
     int b;
     int64_t cur, end, acc, total;
     int ctas;
-    if (!my_units<AD_THREADS>(a.c, a.lens, UNIT, n_pairs, scan, b, acc, cur, end, total, ctas)) return;
+    if (!my_units<AD_THREADS>(a.c, a.lens, UNIT, n_pairs, blockIdx.x, gridDim.x, scan, b, acc, cur, end, total, ctas)) return;
     const int64_t first_unit = cur;
     int nu = units_of(a.c, a.lens, b, UNIT);
     int pi = (int)((cur - acc * n_pairs) / nu), u = (int)((cur - acc * n_pairs) % nu);
@@ -230,14 +211,10 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                 for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
 #pragma unroll
                 for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                // 2^k with k = 13 - floor(log2 max), kept where both it and its inverse are normal
-                int k = 140 - (int)(__float_as_uint(m) >> 23);
-                if (m == 0.0f || !(m < kv_inf())) k = 0;
-                k = min(k, 120);
-                const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+                const int k = f16_lift(m);
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = __fmul_rn(x[i], up);
-                fac = __fmul_rn(fac, __uint_as_float((uint32_t)(127 - k) << 23));
+                for (int i = 0; i < 8; i++) x[i] = __fmul_rn(x[i], pow2i(k));
+                fac = __fmul_rn(fac, pow2i(-k));
             }
             if (lane == 0) qfac[h] = fac;
             if (lane < 8 * NJ) {
@@ -245,8 +222,8 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
 #pragma unroll
                 for (int k = 0; k < NTQ; k++) {
                     uint4 w;
-                    w.x = take_pair<CACHE>(x[0], x[1]), w.y = take_pair<CACHE>(x[2], x[3]);
-                    w.z = take_pair<CACHE>(x[4], x[5]), w.w = take_pair<CACHE>(x[6], x[7]);
+                    w.x = take_pair<OT>(x[0], x[1]), w.y = take_pair<OT>(x[2], x[3]);
+                    w.z = take_pair<OT>(x[4], x[5]), w.w = take_pair<OT>(x[6], x[7]);
                     qs[((k * NHT + (h >> 3)) * 2 * NJ + step) * 32 + (h & 7) * 4 + tt] = w;
                 }
             }
@@ -283,7 +260,7 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
 #pragma unroll
                                 for (int k = NTQ - 1; k >= 0; k--) {
                                     const uint4 q = qs[((k * NHT + c) * 2 * NJ + 2 * j + (e >> 1)) * 32 + lane];
-                                    mma16<CACHE>(p, a0, a1, a2, a3, e & 1 ? q.z : q.x, e & 1 ? q.w : q.y);
+                                    mma16<OT>(p, a0, a1, a2, a3, e & 1 ? q.z : q.x, e & 1 ? q.w : q.y);
                                 }
                             }
                             s[z][c][0] = __fmaf_rn(p[0], ks[z][0][j], s[z][c][0]);
@@ -297,8 +274,8 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
 #pragma unroll
                             for (int k = NTQ - 1; k >= 0; k--) {
                                 const uint4 q = qs[((k * NHT + c) * 2 * NJ + j) * 32 + lane];
-                                mma16<CACHE>(s[z][c], kr[z][0][j].x, kr[z][1][j].x, kr[z][0][j].y, kr[z][1][j].y, q.x, q.y);
-                                mma16<CACHE>(s[z][c], kr[z][0][j].z, kr[z][1][j].z, kr[z][0][j].w, kr[z][1][j].w, q.z, q.w);
+                                mma16<OT>(s[z][c], kr[z][0][j].x, kr[z][1][j].x, kr[z][0][j].y, kr[z][1][j].y, q.x, q.y);
+                                mma16<OT>(s[z][c], kr[z][0][j].z, kr[z][1][j].z, kr[z][0][j].w, kr[z][1][j].w, q.z, q.w);
                             }
                     }
                 }
@@ -368,8 +345,8 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                         }
 #pragma unroll
                         for (int k = 0; k < NTP; k++) {
-                            bp[c][j][k][0] = trans8x8(take_pair<CACHE>(x[0], x[1]));
-                            bp[c][j][k][1] = trans8x8(take_pair<CACHE>(x[2], x[3]));
+                            bp[c][j][k][0] = trans8x8(take_pair<OT>(x[0], x[1]));
+                            bp[c][j][k][1] = trans8x8(take_pair<OT>(x[2], x[3]));
                         }
                     }
 #pragma unroll
@@ -389,7 +366,7 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                         for (int c = 0; c < NHT; c++)
 #pragma unroll
                             for (int x = NTP - 1; x >= 0; x--)
-                                mma16<CACHE>(o[c][j][k], a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
+                                mma16<OT>(o[c][j][k], a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
                     }
             }
             if (i + 1 < nseg) load_v(pgv, i + 1);
@@ -463,21 +440,23 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
 
 constexpr int JOIN_THREADS = 256;
 
-// A CTA a (head, sequence): 256 / (D / 4) groups of threads take every such piece in turn, four dims a thread.
+// A CTA a (head, sequence): the pieces of a pair that several CTAs worked on are added with weights 2^(m_i - max m),
+// in CTA order; 256 / (D / 4) groups of threads take every such piece in turn, four dims a thread. Empty
+// sequences get zeros and -inf, ones longer than their table NaN.
 __global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constant__ SplitArgs a, const __grid_constant__ JoinArgs j,
                                                             float off) {
     __shared__ float w[ATTN_SMS * 4], red[2][JOIN_THREADS / 32];
     __shared__ float4 part[JOIN_THREADS];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = j.D;
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = a.D;
     const int kvh = h / a.group, hg = h - kvh * a.group, pass = hg / j.cols, col = hg - pass * j.cols;
     pdl_wait();
-    const int n = j.lens[b];
+    const int n = a.lens[b];
     if (n <= 0 || n > j.capacity) {
         for (int d = tid; d < D; d += JOIN_THREADS) io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + d, n <= 0 ? 0.0f : kv_nan());
         if (tid == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = n <= 0 ? -kv_inf() : kv_nan();
         return;
     }
-    const int4 ds = j.desc[(int64_t)b * j.n_pairs + kvh * a.passes + pass];
+    const int4 ds = a.desc[(int64_t)b * a.c.Hkv * a.passes + kvh * a.passes + pass];
     if (!ds.w) return;
     const int count = ds.z - ds.x + 1;
     auto piece = [&](int i) { return ((int64_t)(ds.x + i) * 2 + (i == 0 ? ds.y : 0)) * j.cols + col; };
@@ -485,7 +464,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constan
     float2 mine[2];
     for (int k = 0; k < 2; k++) {
         const int i = tid + k * JOIN_THREADS;
-        mine[k] = i < count ? j.ml[piece(i)] : make_float2(-kv_inf(), 0.0f);
+        mine[k] = i < count ? a.ml[piece(i)] : make_float2(-kv_inf(), 0.0f);
         m = fmaxf(m, mine[k].x);
     }
     for (int s = 16; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
@@ -508,7 +487,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constan
     if (gr < groups)
 #pragma unroll 4
         for (int i = gr; i < count; i += groups) {
-            const float4 x = *reinterpret_cast<const float4 *>(j.o + piece(i) * D + 4 * qd);
+            const float4 x = *reinterpret_cast<const float4 *>(a.o + piece(i) * D + 4 * qd);
             o.x = __fmaf_rn(w[i], x.x, o.x), o.y = __fmaf_rn(w[i], x.y, o.y), o.z = __fmaf_rn(w[i], x.z, o.z), o.w = __fmaf_rn(w[i], x.w, o.w);
         }
     part[tid] = o;
@@ -615,7 +594,7 @@ extern "C" HXB_API int hxb_attn_decode_dev(const hxb_kv_cache *c, const int32_t 
     a.sc2 = scale * 1.44269504088896f;
     uint8_t *w = static_cast<uint8_t *>(ws);
     a.desc = reinterpret_cast<int4 *>(w), a.ml = reinterpret_cast<float2 *>(w + p.desc), a.o = reinterpret_cast<float *>(w + p.desc + p.ml);
-    JoinArgs j = {lens, a.desc, a.ml, a.o, (int64_t)c->table_pages * c->page_tokens, c->n_kv_heads * p.passes, 8 * p.nht, c->head_dim, p.ctas};
+    const JoinArgs j = {(int64_t)c->table_pages * c->page_tokens, 8 * p.nht};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (c->dtype == F16) e = dtype == F32 ? split_shape<F16, 2, 2>(a, j, p, s) : split_shape<F16, 1, 2>(a, j, p, s);

@@ -1,5 +1,35 @@
 // hx_latent.cu — absorbed latent attention of one new token a sequence (hxb_latent_decode_dev; the reference's
-// engine/src/model.c:739-787 in another order of summation).
+// engine/src/model.c:739-787 in another order of summation), in three launches chained by programmatic
+// dependent launch:
+//
+//   k_latent_absorb  qa[b][h] = [sum_d q[d] w[h][d] | q's rotated part], f32 into the scratch; mma.sync, a
+//                    warp 64 latent dims of a head for 32 sequences, weights straight into registers.
+//   k_latent_core    softmax(scale qa C^T) C over the pages, on the fifth-generation tensor cores.
+//   k_latent_expand  joins the core's pieces and multiplies by w's value rows.
+//
+// The core. One row of 576 values (1152 bytes) serves every head as key and as value: 2 (576 + 512) H operations for
+// 1152 bytes, 121 a byte at 64 heads, about half of what the machine can do per byte read: HBM bounds it while the
+// tensor cores run at half their rate, so they have to be fed by the fifth-generation unit. A CTA takes up to 64
+// heads and a run of 64-position tiles (the shares of all CTAs are equal, as in hx_attn_decode.cu; with more
+// heads, groups of CTAs take the same runs side by side and share the rows through L2):
+//
+//   S [heads x 64]    = Q [64 x 576] K^T          tcgen05 M 64, N 64: both from shared memory, row-major
+//   P                 = 2^(S - ref) -> shared memory, a thread a head
+//   O^T [512 x heads] += V^T [512 x 64] P^T       M 128 x 4, N heads: V is the K tile itself, read column-major
+//
+// With O transposed its 4 x 64 columns and two S buffers take 384 of the 512 tensor-memory columns at 64 heads (O
+// itself, 64 rows high, would leave half of the lanes empty), and the tile in shared memory is used twice. Shared
+// memory: Q 72 KB, two tiles of 72 KB, P 8 KB. Warps 0-3 softmax, 4 issues the MMAs, 5-12 load, four for each of
+// the two tiles, so that the one in flight never waits for the one at work. Rows are fetched by 16-byte
+// asynchronous copies rather than tensor maps: they take any page size, and rows past the end arrive as zeros
+// (an unused slot may hold NaN, and 0 x NaN would reach every sum).
+//
+// ref is the running maximum, moved only when a score passes it by 2^7 (O^T is then rescaled in tensor memory):
+// the weights relative to it stay below 2^7 (f16 operands: 2^15, lifted by 2^8), and most tiles skip the rescale.
+//
+// Bits. Operands have the cache's type; Q8 rows are expanded to f16 (code x scale in f32, rounded once to 11 bits; bf16's 8
+// would add an error as large as the output's own). f16 queries are lifted by a power of two a head. bf16 weights
+// go in as two terms for the same reason, the second into the tile's rotated part, which S no longer needs.
 #include "hx_attn.cuh"
 
 #include <algorithm>
@@ -7,113 +37,715 @@
 namespace hx {
 namespace {
 
-constexpr int AD_THREADS = 128;
+constexpr int LT = 64;                  // positions a tile
+constexpr int LH = 64;                  // heads a CTA (rows of S)
+constexpr int SEG = LT * 128;           // 64 dims of 64 rows: a 128-byte swizzled block column
+constexpr int LD_WARPS = 4;             // loading warps a tile buffer
+constexpr int CORE_WARPS = 5 + 2 * LD_WARPS, CORE_THREADS = 32 * CORE_WARPS;
+constexpr float REF_SLACK = 7.0f;
 
-__device__ __forceinline__ float pool_load(const void *pool, const float *scale, int dtype, int hd, int64_t row, int e) {
-    if (dtype == Q8) return (float)static_cast<const int8_t *>(pool)[row * hd + e] * scale[row * (hd / KV_BLOCK) + e / KV_BLOCK];
-    return io_load(pool, dtype, row * hd + e);
-}
-
-struct CoreArgs {
+struct LatentArgs {
     KvView c;
     const int32_t *lens;
-    const void *q;
-    void *out;
-    float *lse;
-    int64_t qs, qh, os, oh;
-    int H, dtype_c, dtype_q, dtype_o, vd, latent;
-    float scale;
-};
-
-// One CTA a (head, sequence): tiles of AD_THREADS positions, a thread a score, then a thread an output value.
-__global__ void __launch_bounds__(AD_THREADS) k_attn_core(const __grid_constant__ CoreArgs a) {
-    __shared__ float q[1024], p[AD_THREADS], red[AD_THREADS / 32];
-    __shared__ int64_t rows[AD_THREADS];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const int g = h / (a.H / a.c.Hkv);
-    for (int i = tid; i < a.c.hd; i += AD_THREADS) q[i] = io_load(a.q, a.dtype_q, b * a.qs + h * a.qh + i);
-    const int n = a.lens[b];
-    float m = -kv_inf(), l = 0.0f, o[8] = {};
-    for (int r0 = 0; r0 < n; r0 += AD_THREADS) {
-        __syncthreads();
-        float s = -kv_inf();
-        int64_t row = -1;
-        if (r0 + tid < n) {
-            row = kv_row(a.c, b, r0 + tid);
-            if (row >= 0) row += (int64_t)g << a.c.pt_log2;
-            float d = 0.0f;
-            for (int i = 0; row >= 0 && i < a.c.hd; i++) d = __fmaf_rn(q[i], pool_load(a.c.k, a.c.ks, a.dtype_c, a.c.hd, row, i), d);
-            s = row < 0 ? kv_nan() : d * a.scale;
-        }
-        rows[tid] = row;
-        float mx = s;
-        for (int k = 16; k >= 1; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-        if (tid % 32 == 0) red[tid / 32] = mx;
-        __syncthreads();
-        float m2 = m;
-        for (int k = 0; k < AD_THREADS / 32; k++) m2 = fmaxf(m2, red[k]);
-        const float base = m2 == -kv_inf() ? 0.0f : m2;
-        const float fade = expf(m - base);
-        p[tid] = expf(s - base);
-        __syncthreads();
-        l *= fade;
-        for (int k = 0; k < AD_THREADS; k++) l += p[k];
-        const int lim = min(AD_THREADS, n - r0);
-        for (int j = 0; j < 8; j++) {
-            const int e = tid + j * AD_THREADS;
-            if (e >= a.vd) break;
-            float x = o[j] * fade;
-            for (int k = 0; k < lim; k++)
-                if (rows[k] >= 0)
-                    x = __fmaf_rn(p[k], a.latent ? pool_load(a.c.k, a.c.ks, a.dtype_c, a.c.hd, rows[k], e)
-                                                 : pool_load(a.c.v, a.c.vs, a.dtype_c, a.c.hd, rows[k], e), x);
-                else x = kv_nan();
-            o[j] = x;
-        }
-        m = m2;
-    }
-    for (int j = 0; j < 8; j++) {
-        const int e = tid + j * AD_THREADS;
-        if (e < a.vd) io_store(a.out, a.dtype_o, b * a.os + h * a.oh + e, l == 0.0f ? 0.0f : o[j] / l);
-    }
-    if (a.lse && tid == 0) a.lse[(int64_t)b * a.H + h] = l == 0.0f ? -kv_inf() : (m == -kv_inf() ? 0.0f : m) + logf(l);
-}
-
-struct SideArgs {
     const void *q, *w;
-    float *qa, *o;
     void *out;
+    float *qa;              // [n_seqs][H][R + dr]; a head whose work one CTA did leaves its o, maximum and sum here
+    float2 *ml;             // [CTAs][2][hp]
+    float *o;               // [CTAs][2][hp][R]
+    int4 *desc;             // [n_seqs][passes]: {first CTA of the pass, its slot, last CTA, 1 if split}
+    int *err;
     int64_t qs, qh, os, oh;
-    int H, R, dr, dn, dv, dtype;
+    int H, R, dr, dn, dv, passes, hp;   // hp heads a pass
+    float sc2;
 };
 
-// qa[b][h] = [sum_d q[d] w[h][d] | q's rotated part] in f32.
-__global__ void k_latent_absorb(const __grid_constant__ SideArgs a) {
-    const int h = blockIdx.x, b = blockIdx.y;
-    float *qa = a.qa + ((int64_t)b * a.H + h) * (a.R + a.dr);
-    const int64_t q0 = b * a.qs + h * a.qh, w0 = (int64_t)h * (a.dn + a.dv) * a.R;
-    for (int r = threadIdx.x; r < a.R + a.dr; r += blockDim.x) {
-        float x = 0.0f;
-        if (r < a.R)
-            for (int d = 0; d < a.dn; d++) x = __fmaf_rn(io_load(a.q, a.dtype, q0 + d), io_load(a.w, a.dtype, w0 + (int64_t)d * a.R + r), x);
-        else x = io_load(a.q, a.dtype, q0 + a.dn + r - a.R);
-        qa[r] = x;
+// ------------------------------------------------------------------------------------------- absorb
+
+constexpr int AB_WARPS = 4, AB_ROWS = 32;
+
+template <int T>
+__global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_constant__ LatentArgs a) {
+    __shared__ uint16_t qsm[AB_ROWS][256 + 8];
+    const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS);
+    const int h = blockIdx.x / nc, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int r0 = ((blockIdx.x - h * nc) * AB_WARPS + warp) * 64, b0 = blockIdx.y * AB_ROWS, rows = min(AB_ROWS, a.c.n_seqs - b0);
+    pdl_trigger();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.err = 0;
+    const uint16_t *q = static_cast<const uint16_t *>(a.q);
+    for (int i = threadIdx.x; i < AB_ROWS * a.dn; i += 32 * AB_WARPS) {
+        const int r = i / a.dn, d = i - r * a.dn;
+        qsm[r][d] = r < rows ? q[(b0 + r) * a.qs + h * a.qh + d] : 0;
+    }
+    const int row = a.R + a.dr;
+    if (r0 == 0)
+        for (int i = lane; i < rows * a.dr; i += 32) {
+            const int r = i / a.dr, d = i - r * a.dr;
+            a.qa[((int64_t)(b0 + r) * a.H + h) * row + a.R + d] = io_load(a.q, T, (b0 + r) * a.qs + h * a.qh + a.dn + d);
+        }
+    __syncthreads();
+    if (r0 >= a.R) return;
+    float acc[2][8][4] = {};
+    const uint16_t *w = static_cast<const uint16_t *>(a.w) + (int64_t)h * (a.dn + a.dv) * a.R + r0 + 8 * g;
+#pragma unroll 2
+    for (int d0 = 0; d0 < a.dn; d0 += 16) {
+        uint32_t v[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(w + (int64_t)(d0 + 2 * t + (k & 1) + 8 * (k >> 1)) * a.R));
+            v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+        }
+        uint32_t f[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                f[m][k] = *reinterpret_cast<const uint32_t *>(&qsm[16 * m + g + 8 * (k & 1)][d0 + 2 * t + 8 * (k >> 1)]);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t p0 = __byte_perm(v[0][i], v[1][i], e ? 0x7632 : 0x5410), p1 = __byte_perm(v[2][i], v[3][i], e ? 0x7632 : 0x5410);
+#pragma unroll
+                for (int m = 0; m < 2; m++) mma16<T>(acc[m][2 * i + e], f[m][0], f[m][1], f[m][2], f[m][3], p0, p1);
+            }
+    }
+    // column n of product i is latent dim 8 n + i
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = 16 * m + g + 8 * e;
+            if (r >= rows) continue;
+            float *dst = a.qa + ((int64_t)(b0 + r) * a.H + h) * row + r0 + 16 * t;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 8; i += 4)
+                    *reinterpret_cast<float4 *>(dst + 8 * n + i) = make_float4(acc[m][i][2 * e + n], acc[m][i + 1][2 * e + n], acc[m][i + 2][2 * e + n], acc[m][i + 3][2 * e + n]);
+        }
+}
+
+// ------------------------------------------------------------------------------------------- core
+
+struct CoreShared {
+    uint64_t full[2], sfull[2], done[2], pready;
+    int64_t scan[CORE_WARPS];
+    uint32_t tmem, failed;
+    uint32_t dead[2][2];     // positions of a tile without a row
+    float alpha[LH], fac[LH];
+};
+
+// Shared-memory matrix descriptors of 128-byte swizzled operands (8-row groups 1024 bytes apart). Row-major (K along
+// the 128 bytes): one block column. Column-major (the 64 outer elements along the 128 bytes): `lead` bytes to the
+// next 64 of them.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void umma_done(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_ld32(uint32_t addr, float v[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_ld16(uint32_t addr, float v[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t addr, const float v[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// A barrier of the softmax warps, with the or of x.
+__device__ __forceinline__ bool softmax_any(bool x) {
+    __syncwarp();
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred.aligned q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(x ? 1u : 0u)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool on) {   // zeros when off
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+// A wait that ends: on the phase, when another role has given up, or at the spin limit (the error word, so
+// that the outputs become NaN).
+__device__ __forceinline__ bool core_wait(CoreShared &y, uint64_t *bar, uint32_t parity, int *err) {
+    for (uint32_t i = 0; i < kSpinLimit; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*reinterpret_cast<volatile uint32_t *>(&y.failed)) return false;
+    }
+    *reinterpret_cast<volatile uint32_t *>(&y.failed) = 1;
+    set_error(err, DEV_E_WAIT_TIMEOUT);
+    return false;
+}
+
+// One run of tiles of a sequence; every role walks the same list.
+struct Run {
+    int b, u, nu, n, tiles;     // sequence, first tile, its tiles, its length, tiles of the run
+};
+struct Walk {
+    const LatentArgs &a;
+    int64_t cur, end;
+    int b, u, nu;
+    __device__ __forceinline__ Walk(const LatentArgs &a_, int b_, int64_t before, int64_t cur_, int64_t end_)
+        : a(a_), cur(cur_), end(end_), b(b_), u((int)(cur_ - before)), nu(units_of(a_.c, a_.lens, b_, LT)) {}
+    __device__ __forceinline__ bool next(Run &r) {
+        if (cur >= end) return false;
+        while (u >= nu) nu = units_of(a.c, a.lens, ++b, LT), u = 0;
+        r.b = b, r.u = u, r.nu = nu, r.n = a.lens[b], r.tiles = (int)min((int64_t)(nu - u), end - cur);
+        cur += r.tiles, u += r.tiles;
+        return true;
+    }
+};
+
+template <int CACHE>
+__device__ __forceinline__ void load_tile(const LatentArgs &a, CoreShared &y, uint32_t dst, int segs, int buf, const Run &r, int tile,
+                                          int lt, bool wait, uint32_t parity, bool &ok) {
+    // eight lanes a 128-byte block row, 16 rows at once
+    const int c8 = lt & 7, rr = lt >> 3;
+    int64_t row[4];
+    uint32_t dead = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int pos = (r.u + tile) * LT + rr + 16 * k;
+        row[k] = pos < r.n ? kv_row(a.c, r.b, pos) : -1;
+        if (pos < r.n && row[k] < 0) dead |= 1u << k;
+    }
+    const int tail = a.dr / 8;     // 16-byte pieces of the last block column
+    if constexpr (CACHE == Q8) {
+        // codes and scales into registers while the buffer is still at work
+        uint2 code[9][4];
+        float d[9][4];
+#pragma unroll
+        for (int s = 0; s < 9; s++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool on = row[k] >= 0 && s < segs;
+                code[s][k] = on ? __ldg(reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(a.c.k) + row[k] * a.c.hd + s * 64) + c8) : make_uint2(0, 0);
+                d[s][k] = on ? __ldg(a.c.ks + row[k] * segs + s) : 0.0f;
+            }
+        if (wait) ok = core_wait(y, &y.done[buf], parity, a.err);
+        if (!ok) return;
+#pragma unroll
+        for (int s = 0; s < 9; s++) {
+            if (s >= segs) break;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t w = (e < 2 ? code[s][k].x : code[s][k].y) ^ 0x80808080u;
+                    // 2^23 + (code + 128) as a float's bits
+                    const float lo = __uint_as_float(__byte_perm(w, 0x4b000000u, e & 1 ? 0x7542 : 0x7540)) - 8388736.0f;
+                    const float hi = __uint_as_float(__byte_perm(w, 0x4b000000u, e & 1 ? 0x7543 : 0x7541)) - 8388736.0f;
+                    const __half2 h = __floats2half2_rn(__fmul_rn(lo, d[s][k]), __fmul_rn(hi, d[s][k]));
+                    o[e] = reinterpret_cast<const uint32_t &>(h);
+                }
+                const int rw = rr + 16 * k;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + s * SEG + rw * 128 + ((c8 ^ (rw & 7)) << 4)),
+                             "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
+                             : "memory");
+            }
+        }
+    } else {
+        if (wait) ok = core_wait(y, &y.done[buf], parity, a.err);
+        if (!ok) return;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int rw = rr + 16 * k;
+            const uint8_t *src = static_cast<const uint8_t *>(a.c.k) + (row[k] < 0 ? 0 : row[k]) * a.c.hd * 2 + c8 * 16;
+            const uint32_t at = dst + rw * 128 + ((c8 ^ (rw & 7)) << 4);
+            for (int s = 0; s < segs - 1; s++) cp16(at + s * SEG, src + s * 128, row[k] >= 0);
+            const bool on = row[k] >= 0 && c8 < tail;
+            cp16(at + (segs - 1) * SEG, on ? src + (segs - 1) * 128 : static_cast<const uint8_t *>(a.c.k), on);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // rows without a page: bit position of the tile, one word of 32 rows each
+    if (c8 == 0 && dead)
+        for (int k = 0; k < 4; k++)
+            if (dead >> k & 1) atomicOr(&y.dead[buf][(rr + 16 * k) >> 5], 1u << ((rr + 16 * k) & 31));
+}
+
+// Query rows of a run as the S product's first operand: eight lanes a head.
+template <int OT>
+__device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint32_t dst, int segs, const Run &r, int h0, int nh, int lt) {
+    const int c8 = lt & 7, W = a.R + a.dr;
+    for (int h = lt >> 3; h < LH; h += 16) {
+        const float *src = a.qa + ((int64_t)r.b * a.H + h0 + h) * W;
+        float fac = a.sc2;
+        float up = 1.0f;
+        auto piece = [&](int s, float x[8]) {
+            const int e = s * 64 + c8 * 8;
+            if (h < nh && e < W) {
+                const float4 u = __ldcg(reinterpret_cast<const float4 *>(src + e)), v = __ldcg(reinterpret_cast<const float4 *>(src + e) + 1);
+                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = 0.0f;
+            }
+        };
+        if constexpr (OT == F16) {
+            float m = 0.0f;
+            for (int s = 0; s < segs; s++) {
+                float x[8];
+                piece(s, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
+            }
+#pragma unroll
+            for (int o = 4; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int k = f16_lift(m);
+            up = pow2i(k), fac = __fmul_rn(fac, pow2i(-k));
+        }
+        if (c8 == 0) y.fac[h] = fac;
+        for (int s = 0; s < segs; s++) {
+            float x[8];
+            piece(s, x);
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float u = __fmul_rn(x[2 * i], up), v = __fmul_rn(x[2 * i + 1], up);
+                o[i] = take_pair<OT>(u, v);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + s * SEG + h * 128 + ((c8 ^ (h & 7)) << 4)), "r"(o[0]),
+                         "r"(o[1]), "r"(o[2]), "r"(o[3])
+                         : "memory");
+        }
     }
 }
 
-// out[b][h][j] = o[b][h] . w[h][dn + j]
-__global__ void k_latent_expand(const __grid_constant__ SideArgs a) {
-    const int h = blockIdx.x, b = blockIdx.y;
-    const float *o = a.o + ((int64_t)b * a.H + h) * a.R;
-    for (int j = threadIdx.x; j < a.dv; j += blockDim.x) {
-        const int64_t w0 = ((int64_t)h * (a.dn + a.dv) + a.dn + j) * a.R;
-        float x = 0.0f;
-        for (int r = 0; r < a.R; r++) x = __fmaf_rn(o[r], io_load(a.w, a.dtype, w0 + r), x);
-        io_store(a.out, a.dtype, b * a.os + h * a.oh + j, x);
+template <int CACHE>
+__global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_constant__ LatentArgs a) {
+    constexpr int OT = CACHE == BF16 ? BF16 : F16;
+    constexpr int NTP = OT == BF16 ? 2 : 1;
+    constexpr float POFF = OT == F16 ? 8.0f : 0.0f;
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const int segs = a.R / 64 + 1;
+    uint8_t *qb = base, *kvb = qb + segs * SEG, *pb = kvb + 2 * segs * SEG;
+    CoreShared &y = *reinterpret_cast<CoreShared *>(pb + SEG);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int pass = blockIdx.x % a.passes, cta = blockIdx.x / a.passes, grid = gridDim.x / a.passes;
+    const int h0 = pass * a.hp, nh = min(a.hp, a.H - h0), cols = (nh + 15) & ~15;
+
+    pdl_trigger();
+    int b0, ctas;
+    int64_t before, cur, end, total;
+    const bool have = my_units<CORE_THREADS>(a.c, a.lens, LT, 1, cta, grid, y.scan, b0, before, cur, end, total, ctas);
+    if (!have) {
+        pdl_wait();
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&y.full[i], 32 * LD_WARPS);
+            mbar_init(&y.sfull[i], 1);
+            mbar_init(&y.done[i], 1);
+            y.dead[i][0] = y.dead[i][1] = 0;
+        }
+        mbar_init(&y.pready, 128);
+        y.failed = 0;
+        fence_mbar_init();
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y.tmem)), "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tm = y.tmem, tm_o = tm + 128;      // S in columns 0-63 and 64-127, O^T from 128 on
+    Walk walk(a, b0, before, cur, end);
+    Run r;
+
+    if (warp >= 5) {
+        // ---- loading: warps 5-8 the even tiles, 9-12 the odd ones
+        const int buf = (warp - 5) / LD_WARPS, lt = tid - 160 - buf * 32 * LD_WARPS;
+        const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
+        bool ok = true, waited = false;
+        int ti = 0;      // tiles before this run
+        while (ok && walk.next(r)) {
+            for (int i = (ti ^ buf) & 1; ok && i < r.tiles; i += 2) {
+                const int k = ti + i;
+                load_tile<CACHE>(a, y, dst, segs, buf, r, i, lt, k >= 2, ((k >> 1) - 1) & 1, ok);
+                if (!ok) break;
+                if (i == 0) {     // the first tile's warps bring the queries, once the last run's products are done
+                    if (!waited) pdl_wait(), waited = true;
+                    if (k >= 1) ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err);
+                    if (!ok) break;
+                    load_q<OT>(a, y, smem_u32(qb), segs, r, h0, nh, lt);
+                }
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                fence_proxy_async();
+                arrive(&y.full[buf]);
+            }
+            ti += r.tiles;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!waited) pdl_wait();
+    } else if (warp == 4) {
+        // ---- products, one thread
+        if (lane == 0) {
+            const uint32_t fmt = OT == BF16 ? (1u << 7) | (1u << 10) : 0u;
+            const uint32_t is = (1u << 4) | fmt | ((uint32_t)(LT >> 3) << 17) | ((uint32_t)(LH >> 4) << 24);
+            const uint32_t ip = (1u << 4) | fmt | (1u << 15) | ((uint32_t)(cols >> 3) << 17) | (8u << 24);
+            const uint32_t qa = smem_u32(qb), ka = smem_u32(kvb), pa = smem_u32(pb);
+            int k = 0;       // tile count
+            bool ok = true;
+            auto values = [&](int kt, bool first) {      // O^T += V^T P^T of tile kt
+                if (!core_wait(y, &y.pready, kt & 1, a.err)) return false;
+                tc_after();
+                const uint32_t kv = ka + (kt & 1) * segs * SEG;
+                for (int blk = 0; blk < a.R / 128; blk++)
+#pragma unroll
+                    for (int x = 0; x < NTP; x++)
+#pragma unroll
+                        for (int e = 0; e < LT / 16; e++)
+                            umma_f16(tm_o + blk * cols, sw128_desc(kv + 2 * blk * SEG + e * 2048, SEG),
+                                     sw128_desc((x == 0 ? pa : kv + (segs - 1) * SEG) + e * 32, 16), ip, !(first && x == 0 && e == 0));
+                umma_done(&y.done[kt & 1]);
+                return true;
+            };
+            bool first = true, pending = false;
+            while (ok && walk.next(r))
+                for (int i = 0; ok && i < r.tiles; i++, k++) {
+                    ok = core_wait(y, &y.full[k & 1], (k >> 1) & 1, a.err);
+                    if (!ok) break;
+                    fence_proxy_async();
+                    const uint32_t kv = ka + (k & 1) * segs * SEG, ds = tm + (k & 1) * 64;
+                    for (int s = 0; s < segs; s++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            umma_f16(ds, sw128_desc(qa + s * SEG + e * 32, 16), sw128_desc(kv + s * SEG + e * 32, 16), is, s + e != 0);
+                    umma_done(&y.sfull[k & 1]);
+                    if (pending) ok = values(k - 1, first), first = false;
+                    pending = true;
+                    if (i == r.tiles - 1) {      // the run's last tile: its values before the next run's queries can come
+                        if (ok) ok = values(k, i == 0);
+                        pending = false, first = true;
+                    }
+                }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: thread = head for S (rows 16 w .. 16 w + 15 of a 64-row product lie in lanes 32 w .. 32 w + 15),
+        // dim for O^T
+        const int head = 16 * warp + (lane & 15);
+        const bool mine = lane < 16;
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        int k = 0;
+        bool ok = true, up = false;
+        while (!up && walk.next(r)) {
+            float ref = -kv_inf(), sum = 0.0f, fac = 0.0f;
+            for (int i = 0; i < r.tiles; i++, k++) {
+                const int buf = k & 1;
+                // a wait that fails shows at the next barrier of the four warps, where all of them give up
+                ok = core_wait(y, &y.sfull[buf], (k >> 1) & 1, a.err) && ok;
+                if (softmax_any(!ok)) { up = true; break; }
+                tc_after();
+                if (i == 0) fac = y.fac[head];
+                float v[64];
+                tm_ld32(tm + lanes + buf * 64, v);
+                tm_ld32(tm + lanes + buf * 64 + 32, v + 32);
+                tm_wait_ld();
+                const int live = r.n - (r.u + i) * LT;
+                const uint32_t d0 = y.dead[buf][0], d1 = y.dead[buf][1];
+                float mx = -kv_inf();
+#pragma unroll
+                for (int j = 0; j < 64; j++) v[j] = __fmul_rn(v[j], fac);
+                if (live < LT || (d0 | d1)) {
+#pragma unroll
+                    for (int j = 0; j < 64; j++) {
+                        if (j >= live) v[j] = -kv_inf();
+                        else if ((j < 32 ? d0 >> j : d1 >> (j - 32)) & 1) v[j] = kv_nan();
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 64; j++) mx = fmaxf(mx, v[j]);
+                float fade = 1.0f;
+                if (mx > ref + REF_SLACK || ref == -kv_inf()) {
+                    fade = exp2_fast(__fsub_rn(ref, mx == -kv_inf() ? 0.0f : mx));
+                    ref = mx;
+                }
+                if (softmax_any(mine && i > 0 && fade != 1.0f)) {
+                    if (mine) y.alpha[head] = fade;
+                    ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err) && ok;
+                    if (softmax_any(!ok)) { up = true; break; }
+                    tc_after();
+                    for (int c = 0; c < a.R / 128 * cols; c += 16) {
+                        float o[16];
+                        tm_ld16(tm_o + lanes + c, o);
+                        tm_wait_ld();
+                        const float *al = y.alpha + c % cols;
+#pragma unroll
+                        for (int j = 0; j < 16; j++) o[j] = __fmul_rn(o[j], al[j]);
+                        tm_st16(tm_o + lanes + c, o);
+                    }
+                    tm_wait_st();
+                }
+                const float shift = __fsub_rn(ref == -kv_inf() ? 0.0f : ref, POFF);
+                sum = __fmul_rn(sum, fade);
+                float part[4] = {};
+#pragma unroll
+                for (int j = 0; j < 64; j++) {
+                    v[j] = exp2_fast(__fsub_rn(v[j], shift));
+                    part[j & 3] = __fadd_rn(part[j & 3], v[j]);
+                }
+                sum = __fadd_rn(sum, __fadd_rn(__fadd_rn(part[0], part[1]), __fadd_rn(part[2], part[3])));
+                // P's buffer is free once the previous values' product is done
+                if (k >= 1) ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err) && ok;
+                if (mine && head < cols) {
+                    const uint32_t p0 = smem_u32(pb) + head * 128, p1 = smem_u32(kvb) + buf * segs * SEG + (segs - 1) * SEG + head * 128;
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+#pragma unroll
+                        for (int x = 0; x < NTP; x++) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[e] = take_pair<OT>(v[8 * c + 2 * e], v[8 * c + 2 * e + 1]);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((x == 0 ? p0 : p1) + ((c ^ (head & 7)) << 4)),
+                                         "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
+                                         : "memory");
+                        }
+                }
+                if (tid == 0) y.dead[buf][0] = y.dead[buf][1] = 0;
+                fence_proxy_async();
+                tc_before();
+                arrive(&y.pready);
+            }
+            if (up) break;
+            ok = core_wait(y, &y.done[(k - 1) & 1], ((k - 1) >> 1) & 1, a.err) && ok;
+            if (softmax_any(!ok)) break;
+            tc_after();
+            const bool whole = r.tiles == r.nu;
+            const int slot = r.b == b0 && r.u == (int)(cur - before) ? 0 : 1, W = a.R + a.dr;
+            const int64_t piece = (int64_t)blockIdx.x * 2 + slot;
+            float *o0 = whole ? a.qa + ((int64_t)r.b * a.H + h0) * W : a.o + piece * a.hp * a.R;
+            const int pitch = whole ? W : a.R;
+            for (int c = 0; c < a.R / 128 * cols; c += 16) {
+                float o[16];
+                tm_ld16(tm_o + lanes + c, o);
+                tm_wait_ld();
+                const int hc = c % cols, d = c / cols * 128 + 32 * warp + lane;
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (hc + j < nh) o0[(int64_t)(hc + j) * pitch + d] = o[j];
+            }
+            if (mine && head < nh) {
+                if (whole) o0[(int64_t)head * W + a.R] = ref, o0[(int64_t)head * W + a.R + 1] = sum;
+                else a.ml[piece * a.hp + head] = make_float2(ref, sum);
+            }
+            if (tid == 0 && r.u == 0) {
+                const int64_t upto = walk.cur - r.tiles + r.nu;
+                a.desc[(int64_t)r.b * a.passes + pass] = make_int4(cta, slot, (int)((upto * ctas - 1) / total), whole ? 0 : 1);
+            }
+            tc_before();
+        }
+    }
+    __syncthreads();
+    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u));
+}
+
+// ------------------------------------------------------------------------------------------- expand
+
+constexpr int EX_WARPS = 16, EX_ROWS = 8;
+
+struct ExpandShared {
+    uint4 ops[2][16][32];                // [term][32-dim step][lane]
+    float join[EX_WARPS][512];
+    float wgt[EX_WARPS][ATTN_SMS], red[EX_WARPS][16 * EX_ROWS];
+};
+
+// A CTA a head and eight sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as two
+// terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o.
+template <int T>
+__global__ void __launch_bounds__(32 * EX_WARPS) k_latent_expand(const __grid_constant__ LatentArgs a) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    ExpandShared &y = *reinterpret_cast<ExpandShared *>(raw);
+    auto &ops = y.ops;
+    auto &wgt = y.wgt;
+    auto &red = y.red;
+    auto &join = y.join;
+    const int h = blockIdx.x, b0 = blockIdx.y * EX_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rows = min(EX_ROWS, a.c.n_seqs - b0), pass = h / a.hp, hc = h - pass * a.hp, W = a.R + a.dr, steps = a.R / 32;
+    const int mt = a.dv / 16, ksplit = EX_WARPS / mt, m = warp % mt, kq = warp / mt;
+    const bool live = warp < mt * ksplit;
+    const int s0 = live ? kq * steps / ksplit : 0, s1 = live ? (kq + 1) * steps / ksplit : 0;
+    const uint16_t *w = static_cast<const uint16_t *>(a.w) + ((int64_t)h * (a.dn + a.dv) + a.dn + 16 * m + g) * a.R + 8 * t;
+    uint4 w0[8], w1[8];      // the first 256 dims of its part, under way before the core has ended
+#pragma unroll
+    for (int s = 0; s < 8; s++)
+        if (s0 + s < s1) {
+            w0[s] = __ldg(reinterpret_cast<const uint4 *>(w + (s0 + s) * 32));
+            w1[s] = __ldg(reinterpret_cast<const uint4 *>(w + 8 * (int64_t)a.R + (s0 + s) * 32));
+        }
+    for (int i = threadIdx.x; i < 2 * 16 * 32; i += 32 * EX_WARPS) (&ops[0][0][0])[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    pdl_wait();
+
+    int wpr = EX_WARPS;                                  // warps a row
+    while (wpr * rows > EX_WARPS) wpr >>= 1;
+    const int row = warp / wpr, part = warp % wpr;
+    const bool work = row < rows;
+    float inv = 0.0f;
+    if (work) {
+        const int b = b0 + row, n = a.lens[b];
+        const int64_t cap = table_capacity(a.c);
+        float o[4][4] = {};
+        if (*a.err || n > cap) {
+            inv = kv_nan();
+        } else if (n > 0) {
+            const int4 ds = a.desc[(int64_t)b * a.passes + pass];
+            const float *whole = a.qa + ((int64_t)b * a.H + h) * W;
+            const int count = ds.w ? ds.z - ds.x + 1 : 1;
+            auto piece = [&](int i) { return ((int64_t)((ds.x + i) * a.passes + pass) * 2 + (i == 0 ? ds.y : 0)) * a.hp + hc; };
+            float mx = -kv_inf(), l = 0.0f;
+            for (int i = lane; i < count; i += 32) mx = fmaxf(mx, ds.w ? a.ml[piece(i)].x : whole[a.R]);
+            for (int s = 16; s >= 1; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+            for (int i = lane; i < count; i += 32) {
+                const float2 x = ds.w ? a.ml[piece(i)] : make_float2(whole[a.R], whole[a.R + 1]);
+                const float f = exp2_fast(__fsub_rn(x.x, mx == -kv_inf() ? 0.0f : mx));
+                wgt[warp][i] = f;
+                l = __fmaf_rn(f, x.y, l);
+            }
+            for (int s = 16; s >= 1; s >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, s));
+            __syncwarp();
+            inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+#pragma unroll 2
+            for (int i = part; i < count; i += wpr) {
+                const float *src = ds.w ? a.o + piece(i) * a.R : whole;
+                const float f = wgt[warp][i];
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (k < a.R / 128) {
+                        const float *at = src + 128 * k + 4 * lane;
+                        o[k][0] = __fmaf_rn(f, at[0], o[k][0]), o[k][1] = __fmaf_rn(f, at[1], o[k][1]);
+                        o[k][2] = __fmaf_rn(f, at[2], o[k][2]), o[k][3] = __fmaf_rn(f, at[3], o[k][3]);
+                    }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k < a.R / 128) *reinterpret_cast<float4 *>(&join[warp][128 * k + 4 * lane]) = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
+    }
+    __syncthreads();
+    // eight dims a lane of the row's first warp, over its warps' sums
+    if (work && part == 0)
+        for (int c = lane; c < a.R / 8; c += 32) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = join[warp][8 * c + i];
+            for (int p = 1; p < wpr; p++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = __fadd_rn(x[i], join[warp + p][8 * c + i]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = inv == 0.0f ? 0.0f : __fmul_rn(x[i], inv);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                uint4 v;
+                v.x = take_pair<T>(x[0], x[1]), v.y = take_pair<T>(x[2], x[3]), v.z = take_pair<T>(x[4], x[5]), v.w = take_pair<T>(x[6], x[7]);
+                ops[k][c >> 2][row * 4 + (c & 3)] = v;
+            }
+        }
+    __syncthreads();
+    float acc[4] = {};
+    auto step = [&](int s, const uint4 &u, const uint4 &v) {
+#pragma unroll
+        for (int k = 1; k >= 0; k--) {
+            const uint4 x = ops[k][s][lane];
+            mma16<T>(acc, u.x, v.x, u.y, v.y, x.x, x.y);
+            mma16<T>(acc, u.z, v.z, u.w, v.w, x.z, x.w);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < 8; s++)
+        if (s0 + s < s1) step(s0 + s, w0[s], w1[s]);
+    for (int s = s0 + 8; s < s1; s++)
+        step(s, __ldg(reinterpret_cast<const uint4 *>(w + s * 32)), __ldg(reinterpret_cast<const uint4 *>(w + 8 * (int64_t)a.R + s * 32)));
+    if (live) {
+        red[warp][g * EX_ROWS + 2 * t] = acc[0], red[warp][g * EX_ROWS + 2 * t + 1] = acc[1];
+        red[warp][(g + 8) * EX_ROWS + 2 * t] = acc[2], red[warp][(g + 8) * EX_ROWS + 2 * t + 1] = acc[3];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
+        const int rw = i / a.dv, j = i - rw * a.dv;
+        float x = red[j >> 4][(j & 15) * EX_ROWS + rw];
+        for (int k = 1; k < ksplit; k++) x = __fadd_rn(x, red[k * mt + (j >> 4)][(j & 15) * EX_ROWS + rw]);
+        io_store(a.out, T, (b0 + rw) * a.os + h * a.oh + j, x);
     }
 }
 
-bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// ------------------------------------------------------------------------------------------- host side
+
+struct Plan {
+    int passes, hp, grid, segs;
+    size_t qa, o, ml, desc, bytes, smem;
+};
+
+Plan plan_of(const hxb_kv_cache *c, int H, int R) {
+    Plan p = {};
+    p.passes = (H + LH - 1) / LH;
+    p.hp = (H + p.passes - 1) / p.passes;
+    p.grid = ATTN_SMS / p.passes * p.passes;
+    p.segs = R / 64 + 1;
+    auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+    p.qa = up((size_t)c->n_seqs * H * c->head_dim * sizeof(float));
+    p.o = (size_t)p.grid * 2 * p.hp * R * sizeof(float);
+    p.ml = (size_t)p.grid * 2 * p.hp * sizeof(float2);
+    p.desc = (size_t)c->n_seqs * p.passes * sizeof(int4);
+    p.bytes = p.qa + p.o + p.ml + p.desc + 16;
+    p.smem = 1024 + (size_t)(3 * p.segs + 1) * SEG + sizeof(CoreShared);
+    return p;
+}
+
+template <int CACHE, int T>
+cudaError_t launch(const LatentArgs &a, const Plan &p, cudaStream_t s) {
+    cudaError_t e = cudaFuncSetAttribute(k_latent_core<CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(k_latent_expand<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ExpandShared));
+    if (e != cudaSuccess) return e;
+    const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS), B = a.c.n_seqs;
+    e = launch_pdl(false, k_latent_absorb<T>, dim3(a.H * nc, (B + AB_ROWS - 1) / AB_ROWS), dim3(32 * AB_WARPS), 0, s, a);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(true, k_latent_expand<T>, dim3(a.H, (B + EX_ROWS - 1) / EX_ROWS), dim3(32 * EX_WARPS), sizeof(ExpandShared), s, a);
+}
 
 }  // namespace
 }  // namespace hx
@@ -121,46 +753,48 @@ bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % 
 using namespace hx;
 
 extern "C" HXB_API size_t hxb_latent_decode_workspace(const hxb_kv_cache *c, int n_heads, int rank) {
-    if (!c || n_heads < 1 || rank < 1 || c->n_seqs < 0) return 0;
-    return ((size_t)c->n_seqs * n_heads * ((size_t)c->head_dim + rank)) * 4 + 16;
+    if (!c || n_heads < 1 || n_heads > 256 || rank < 1 || rank > 512 || c->n_seqs < 0 || c->head_dim < 1) return 0;
+    return plan_of(c, n_heads, rank).bytes;
 }
 
 extern "C" HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_t *lens, const void *q, int64_t q_stride,
                                              int64_t q_head_stride, const void *w, int n_heads, int rank, int nope,
                                              int v_dim, int dtype, float scale, void *out, int64_t out_stride,
                                              int64_t out_head_stride, void *ws, size_t ws_bytes, void *stream) {
-    CoreArgs a = {};
-    int rc = kv_view(c, "latent_decode", true, &a.c);
+    const char *who = "latent_decode";
+    LatentArgs a = {};
+    int rc = kv_view(c, who, true, &a.c);
     if (rc != HXB_OK) return rc;
-    if (dtype != F16 && dtype != BF16) return attn_fail(HXB_E_ARG, "latent_decode: dtype %d (F16 or BF16)", dtype);
-    if (c->dtype != Q8 && c->dtype != dtype)
-        return attn_fail(HXB_E_ARG, "latent_decode: the cache is Q8 or has the type of q");
+    if (dtype != F16 && dtype != BF16) return attn_fail(HXB_E_ARG, "%s: dtype %d (F16 or BF16)", who, dtype);
+    if (c->dtype != Q8 && c->dtype != dtype) return attn_fail(HXB_E_ARG, "%s: the cache is Q8 or has the type of q", who);
     const int dr = c->head_dim - rank;
     if (rank < 128 || rank > 512 || rank % 128 || dr < 16 || dr > 64 || dr % 16)
-        return attn_fail(HXB_E_UNSUPPORTED, "latent_decode: rank %d in rows of %d (rank a multiple of 128 up to 512, 16 to 64 more)",
-                         rank, c->head_dim);
+        return attn_fail(HXB_E_UNSUPPORTED, "%s: rank %d in rows of %d (rank a multiple of 128 up to 512, and 16 to 64 more)", who, rank,
+                         c->head_dim);
     if (nope < 16 || nope > 256 || nope % 16 || v_dim < 16 || v_dim > 256 || v_dim % 16)
-        return attn_fail(HXB_E_UNSUPPORTED, "latent_decode: nope %d, v_dim %d (multiples of 16 up to 256)", nope, v_dim);
-    if (n_heads < 1 || n_heads > 256) return attn_fail(HXB_E_ARG, "latent_decode: %d heads (up to 256)", n_heads);
+        return attn_fail(HXB_E_UNSUPPORTED, "%s: nope %d, v_dim %d (multiples of 16 up to 256)", who, nope, v_dim);
+    if (n_heads < 1 || n_heads > 256 || c->n_seqs > 65535)
+        return attn_fail(HXB_E_ARG, "%s: %d heads (up to 256), %d sequences (up to 65535)", who, n_heads, c->n_seqs);
     if (c->n_seqs == 0) return HXB_OK;
-    rc = attn_check_io("latent_decode", c->n_seqs, n_heads, q, q_stride, q_head_stride, out, out_stride, out_head_stride, v_dim, dtype,
-                       lens, scale);
+    rc = attn_check_io(who, c->n_seqs, n_heads, q, q_stride, q_head_stride, out, out_stride, out_head_stride, v_dim, dtype, lens, scale);
     if (rc != HXB_OK) return rc;
-    if (!w || !aligned(w, 16)) return attn_fail(HXB_E_ARG, "latent_decode: w must be 16-byte aligned");
-    if (!ws || !aligned(ws, 16) || ws_bytes < hxb_latent_decode_workspace(c, n_heads, rank))
-        return attn_fail(HXB_E_ARG, "latent_decode: workspace of %zu bytes, 16-byte aligned, needed",
-                         hxb_latent_decode_workspace(c, n_heads, rank));
+    if (!w || reinterpret_cast<uintptr_t>(w) % 16) return attn_fail(HXB_E_ARG, "%s: w must be 16-byte aligned", who);
+    const Plan p = plan_of(c, n_heads, rank);
+    if (!ws || reinterpret_cast<uintptr_t>(ws) % 16 || ws_bytes < p.bytes)
+        return attn_fail(HXB_E_ARG, "%s: workspace of %zu bytes, 16-byte aligned, needed", who, p.bytes);
+    uint8_t *at = static_cast<uint8_t *>(ws);
+    a.qa = reinterpret_cast<float *>(at), at += p.qa;
+    a.o = reinterpret_cast<float *>(at), at += p.o;
+    a.ml = reinterpret_cast<float2 *>(at), at += p.ml;
+    a.desc = reinterpret_cast<int4 *>(at), at += p.desc;
+    a.err = reinterpret_cast<int *>(at);
+    a.lens = lens, a.q = q, a.w = w, a.out = out, a.qs = q_stride, a.qh = q_head_stride, a.os = out_stride, a.oh = out_head_stride;
+    a.H = n_heads, a.R = rank, a.dr = dr, a.dn = nope, a.dv = v_dim, a.passes = p.passes, a.hp = p.hp;
+    a.sc2 = scale * 1.44269504088896f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    SideArgs e = {};
-    e.q = q, e.w = w, e.qa = static_cast<float *>(ws), e.o = e.qa + (size_t)c->n_seqs * n_heads * c->head_dim, e.out = out;
-    e.qs = q_stride, e.qh = q_head_stride, e.os = out_stride, e.oh = out_head_stride;
-    e.H = n_heads, e.R = rank, e.dr = dr, e.dn = nope, e.dv = v_dim, e.dtype = dtype;
-    a.lens = lens, a.q = e.qa, a.qs = (int64_t)n_heads * c->head_dim, a.qh = c->head_dim, a.out = e.o;
-    a.os = (int64_t)n_heads * rank, a.oh = rank, a.H = n_heads, a.dtype_c = c->dtype, a.dtype_q = a.dtype_o = F32;
-    a.vd = rank, a.latent = 1, a.scale = scale;
-    const dim3 grid(n_heads, c->n_seqs);
-    k_latent_absorb<<<grid, 128, 0, s>>>(e);
-    k_attn_core<<<grid, AD_THREADS, 0, s>>>(a);
-    k_latent_expand<<<grid, 128, 0, s>>>(e);
-    return attn_launched("latent_decode") ? HXB_OK : HXB_E_DEVICE;
+    cudaError_t e;
+    if (c->dtype == Q8) e = dtype == F16 ? launch<Q8, F16>(a, p, s) : launch<Q8, BF16>(a, p, s);
+    else e = dtype == F16 ? launch<F16, F16>(a, p, s) : launch<BF16, BF16>(a, p, s);
+    if (e != cudaSuccess) return attn_fail(HXB_E_DEVICE, "%s: %s", who, cudaGetErrorString(e));
+    return HXB_OK;
 }

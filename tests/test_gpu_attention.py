@@ -470,7 +470,7 @@ def test_latent_attention_bad_pages_strides_and_scratch(gpu):
     lens = torch.tensor([100, 100, 100], dtype=torch.int32).cuda()
     good = hb.latent_attention(q, w, cp, table.cuda(), lens, scale=0.07)
     out = torch.full((3, 17, 131), 5.0, dtype=torch.bfloat16).cuda()
-    ws = torch.full((1 << 25,), 255, dtype=torch.uint8).cuda()
+    ws = torch.full((1 << 26,), 255, dtype=torch.uint8).cuda()
     hb.latent_attention(q, w, cp, table.cuda(), lens, scale=0.07, out=out[:, :16, 2:130], workspace=ws)
     assert torch.equal(out[:, :16, 2:130], good)
     rest = out.clone()
