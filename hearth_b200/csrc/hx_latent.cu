@@ -33,6 +33,7 @@
 #include "hx_attn.cuh"
 
 #include <algorithm>
+#include <cuda.h>
 
 namespace hx {
 namespace {
@@ -40,8 +41,9 @@ namespace {
 constexpr int LT = 64;                  // positions a tile
 constexpr int LH = 64;                  // heads a CTA (rows of S)
 constexpr int SEG = LT * 128;           // 64 dims of 64 rows: a 128-byte swizzled block column
-constexpr int LD_WARPS = 4;             // loading warps a tile buffer
-constexpr int CORE_WARPS = 5 + 2 * LD_WARPS, CORE_THREADS = 32 * CORE_WARPS;
+constexpr int LD_WARPS = 8, LD_THREADS = 32 * LD_WARPS;
+constexpr int CORE_WARPS = 6 + LD_WARPS, CORE_THREADS = 32 * CORE_WARPS;
+constexpr int MMA_WARP = 4, MAP_WARP = 5, LD_WARP0 = 6;
 constexpr float REF_SLACK = 7.0f;
 
 struct LatentArgs {
@@ -57,6 +59,7 @@ struct LatentArgs {
     int64_t qs, qh, os, oh;
     int H, R, dr, dn, dv, passes, hp;   // hp heads a pass
     float sc2;
+    int box;                // rows of a tensor-map load; 0: rows by 16-byte copies only
 };
 
 // ------------------------------------------------------------------------------------------- absorb
@@ -128,40 +131,44 @@ __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_co
 // ------------------------------------------------------------------------------------------- core
 
 struct CoreShared {
-    uint64_t full[2], sfull[2], done[2], pready;
+    uint64_t full[2], freed[2][3], sfull[2], done[2], pready, qfull;   // freed: 128-dim pieces of a buffer, before done
     int64_t scan[CORE_WARPS];
     uint32_t tmem, failed;
     uint32_t dead[2][2];     // positions of a tile without a row
     float alpha[LH], fac[LH];
 };
 
-// Shared-memory matrix descriptors of 128-byte swizzled operands (8-row groups 1024 bytes apart). Row-major (K along
-// the 128 bytes): one block column. Column-major (the 64 outer elements along the 128 bytes): `lead` bytes to the
-// next 64 of them.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// Shared-memory matrix descriptors of 128-byte swizzled operands (8-row groups 1024 bytes apart): the high word is
+// the same for all of them, the low word is the address in 16-byte units under the distance `lead` between blocks of
+// 64 outer elements (column-major operands; ignored for row-major ones). Steps through an operand add to the low word.
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) { return ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16); }
 
-__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool accumulate) {
+template <bool ACC>
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t da, uint32_t db, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(da), "r"(db), "n"(DESC_HI), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
+}
+// One lane of the calling warp, the same at every call.
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void umma_done(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tm_ld32(uint32_t addr, float v[32]) {
+// 16 lanes by 64 columns, as the accumulators of 16 x 8 products: [8-column block][row g: 2 t, 2 t + 1; row g + 8].
+__device__ __forceinline__ void tm_ld_rows16(uint32_t addr, float v[8][4]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
-          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]), "=f"(v[2][0]), "=f"(v[2][1]), "=f"(v[2][2]), "=f"(v[2][3]), "=f"(v[3][0]), "=f"(v[3][1]), "=f"(v[3][2]), "=f"(v[3][3]), "=f"(v[4][0]), "=f"(v[4][1]), "=f"(v[4][2]), "=f"(v[4][3]), "=f"(v[5][0]), "=f"(v[5][1]), "=f"(v[5][2]), "=f"(v[5][3]), "=f"(v[6][0]), "=f"(v[6][1]), "=f"(v[6][2]), "=f"(v[6][3]), "=f"(v[7][0]), "=f"(v[7][1]), "=f"(v[7][2]), "=f"(v[7][3])
         : "r"(addr)
         : "memory");
 }
@@ -185,20 +192,34 @@ __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// A barrier of the softmax warps, with the or of x.
-__device__ __forceinline__ bool softmax_any(bool x) {
+// Barrier BAR of N threads, with the or of x.
+template <int BAR, int N>
+__device__ __forceinline__ bool any_of(bool x) {
     __syncwarp();
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred.aligned q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        "barrier.cta.red.or.pred.aligned q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"(x ? 1u : 0u)
+        : "r"(x ? 1u : 0u), "n"(BAR), "n"(N)
         : "memory");
     return r != 0;
 }
+__device__ __forceinline__ bool softmax_any(bool x) { return any_of<1, 128>(x); }
+__device__ __forceinline__ bool loaders_any(bool x) { return any_of<2, LD_THREADS>(x); }
+
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool on) {   // zeros when off
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {   // without suspending the thread
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 // A wait that ends: on the phase, when another role has given up, or at the spin limit (the error word, so
@@ -206,6 +227,18 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool on) {  
 __device__ __forceinline__ bool core_wait(CoreShared &y, uint64_t *bar, uint32_t parity, int *err) {
     for (uint32_t i = 0; i < kSpinLimit; i++) {
         if (mbar_try_wait(bar, parity)) return true;
+        if (*reinterpret_cast<volatile uint32_t *>(&y.failed)) return false;
+    }
+    *reinterpret_cast<volatile uint32_t *>(&y.failed) = 1;
+    set_error(err, DEV_E_WAIT_TIMEOUT);
+    return false;
+}
+
+// The first of two waits (null: not asked for) whose phase is over, a before b; first_is_a says which.
+__device__ __forceinline__ bool core_wait2(CoreShared &y, uint64_t *a, uint32_t pa, uint64_t *b, uint32_t pb, int *err, bool &first_is_a) {
+    for (uint32_t i = 0; i < kSpinLimit; i++) {
+        if (a && mbar_test(a, pa)) return first_is_a = true, true;
+        if (b && mbar_test(b, pb)) return first_is_a = false, true;
         if (*reinterpret_cast<volatile uint32_t *>(&y.failed)) return false;
     }
     *reinterpret_cast<volatile uint32_t *>(&y.failed) = 1;
@@ -232,80 +265,70 @@ struct Walk {
     }
 };
 
+// The loading threads' view of a tile: the rows each of them fetches from, looked up one tile ahead. 16-bit rows: eight
+// lanes a 128-byte block row, 32 rows at once; Q8: four lanes a row's 64 codes.
 template <int CACHE>
-__device__ __forceinline__ void load_tile(const LatentArgs &a, CoreShared &y, uint32_t dst, int segs, int buf, const Run &r, int tile,
-                                          int lt, bool wait, uint32_t parity, bool &ok) {
-    // eight lanes a 128-byte block row, 16 rows at once
-    const int c8 = lt & 7, rr = lt >> 3;
-    int64_t row[4];
-    uint32_t dead = 0;
+struct TileRows {
+    static constexpr int N = CACHE == Q8 ? 1 : 2;
+    int64_t row[N];
+    uint32_t dead;      // positions in range that have no row
+    __device__ __forceinline__ void find(const LatentArgs &a, const Run &r, int tile, int lt) {
+        dead = 0;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const int pos = (r.u + tile) * LT + rr + 16 * k;
-        row[k] = pos < r.n ? kv_row(a.c, r.b, pos) : -1;
-        if (pos < r.n && row[k] < 0) dead |= 1u << k;
+        for (int k = 0; k < N; k++) {
+            const int pos = (r.u + tile) * LT + (CACHE == Q8 ? lt >> 2 : (lt >> 3) + 32 * k);
+            row[k] = pos < r.n ? kv_row(a.c, r.b, pos) : -1;
+            if (pos < r.n && row[k] < 0) dead |= 1u << k;
+        }
     }
-    const int tail = a.dr / 8;     // 16-byte pieces of the last block column
-    if constexpr (CACHE == Q8) {
-        // codes and scales into registers while the buffer is still at work
-        uint2 code[9][4];
-        float d[9][4];
+    // marks them for the softmax (bit position of the tile)
+    __device__ __forceinline__ void mark(CoreShared &y, int buf, int lt) const {
+        if (!dead) return;
 #pragma unroll
-        for (int s = 0; s < 9; s++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const bool on = row[k] >= 0 && s < segs;
-                code[s][k] = on ? __ldg(reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(a.c.k) + row[k] * a.c.hd + s * 64) + c8) : make_uint2(0, 0);
-                d[s][k] = on ? __ldg(a.c.ks + row[k] * segs + s) : 0.0f;
-            }
-        if (wait) ok = core_wait(y, &y.done[buf], parity, a.err);
-        if (!ok) return;
+        for (int k = 0; k < N; k++) {
+            const int rw = CACHE == Q8 ? lt >> 2 : (lt >> 3) + 32 * k;
+            if ((dead >> k & 1) && (lt & (CACHE == Q8 ? 3 : 7)) == 0) atomicOr(&y.dead[buf][rw >> 5], 1u << (rw & 31));
+        }
+    }
+};
+
+// Raw Q8 rows of a tile, in registers while the buffer is still at work.
+struct RawRows {
+    uint4 code[9];
+    float d[9];
+    __device__ __forceinline__ void fetch(const LatentArgs &a, int64_t row, int segs, int lt) {
 #pragma unroll
         for (int s = 0; s < 9; s++) {
-            if (s >= segs) break;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                uint32_t o[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t w = (e < 2 ? code[s][k].x : code[s][k].y) ^ 0x80808080u;
-                    // 2^23 + (code + 128) as a float's bits
-                    const float lo = __uint_as_float(__byte_perm(w, 0x4b000000u, e & 1 ? 0x7542 : 0x7540)) - 8388736.0f;
-                    const float hi = __uint_as_float(__byte_perm(w, 0x4b000000u, e & 1 ? 0x7543 : 0x7541)) - 8388736.0f;
-                    const __half2 h = __floats2half2_rn(__fmul_rn(lo, d[s][k]), __fmul_rn(hi, d[s][k]));
-                    o[e] = reinterpret_cast<const uint32_t &>(h);
-                }
-                const int rw = rr + 16 * k;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + s * SEG + rw * 128 + ((c8 ^ (rw & 7)) << 4)),
-                             "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
-                             : "memory");
-            }
+            const bool on = row >= 0 && s < segs;
+            code[s] = on ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(a.c.k) + row * a.c.hd + s * 64) + (lt & 3)) : make_uint4(0, 0, 0, 0);
+            d[s] = on ? __ldg(a.c.ks + row * segs + s) : 0.0f;
         }
-    } else {
-        if (wait) ok = core_wait(y, &y.done[buf], parity, a.err);
-        if (!ok) return;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int rw = rr + 16 * k;
-            const uint8_t *src = static_cast<const uint8_t *>(a.c.k) + (row[k] < 0 ? 0 : row[k]) * a.c.hd * 2 + c8 * 16;
-            const uint32_t at = dst + rw * 128 + ((c8 ^ (rw & 7)) << 4);
-            for (int s = 0; s < segs - 1; s++) cp16(at + s * SEG, src + s * 128, row[k] >= 0);
-            const bool on = row[k] >= 0 && c8 < tail;
-            cp16(at + (segs - 1) * SEG, on ? src + (segs - 1) * 128 : static_cast<const uint8_t *>(a.c.k), on);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    // rows without a page: bit position of the tile, one word of 32 rows each
-    if (c8 == 0 && dead)
-        for (int k = 0; k < 4; k++)
-            if (dead >> k & 1) atomicOr(&y.dead[buf][(rr + 16 * k) >> 5], 1u << ((rr + 16 * k) & 31));
+};
+// 16 codes times d as f16, into pieces 2 q and 2 q + 1 of a block row.
+__device__ __forceinline__ void expand16(uint32_t at, int rw, int q, const uint4 &code, float d) {
+    const uint32_t in[4] = {code.x ^ 0x80808080u, code.y ^ 0x80808080u, code.z ^ 0x80808080u, code.w ^ 0x80808080u};
+    uint32_t o[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        // 2^23 + (code + 128) as a float's bits
+        const float lo = __uint_as_float(__byte_perm(in[e >> 1], 0x4b000000u, e & 1 ? 0x7542 : 0x7540)) - 8388736.0f;
+        const float hi = __uint_as_float(__byte_perm(in[e >> 1], 0x4b000000u, e & 1 ? 0x7543 : 0x7541)) - 8388736.0f;
+        const __half2 h = __floats2half2_rn(__fmul_rn(lo, d), __fmul_rn(hi, d));
+        o[e] = reinterpret_cast<const uint32_t &>(h);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + rw * 128 + (((2 * q + c) ^ (rw & 7)) << 4)), "r"(o[4 * c]),
+                     "r"(o[4 * c + 1]), "r"(o[4 * c + 2]), "r"(o[4 * c + 3])
+                     : "memory");
 }
 
 // Query rows of a run as the S product's first operand: eight lanes a head.
 template <int OT>
 __device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint32_t dst, int segs, const Run &r, int h0, int nh, int lt) {
     const int c8 = lt & 7, W = a.R + a.dr;
-    for (int h = lt >> 3; h < LH; h += 16) {
+    for (int h = lt >> 3; h < LH; h += LD_THREADS / 8) {
         const float *src = a.qa + ((int64_t)r.b * a.H + h0 + h) * W;
         float fac = a.sc2;
         float up = 1.0f;
@@ -349,8 +372,16 @@ __device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint3
     }
 }
 
+// One box of the pool's rows: 64 values from column x on of rows y ..., 128-byte swizzled. x is a multiple of 64.
+__device__ __forceinline__ void map_load(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+
 template <int CACHE>
-__global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_constant__ LatentArgs a) {
+__global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_constant__ LatentArgs a, const __grid_constant__ CUtensorMap map) {
     constexpr int OT = CACHE == BF16 ? BF16 : F16;
     constexpr int NTP = OT == BF16 ? 2 : 1;
     constexpr float POFF = OT == F16 ? 8.0f : 0.0f;
@@ -373,16 +404,18 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
     }
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&y.full[i], 32 * LD_WARPS);
+            mbar_init(&y.full[i], 1);
+            for (int j = 0; j < 3; j++) mbar_init(&y.freed[i][j], 1);
             mbar_init(&y.sfull[i], 1);
             mbar_init(&y.done[i], 1);
             y.dead[i][0] = y.dead[i][1] = 0;
         }
         mbar_init(&y.pready, 128);
+        mbar_init(&y.qfull, LD_THREADS);
         y.failed = 0;
         fence_mbar_init();
     }
-    if (warp == 4) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y.tmem)), "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -393,117 +426,221 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
     Walk walk(a, b0, before, cur, end);
     Run r;
 
-    if (warp >= 5) {
-        // ---- loading: warps 5-8 the even tiles, 9-12 the odd ones
-        const int buf = (warp - 5) / LD_WARPS, lt = tid - 160 - buf * 32 * LD_WARPS;
-        const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
-        bool ok = true, waited = false;
-        int ti = 0;      // tiles before this run
-        while (ok && walk.next(r)) {
-            for (int i = (ti ^ buf) & 1; ok && i < r.tiles; i += 2) {
-                const int k = ti + i;
-                load_tile<CACHE>(a, y, dst, segs, buf, r, i, lt, k >= 2, ((k >> 1) - 1) & 1, ok);
-                if (!ok) break;
-                if (i == 0) {     // the first tile's warps bring the queries, once the last run's products are done
-                    if (!waited) pdl_wait(), waited = true;
-                    if (k >= 1) ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err);
-                    if (!ok) break;
-                    load_q<OT>(a, y, smem_u32(qb), segs, r, h0, nh, lt);
-                }
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                fence_proxy_async();
-                arrive(&y.full[buf]);
-            }
-            ti += r.tiles;
-        }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (!waited) pdl_wait();
-    } else if (warp == 4) {
-        // ---- products, one thread
-        if (lane == 0) {
-            const uint32_t fmt = OT == BF16 ? (1u << 7) | (1u << 10) : 0u;
-            const uint32_t is = (1u << 4) | fmt | ((uint32_t)(LT >> 3) << 17) | ((uint32_t)(LH >> 4) << 24);
-            const uint32_t ip = (1u << 4) | fmt | (1u << 15) | ((uint32_t)(cols >> 3) << 17) | (8u << 24);
-            const uint32_t qa = smem_u32(qb), ka = smem_u32(kvb), pa = smem_u32(pb);
-            int k = 0;       // tile count
+    // A tile whose 64 positions are all in range comes by tensor map where the pages allow it; a sequence's last rows
+    // (past them a slot may hold NaN, and 0 x NaN would reach every sum), small pages and Q8 rows go through the
+    // loading warps. Either way a buffer's pieces are refilled as the products of the tile before last free them.
+    const int pieces = a.R / 128;
+    auto by_map = [&](const Run &r, int i) { return CACHE != Q8 && a.box && r.n - (r.u + i) * LT >= LT; };
+    auto wait_free = [&](int k, int j) {     // piece j of tile k's buffer (pieces: the rotated part)
+        return k < 2 || core_wait(y, j < pieces - 1 ? &y.freed[k & 1][j] : &y.done[k & 1], ((k >> 1) - 1) & 1, a.err);
+    };
+    if (warp == MAP_WARP) {
+        // ---- tensor-map loads: lane i a box of rows
+        if constexpr (CACHE != Q8) {
+            const int boxes = a.box ? LT / a.box : 0;
+            int k = 0;
             bool ok = true;
-            auto values = [&](int kt, bool first) {      // O^T += V^T P^T of tile kt
-                if (!core_wait(y, &y.pready, kt & 1, a.err)) return false;
-                tc_after();
-                const uint32_t kv = ka + (kt & 1) * segs * SEG;
-                for (int blk = 0; blk < a.R / 128; blk++)
-#pragma unroll
-                    for (int x = 0; x < NTP; x++)
-#pragma unroll
-                        for (int e = 0; e < LT / 16; e++)
-                            umma_f16(tm_o + blk * cols, sw128_desc(kv + 2 * blk * SEG + e * 2048, SEG),
-                                     sw128_desc((x == 0 ? pa : kv + (segs - 1) * SEG) + e * 32, 16), ip, !(first && x == 0 && e == 0));
-                umma_done(&y.done[kt & 1]);
-                return true;
-            };
-            bool first = true, pending = false;
             while (ok && walk.next(r))
                 for (int i = 0; ok && i < r.tiles; i++, k++) {
-                    ok = core_wait(y, &y.full[k & 1], (k >> 1) & 1, a.err);
-                    if (!ok) break;
-                    fence_proxy_async();
-                    const uint32_t kv = ka + (k & 1) * segs * SEG, ds = tm + (k & 1) * 64;
-                    for (int s = 0; s < segs; s++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            umma_f16(ds, sw128_desc(qa + s * SEG + e * 32, 16), sw128_desc(kv + s * SEG + e * 32, 16), is, s + e != 0);
-                    umma_done(&y.sfull[k & 1]);
-                    if (pending) ok = values(k - 1, first), first = false;
-                    pending = true;
-                    if (i == r.tiles - 1) {      // the run's last tile: its values before the next run's queries can come
-                        if (ok) ok = values(k, i == 0);
-                        pending = false, first = true;
+                    const int buf = k & 1;
+                    if (!by_map(r, i)) {     // passed in step all the same: a phase is told from the one before last only
+                        ok = __all_sync(0xffffffffu, wait_free(k, pieces));
+                        continue;
+                    }
+                    int64_t row = -1;
+                    if (lane < boxes) row = kv_row(a.c, r.b, (r.u + i) * LT + lane * a.box);
+                    const bool dead = lane < boxes && row < 0;
+                    const int y0 = dead ? (int)(a.c.n_pages << a.c.pt_log2) : (int)row;      // past the last row: zeros
+                    const uint32_t no_rows = __ballot_sync(0xffffffffu, dead);
+                    for (int j = 0; ok && j <= pieces; j++) {
+                        ok = __all_sync(0xffffffffu, wait_free(k, j));
+                        if (!ok) break;
+                        if (j == pieces && no_rows && lane == 0)     // the buffer's last tile has been read: new marks
+                            for (int p = 0; p < LT; p++)
+                                if (no_rows >> (p / a.box) & 1) y.dead[buf][p >> 5] |= 1u << (p & 31);
+                        if (j == pieces && lane == 0) mbar_expect_tx(&y.full[buf], segs * SEG);
+                        __syncwarp();
+                        if (lane < boxes)
+                            for (int s = 2 * j; s < min(2 * j + 2, segs); s++)
+                                map_load(kvb + buf * segs * SEG + s * SEG + lane * a.box * 128, &map, s * 64, y0, &y.full[buf]);
                     }
                 }
         }
-        __syncwarp();
+    } else if (warp >= LD_WARP0) {
+        const int lt = tid - 32 * LD_WARP0;
+        TileRows<CACHE> rows;
+        RawRows raws;
+        bool ok = true, up = false, waited = false;      // up: all of them give up, at a barrier
+        int k = 0;
+        while (!up && walk.next(r)) {
+            for (int i = 0; i < r.tiles; i++, k++) {
+                const int buf = k & 1;
+                if (by_map(r, i)) {
+                    ok = wait_free(k, pieces) && ok;     // in step with the buffers
+                } else {
+                    const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
+                    rows.find(a, r, i, lt);
+                    if constexpr (CACHE == Q8) raws.fetch(a, rows.row[0], segs, lt);
+                    for (int j = 0; j <= pieces; j++) {
+                        ok = wait_free(k, j) && ok;
+                        if (!ok) break;
+                        if constexpr (CACHE == Q8) {
+#pragma unroll
+                            for (int s = 0; s < 9; s++)
+                                if (s >> 1 == j && s < segs) expand16(dst + s * SEG, lt >> 2, lt & 3, raws.code[s], raws.d[s]);
+                        } else {
+                            const int c8 = lt & 7, tail = j == pieces ? a.dr / 8 : 8;
+#pragma unroll
+                            for (int n = 0; n < 2; n++) {
+                                const int rw = (lt >> 3) + 32 * n;
+                                const bool on = rows.row[n] >= 0 && c8 < tail;
+                                const uint8_t *src = static_cast<const uint8_t *>(a.c.k) + (on ? rows.row[n] * a.c.hd * 2 + j * 256 + c8 * 16 : 0);
+                                const uint32_t at = dst + 2 * j * SEG + rw * 128 + ((c8 ^ (rw & 7)) << 4);
+                                cp16(at, src, on);
+                                if (j < pieces) cp16(at + SEG, src + (on ? 128 : 0), on);
+                            }
+                        }
+                    }
+                    rows.mark(y, buf, lt);
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_proxy_async();
+                    up = loaders_any(!ok);
+                    if (up) break;
+                    if (lt == 0) arrive(&y.full[buf]);
+                }
+                if (i == 0) {     // the queries, once the last run's products are done
+                    if (!waited) pdl_wait(), waited = true;
+                    if (k >= 1) ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err) && ok;
+                    up = loaders_any(!ok);
+                    if (up) break;
+                    load_q<OT>(a, y, smem_u32(qb), segs, r, h0, nh, lt);
+                    fence_proxy_async();
+                    arrive(&y.qfull);
+                }
+            }
+        }
+        if (!waited) pdl_wait();
+    } else if (warp == MMA_WARP) {
+        // ---- products: the whole warp walks and waits, one lane issues. Descriptors are stepped by constants: the unit
+        // takes a product every 32 cycles, fewer than a thread needs to build two descriptors from scratch.
+        const uint32_t fmt = OT == BF16 ? (1u << 7) | (1u << 10) : 0u;
+        const uint32_t is = (1u << 4) | fmt | ((uint32_t)(LT >> 3) << 17) | ((uint32_t)(LH >> 4) << 24);
+        const uint32_t ip = (1u << 4) | fmt | (1u << 15) | ((uint32_t)(cols >> 3) << 17) | (8u << 24);
+        const uint32_t q_lo = desc_lo(smem_u32(qb), 16), p_lo = desc_lo(smem_u32(pb), 16);
+        const uint32_t k_lo[2] = {desc_lo(smem_u32(kvb), 16), desc_lo(smem_u32(kvb) + segs * SEG, 16)};
+        const uint32_t v_lo[2] = {desc_lo(smem_u32(kvb), SEG), desc_lo(smem_u32(kvb) + segs * SEG, SEG)};
+        constexpr uint32_t SEG16 = SEG >> 4, STEP = 32 >> 4, VSTEP = 2048 >> 4;
+        const bool lead = elected();
+        int k = 0, run = 0;
+        bool ok = true;
+        auto scores = [&](int kt) {      // S = Q K^T of tile kt
+            if (lead) {
+                const uint32_t d = tm + (kt & 1) * 64;
+                uint32_t da = q_lo, db = k_lo[kt & 1];
+                umma_f16<false>(d, da, db, is);
+#pragma unroll
+                for (int e = 1; e < 4; e++) umma_f16<true>(d, da + e * STEP, db + e * STEP, is);
+#pragma unroll 2
+                for (int s = 1; s < segs; s++) {
+                    da += SEG16, db += SEG16;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) umma_f16<true>(d, da + e * STEP, db + e * STEP, is);
+                }
+                umma_done(&y.sfull[kt & 1]);
+            }
+            __syncwarp();
+        };
+        auto values = [&](int kt, bool first) {      // O^T += V^T P^T of tile kt, freeing its pieces one by one
+            if (lead) {
+                uint32_t da = v_lo[kt & 1], d = tm_o;
+                const uint32_t rest = k_lo[kt & 1] + (segs - 1) * SEG16;
+                for (int blk = 0; blk < pieces; blk++, d += cols, da += 2 * SEG16) {
+                    if (first) umma_f16<false>(d, da, p_lo, ip);
+                    else umma_f16<true>(d, da, p_lo, ip);
+#pragma unroll
+                    for (int e = 1; e < LT / 16; e++) umma_f16<true>(d, da + e * VSTEP, p_lo + e * STEP, ip);
+                    if constexpr (NTP == 2)
+#pragma unroll
+                        for (int e = 0; e < LT / 16; e++) umma_f16<true>(d, da + e * VSTEP, rest + e * STEP, ip);
+                    umma_done(blk < pieces - 1 ? &y.freed[kt & 1][blk] : &y.done[kt & 1]);
+                }
+            }
+            __syncwarp();
+        };
+        // Within a run the next product is the next tile's scores or the last tile's values, whichever has its operands
+        // first: values free a buffer, scores keep the softmax busy while values run.
+        while (ok && walk.next(r)) {
+            int s = 0, v = 0;
+            ok = __all_sync(0xffffffffu, core_wait(y, &y.qfull, run & 1, a.err));
+            run++;
+            while (ok && v < r.tiles) {
+                const int ks = k + s, kv = k + v;
+                bool do_s = s < r.tiles && s - v < 2;
+                const bool can_v = v < s;
+                if (do_s && can_v) {
+                    ok = core_wait2(y, &y.full[ks & 1], (ks >> 1) & 1, &y.pready, kv & 1, a.err, do_s);
+                    do_s = __shfl_sync(0xffffffffu, do_s, 0);      // one choice for the warp
+                }
+                // every lane sees the phase of the choice
+                if (ok) ok = do_s ? core_wait(y, &y.full[ks & 1], (ks >> 1) & 1, a.err) : core_wait(y, &y.pready, kv & 1, a.err);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_after();
+                if (do_s) scores(ks), s++;
+                else values(kv, v == 0), v++;
+            }
+            k += r.tiles;
+        }
     } else {
-        // ---- softmax: thread = head for S (rows 16 w .. 16 w + 15 of a 64-row product lie in lanes 32 w .. 32 w + 15),
-        // dim for O^T
-        const int head = 16 * warp + (lane & 15);
-        const bool mine = lane < 16;
+        // ---- softmax. The 64 rows (heads) of S lie in lanes 0-15 of the four warps' quarters of tensor memory; read 16
+        // lanes by 256 bits, lane (g, t) gets heads 16 w + g and + 8, columns 8 j + 2 t and + 1. O^T: a lane a dim.
+        const int g = lane >> 2, t = lane & 3, hd[2] = {16 * warp + g, 16 * warp + g + 8};
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        // where this lane's rows of 8 x 8 blocks go in P: lanes 0-7 block j, rows g; 8-15 rows g + 8; 16-31 block j + 1
+        const int prow = 16 * warp + (lane & 15), pcol = lane >> 4;
         int k = 0;
         bool ok = true, up = false;
         while (!up && walk.next(r)) {
-            float ref = -kv_inf(), sum = 0.0f, fac = 0.0f;
+            float ref[2] = {-kv_inf(), -kv_inf()}, sum[2] = {}, fac[2] = {};
             for (int i = 0; i < r.tiles; i++, k++) {
                 const int buf = k & 1;
                 // a wait that fails shows at the next barrier of the four warps, where all of them give up
                 ok = core_wait(y, &y.sfull[buf], (k >> 1) & 1, a.err) && ok;
-                if (softmax_any(!ok)) { up = true; break; }
+                __syncwarp();
                 tc_after();
-                if (i == 0) fac = y.fac[head];
-                float v[64];
-                tm_ld32(tm + lanes + buf * 64, v);
-                tm_ld32(tm + lanes + buf * 64 + 32, v + 32);
-                tm_wait_ld();
+                if (i == 0) fac[0] = y.fac[hd[0]], fac[1] = y.fac[hd[1]];
+                float v[8][4];
+                tm_ld_rows16(tm + lanes + buf * 64, v);
                 const int live = r.n - (r.u + i) * LT;
                 const uint32_t d0 = y.dead[buf][0], d1 = y.dead[buf][1];
-                float mx = -kv_inf();
+                float mx[2] = {-kv_inf(), -kv_inf()}, fade[2] = {1.0f, 1.0f};
+                const bool whole_tile = live >= LT && !(d0 | d1);
 #pragma unroll
-                for (int j = 0; j < 64; j++) v[j] = __fmul_rn(v[j], fac);
-                if (live < LT || (d0 | d1)) {
+                for (int j = 0; j < 8; j++)
 #pragma unroll
-                    for (int j = 0; j < 64; j++) {
-                        if (j >= live) v[j] = -kv_inf();
-                        else if ((j < 32 ? d0 >> j : d1 >> (j - 32)) & 1) v[j] = kv_nan();
+                    for (int e = 0; e < 4; e++) {
+                        float x = __fmul_rn(v[j][e], fac[e >> 1]);
+                        if (!whole_tile) {
+                            const int c = 8 * j + 2 * t + (e & 1);
+                            if (c >= live) x = -kv_inf();
+                            else if ((c < 32 ? d0 >> c : d1 >> (c - 32)) & 1) x = kv_nan();
+                        }
+                        v[j][e] = x;
+                        mx[e >> 1] = fmaxf(mx[e >> 1], x);
+                    }
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                    mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+                    if (mx[e] > ref[e] + REF_SLACK || ref[e] == -kv_inf()) {
+                        fade[e] = exp2_fast(__fsub_rn(ref[e], mx[e] == -kv_inf() ? 0.0f : mx[e]));
+                        ref[e] = mx[e];
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 64; j++) mx = fmaxf(mx, v[j]);
-                float fade = 1.0f;
-                if (mx > ref + REF_SLACK || ref == -kv_inf()) {
-                    fade = exp2_fast(__fsub_rn(ref, mx == -kv_inf() ? 0.0f : mx));
-                    ref = mx;
-                }
-                if (softmax_any(mine && i > 0 && fade != 1.0f)) {
-                    if (mine) y.alpha[head] = fade;
+                const bool rescale = i > 0 && (fade[0] != 1.0f || fade[1] != 1.0f);
+                if (softmax_any(!ok || rescale)) {
+                    if (softmax_any(!ok)) { up = true; break; }
+                    if (t == 0) y.alpha[hd[0]] = fade[0], y.alpha[hd[1]] = fade[1];
                     ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err) && ok;
                     if (softmax_any(!ok)) { up = true; break; }
                     tc_after();
@@ -518,28 +655,30 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                     }
                     tm_wait_st();
                 }
-                const float shift = __fsub_rn(ref == -kv_inf() ? 0.0f : ref, POFF);
-                sum = __fmul_rn(sum, fade);
-                float part[4] = {};
 #pragma unroll
-                for (int j = 0; j < 64; j++) {
-                    v[j] = exp2_fast(__fsub_rn(v[j], shift));
-                    part[j & 3] = __fadd_rn(part[j & 3], v[j]);
-                }
-                sum = __fadd_rn(sum, __fadd_rn(__fadd_rn(part[0], part[1]), __fadd_rn(part[2], part[3])));
+                for (int e = 0; e < 2; e++) sum[e] = __fmul_rn(sum[e], fade[e]);
+                const float shift[2] = {__fsub_rn(ref[0] == -kv_inf() ? 0.0f : ref[0], POFF), __fsub_rn(ref[1] == -kv_inf() ? 0.0f : ref[1], POFF)};
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[j][e] = exp2_fast(__fsub_rn(v[j][e], shift[e >> 1]));
+                        sum[e >> 1] = __fadd_rn(sum[e >> 1], v[j][e]);
+                    }
                 // P's buffer is free once the previous values' product is done
                 if (k >= 1) ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err) && ok;
-                if (mine && head < cols) {
-                    const uint32_t p0 = smem_u32(pb) + head * 128, p1 = smem_u32(kvb) + buf * segs * SEG + (segs - 1) * SEG + head * 128;
+                __syncwarp();
+                if (16 * warp < cols) {
+                    const uint32_t p0 = smem_u32(pb) + prow * 128, p1 = smem_u32(kvb) + buf * segs * SEG + (segs - 1) * SEG + prow * 128;
 #pragma unroll
-                    for (int c = 0; c < 8; c++)
+                    for (int j = 0; j < 8; j += 2)
 #pragma unroll
                         for (int x = 0; x < NTP; x++) {
-                            uint32_t o[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[e] = take_pair<OT>(v[8 * c + 2 * e], v[8 * c + 2 * e + 1]);
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((x == 0 ? p0 : p1) + ((c ^ (head & 7)) << 4)),
-                                         "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3])
+                            const uint32_t m0 = take_pair<OT>(v[j][0], v[j][1]), m1 = take_pair<OT>(v[j][2], v[j][3]);
+                            const uint32_t m2 = take_pair<OT>(v[j + 1][0], v[j + 1][1]), m3 = take_pair<OT>(v[j + 1][2], v[j + 1][3]);
+                            asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                                             (x == 0 ? p0 : p1) + (((j + pcol) ^ (prow & 7)) << 4)),
+                                         "r"(m0), "r"(m1), "r"(m2), "r"(m3)
                                          : "memory");
                         }
                 }
@@ -566,9 +705,13 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                 for (int j = 0; j < 16; j++)
                     if (hc + j < nh) o0[(int64_t)(hc + j) * pitch + d] = o[j];
             }
-            if (mine && head < nh) {
-                if (whole) o0[(int64_t)head * W + a.R] = ref, o0[(int64_t)head * W + a.R + 1] = sum;
-                else a.ml[piece * a.hp + head] = make_float2(ref, sum);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                sum[e] = __fadd_rn(sum[e], __shfl_xor_sync(0xffffffffu, sum[e], 1));
+                sum[e] = __fadd_rn(sum[e], __shfl_xor_sync(0xffffffffu, sum[e], 2));
+                if (t != 0 || hd[e] >= nh) continue;
+                if (whole) o0[(int64_t)hd[e] * W + a.R] = ref[e], o0[(int64_t)hd[e] * W + a.R + 1] = sum[e];
+                else a.ml[piece * a.hp + hd[e]] = make_float2(ref[e], sum[e]);
             }
             if (tid == 0 && r.u == 0) {
                 const int64_t upto = walk.cur - r.tiles + r.nu;
@@ -577,8 +720,11 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
             tc_before();
         }
     }
+    // after a failed wait loads may still be on their way to shared memory: time to land
+    if (*reinterpret_cast<volatile uint32_t *>(&y.failed))
+        for (int i = 0; i < 200; i++) __nanosleep(1000);
     __syncthreads();
-    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u));
+    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u));
 }
 
 // ------------------------------------------------------------------------------------------- expand
@@ -733,8 +879,32 @@ Plan plan_of(const hxb_kv_cache *c, int H, int R) {
     return p;
 }
 
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The pool as rows of R + dr values, in boxes of 64 values by 16 to 64 rows of a page; false where pages are smaller (36
+// loads a tile already cost as much as the copies of the loading warps) or rows do not fit a coordinate.
+bool row_map(const hxb_kv_cache *c, CUtensorMap *map, int *box) {
+    static const EncodeFn encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess)
+            cudaGetLastError(), fn = nullptr;
+        return reinterpret_cast<EncodeFn>(fn);
+    }();
+    const int64_t rows = c->n_pages * c->page_tokens;
+    if (!encode || c->dtype == Q8 || c->page_tokens < 16 || rows < LT || rows > 0x7fffffff) return false;
+    *box = std::min(c->page_tokens, LT);
+    const cuuint64_t dims[2] = {(cuuint64_t)c->head_dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)c->head_dim * 2};
+    const cuuint32_t boxd[2] = {64, (cuuint32_t)*box}, step[2] = {1, 1};
+    return encode(map, c->dtype == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, c->k, dims, strides, boxd,
+                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int CACHE, int T>
-cudaError_t launch(const LatentArgs &a, const Plan &p, cudaStream_t s) {
+cudaError_t launch(const LatentArgs &a, const CUtensorMap &map, const Plan &p, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(k_latent_core<CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(k_latent_expand<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ExpandShared));
@@ -742,7 +912,7 @@ cudaError_t launch(const LatentArgs &a, const Plan &p, cudaStream_t s) {
     const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS), B = a.c.n_seqs;
     e = launch_pdl(false, k_latent_absorb<T>, dim3(a.H * nc, (B + AB_ROWS - 1) / AB_ROWS), dim3(32 * AB_WARPS), 0, s, a);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a);
+    e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a, map);
     if (e != cudaSuccess) return e;
     return launch_pdl(true, k_latent_expand<T>, dim3(a.H, (B + EX_ROWS - 1) / EX_ROWS), dim3(32 * EX_WARPS), sizeof(ExpandShared), s, a);
 }
@@ -792,9 +962,11 @@ extern "C" HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_
     a.H = n_heads, a.R = rank, a.dr = dr, a.dn = nope, a.dv = v_dim, a.passes = p.passes, a.hp = p.hp;
     a.sc2 = scale * 1.44269504088896f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    CUtensorMap map = {};
+    if (!row_map(c, &map, &a.box)) a.box = 0;
     cudaError_t e;
-    if (c->dtype == Q8) e = dtype == F16 ? launch<Q8, F16>(a, p, s) : launch<Q8, BF16>(a, p, s);
-    else e = dtype == F16 ? launch<F16, F16>(a, p, s) : launch<BF16, BF16>(a, p, s);
+    if (c->dtype == Q8) e = dtype == F16 ? launch<Q8, F16>(a, map, p, s) : launch<Q8, BF16>(a, map, p, s);
+    else e = dtype == F16 ? launch<F16, F16>(a, map, p, s) : launch<BF16, BF16>(a, map, p, s);
     if (e != cudaSuccess) return attn_fail(HXB_E_DEVICE, "%s: %s", who, cudaGetErrorString(e));
     return HXB_OK;
 }

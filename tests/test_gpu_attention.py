@@ -461,6 +461,36 @@ def test_latent_attention_many_sequences(gpu):
     check_latent([int(v) for v in torch.randint(0, 30, (331,), generator=g)], 8, 128, 64, 16, 16, 8, "bf16", "bf16")
 
 
+@pytest.mark.parametrize("cache,x,pt", [("bf16", "bf16", 64), ("f16", "f16", 16), ("bf16", "bf16", 128), ("bf16", "bf16", 8), ("q8", "bf16", 32)])
+@pytest.mark.parametrize("H,R", [(64, 512), (16, 512), (100, 512), (24, 256), (8, 128)])
+def test_latent_attention_many_tiles_a_cta(gpu, cache, x, pt, H, R):
+    """Long rows of tiles in every CTA, runs that end inside and at the end of a tile, in any order: the buffers turn over
+    many times. Pages are drawn from a small pool, so sequences share them."""
+    g = gen(23)
+    lens = [6000, 64, 640, 1, 5993, 0, 128, 4097, 63, 6001, 3000, 2000, 64 * 90, 17, 5000, 6003] + [64 * i + i % 3 - 1 for i in range(1, 60)]
+    W, pages = R + 64, 12000 // pt
+    if cache == "q8":
+        cp, cs = torch.randint(-127, 128, (pages, 1, pt, W), generator=g).to(torch.int8), torch.rand((pages, 1, pt, W // 64), generator=g) / 64
+        val = dequant(cp.reshape(-1, W), cs.reshape(-1, W // 64)).view(pages, pt, W)
+    else:
+        cp, cs = randn(g, pages, 1, pt, W, dtype=F[x]), None
+        val = cp.double()[:, 0]
+    table = torch.randint(0, pages, (len(lens), -(-6003 // pt)), generator=g, dtype=torch.int32)
+    q, w = randn(g, len(lens), H, 64 + 64, dtype=F[x]), randn(g, H, 128, R, dtype=F[x], scale=R ** -0.5)
+    out = hb.latent_attention(q.cuda(), w.cuda(), cp.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scale=0.09, c_scale=cu(cs))
+    val, wd, qd, td = val.cuda(), w.cuda().double(), q.cuda().double(), table.cuda().long()
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        c = val[td[b, :-(-n // pt)]].reshape(-1, W)[:n]
+        qa = torch.cat([torch.einsum("hd,hdr->hr", qd[b, :, :64], wd[:, :64]), qd[b, :, 64:]], -1)
+        p = torch.softmax((qa @ c.T) * 0.09, -1)
+        want = torch.einsum("hr,hvr->hv", p @ c[:, :R], wd[:, 64:])
+        err = (out[b].double() - want).norm() / want.norm()
+        assert err <= 4 * half_step(torch.bfloat16 if x == "bf16" else F[x]), (b, n, err)   # qa, the weights, o's rest, out
+
+
 def test_latent_attention_bad_pages_strides_and_scratch(gpu):
     g = gen(22)
     pools, table, (rows,) = filled(g, [100, 100, 100], 1, 16, 576, "bf16", sides=1)
