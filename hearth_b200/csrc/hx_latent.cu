@@ -33,7 +33,6 @@
 #include "hx_attn.cuh"
 
 #include <algorithm>
-#include <cuda.h>
 
 namespace hx {
 namespace {
@@ -41,9 +40,9 @@ namespace {
 constexpr int LT = 64;                  // positions a tile
 constexpr int LH = 64;                  // heads a CTA (rows of S)
 constexpr int SEG = LT * 128;           // 64 dims of 64 rows: a 128-byte swizzled block column
-constexpr int LD_WARPS = 8, LD_THREADS = 32 * LD_WARPS;
-constexpr int CORE_WARPS = 6 + LD_WARPS, CORE_THREADS = 32 * CORE_WARPS;
-constexpr int MMA_WARP = 4, MAP_WARP = 5, LD_WARP0 = 6;
+constexpr int LD_WARPS = 4, LD_THREADS = 32 * LD_WARPS;      // loading warps a tile buffer
+constexpr int SCORE_WARP = 4, VALUE_WARP = 5, LD_WARP0 = 6;
+constexpr int CORE_WARPS = LD_WARP0 + 2 * LD_WARPS, CORE_THREADS = 32 * CORE_WARPS;
 constexpr float REF_SLACK = 7.0f;
 
 struct LatentArgs {
@@ -59,7 +58,6 @@ struct LatentArgs {
     int64_t qs, qh, os, oh;
     int H, R, dr, dn, dv, passes, hp;   // hp heads a pass
     float sc2;
-    int box;                // rows of a tensor-map load; 0: rows by 16-byte copies only
 };
 
 // ------------------------------------------------------------------------------------------- absorb
@@ -74,44 +72,59 @@ __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_co
     const int r0 = ((blockIdx.x - h * nc) * AB_WARPS + warp) * 64, b0 = blockIdx.y * AB_ROWS, rows = min(AB_ROWS, a.c.n_seqs - b0);
     pdl_trigger();
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.err = 0;
-    const uint16_t *q = static_cast<const uint16_t *>(a.q);
-    for (int i = threadIdx.x; i < AB_ROWS * a.dn; i += 32 * AB_WARPS) {
-        const int r = i / a.dn, d = i - r * a.dn;
-        qsm[r][d] = r < rows ? q[(b0 + r) * a.qs + h * a.qh + d] : 0;
-    }
+    // weights of the first 64 dims on their way before the queries are staged
+    const uint16_t *w = static_cast<const uint16_t *>(a.w) + (int64_t)h * (a.dn + a.dv) * a.R + r0 + 8 * g;
+    uint4 pre[4][4];
+    auto fetch = [&](uint4 v[4], int d0) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            v[k] = r0 < a.R && d0 < a.dn ? __ldg(reinterpret_cast<const uint4 *>(w + (int64_t)(d0 + 2 * t + (k & 1) + 8 * (k >> 1)) * a.R)) : make_uint4(0, 0, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; i++) fetch(pre[i], 16 * i);
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + h * a.qh;
+#pragma unroll 4
+    for (int r = warp; r < AB_ROWS; r += AB_WARPS)
+#pragma unroll
+        for (int d = 0; d < 256; d += 32)
+            if (d + lane < a.dn) qsm[r][d + lane] = r < rows ? q[(b0 + r) * a.qs + d + lane] : 0;
     const int row = a.R + a.dr;
-    if (r0 == 0)
-        for (int i = lane; i < rows * a.dr; i += 32) {
-            const int r = i / a.dr, d = i - r * a.dr;
-            a.qa[((int64_t)(b0 + r) * a.H + h) * row + a.R + d] = io_load(a.q, T, (b0 + r) * a.qs + h * a.qh + a.dn + d);
-        }
+    if (blockIdx.x == h * nc)      // the rotated parts, with the head's first CTA
+#pragma unroll 4
+        for (int r = warp; r < rows; r += AB_WARPS)
+#pragma unroll
+            for (int d = 0; d < 64; d += 32)
+                if (d + lane < a.dr) {
+                    const uint16_t x = q[(b0 + r) * a.qs + a.dn + d + lane];
+                    a.qa[((int64_t)(b0 + r) * a.H + h) * row + a.R + d + lane] = T == F16 ? f16_to_f32_hw(x) : bf16_to_f32(x);
+                }
     __syncthreads();
     if (r0 >= a.R) return;
     float acc[2][8][4] = {};
-    const uint16_t *w = static_cast<const uint16_t *>(a.w) + (int64_t)h * (a.dn + a.dv) * a.R + r0 + 8 * g;
-#pragma unroll 2
-    for (int d0 = 0; d0 < a.dn; d0 += 16) {
-        uint32_t v[4][4];
+    for (int d0 = 0; d0 < a.dn; d0 += 64)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(w + (int64_t)(d0 + 2 * t + (k & 1) + 8 * (k >> 1)) * a.R));
-            v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+        for (int s = 0; s < 4; s++) {
+            const int d = d0 + 16 * s;
+            if (d >= a.dn) break;
+            uint32_t v[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k][0] = pre[s][k].x, v[k][1] = pre[s][k].y, v[k][2] = pre[s][k].z, v[k][3] = pre[s][k].w;
+            fetch(pre[s], d + 64);
+            uint32_t f[2][4];
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    f[m][k] = *reinterpret_cast<const uint32_t *>(&qsm[16 * m + g + 8 * (k & 1)][d + 2 * t + 8 * (k >> 1)]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t p0 = __byte_perm(v[0][i], v[1][i], e ? 0x7632 : 0x5410), p1 = __byte_perm(v[2][i], v[3][i], e ? 0x7632 : 0x5410);
+#pragma unroll
+                    for (int m = 0; m < 2; m++) mma16<T>(acc[m][2 * i + e], f[m][0], f[m][1], f[m][2], f[m][3], p0, p1);
+                }
         }
-        uint32_t f[2][4];
-#pragma unroll
-        for (int m = 0; m < 2; m++)
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                f[m][k] = *reinterpret_cast<const uint32_t *>(&qsm[16 * m + g + 8 * (k & 1)][d0 + 2 * t + 8 * (k >> 1)]);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const uint32_t p0 = __byte_perm(v[0][i], v[1][i], e ? 0x7632 : 0x5410), p1 = __byte_perm(v[2][i], v[3][i], e ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int m = 0; m < 2; m++) mma16<T>(acc[m][2 * i + e], f[m][0], f[m][1], f[m][2], f[m][3], p0, p1);
-            }
-    }
     // column n of product i is latent dim 8 n + i
 #pragma unroll
     for (int m = 0; m < 2; m++)
@@ -131,7 +144,7 @@ __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_co
 // ------------------------------------------------------------------------------------------- core
 
 struct CoreShared {
-    uint64_t full[2], freed[2][3], sfull[2], done[2], pready, qfull;   // freed: 128-dim pieces of a buffer, before done
+    uint64_t full[2], freed[2], sfull[2], sfree[2], done[2], pready;   // freed: the first half of a buffer's dims, before done
     int64_t scan[CORE_WARPS];
     uint32_t tmem, failed;
     uint32_t dead[2][2];     // positions of a tile without a row
@@ -149,6 +162,23 @@ __device__ __forceinline__ void umma_f16(uint32_t d, uint32_t da, uint32_t db, u
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(da), "r"(db), "n"(DESC_HI), "r"(idesc), "n"(ACC ? 1 : 0)
+        : "memory");
+}
+// A pair of products with one first operand: the first keeps it in the unit, the second takes it from there.
+template <bool ACC>
+__device__ __forceinline__ void umma_f16_keep(uint32_t d, uint32_t da, uint32_t db, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16.collector::a::fill [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(da), "r"(db), "n"(DESC_HI), "r"(idesc), "n"(ACC ? 1 : 0)
+        : "memory");
+}
+template <bool ACC>
+__device__ __forceinline__ void umma_f16_kept(uint32_t d, uint32_t da, uint32_t db, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16.collector::a::lastuse [%0], a, b, %4, p;\n\t}" ::"r"(d),
         "r"(da), "r"(db), "n"(DESC_HI), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
 }
@@ -206,20 +236,9 @@ __device__ __forceinline__ bool any_of(bool x) {
     return r != 0;
 }
 __device__ __forceinline__ bool softmax_any(bool x) { return any_of<1, 128>(x); }
-__device__ __forceinline__ bool loaders_any(bool x) { return any_of<2, LD_THREADS>(x); }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool on) {   // zeros when off
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {   // without suspending the thread
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
 }
 
 // A wait that ends: on the phase, when another role has given up, or at the spin limit (the error word, so
@@ -227,18 +246,6 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {   //
 __device__ __forceinline__ bool core_wait(CoreShared &y, uint64_t *bar, uint32_t parity, int *err) {
     for (uint32_t i = 0; i < kSpinLimit; i++) {
         if (mbar_try_wait(bar, parity)) return true;
-        if (*reinterpret_cast<volatile uint32_t *>(&y.failed)) return false;
-    }
-    *reinterpret_cast<volatile uint32_t *>(&y.failed) = 1;
-    set_error(err, DEV_E_WAIT_TIMEOUT);
-    return false;
-}
-
-// The first of two waits (null: not asked for) whose phase is over, a before b; first_is_a says which.
-__device__ __forceinline__ bool core_wait2(CoreShared &y, uint64_t *a, uint32_t pa, uint64_t *b, uint32_t pb, int *err, bool &first_is_a) {
-    for (uint32_t i = 0; i < kSpinLimit; i++) {
-        if (a && mbar_test(a, pa)) return first_is_a = true, true;
-        if (b && mbar_test(b, pb)) return first_is_a = false, true;
         if (*reinterpret_cast<volatile uint32_t *>(&y.failed)) return false;
     }
     *reinterpret_cast<volatile uint32_t *>(&y.failed) = 1;
@@ -265,44 +272,41 @@ struct Walk {
     }
 };
 
-// The loading threads' view of a tile: the rows each of them fetches from, looked up one tile ahead. 16-bit rows: eight
-// lanes a 128-byte block row, 32 rows at once; Q8: four lanes a row's 64 codes.
+// A loading thread's rows of a tile. 16-bit rows: eight lanes a 128-byte block row, 16 rows at once; Q8: two lanes a row.
 template <int CACHE>
 struct TileRows {
-    static constexpr int N = CACHE == Q8 ? 1 : 2;
+    static constexpr int N = CACHE == Q8 ? 1 : 4;
     int64_t row[N];
     uint32_t dead;      // positions in range that have no row
+    static __device__ __forceinline__ int at(int lt, int k) { return CACHE == Q8 ? lt >> 1 : (lt >> 3) + 16 * k; }
     __device__ __forceinline__ void find(const LatentArgs &a, const Run &r, int tile, int lt) {
         dead = 0;
 #pragma unroll
         for (int k = 0; k < N; k++) {
-            const int pos = (r.u + tile) * LT + (CACHE == Q8 ? lt >> 2 : (lt >> 3) + 32 * k);
+            const int pos = (r.u + tile) * LT + at(lt, k);
             row[k] = pos < r.n ? kv_row(a.c, r.b, pos) : -1;
             if (pos < r.n && row[k] < 0) dead |= 1u << k;
         }
     }
     // marks them for the softmax (bit position of the tile)
     __device__ __forceinline__ void mark(CoreShared &y, int buf, int lt) const {
-        if (!dead) return;
+        if (!dead || (lt & (CACHE == Q8 ? 1 : 7))) return;
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-            const int rw = CACHE == Q8 ? lt >> 2 : (lt >> 3) + 32 * k;
-            if ((dead >> k & 1) && (lt & (CACHE == Q8 ? 3 : 7)) == 0) atomicOr(&y.dead[buf][rw >> 5], 1u << (rw & 31));
-        }
+        for (int k = 0; k < N; k++)
+            if (dead >> k & 1) atomicOr(&y.dead[buf][at(lt, k) >> 5], 1u << (at(lt, k) & 31));
     }
 };
 
-// Raw Q8 rows of a tile, in registers while the buffer is still at work.
+// Raw Q8 codes of half a block column, and the scales: asked for a step ahead of their use.
 struct RawRows {
-    uint4 code[9];
-    float d[9];
-    __device__ __forceinline__ void fetch(const LatentArgs &a, int64_t row, int segs, int lt) {
-#pragma unroll
-        for (int s = 0; s < 9; s++) {
-            const bool on = row >= 0 && s < segs;
-            code[s] = on ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(a.c.k) + row * a.c.hd + s * 64) + (lt & 3)) : make_uint4(0, 0, 0, 0);
-            d[s] = on ? __ldg(a.c.ks + row * segs + s) : 0.0f;
-        }
+    uint4 code[2];
+    float d;
+    __device__ __forceinline__ void fetch(const LatentArgs &a, int64_t row, int s, int segs, int lt) {
+        const bool on = row >= 0 && s < segs;
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(a.c.k) + row * a.c.hd + s * 64) + 2 * (lt & 1);
+        code[0] = on ? __ldg(p) : make_uint4(0, 0, 0, 0);
+        code[1] = on ? __ldg(p + 1) : make_uint4(0, 0, 0, 0);
+        d = on ? __ldg(a.c.ks + row * segs + s) : 0.0f;
     }
 };
 // 16 codes times d as f16, into pieces 2 q and 2 q + 1 of a block row.
@@ -372,16 +376,8 @@ __device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint3
     }
 }
 
-// One box of the pool's rows: 64 values from column x on of rows y ..., 128-byte swizzled. x is a multiple of 64.
-__device__ __forceinline__ void map_load(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-
 template <int CACHE>
-__global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_constant__ LatentArgs a, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_constant__ LatentArgs a) {
     constexpr int OT = CACHE == BF16 ? BF16 : F16;
     constexpr int NTP = OT == BF16 ? 2 : 1;
     constexpr float POFF = OT == F16 ? 8.0f : 0.0f;
@@ -404,18 +400,18 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
     }
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&y.full[i], 1);
-            for (int j = 0; j < 3; j++) mbar_init(&y.freed[i][j], 1);
+            mbar_init(&y.full[i], LD_THREADS);
+            mbar_init(&y.freed[i], 1);
             mbar_init(&y.sfull[i], 1);
+            mbar_init(&y.sfree[i], 128);
             mbar_init(&y.done[i], 1);
             y.dead[i][0] = y.dead[i][1] = 0;
         }
         mbar_init(&y.pready, 128);
-        mbar_init(&y.qfull, LD_THREADS);
         y.failed = 0;
         fence_mbar_init();
     }
-    if (warp == MMA_WARP) {
+    if (warp == SCORE_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y.tmem)), "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -426,170 +422,143 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
     Walk walk(a, b0, before, cur, end);
     Run r;
 
-    // A tile whose 64 positions are all in range comes by tensor map where the pages allow it; a sequence's last rows
-    // (past them a slot may hold NaN, and 0 x NaN would reach every sum), small pages and Q8 rows go through the
-    // loading warps. Either way a buffer's pieces are refilled as the products of the tile before last free them.
-    const int pieces = a.R / 128;
-    auto by_map = [&](const Run &r, int i) { return CACHE != Q8 && a.box && r.n - (r.u + i) * LT >= LT; };
-    auto wait_free = [&](int k, int j) {     // piece j of tile k's buffer (pieces: the rotated part)
-        return k < 2 || core_wait(y, j < pieces - 1 ? &y.freed[k & 1][j] : &y.done[k & 1], ((k >> 1) - 1) & 1, a.err);
-    };
-    if (warp == MAP_WARP) {
-        // ---- tensor-map loads: lane i a box of rows
-        if constexpr (CACHE != Q8) {
-            const int boxes = a.box ? LT / a.box : 0;
-            int k = 0;
-            bool ok = true;
-            while (ok && walk.next(r))
-                for (int i = 0; ok && i < r.tiles; i++, k++) {
-                    const int buf = k & 1;
-                    if (!by_map(r, i)) {     // passed in step all the same: a phase is told from the one before last only
-                        ok = __all_sync(0xffffffffu, wait_free(k, pieces));
-                        continue;
-                    }
-                    int64_t row = -1;
-                    if (lane < boxes) row = kv_row(a.c, r.b, (r.u + i) * LT + lane * a.box);
-                    const bool dead = lane < boxes && row < 0;
-                    const int y0 = dead ? (int)(a.c.n_pages << a.c.pt_log2) : (int)row;      // past the last row: zeros
-                    const uint32_t no_rows = __ballot_sync(0xffffffffu, dead);
-                    for (int j = 0; ok && j <= pieces; j++) {
-                        ok = __all_sync(0xffffffffu, wait_free(k, j));
-                        if (!ok) break;
-                        if (j == pieces && no_rows && lane == 0)     // the buffer's last tile has been read: new marks
-                            for (int p = 0; p < LT; p++)
-                                if (no_rows >> (p / a.box) & 1) y.dead[buf][p >> 5] |= 1u << (p & 31);
-                        if (j == pieces && lane == 0) mbar_expect_tx(&y.full[buf], segs * SEG);
-                        __syncwarp();
-                        if (lane < boxes)
-                            for (int s = 2 * j; s < min(2 * j + 2, segs); s++)
-                                map_load(kvb + buf * segs * SEG + s * SEG + lane * a.box * 128, &map, s * 64, y0, &y.full[buf]);
-                    }
-                }
-        }
-    } else if (warp >= LD_WARP0) {
-        const int lt = tid - 32 * LD_WARP0;
+    const int pieces = a.R / 128, half = (pieces + 1) / 2;      // blocks of 128 dims; those freed first
+    if (warp >= LD_WARP0) {
+        // ---- loading: the first four warps the even tiles, the others the odd ones
+        const int buf = (warp - LD_WARP0) / LD_WARPS, lt = tid - 32 * (LD_WARP0 + buf * LD_WARPS);
+        const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
         TileRows<CACHE> rows;
-        RawRows raws;
-        bool ok = true, up = false, waited = false;      // up: all of them give up, at a barrier
-        int k = 0;
-        while (!up && walk.next(r)) {
-            for (int i = 0; i < r.tiles; i++, k++) {
-                const int buf = k & 1;
-                if (by_map(r, i)) {
-                    ok = wait_free(k, pieces) && ok;     // in step with the buffers
+        auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, core_wait(y, bar, parity, a.err)); };
+        bool ok = true, waited = false;
+        int k0 = 0;      // tiles before this run
+        while (ok && walk.next(r)) {
+            for (int i = (k0 ^ buf) & 1; ok && i < r.tiles; i += 2) {
+                const int k = k0 + i;
+                rows.find(a, r, i, lt);
+                if constexpr (CACHE == Q8) {
+                    RawRows raw[5];
+#pragma unroll
+                    for (int s = 0; s < 5; s++) raw[s].fetch(a, rows.row[0], s, segs, lt);
+                    if (k >= 2) ok = wait(&y.freed[buf], ((k >> 1) - 1) & 1);
+                    if (!ok) break;
+                    bool all = k < 2;
+#pragma unroll
+                    for (int s = 0; s < 9; s++) {
+                        if (s < segs) {
+                            if (s >= 2 * half && !all) {
+                                ok = wait(&y.done[buf], ((k >> 1) - 1) & 1), all = true;
+                                if (!ok) break;
+                            }
+                            expand16(dst + s * SEG, lt >> 1, 2 * (lt & 1), raw[s % 5].code[0], raw[s % 5].d);
+                            expand16(dst + s * SEG, lt >> 1, 2 * (lt & 1) + 1, raw[s % 5].code[1], raw[s % 5].d);
+                        }
+                        if (s < 4) raw[s % 5].fetch(a, rows.row[0], s + 5, segs, lt);
+                    }
                 } else {
-                    const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
-                    rows.find(a, r, i, lt);
-                    if constexpr (CACHE == Q8) raws.fetch(a, rows.row[0], segs, lt);
-                    for (int j = 0; j <= pieces; j++) {
-                        ok = wait_free(k, j) && ok;
-                        if (!ok) break;
-                        if constexpr (CACHE == Q8) {
+                    const int c8 = lt & 7, tail = a.dr / 8;
+                    auto copy = [&](int s0, int s1) {
 #pragma unroll
-                            for (int s = 0; s < 9; s++)
-                                if (s >> 1 == j && s < segs) expand16(dst + s * SEG, lt >> 2, lt & 3, raws.code[s], raws.d[s]);
-                        } else {
-                            const int c8 = lt & 7, tail = j == pieces ? a.dr / 8 : 8;
-#pragma unroll
-                            for (int n = 0; n < 2; n++) {
-                                const int rw = (lt >> 3) + 32 * n;
-                                const bool on = rows.row[n] >= 0 && c8 < tail;
-                                const uint8_t *src = static_cast<const uint8_t *>(a.c.k) + (on ? rows.row[n] * a.c.hd * 2 + j * 256 + c8 * 16 : 0);
-                                const uint32_t at = dst + 2 * j * SEG + rw * 128 + ((c8 ^ (rw & 7)) << 4);
-                                cp16(at, src, on);
-                                if (j < pieces) cp16(at + SEG, src + (on ? 128 : 0), on);
+                        for (int n = 0; n < 4; n++) {
+                            const int rw = (lt >> 3) + 16 * n;
+                            const bool on = rows.row[n] >= 0;
+                            const uint8_t *src = static_cast<const uint8_t *>(a.c.k) + (on ? rows.row[n] * a.c.hd * 2 + c8 * 16 : 0);
+                            const uint32_t at = dst + rw * 128 + ((c8 ^ (rw & 7)) << 4);
+                            for (int s = s0; s < s1; s++) {
+                                const bool use = on && (s < segs - 1 || c8 < tail);
+                                cp16(at + s * SEG, use ? src + s * 128 : src, use);
                             }
                         }
-                    }
-                    rows.mark(y, buf, lt);
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    fence_proxy_async();
-                    up = loaders_any(!ok);
-                    if (up) break;
-                    if (lt == 0) arrive(&y.full[buf]);
+                    };
+                    if (k >= 2) ok = wait(&y.freed[buf], ((k >> 1) - 1) & 1);
+                    if (!ok) break;
+                    copy(0, 2 * half);
+                    if (k >= 2) ok = wait(&y.done[buf], ((k >> 1) - 1) & 1);
+                    if (!ok) break;
+                    copy(2 * half, segs);
                 }
-                if (i == 0) {     // the queries, once the last run's products are done
+                rows.mark(y, buf, lt);
+                if (i == 0) {     // the first tile's warps bring the queries, once the last run's products are done
                     if (!waited) pdl_wait(), waited = true;
-                    if (k >= 1) ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err) && ok;
-                    up = loaders_any(!ok);
-                    if (up) break;
+                    if (k >= 1) ok = wait(&y.done[buf ^ 1], ((k - 1) >> 1) & 1);
+                    if (!ok) break;
                     load_q<OT>(a, y, smem_u32(qb), segs, r, h0, nh, lt);
-                    fence_proxy_async();
-                    arrive(&y.qfull);
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async();
+                arrive(&y.full[buf]);
             }
+            k0 += r.tiles;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         if (!waited) pdl_wait();
-    } else if (warp == MMA_WARP) {
-        // ---- products: the whole warp walks and waits, one lane issues. Descriptors are stepped by constants: the unit
-        // takes a product every 32 cycles, fewer than a thread needs to build two descriptors from scratch.
+    } else if (warp >= SCORE_WARP) {
+        // ---- products: a warp each for scores and values walks and waits, one of its lanes issues. One warp for both spent as
+        // long between its products as on them: a wait costs some 100 cycles beside a busy shared memory.
         const uint32_t fmt = OT == BF16 ? (1u << 7) | (1u << 10) : 0u;
-        const uint32_t is = (1u << 4) | fmt | ((uint32_t)(LT >> 3) << 17) | ((uint32_t)(LH >> 4) << 24);
-        const uint32_t ip = (1u << 4) | fmt | (1u << 15) | ((uint32_t)(cols >> 3) << 17) | (8u << 24);
-        const uint32_t q_lo = desc_lo(smem_u32(qb), 16), p_lo = desc_lo(smem_u32(pb), 16);
-        const uint32_t k_lo[2] = {desc_lo(smem_u32(kvb), 16), desc_lo(smem_u32(kvb) + segs * SEG, 16)};
-        const uint32_t v_lo[2] = {desc_lo(smem_u32(kvb), SEG), desc_lo(smem_u32(kvb) + segs * SEG, SEG)};
         constexpr uint32_t SEG16 = SEG >> 4, STEP = 32 >> 4, VSTEP = 2048 >> 4;
         const bool lead = elected();
-        int k = 0, run = 0;
         bool ok = true;
-        auto scores = [&](int kt) {      // S = Q K^T of tile kt
-            if (lead) {
-                const uint32_t d = tm + (kt & 1) * 64;
-                uint32_t da = q_lo, db = k_lo[kt & 1];
-                umma_f16<false>(d, da, db, is);
+        int k = 0;
+        if (warp == SCORE_WARP) {      // S = Q K^T
+            const uint32_t is = (1u << 4) | fmt | ((uint32_t)(LT >> 3) << 17) | ((uint32_t)(LH >> 4) << 24);
+            const uint32_t q_lo = desc_lo(smem_u32(qb), 16), k0 = desc_lo(smem_u32(kvb), 16);
+            while (ok && walk.next(r))
+                for (int i = 0; ok && i < r.tiles; i++, k++) {
+                    if (k >= 2) ok = core_wait(y, &y.sfree[k & 1], ((k >> 1) - 1) & 1, a.err);
+                    ok = ok && core_wait(y, &y.full[k & 1], (k >> 1) & 1, a.err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_after();
+                    if (lead) {
+                        const uint32_t d = tm + (k & 1) * 64;
+                        uint32_t da = q_lo, db = k0 + (k & 1) * segs * SEG16;
+                        umma_f16<false>(d, da, db, is);
 #pragma unroll
-                for (int e = 1; e < 4; e++) umma_f16<true>(d, da + e * STEP, db + e * STEP, is);
+                        for (int e = 1; e < 4; e++) umma_f16<true>(d, da + e * STEP, db + e * STEP, is);
 #pragma unroll 2
-                for (int s = 1; s < segs; s++) {
-                    da += SEG16, db += SEG16;
+                        for (int s = 1; s < segs; s++) {
+                            da += SEG16, db += SEG16;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) umma_f16<true>(d, da + e * STEP, db + e * STEP, is);
+                            for (int e = 0; e < 4; e++) umma_f16<true>(d, da + e * STEP, db + e * STEP, is);
+                        }
+                        umma_done(&y.sfull[k & 1]);
+                    }
+                    __syncwarp();
                 }
-                umma_done(&y.sfull[kt & 1]);
-            }
-            __syncwarp();
-        };
-        auto values = [&](int kt, bool first) {      // O^T += V^T P^T of tile kt, freeing its pieces one by one
-            if (lead) {
-                uint32_t da = v_lo[kt & 1], d = tm_o;
-                const uint32_t rest = k_lo[kt & 1] + (segs - 1) * SEG16;
-                for (int blk = 0; blk < pieces; blk++, d += cols, da += 2 * SEG16) {
-                    if (first) umma_f16<false>(d, da, p_lo, ip);
-                    else umma_f16<true>(d, da, p_lo, ip);
+        } else {      // O^T += V^T P^T
+            const uint32_t ip = (1u << 4) | fmt | (1u << 15) | ((uint32_t)(cols >> 3) << 17) | (8u << 24);
+            const uint32_t p_lo = desc_lo(smem_u32(pb), 16), v0 = desc_lo(smem_u32(kvb), SEG), r0 = desc_lo(smem_u32(kvb), 16) + (segs - 1) * SEG16;
+            while (ok && walk.next(r))
+                for (int i = 0; ok && i < r.tiles; i++, k++) {
+                    ok = __all_sync(0xffffffffu, core_wait(y, &y.pready, k & 1, a.err));
+                    if (!ok) break;
+                    tc_after();
+                    if (lead) {
+                        uint32_t da = v0 + (k & 1) * segs * SEG16, d = tm_o;
+                        const uint32_t rest = r0 + (k & 1) * segs * SEG16;
+                        for (int blk = 0; blk < pieces; blk++, d += cols, da += 2 * SEG16) {
+                            if constexpr (NTP == 2) {
+                                if (i == 0) umma_f16_keep<false>(d, da, p_lo, ip);
+                                else umma_f16_keep<true>(d, da, p_lo, ip);
+                                umma_f16_kept<true>(d, da, rest, ip);
 #pragma unroll
-                    for (int e = 1; e < LT / 16; e++) umma_f16<true>(d, da + e * VSTEP, p_lo + e * STEP, ip);
-                    if constexpr (NTP == 2)
+                                for (int e = 1; e < LT / 16; e++) {
+                                    umma_f16_keep<true>(d, da + e * VSTEP, p_lo + e * STEP, ip);
+                                    umma_f16_kept<true>(d, da + e * VSTEP, rest + e * STEP, ip);
+                                }
+                            } else {
+                                if (i == 0) umma_f16<false>(d, da, p_lo, ip);
+                                else umma_f16<true>(d, da, p_lo, ip);
 #pragma unroll
-                        for (int e = 0; e < LT / 16; e++) umma_f16<true>(d, da + e * VSTEP, rest + e * STEP, ip);
-                    umma_done(blk < pieces - 1 ? &y.freed[kt & 1][blk] : &y.done[kt & 1]);
+                                for (int e = 1; e < LT / 16; e++) umma_f16<true>(d, da + e * VSTEP, p_lo + e * STEP, ip);
+                            }
+                            // a commit costs the unit about as long as five products: one half way, one at the end
+                            if (blk == half - 1) umma_done(&y.freed[k & 1]);
+                        }
+                        umma_done(&y.done[k & 1]);
+                    }
+                    __syncwarp();
                 }
-            }
-            __syncwarp();
-        };
-        // Within a run the next product is the next tile's scores or the last tile's values, whichever has its operands
-        // first: values free a buffer, scores keep the softmax busy while values run.
-        while (ok && walk.next(r)) {
-            int s = 0, v = 0;
-            ok = __all_sync(0xffffffffu, core_wait(y, &y.qfull, run & 1, a.err));
-            run++;
-            while (ok && v < r.tiles) {
-                const int ks = k + s, kv = k + v;
-                bool do_s = s < r.tiles && s - v < 2;
-                const bool can_v = v < s;
-                if (do_s && can_v) {
-                    ok = core_wait2(y, &y.full[ks & 1], (ks >> 1) & 1, &y.pready, kv & 1, a.err, do_s);
-                    do_s = __shfl_sync(0xffffffffu, do_s, 0);      // one choice for the warp
-                }
-                // every lane sees the phase of the choice
-                if (ok) ok = do_s ? core_wait(y, &y.full[ks & 1], (ks >> 1) & 1, a.err) : core_wait(y, &y.pready, kv & 1, a.err);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_after();
-                if (do_s) scores(ks), s++;
-                else values(kv, v == 0), v++;
-            }
-            k += r.tiles;
         }
     } else {
         // ---- softmax. The 64 rows (heads) of S lie in lanes 0-15 of the four warps' quarters of tensor memory; read 16
@@ -611,23 +580,29 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                 if (i == 0) fac[0] = y.fac[hd[0]], fac[1] = y.fac[hd[1]];
                 float v[8][4];
                 tm_ld_rows16(tm + lanes + buf * 64, v);
+                tc_before();
+                arrive(&y.sfree[buf]);
                 const int live = r.n - (r.u + i) * LT;
                 const uint32_t d0 = y.dead[buf][0], d1 = y.dead[buf][1];
                 float mx[2] = {-kv_inf(), -kv_inf()}, fade[2] = {1.0f, 1.0f};
-                const bool whole_tile = live >= LT && !(d0 | d1);
 #pragma unroll
                 for (int j = 0; j < 8; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x = __fmul_rn(v[j][e], fac[e >> 1]);
-                        if (!whole_tile) {
+                    for (int e = 0; e < 4; e++) v[j][e] = __fmul_rn(v[j][e], fac[e >> 1]);
+                if (live < LT || (d0 | d1)) {      // a sequence's last tile, or positions without a row
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
                             const int c = 8 * j + 2 * t + (e & 1);
-                            if (c >= live) x = -kv_inf();
-                            else if ((c < 32 ? d0 >> c : d1 >> (c - 32)) & 1) x = kv_nan();
+                            if ((j < 4 ? d0 >> c : d1 >> (c - 32)) & 1) v[j][e] = kv_nan();
+                            if (c >= live) v[j][e] = -kv_inf();
                         }
-                        v[j][e] = x;
-                        mx[e >> 1] = fmaxf(mx[e >> 1], x);
-                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e >> 1] = fmaxf(mx[e >> 1], v[j][e]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
@@ -696,14 +671,19 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
             const int64_t piece = (int64_t)blockIdx.x * 2 + slot;
             float *o0 = whole ? a.qa + ((int64_t)r.b * a.H + h0) * W : a.o + piece * a.hp * a.R;
             const int pitch = whole ? W : a.R;
-            for (int c = 0; c < a.R / 128 * cols; c += 16) {
-                float o[16];
-                tm_ld16(tm_o + lanes + c, o);
+            // the next 16 columns are read while these are stored
+            float o[2][16];
+            const int all = pieces * cols;
+            tm_ld16(tm_o + lanes, o[0]);
+#pragma unroll 2
+            for (int c = 0, z = 0; c < all; c += 16, z ^= 1) {
                 tm_wait_ld();
+                if (c + 16 < all) tm_ld16(tm_o + lanes + c + 16, o[z ^ 1]);
                 const int hc = c % cols, d = c / cols * 128 + 32 * warp + lane;
+                float *at = o0 + (int64_t)hc * pitch + d;
 #pragma unroll
                 for (int j = 0; j < 16; j++)
-                    if (hc + j < nh) o0[(int64_t)(hc + j) * pitch + d] = o[j];
+                    if (hc + j < nh) at[(int64_t)j * pitch] = o[z][j];
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -720,46 +700,44 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
             tc_before();
         }
     }
-    // after a failed wait loads may still be on their way to shared memory: time to land
-    if (*reinterpret_cast<volatile uint32_t *>(&y.failed))
-        for (int i = 0; i < 200; i++) __nanosleep(1000);
     __syncthreads();
-    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u));
+    if (warp == SCORE_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u));
 }
 
 // ------------------------------------------------------------------------------------------- expand
 
-constexpr int EX_WARPS = 16, EX_ROWS = 8;
+constexpr int EX_WARPS = 8, EX_ROWS = 8;
 
 struct ExpandShared {
     uint4 ops[2][16][32];                // [term][32-dim step][lane]
     float join[EX_WARPS][512];
-    float wgt[EX_WARPS][ATTN_SMS], red[EX_WARPS][16 * EX_ROWS];
+    float wgt[EX_WARPS][ATTN_SMS], red[16][16 * EX_ROWS];
 };
 
 // A CTA a head and eight sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as two
 // terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o.
 template <int T>
-__global__ void __launch_bounds__(32 * EX_WARPS) k_latent_expand(const __grid_constant__ LatentArgs a) {
+__global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid_constant__ LatentArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     ExpandShared &y = *reinterpret_cast<ExpandShared *>(raw);
     auto &ops = y.ops;
     auto &wgt = y.wgt;
-    auto &red = y.red;
     auto &join = y.join;
     const int h = blockIdx.x, b0 = blockIdx.y * EX_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rows = min(EX_ROWS, a.c.n_seqs - b0), pass = h / a.hp, hc = h - pass * a.hp, W = a.R + a.dr, steps = a.R / 32;
-    const int mt = a.dv / 16, ksplit = EX_WARPS / mt, m = warp % mt, kq = warp / mt;
-    const bool live = warp < mt * ksplit;
-    const int s0 = live ? kq * steps / ksplit : 0, s1 = live ? (kq + 1) * steps / ksplit : 0;
-    const uint16_t *w = static_cast<const uint16_t *>(a.w) + ((int64_t)h * (a.dn + a.dv) + a.dn + 16 * m + g) * a.R + 8 * t;
-    uint4 w0[8], w1[8];      // the first 256 dims of its part, under way before the core has ended
+    // warps over (16 value rows, part of the latent dims): ksplit parts where there are fewer row tiles than warps
+    const int mt = a.dv / 16, ksplit = max(1, EX_WARPS / mt), items = mt * ksplit;
+    const uint16_t *w = static_cast<const uint16_t *>(a.w) + ((int64_t)h * (a.dn + a.dv) + a.dn + g) * a.R + 8 * t;
+    auto first = [&](int item) { return item / mt * steps / ksplit; };
+    auto last = [&](int item) { return item < items ? (item / mt + 1) * steps / ksplit : 0; };
+    auto fetch = [&](int item, int s, uint4 v[2]) {
+        const uint16_t *p = w + (int64_t)(item % mt) * 16 * a.R + s * 32;
+        v[0] = __ldg(reinterpret_cast<const uint4 *>(p)), v[1] = __ldg(reinterpret_cast<const uint4 *>(p + 8 * (int64_t)a.R));
+    };
+    uint4 pre[8][2];      // the first 256 dims of the warp's first part, under way before the core has ended
 #pragma unroll
     for (int s = 0; s < 8; s++)
-        if (s0 + s < s1) {
-            w0[s] = __ldg(reinterpret_cast<const uint4 *>(w + (s0 + s) * 32));
-            w1[s] = __ldg(reinterpret_cast<const uint4 *>(w + 8 * (int64_t)a.R + (s0 + s) * 32));
-        }
+        if (first(warp) + s < last(warp)) fetch(warp, first(warp) + s, pre[s]);
     for (int i = threadIdx.x; i < 2 * 16 * 32; i += 32 * EX_WARPS) (&ops[0][0][0])[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     pdl_wait();
@@ -792,16 +770,16 @@ __global__ void __launch_bounds__(32 * EX_WARPS) k_latent_expand(const __grid_co
             for (int s = 16; s >= 1; s >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, s));
             __syncwarp();
             inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-#pragma unroll 2
+#pragma unroll 4
             for (int i = part; i < count; i += wpr) {
                 const float *src = ds.w ? a.o + piece(i) * a.R : whole;
                 const float f = wgt[warp][i];
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                     if (k < a.R / 128) {
-                        const float *at = src + 128 * k + 4 * lane;
-                        o[k][0] = __fmaf_rn(f, at[0], o[k][0]), o[k][1] = __fmaf_rn(f, at[1], o[k][1]);
-                        o[k][2] = __fmaf_rn(f, at[2], o[k][2]), o[k][3] = __fmaf_rn(f, at[3], o[k][3]);
+                        const float4 x = *reinterpret_cast<const float4 *>(src + 128 * k + 4 * lane);
+                        o[k][0] = __fmaf_rn(f, x.x, o[k][0]), o[k][1] = __fmaf_rn(f, x.y, o[k][1]);
+                        o[k][2] = __fmaf_rn(f, x.z, o[k][2]), o[k][3] = __fmaf_rn(f, x.w, o[k][3]);
                     }
             }
         }
@@ -829,23 +807,32 @@ __global__ void __launch_bounds__(32 * EX_WARPS) k_latent_expand(const __grid_co
             }
         }
     __syncthreads();
-    float acc[4] = {};
-    auto step = [&](int s, const uint4 &u, const uint4 &v) {
+    float (&red)[16][16 * EX_ROWS] = y.red;
+    for (int item = warp; item < items; item += EX_WARPS) {
+        float acc[4] = {};
+        auto step = [&](int s, const uint4 v[2]) {
 #pragma unroll
-        for (int k = 1; k >= 0; k--) {
-            const uint4 x = ops[k][s][lane];
-            mma16<T>(acc, u.x, v.x, u.y, v.y, x.x, x.y);
-            mma16<T>(acc, u.z, v.z, u.w, v.w, x.z, x.w);
+            for (int k = 1; k >= 0; k--) {
+                const uint4 x = ops[k][s][lane];
+                mma16<T>(acc, v[0].x, v[1].x, v[0].y, v[1].y, x.x, x.y);
+                mma16<T>(acc, v[0].z, v[1].z, v[0].w, v[1].w, x.z, x.w);
+            }
+        };
+        int s = first(item);
+        if (item == warp) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (s + i < last(item)) step(s + i, pre[i]);
+            s += 8;
         }
-    };
-#pragma unroll
-    for (int s = 0; s < 8; s++)
-        if (s0 + s < s1) step(s0 + s, w0[s], w1[s]);
-    for (int s = s0 + 8; s < s1; s++)
-        step(s, __ldg(reinterpret_cast<const uint4 *>(w + s * 32)), __ldg(reinterpret_cast<const uint4 *>(w + 8 * (int64_t)a.R + s * 32)));
-    if (live) {
-        red[warp][g * EX_ROWS + 2 * t] = acc[0], red[warp][g * EX_ROWS + 2 * t + 1] = acc[1];
-        red[warp][(g + 8) * EX_ROWS + 2 * t] = acc[2], red[warp][(g + 8) * EX_ROWS + 2 * t + 1] = acc[3];
+#pragma unroll 4
+        for (; s < last(item); s++) {
+            uint4 v[2];
+            fetch(item, s, v);
+            step(s, v);
+        }
+        red[item][g * EX_ROWS + 2 * t] = acc[0], red[item][g * EX_ROWS + 2 * t + 1] = acc[1];
+        red[item][(g + 8) * EX_ROWS + 2 * t] = acc[2], red[item][(g + 8) * EX_ROWS + 2 * t + 1] = acc[3];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
@@ -879,32 +866,8 @@ Plan plan_of(const hxb_kv_cache *c, int H, int R) {
     return p;
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The pool as rows of R + dr values, in boxes of 64 values by 16 to 64 rows of a page; false where pages are smaller (36
-// loads a tile already cost as much as the copies of the loading warps) or rows do not fit a coordinate.
-bool row_map(const hxb_kv_cache *c, CUtensorMap *map, int *box) {
-    static const EncodeFn encode = [] {
-        void *fn = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess)
-            cudaGetLastError(), fn = nullptr;
-        return reinterpret_cast<EncodeFn>(fn);
-    }();
-    const int64_t rows = c->n_pages * c->page_tokens;
-    if (!encode || c->dtype == Q8 || c->page_tokens < 16 || rows < LT || rows > 0x7fffffff) return false;
-    *box = std::min(c->page_tokens, LT);
-    const cuuint64_t dims[2] = {(cuuint64_t)c->head_dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)c->head_dim * 2};
-    const cuuint32_t boxd[2] = {64, (cuuint32_t)*box}, step[2] = {1, 1};
-    return encode(map, c->dtype == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, c->k, dims, strides, boxd,
-                  step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int CACHE, int T>
-cudaError_t launch(const LatentArgs &a, const CUtensorMap &map, const Plan &p, cudaStream_t s) {
+cudaError_t launch(const LatentArgs &a, const Plan &p, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(k_latent_core<CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(k_latent_expand<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ExpandShared));
@@ -912,7 +875,7 @@ cudaError_t launch(const LatentArgs &a, const CUtensorMap &map, const Plan &p, c
     const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS), B = a.c.n_seqs;
     e = launch_pdl(false, k_latent_absorb<T>, dim3(a.H * nc, (B + AB_ROWS - 1) / AB_ROWS), dim3(32 * AB_WARPS), 0, s, a);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a, map);
+    e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a);
     if (e != cudaSuccess) return e;
     return launch_pdl(true, k_latent_expand<T>, dim3(a.H, (B + EX_ROWS - 1) / EX_ROWS), dim3(32 * EX_WARPS), sizeof(ExpandShared), s, a);
 }
@@ -962,11 +925,9 @@ extern "C" HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_
     a.H = n_heads, a.R = rank, a.dr = dr, a.dn = nope, a.dv = v_dim, a.passes = p.passes, a.hp = p.hp;
     a.sc2 = scale * 1.44269504088896f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    CUtensorMap map = {};
-    if (!row_map(c, &map, &a.box)) a.box = 0;
     cudaError_t e;
-    if (c->dtype == Q8) e = dtype == F16 ? launch<Q8, F16>(a, map, p, s) : launch<Q8, BF16>(a, map, p, s);
-    else e = dtype == F16 ? launch<F16, F16>(a, map, p, s) : launch<BF16, BF16>(a, map, p, s);
+    if (c->dtype == Q8) e = dtype == F16 ? launch<Q8, F16>(a, p, s) : launch<Q8, BF16>(a, p, s);
+    else e = dtype == F16 ? launch<F16, F16>(a, p, s) : launch<BF16, BF16>(a, p, s);
     if (e != cudaSuccess) return attn_fail(HXB_E_DEVICE, "%s: %s", who, cudaGetErrorString(e));
     return HXB_OK;
 }
