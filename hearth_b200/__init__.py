@@ -17,8 +17,8 @@ from ._lib import (BF16, F16, F32, POLICY_LFU, POLICY_LRU, Q4, Q8, SCORE_SIGMOID
 from . import native  # noqa: F401
 from .moe import MoeBackend, container_probe  # noqa: F401
 from .model import Model  # noqa: F401
-from .attention import (decode_attention, kv_read, kv_write, latent_attention, rope, rope_freqs,  # noqa: F401
-                        rope_table)
+from .attention import (attention_workspace, decode_attention, kv_read, kv_write, latent_attention,  # noqa: F401
+                        latent_workspace, rope, rope_freqs, rope_table)
 
 __all__ = ["lib", "last_error", "native", "MoeBackend", "Model", "container_probe", "rope_freqs", "rope_table", "rope",
-           "kv_write", "kv_read", "decode_attention", "latent_attention", "F32", "F16", "BF16", "Q8", "Q4"]
+           "kv_write", "kv_read", "decode_attention", "latent_attention", "attention_workspace", "latent_workspace", "F32", "F16", "BF16", "Q8", "Q4"]

@@ -17,168 +17,210 @@ raises ValueError before anything is enqueued.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import numpy as np
 
 from . import _lib
 from ._lib import KvCache, Rope, check, lib
-from .moe import _stream
+from .moe import _CUDA_STREAM_LEGACY, _stream
 
 _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
 
-def _dtype(t, what):
+@functools.lru_cache(None)
+def _torch():
+    """torch (imported with the first call), its element types as the library's, and a device's current stream."""
     import torch
-    d = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}.get(t.dtype)
-    if d is None:
-        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
-    return d
+    io = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+    cache = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.int8: _lib.Q8}
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return torch, io, cache, raw
 
 
-def _need(ok, msg):
-    if not ok:
-        raise ValueError(msg)
+def _bad(msg):
+    raise ValueError(msg)
 
 
 def _rows(t, what):
-    """A [tokens, heads, dim] tensor's pointer and strides."""
-    _need(t.dim() == 3, f"{what} must be [tokens, heads, dim], got {tuple(t.shape)}")
-    _need(t.shape[2] < 2 or t.stride(2) == 1, f"{what}'s last dimension must be contiguous")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    """Pointer, strides and shape of a [tokens, heads, dim] tensor."""
+    shape = t.shape
+    if len(shape) != 3:
+        _bad(f"{what} must be [tokens, heads, dim], got {tuple(shape)}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and shape[2] > 1:
+        _bad(f"{what}'s last dimension must be contiguous")
+    return t.data_ptr(), s0, s1, shape
 
 
-def _ints(t, what, n=None):
-    import torch
-    _need(t.dtype == torch.int32 and t.dim() == 1 and (t.numel() < 2 or t.stride(0) == 1),
-          f"{what} must be a contiguous int32 vector")
-    _need(n is None or t.numel() == n, f"{what} must have {n} values, got {t.numel()}")
+def _ints(t, what, n):
+    if t.dtype != _torch()[0].int32 or t.dim() != 1 or (t.stride(0) != 1 and t.numel() > 1):
+        _bad(f"{what} must be a contiguous int32 vector")
+    if t.numel() != n:
+        _bad(f"{what} must have {n} values, got {t.numel()}")
     return t.data_ptr()
 
 
 class _on:
-    """The tensors' device as the current one, and the stream to use there."""
+    """The tensors' device as the current one, and the stream to use there (`ptr` inside the with block)."""
+    __slots__ = ("guard", "dev", "user", "ptr")
 
     def __init__(self, stream, *tensors):
-        import torch
+        cuda = _torch()[0].cuda
         dev = tensors[0].device
+        if dev.type != "cuda":
+            _bad("tensors must be on a CUDA device")
         for t in tensors:
-            if t is not None:
-                _need(t.is_cuda, "tensors must be on a CUDA device")
-                _need(t.device == dev, "tensors must be on one device")
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+            if t is not None and t.device != dev:
+                _bad("tensors must be on one CUDA device")
+        self.guard = None if cuda.current_device() == dev.index else cuda.device(dev)
         self.dev, self.user = dev, stream
+        self.ptr = (_torch()[3](dev.index) or _CUDA_STREAM_LEGACY) if stream is None else _stream(stream)
 
     def __enter__(self):
-        import torch
         if self.guard is not None:
             self.guard.__enter__()
-        return _stream(torch.cuda.current_stream(self.dev) if self.user is None else self.user)
+        return self.ptr
 
     def __exit__(self, *a):
         if self.guard is not None:
             self.guard.__exit__(*a)
 
-    def scratch(self, n):
+    def scratch(self, given, n):
         """n bytes for work on the call's stream."""
-        import torch
+        torch = _torch()[0]
+        if given is not None:
+            if given.dtype != torch.uint8 or not given.is_contiguous() or given.numel() < n:
+                _bad(f"workspace must be a contiguous uint8 tensor of at least {n} bytes")
+            return given
         t = torch.empty(n, dtype=torch.uint8, device=self.dev)
         if self.user is not None:
-            s = self.user if hasattr(self.user, "cuda_stream") else torch.cuda.ExternalStream(int(self.user), self.dev)
-            t.record_stream(s)
+            t.record_stream(self.user if hasattr(self.user, "cuda_stream") else torch.cuda.ExternalStream(int(self.user), self.dev))
         return t
 
 
-def _call(name, *args):
-    rc = getattr(lib(), name)(*args)
-    if rc in (_lib.HXB_E_ARG, _lib.HXB_E_UNSUPPORTED):
-        raise ValueError(f"{name}: {_lib.last_error()}")
-    check(rc, name)
+def _done(rc, name):
+    if rc:
+        if rc in (_lib.HXB_E_ARG, _lib.HXB_E_UNSUPPORTED):
+            _bad(f"{name}: {_lib.last_error()}")
+        check(rc, name)
+
+
+def _scales(dt, k, s, what):
+    if k is None or dt != _lib.Q8:
+        if s is not None:
+            _bad(f"{what} goes with an int8 cache")
+        return 0
+    want = (*k.shape[:3], k.shape[3] // 64)
+    if s is None or s.dtype != _torch()[0].float32 or s.shape != want or not s.is_contiguous():
+        _bad(f"{what} must be float32 [pages, heads, page_tokens, dim / 64]")
+    return s.data_ptr()
 
 
 def _cache(k, v, table, k_scale, v_scale):
-    import torch
-    _need(k.dim() == 4 and k.is_contiguous(), "k_cache must be contiguous [pages, heads, page_tokens, dim]")
-    n_pages, heads, pt, hd = k.shape
-    dt = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.int8: _lib.Q8}.get(k.dtype)
-    _need(dt is not None, f"a cache is float16, bfloat16 or int8, got {k.dtype}")
-    _need(v is None or (v.dtype == k.dtype and v.shape == k.shape and v.is_contiguous()), "v_cache must be like k_cache")
-    for s, p, what in ((k_scale, k, "k_scale"), (v_scale, v, "v_scale")):
-        if p is None or dt != _lib.Q8:
-            _need(s is None, f"{what} goes with an int8 cache")
-        else:
-            _need(s is not None and s.dtype == torch.float32 and s.is_contiguous()
-                  and s.shape == (n_pages, heads, pt, hd // 64), f"{what} must be float32 [pages, heads, page_tokens, dim / 64]")
-    _need(table.dtype == torch.int32 and table.dim() == 2, "table must be int32 [sequences, pages]")
+    torch, _, types, _ = _torch()
+    shape = k.shape
+    if len(shape) != 4 or not k.is_contiguous():
+        _bad("k_cache must be contiguous [pages, heads, page_tokens, dim]")
+    dt = types.get(k.dtype)
+    if dt is None:
+        _bad(f"a cache is float16, bfloat16 or int8, got {k.dtype}")
+    if v is not None and (v.dtype != k.dtype or v.shape != shape or not v.is_contiguous()):
+        _bad("v_cache must be like k_cache")
+    ks, vs = _scales(dt, k, k_scale, "k_scale"), _scales(dt, v, v_scale, "v_scale")
+    if table.dtype != torch.int32 or table.dim() != 2:
+        _bad("table must be int32 [sequences, pages]")
     B, P = table.shape
-    _need(P < 2 or table.stride(1) == 1, "table rows must be contiguous")
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    return KvCache(dt, heads, hd, pt, n_pages, ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), ptr(table),
-                   table.stride(0) if B > 1 else P, P, B)
+    s0, s1 = table.stride()
+    if s1 != 1 and P > 1:
+        _bad("table rows must be contiguous")
+    return KvCache(dt, shape[1], shape[3], shape[2], shape[0], k.data_ptr(), 0 if v is None else v.data_ptr(), ks, vs, table.data_ptr(),
+                   s0 if B > 1 else P, P, B)
 
 
 def _rope(cs, interleaved, offset):
-    import torch
-    _need(cs.dtype == torch.float32 and cs.dim() == 3 and cs.shape[2] == 2 and cs.is_contiguous(),
-          "cs must be a contiguous float32 [positions, rope_dim / 2, 2] table")
+    if cs.dtype != _torch()[0].float32 or cs.dim() != 3 or cs.shape[2] != 2 or not cs.is_contiguous():
+        _bad("cs must be a contiguous float32 [positions, rope_dim / 2, 2] table")
     return Rope(cs.data_ptr(), cs.shape[0], 2 * cs.shape[1], offset, int(bool(interleaved)))
+
+
+def _like(t, shape, dtype):
+    """A new contiguous tensor beside t."""
+    if t.is_contiguous() and t.dtype == dtype and t.shape == shape:
+        return _torch()[0].empty_like(t)
+    return t.new_empty(shape, dtype=dtype)
+
+
+def _io(t, what):
+    d = _torch()[1].get(t.dtype)
+    if d is None:
+        _bad(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    return d
 
 
 def rope_freqs(rope_dim: int, theta: float, *, scaling: str = "none", factor: float = 1.0, original: int = 4096,
                beta_fast: float = 32.0, beta_slow: float = 1.0) -> tuple[np.ndarray, float]:
     """Frequencies (float64 [rope_dim / 2]) and the factor for the table's values; scaling "none", "linear",
     "ntk" or "yarn" (hxb_rope_freqs)."""
-    _need(scaling in _SCALINGS, f"scaling must be one of {sorted(_SCALINGS)}, got {scaling!r}")
-    _need(2 <= rope_dim <= 1024 and rope_dim % 2 == 0, f"rope_dim must be even, 2 to 1024, got {rope_dim}")
+    if scaling not in _SCALINGS:
+        _bad(f"scaling must be one of {sorted(_SCALINGS)}, got {scaling!r}")
+    if not 2 <= rope_dim <= 1024 or rope_dim % 2:
+        _bad(f"rope_dim must be even, 2 to 1024, got {rope_dim}")
     f, a = np.empty(rope_dim // 2, np.float64), C.c_double()
-    _call("hxb_rope_freqs", rope_dim, theta, _SCALINGS[scaling], factor, original, beta_fast, beta_slow, f.ctypes.data,
-          C.byref(a))
+    _done(lib().hxb_rope_freqs(rope_dim, theta, _SCALINGS[scaling], factor, original, beta_fast, beta_slow, f.ctypes.data,
+                               C.byref(a)), "hxb_rope_freqs")
     return f, a.value
 
 
 def rope_table(freqs, n_pos: int, *, first: int = 0, factor: float = 1.0, out=None, device=None, stream=None):
     """cs [n_pos, rope_dim / 2, 2] float32: factor * (cos, sin) of positions first .. first + n_pos - 1."""
-    import torch
+    torch = _torch()[0]
     f = np.ascontiguousarray(freqs, np.float64)
-    _need(f.ndim == 1 and f.size >= 1, "freqs must be a vector")
-    _need(n_pos >= 0, "n_pos must not be negative")
+    if f.ndim != 1 or f.size < 1:
+        _bad("freqs must be a vector")
+    if n_pos < 0:
+        _bad("n_pos must not be negative")
     if out is None:
         out = torch.empty((n_pos, f.size, 2), dtype=torch.float32, device="cuda" if device is None else device)
         if stream is not None and hasattr(stream, "cuda_stream"):
             out.record_stream(stream)
-    _need(out.dtype == torch.float32 and out.shape == (n_pos, f.size, 2) and out.is_contiguous(),
-          "out must be a contiguous float32 [n_pos, len(freqs), 2] tensor")
+    if out.dtype != torch.float32 or out.shape != (n_pos, f.size, 2) or not out.is_contiguous():
+        _bad("out must be a contiguous float32 [n_pos, len(freqs), 2] tensor")
     with _on(stream, out) as s:
-        _call("hxb_rope_table_dev", f.ctypes.data, 2 * f.size, factor, first, n_pos, out.data_ptr(), s)
+        _done(lib().hxb_rope_table_dev(f.ctypes.data, 2 * f.size, factor, first, n_pos, out.data_ptr(), s), "hxb_rope_table_dev")
     return out
 
 
 def rope(x, pos, cs, *, interleaved: bool = False, offset: int = 0, out=None, stream=None):
     """x [T, heads, dim] with values [offset, offset + rope_dim) of every head rotated by position pos[t] (int32
     [T]); into out (another element type is rounded to; x itself: in place), or a new tensor like x."""
-    import torch
-    xa = _rows(x, "x")
-    T, H, D = x.shape
+    xp, xs, xh, shape = _rows(x, "x")
+    T, H, D = shape
     r, p = _rope(cs, interleaved, offset), _ints(pos, "pos", T)
     if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
-    ya = _rows(out, "out")
-    _need(out.shape == x.shape, "out must have x's shape")
-    dx, dy = _dtype(x, "x"), _dtype(out, "out")
+        out = _like(x, shape, x.dtype)
+    yp, ys, yh, yshape = _rows(out, "out")
+    if yshape != shape:
+        _bad("out must have x's shape")
+    dx, dy = _io(x, "x"), _io(out, "out")
     with _on(stream, x, pos, cs, out) as s:
-        _call("hxb_rope_dev", C.byref(r), p, T, H, D, xa[0], dx, xa[1], xa[2], ya[0], dy, ya[1], ya[2], s)
+        _done(lib().hxb_rope_dev(C.byref(r), p, T, H, D, xp, dx, xs, xh, yp, dy, ys, yh, s), "hxb_rope_dev")
     return out
 
 
 def _kv_args(k, v, cache, v_cache, start, pos0, what):
-    ka = _rows(k, what)
-    _need(k.shape[1:] == (cache.n_kv_heads, cache.head_dim), f"{what} must be [tokens, {cache.n_kv_heads}, {cache.head_dim}]")
-    _need((v is None) == (v_cache is None), "v goes with a v_cache")
-    va = (0, 0, 0)
+    kp, ks, kh, shape = _rows(k, what)
+    if shape[1] != cache.n_kv_heads or shape[2] != cache.head_dim:
+        _bad(f"{what} must be [tokens, {cache.n_kv_heads}, {cache.head_dim}]")
+    if (v is None) != (v_cache is None):
+        _bad("v goes with a v_cache")
+    vp = vs = vh = 0
     if v is not None:
-        va = _rows(v, "v")
-        _need(v.shape == k.shape and v.dtype == k.dtype, "v must be like k")
-    return (_ints(start, "start", cache.n_seqs + 1), _ints(pos0, "pos0", cache.n_seqs), k.shape[0], *ka, *va,
-            _dtype(k, what))
+        vp, vs, vh, vshape = _rows(v, "v")
+        if vshape != shape or v.dtype != k.dtype:
+            _bad("v must be like k")
+    B = cache.n_seqs
+    return _ints(start, "start", B + 1), _ints(pos0, "pos0", B), shape[0], kp, ks, kh, vp, vs, vh, _io(k, what)
 
 
 def kv_write(k, v, k_cache, v_cache, table, start, pos0, *, k_scale=None, v_scale=None, cs=None,
@@ -190,7 +232,7 @@ def kv_write(k, v, k_cache, v_cache, table, start, pos0, *, k_scale=None, v_scal
     args = _kv_args(k, v, c, v_cache, start, pos0, "k")
     r = None if cs is None else C.byref(_rope(cs, interleaved, offset))
     with _on(stream, k, v, k_cache, v_cache, table, start, pos0, k_scale, v_scale, cs) as s:
-        _call("hxb_kv_write_dev", C.byref(c), *args, r, s)
+        _done(lib().hxb_kv_write_dev(C.byref(c), *args, r, s), "hxb_kv_write_dev")
 
 
 def kv_read(k_cache, v_cache, table, start, pos0, k_out, v_out, *, k_scale=None, v_scale=None, stream=None) -> None:
@@ -199,16 +241,24 @@ def kv_read(k_cache, v_cache, table, start, pos0, k_out, v_out, *, k_scale=None,
     c = _cache(k_cache, v_cache, table, k_scale, v_scale)
     args = _kv_args(k_out, v_out, c, v_cache, start, pos0, "k_out")
     with _on(stream, k_out, v_out, k_cache, v_cache, table, start, pos0, k_scale, v_scale) as s:
-        _call("hxb_kv_read_dev", C.byref(c), *args, s)
+        _done(lib().hxb_kv_read_dev(C.byref(c), *args, s), "hxb_kv_read_dev")
 
 
-def _workspace(on, given, n):
-    import torch
-    if given is None:
-        return on.scratch(n)
-    _need(given.dtype == torch.uint8 and given.is_contiguous() and given.numel() >= n,
-          f"workspace must be a contiguous uint8 tensor of at least {n} bytes")
-    return given
+@functools.lru_cache(1024)
+def _workspace(n_seqs, n_kv_heads, head_dim, heads, rank):
+    c = KvCache(_lib.BF16, n_kv_heads, head_dim, 1, 0, 0, 0, 0, 0, 0, 0, 0, n_seqs)
+    return int(lib().hxb_latent_decode_workspace(C.byref(c), heads, rank) if rank else lib().hxb_attn_decode_workspace(C.byref(c), heads))
+
+
+def attention_workspace(n_seqs: int, heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch decode_attention needs for these sizes, whatever the cache's type and length
+    (hxb_attn_decode_workspace)."""
+    return _workspace(n_seqs, n_kv_heads, head_dim, heads, 0)
+
+
+def latent_workspace(n_seqs: int, heads: int, rank: int, rope_dim: int) -> int:
+    """Bytes of scratch latent_attention needs for these sizes (hxb_latent_decode_workspace)."""
+    return _workspace(n_seqs, 1, rank + rope_dim, heads, rank)
 
 
 def decode_attention(q, k_cache, v_cache, table, lens, *, scale: float, k_scale=None, v_scale=None, out=None,
@@ -216,54 +266,57 @@ def decode_attention(q, k_cache, v_cache, table, lens, *, scale: float, k_scale=
     """Attention of one new token a sequence, q [n_seqs, heads, head_dim], over positions 0 .. lens[b] - 1 of its
     pages; out like q, with return_lse (out, lse [n_seqs, heads] float32). A sequence of length 0 gives zeros
     and -inf. workspace: uint8 scratch of attention_workspace bytes that no other call in flight uses
-    (default: torch's allocator). (hxb_attn_decode_dev)"""
-    import torch
+    (default: from torch's allocator). (hxb_attn_decode_dev)"""
     c = _cache(k_cache, v_cache, table, k_scale, v_scale)
-    _need(v_cache is not None, "decode_attention needs a v_cache (latent_attention reads a latent cache)")
-    qa = _rows(q, "q")
-    B, H, D = q.shape
-    _need((B, D) == (c.n_seqs, c.head_dim), f"q must be [{c.n_seqs}, heads, {c.head_dim}], got {tuple(q.shape)}")
-    lp, dt = _ints(lens, "lens", B), _dtype(q, "q")
-    if out is None:
-        out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
-    oa = _rows(out, "out")
-    _need(out.shape == q.shape and out.dtype == q.dtype, "out must be like q")
-    if lse is None and return_lse:
-        lse = torch.empty((B, H), dtype=torch.float32, device=q.device)
-    _need(lse is None or (lse.dtype == torch.float32 and lse.shape == (B, H) and lse.is_contiguous()),
-          "lse must be a contiguous float32 [n_seqs, heads] tensor")
+    if v_cache is None:
+        _bad("decode_attention needs a v_cache (latent_attention reads a latent cache)")
+    qp, qs, qh, shape = _rows(q, "q")
+    B, H, D = shape
+    if B != c.n_seqs or D != c.head_dim:
+        _bad(f"q must be [{c.n_seqs}, heads, {c.head_dim}], got {tuple(shape)}")
+    lp, dt = _ints(lens, "lens", B), _io(q, "q")
+    torch = _torch()[0]
     on = _on(stream, q, k_cache, v_cache, table, lens, k_scale, v_scale, out, lse, workspace)
+    if out is None:
+        out = _like(q, shape, q.dtype)
+    op, os, oh, oshape = _rows(out, "out")
+    if oshape != shape or out.dtype != q.dtype:
+        _bad("out must be like q")
+    if lse is None and return_lse:
+        lse = _like(q, (B, H), torch.float32)
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
+        _bad("lse must be a contiguous float32 [n_seqs, heads] tensor")
     with on as s:
-        n = int(lib().hxb_attn_decode_workspace(C.byref(c), H))
-        ws = _workspace(on, workspace, n)
-        _call("hxb_attn_decode_dev", C.byref(c), lp, *qa, H, dt, scale, *oa, 0 if lse is None else lse.data_ptr(),
-              ws.data_ptr(), ws.numel(), s)
+        ws = on.scratch(workspace, _workspace(B, c.n_kv_heads, D, H, 0))
+        _done(lib().hxb_attn_decode_dev(C.byref(c), lp, qp, qs, qh, H, dt, scale, op, os, oh, None if lse is None else lse.data_ptr(),
+                                        ws.data_ptr(), ws.numel(), s), "hxb_attn_decode_dev")
     return (out, lse) if return_lse else out
 
 
 def latent_attention(q, w, c_cache, table, lens, *, scale: float, c_scale=None, out=None, workspace=None, stream=None):
     """Absorbed latent attention of one new token a sequence over a latent cache [n_pages, 1, page_tokens, rank +
     rope]: q [n_seqs, heads, nope + rope] (its rope part rotated), w [heads, nope + v_dim, rank] (the latent's
-    expansion to each head's key and value); out [n_seqs, heads, v_dim]. (hxb_latent_decode_dev)"""
-    import torch
+    expansion to each head's key and value); out [n_seqs, heads, v_dim]. workspace: uint8 scratch of latent_workspace
+    bytes, as for decode_attention. (hxb_latent_decode_dev)"""
     c = _cache(c_cache, None, table, c_scale, None)
-    qa = _rows(q, "q")
-    B, H, dq = q.shape
-    _need(w.dim() == 3 and w.is_contiguous() and w.dtype == q.dtype and w.shape[0] == H,
-          f"w must be contiguous [{H}, nope + v_dim, rank] in q's type")
+    qp, qs, qh, shape = _rows(q, "q")
+    B, H, dq = shape
+    if w.dim() != 3 or not w.is_contiguous() or w.dtype != q.dtype or w.shape[0] != H:
+        _bad(f"w must be contiguous [{H}, nope + v_dim, rank] in q's type")
     R = w.shape[2]
     nope = dq - (c.head_dim - R)
     vd = w.shape[1] - nope
-    _need(B == c.n_seqs and 0 < nope < w.shape[1], f"q {tuple(q.shape)}, w {tuple(w.shape)} and rows of {c.head_dim} do not fit together")
-    lp, dt = _ints(lens, "lens", B), _dtype(q, "q")
-    if out is None:
-        out = torch.empty((B, H, vd), dtype=q.dtype, device=q.device)
-    oa = _rows(out, "out")
-    _need(out.shape == (B, H, vd) and out.dtype == q.dtype, f"out must be [{B}, {H}, {vd}] in q's type")
+    if B != c.n_seqs or nope <= 0 or vd <= 0:
+        _bad(f"q {tuple(shape)}, w {tuple(w.shape)} and rows of {c.head_dim} do not fit together")
+    lp, dt = _ints(lens, "lens", B), _io(q, "q")
     on = _on(stream, q, w, c_cache, table, lens, c_scale, out, workspace)
+    if out is None:
+        out = _like(q, (B, H, vd), q.dtype)
+    op, os, oh, oshape = _rows(out, "out")
+    if oshape != (B, H, vd) or out.dtype != q.dtype:
+        _bad(f"out must be [{B}, {H}, {vd}] in q's type")
     with on as s:
-        n = int(lib().hxb_latent_decode_workspace(C.byref(c), H, R))
-        ws = _workspace(on, workspace, n)
-        _call("hxb_latent_decode_dev", C.byref(c), lp, *qa, w.data_ptr(), H, R, nope, vd, dt, scale, *oa,
-              ws.data_ptr(), ws.numel(), s)
+        ws = on.scratch(workspace, _workspace(B, 1, c.head_dim, H, R))
+        _done(lib().hxb_latent_decode_dev(C.byref(c), lp, qp, qs, qh, w.data_ptr(), H, R, nope, vd, dt, scale, op, os, oh,
+                                          ws.data_ptr(), ws.numel(), s), "hxb_latent_decode_dev")
     return out

@@ -85,6 +85,53 @@ __device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, i
     return true;
 }
 
+// Where a (sequence, pair)'s work went, from the lengths alone: CTAs first .. last, each with one piece, in slot 0 but
+// for the first CTA where the pair is not what it began with. One CTA: it wrote the result itself.
+struct Span {
+    int first, last, slot;
+    __device__ __forceinline__ bool split() const { return first != last; }
+};
+__device__ __forceinline__ Span span_of(int64_t unit0, int nu, int64_t total, int grid) {
+    const int64_t ctas = min((int64_t)grid, total);
+    Span s;
+    // unit u is in the CTA c with c total / ctas <= u < (c + 1) total / ctas
+    s.first = (int)(((unit0 + 1) * ctas - 1) / total), s.last = (int)(((unit0 + nu) * ctas - 1) / total);
+    s.slot = unit0 == s.first * total / ctas ? 0 : 1;
+    return s;
+}
+// Units of the sequences before b, and of all: the same sums my_units forms. Every thread of the CTA calls it.
+template <int THREADS>
+__device__ __forceinline__ void unit_sums(const KvView &c, const int32_t *lens, int unit, int b, int64_t (*scratch)[2], int64_t &before, int64_t &all) {
+    before = all = 0;
+    for (int i = threadIdx.x; i < c.n_seqs; i += THREADS) {
+        const int nu = units_of(c, lens, i, unit);
+        all += nu;
+        if (i < b) before += nu;
+    }
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s), before += __shfl_xor_sync(0xffffffffu, before, s);
+    if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32][0] = before, scratch[threadIdx.x / 32][1] = all;
+    __syncthreads();
+    before = all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) before += scratch[w][0], all += scratch[w][1];
+}
+
+// A running softmax-weighted sum of pieces (maximum, sum, N values each): weights 2^(m_i - max m).
+template <int N>
+struct Joined {
+    float m, l = 0.0f, o[N] = {};
+    __device__ __forceinline__ Joined() : m(-kv_inf()) {}
+    __device__ __forceinline__ void add(float2 ml, const float *x) {
+        const float mx = fmaxf(m, ml.x), base = mx == -kv_inf() ? 0.0f : mx;
+        const float f = exp2_fast(__fsub_rn(m, base)), w = exp2_fast(__fsub_rn(ml.x, base));
+        l = __fmaf_rn(l, f, __fmul_rn(ml.y, w));
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = __fmaf_rn(o[i], f, __fmul_rn(x[i], w));
+        m = mx;
+    }
+};
+
 // Two f32 as a pair of 16-bit matrix operands of TYPE F16 or BF16 (x in the low half); what they leave stays in x, y.
 template <int TYPE>
 __device__ __forceinline__ uint32_t take_pair(float &x, float &y) {

@@ -41,8 +41,9 @@ constexpr int ad_ctas(int nj, int nht) { return nj * nht <= 2 ? 3 : 2; }
 
 // What the join needs beside SplitArgs.
 struct JoinArgs {
-    int64_t capacity;       // positions a table row can name
-    int cols;               // heads of a pair's piece
+    int cols, unit, ctas;   // heads of a pair's piece, positions a unit, CTAs of the split kernel
+    int heads;              // heads a CTA of the join
+    float off;              // exponent the weights carry
 };
 
 struct SplitArgs {
@@ -54,7 +55,6 @@ struct SplitArgs {
     int64_t qs, qh, os, oh;
     int H, group, passes, dtype, D;
     float sc2;              // scale * log2(e)
-    int4 *desc;             // [n_seqs][kv heads * passes]: {first CTA, its slot, last CTA, 1 if split}
     float2 *ml;             // [CTAs][2][columns]: maximum (log2 domain), sum
     float *o;               // [CTAs][2][columns][D]
 };
@@ -421,10 +421,6 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                 else if (a.lse) a.lse[(int64_t)b * a.H + h0 + h] = lse_of(x, sum, POFF);
             }
         }
-        if (u == 0 && tid == 0) {
-            const int64_t upto = cur + nu;   // its last unit is in the CTA c with c total / ctas < upto <= (c + 1) total / ctas
-            a.desc[(int64_t)b * n_pairs + pi] = make_int4(blockIdx.x, slot, (int)((upto * ctas - 1) / total), whole ? 0 : 1);
-        }
         __syncthreads();
 
         cur += nseg, u = 0, pi++;
@@ -438,77 +434,77 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
 
 // ------------------------------------------------------------------------------------------- the join
 
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 512;
 
-// A CTA a (head, sequence): the pieces of a pair that several CTAs worked on are added with weights 2^(m_i - max m),
-// in CTA order; 256 / (D / 4) groups of threads take every such piece in turn, four dims a thread. Empty
+// The pieces of a pair that several CTAs worked on are added with weights 2^(m_i - max m), in a fixed order. A CTA takes
+// `heads` heads of a pair: a thread four dims of one, every `groups`-th piece; then the groups are joined. Which pieces there
+// are follows from the lengths, before the split kernel has ended; after it one round of loads is left. Empty
 // sequences get zeros and -inf, ones longer than their table NaN.
-__global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constant__ SplitArgs a, const __grid_constant__ JoinArgs j,
-                                                            float off) {
-    __shared__ float w[ATTN_SMS * 4], red[2][JOIN_THREADS / 32];
+__global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constant__ SplitArgs a, const __grid_constant__ JoinArgs j) {
+    __shared__ int64_t sums[JOIN_THREADS / 32][2];
     __shared__ float4 part[JOIN_THREADS];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, D = a.D;
-    const int kvh = h / a.group, hg = h - kvh * a.group, pass = hg / j.cols, col = hg - pass * j.cols;
-    pdl_wait();
-    const int n = a.lens[b];
-    if (n <= 0 || n > j.capacity) {
-        for (int d = tid; d < D; d += JOIN_THREADS) io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + d, n <= 0 ? 0.0f : kv_nan());
-        if (tid == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = n <= 0 ? -kv_inf() : kv_nan();
+    __shared__ float2 part_ml[JOIN_THREADS];
+    const int b = blockIdx.y, tid = threadIdx.x, D = a.D, quads = D / 4, each = quads * j.heads, groups = JOIN_THREADS / each;
+    const int nb = (j.cols + j.heads - 1) / j.heads, pair = blockIdx.x / nb, kvh = pair / a.passes, pass = pair - kvh * a.passes;
+    const int gr = tid / each, col = (blockIdx.x - pair * nb) * j.heads + (tid - gr * each) / quads, qd = tid % quads;
+    const int hg = pass * j.cols + col, h = kvh * a.group + hg;
+    const bool live = gr < groups && col < j.cols && hg < a.group;
+    const int n = a.lens[b], nu = units_of(a.c, a.lens, b, j.unit), n_pairs = a.c.Hkv * a.passes;
+    int64_t before, all;
+    unit_sums<JOIN_THREADS>(a.c, a.lens, j.unit, b, sums, before, all);
+    Span sp = {};
+    if (nu) sp = span_of(before * n_pairs + (int64_t)pair * nu, nu, all * n_pairs, j.ctas);
+    if (!nu || !sp.split()) {
+        pdl_wait();      // no CTA ends before the split kernel has: the stream's next kernel waits for this one only
+        if (nu || !live || gr) return;
+        for (int k = 0; k < 4; k++) io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + 4 * qd + k, n <= 0 ? 0.0f : kv_nan());
+        if (qd == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = n <= 0 ? -kv_inf() : kv_nan();
         return;
     }
-    const int4 ds = a.desc[(int64_t)b * a.c.Hkv * a.passes + kvh * a.passes + pass];
-    if (!ds.w) return;
-    const int count = ds.z - ds.x + 1;
-    auto piece = [&](int i) { return ((int64_t)(ds.x + i) * 2 + (i == 0 ? ds.y : 0)) * j.cols + col; };
-    float m = -kv_inf(), l[2] = {};
-    float2 mine[2];
-    for (int k = 0; k < 2; k++) {
-        const int i = tid + k * JOIN_THREADS;
-        mine[k] = i < count ? a.ml[piece(i)] : make_float2(-kv_inf(), 0.0f);
-        m = fmaxf(m, mine[k].x);
-    }
-    for (int s = 16; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-    if (tid % 32 == 0) red[0][tid / 32] = m;
-    __syncthreads();
-    for (int k = 0; k < JOIN_THREADS / 32; k++) m = fmaxf(m, red[0][k]);
-    for (int k = 0; k < 2; k++) {
-        const int i = tid + k * JOIN_THREADS;
-        const float x = exp2_fast(__fsub_rn(mine[k].x, m == -kv_inf() ? 0.0f : m));
-        if (i < count) w[i] = x;
-        l[0] = __fmaf_rn(x, mine[k].y, l[0]);
-    }
-    for (int s = 16; s >= 1; s >>= 1) l[0] = __fadd_rn(l[0], __shfl_xor_sync(0xffffffffu, l[0], s));
-    if (tid % 32 == 0) red[1][tid / 32] = l[0];
-    __syncthreads();
-    float sum = 0.0f;
-    for (int k = 0; k < JOIN_THREADS / 32; k++) sum = __fadd_rn(sum, red[1][k]);
-    const int quads = D / 4, groups = JOIN_THREADS / quads, gr = tid / quads, qd = tid - gr * quads;
-    float4 o = make_float4(0, 0, 0, 0);
-    if (gr < groups)
-#pragma unroll 4
-        for (int i = gr; i < count; i += groups) {
-            const float4 x = *reinterpret_cast<const float4 *>(a.o + piece(i) * D + 4 * qd);
-            o.x = __fmaf_rn(w[i], x.x, o.x), o.y = __fmaf_rn(w[i], x.y, o.y), o.z = __fmaf_rn(w[i], x.z, o.z), o.w = __fmaf_rn(w[i], x.w, o.w);
+    const int count = sp.last - sp.first + 1;
+    // Twice in an SM's first CTA: the first round, on whatever the scratch holds, brings the code near while the split kernel
+    // still runs (code that runs once is fetched slower than it runs); only the second stores.
+#pragma unroll 1
+    for (int round = blockIdx.y * gridDim.x + blockIdx.x < ATTN_SMS ? 0 : 1; round < 2; round++) {
+        if (round) pdl_wait();
+        __syncthreads();
+        Joined<4> mine;
+        if (live)
+#pragma unroll 8
+            for (int i = gr; i < (round ? count : min(count, 8 * groups)); i += groups) {
+                const int64_t at = ((int64_t)(sp.first + i) * 2 + (i == 0 ? sp.slot : 0)) * j.cols + col;
+                const float2 ml = __ldcg(a.ml + at);
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.o + at * D) + qd);
+                const float v[4] = {x.x, x.y, x.z, x.w};
+                mine.add(ml, v);
+            }
+        if (groups > 1) {
+            part[tid] = make_float4(mine.o[0], mine.o[1], mine.o[2], mine.o[3]), part_ml[tid] = make_float2(mine.m, mine.l);
+            __syncthreads();
+            if (gr == 0)
+#pragma unroll 1
+                for (int k = 1; k < min(groups, count); k++) {
+                    const float4 x = part[k * each + tid];
+                    const float v[4] = {x.x, x.y, x.z, x.w};
+                    mine.add(part_ml[k * each + tid], v);
+                }
         }
-    part[tid] = o;
-    __syncthreads();
-    if (gr == 0) {
-        for (int k = 1; k < groups; k++) {
-            const float4 x = part[k * quads + qd];
-            o.x = __fadd_rn(o.x, x.x), o.y = __fadd_rn(o.y, x.y), o.z = __fadd_rn(o.z, x.z), o.w = __fadd_rn(o.w, x.w);
+        if (round && live && gr == 0) {
+#pragma unroll 1
+            for (int k = 0; k < 4; k++) {
+                io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + 4 * qd + k, mine.l == 0.0f ? 0.0f : __fdiv_rn(mine.o[0], mine.l));
+                mine.o[0] = mine.o[1], mine.o[1] = mine.o[2], mine.o[2] = mine.o[3];
+            }
+            if (qd == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = lse_of(mine.m, mine.l, j.off);
         }
-        const float v[4] = {o.x, o.y, o.z, o.w};
-        for (int k = 0; k < 4; k++)
-            io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + 4 * qd + k, sum == 0.0f ? 0.0f : __fdiv_rn(v[k], sum));
     }
-    if (tid == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = lse_of(m, sum, off);
 }
 
 // ------------------------------------------------------------------------------------------- host side
 
 struct Plan {
     int nj, nht, passes, ctas;
-    size_t desc, ml, o, bytes;
+    size_t ml, o, bytes;
 };
 
 Plan plan_of(const hxb_kv_cache *c, int H) {
@@ -519,31 +515,34 @@ Plan plan_of(const hxb_kv_cache *c, int H) {
     p.nht = group > 8 && p.nj <= 2 ? 2 : 1;
     p.passes = (group + 8 * p.nht - 1) / (8 * p.nht);
     p.ctas = ATTN_SMS * ad_ctas(p.nj, p.nht);
-    p.desc = (size_t)c->n_seqs * c->n_kv_heads * p.passes * sizeof(int4);
     p.ml = (size_t)p.ctas * 2 * 8 * p.nht * sizeof(float2);
     p.o = (size_t)p.ctas * 2 * 8 * p.nht * c->head_dim * sizeof(float);
-    p.bytes = p.desc + p.ml + p.o;
+    p.bytes = p.ml + p.o;
     return p;
 }
 
 template <int CACHE, int NTQ, int NTP, int NJ, int NHT>
-cudaError_t split(const SplitArgs &a, const JoinArgs &j, int ctas, cudaStream_t s) {
+cudaError_t split(const SplitArgs &a, int ctas, cudaStream_t s) {
     using Sh = SplitShape<CACHE, NTQ, NTP, NJ, NHT>;
     auto k = k_attn_split<CACHE, NTQ, NTP, NJ, NHT>;
-    if (Sh::SMEM > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM);
-        if (e != cudaSuccess) return e;
-    }
+    static_assert(Sh::SMEM <= 46 * 1024, "dynamic shared memory without an opt-in, beside the kernel's own");
+    // more heads a join CTA while there are two CTAs an SM: with many sequences the pieces of each are few
+    int heads = 1;
+    const int pairs = a.c.Hkv * a.passes;
+    while (heads < Sh::COLS && 2 * heads * (a.D / 4) <= JOIN_THREADS &&
+           (int64_t)pairs * (std::min(a.group, Sh::COLS) / (2 * heads)) * a.c.n_seqs >= 2 * ATTN_SMS)
+        heads *= 2;
+    const JoinArgs j = {Sh::COLS, Sh::UNIT, ctas, heads, CACHE == F16 ? 14.0f : 0.0f};
     const cudaError_t e = launch_pdl(false, k, dim3(ctas), dim3(AD_THREADS), Sh::SMEM, s, a);
     if (e != cudaSuccess) return e;
-    return launch_pdl(true, k_attn_join, dim3(a.H, a.c.n_seqs), dim3(JOIN_THREADS), 0, s, a, j, CACHE == F16 ? 14.0f : 0.0f);
+    return launch_pdl(true, k_attn_join, dim3(pairs * ((Sh::COLS + heads - 1) / heads), a.c.n_seqs), dim3(JOIN_THREADS), 0, s, a, j);
 }
 
 template <int CACHE, int NTQ, int NTP>
-cudaError_t split_shape(const SplitArgs &a, const JoinArgs &j, const Plan &p, cudaStream_t s) {
-    if (p.nj == 1) return p.nht == 1 ? split<CACHE, NTQ, NTP, 1, 1>(a, j, p.ctas, s) : split<CACHE, NTQ, NTP, 1, 2>(a, j, p.ctas, s);
-    if (p.nj == 2) return p.nht == 1 ? split<CACHE, NTQ, NTP, 2, 1>(a, j, p.ctas, s) : split<CACHE, NTQ, NTP, 2, 2>(a, j, p.ctas, s);
-    return split<CACHE, NTQ, NTP, 4, 1>(a, j, p.ctas, s);
+cudaError_t split_shape(const SplitArgs &a, const Plan &p, cudaStream_t s) {
+    if (p.nj == 1) return p.nht == 1 ? split<CACHE, NTQ, NTP, 1, 1>(a, p.ctas, s) : split<CACHE, NTQ, NTP, 1, 2>(a, p.ctas, s);
+    if (p.nj == 2) return p.nht == 1 ? split<CACHE, NTQ, NTP, 2, 1>(a, p.ctas, s) : split<CACHE, NTQ, NTP, 2, 2>(a, p.ctas, s);
+    return split<CACHE, NTQ, NTP, 4, 1>(a, p.ctas, s);
 }
 
 }  // namespace
@@ -593,14 +592,13 @@ extern "C" HXB_API int hxb_attn_decode_dev(const hxb_kv_cache *c, const int32_t 
     a.H = n_heads, a.group = n_heads / c->n_kv_heads, a.passes = p.passes, a.dtype = dtype, a.D = c->head_dim;
     a.sc2 = scale * 1.44269504088896f;
     uint8_t *w = static_cast<uint8_t *>(ws);
-    a.desc = reinterpret_cast<int4 *>(w), a.ml = reinterpret_cast<float2 *>(w + p.desc), a.o = reinterpret_cast<float *>(w + p.desc + p.ml);
-    const JoinArgs j = {(int64_t)c->table_pages * c->page_tokens, 8 * p.nht};
+    a.ml = reinterpret_cast<float2 *>(w), a.o = reinterpret_cast<float *>(w + p.ml);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (c->dtype == F16) e = dtype == F32 ? split_shape<F16, 2, 2>(a, j, p, s) : split_shape<F16, 1, 2>(a, j, p, s);
+    if (c->dtype == F16) e = dtype == F32 ? split_shape<F16, 2, 2>(a, p, s) : split_shape<F16, 1, 2>(a, p, s);
     else if (c->dtype == BF16)
-        e = dtype == F32 ? split_shape<BF16, 3, 3>(a, j, p, s) : dtype == F16 ? split_shape<BF16, 2, 2>(a, j, p, s) : split_shape<BF16, 1, 2>(a, j, p, s);
-    else e = dtype == F32 ? split_shape<Q8, 3, 3>(a, j, p, s) : dtype == F16 ? split_shape<Q8, 2, 2>(a, j, p, s) : split_shape<Q8, 1, 2>(a, j, p, s);
+        e = dtype == F32 ? split_shape<BF16, 3, 3>(a, p, s) : dtype == F16 ? split_shape<BF16, 2, 2>(a, p, s) : split_shape<BF16, 1, 2>(a, p, s);
+    else e = dtype == F32 ? split_shape<Q8, 3, 3>(a, p, s) : dtype == F16 ? split_shape<Q8, 2, 2>(a, p, s) : split_shape<Q8, 1, 2>(a, p, s);
     if (e != cudaSuccess) return attn_fail(HXB_E_DEVICE, "%s: %s", who, cudaGetErrorString(e));
     return HXB_OK;
 }

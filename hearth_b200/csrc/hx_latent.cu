@@ -53,7 +53,6 @@ struct LatentArgs {
     float *qa;              // [n_seqs][H][R + dr]; a head whose work one CTA did leaves its o, maximum and sum here
     float2 *ml;             // [CTAs][2][hp]
     float *o;               // [CTAs][2][hp][R]
-    int4 *desc;             // [n_seqs][passes]: {first CTA of the pass, its slot, last CTA, 1 if split}
     int *err;
     int64_t qs, qh, os, oh;
     int H, R, dr, dn, dv, passes, hp;   // hp heads a pass
@@ -62,7 +61,7 @@ struct LatentArgs {
 
 // ------------------------------------------------------------------------------------------- absorb
 
-constexpr int AB_WARPS = 4, AB_ROWS = 32;
+constexpr int AB_WARPS = 4, AB_ROWS = 32, AB_AHEAD = 4;
 
 template <int T>
 __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_constant__ LatentArgs a) {
@@ -72,59 +71,72 @@ __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_co
     const int r0 = ((blockIdx.x - h * nc) * AB_WARPS + warp) * 64, b0 = blockIdx.y * AB_ROWS, rows = min(AB_ROWS, a.c.n_seqs - b0);
     pdl_trigger();
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.err = 0;
-    // weights of the first 64 dims on their way before the queries are staged
     const uint16_t *w = static_cast<const uint16_t *>(a.w) + (int64_t)h * (a.dn + a.dv) * a.R + r0 + 8 * g;
-    uint4 pre[4][4];
     auto fetch = [&](uint4 v[4], int d0) {
 #pragma unroll
         for (int k = 0; k < 4; k++)
             v[k] = r0 < a.R && d0 < a.dn ? __ldg(reinterpret_cast<const uint4 *>(w + (int64_t)(d0 + 2 * t + (k & 1) + 8 * (k >> 1)) * a.R)) : make_uint4(0, 0, 0, 0);
     };
+    uint4 pre[AB_AHEAD][4];      // weights on their way before the queries are staged, and that far ahead from then on
 #pragma unroll
-    for (int i = 0; i < 4; i++) fetch(pre[i], 16 * i);
+    for (int i = 0; i < AB_AHEAD; i++) fetch(pre[i], 16 * i);
     const uint16_t *q = static_cast<const uint16_t *>(a.q) + h * a.qh;
-#pragma unroll 4
-    for (int r = warp; r < AB_ROWS; r += AB_WARPS)
+    constexpr int AB_EACH = AB_ROWS / AB_WARPS;      // rows a warp stages: all its loads of 64 values before their stores
+    auto row_at = [&](int r, int d, int lim) -> uint16_t {
+        return warp + r * AB_WARPS < rows && d < lim ? __ldg(q + (b0 + warp + r * AB_WARPS) * a.qs + d) : 0;
+    };
+#pragma unroll 1
+    for (int d = lane; d < a.dn; d += 64) {
+        uint16_t x[2][AB_EACH];
 #pragma unroll
-        for (int d = 0; d < 256; d += 32)
-            if (d + lane < a.dn) qsm[r][d + lane] = r < rows ? q[(b0 + r) * a.qs + d + lane] : 0;
+        for (int r = 0; r < AB_EACH; r++) x[0][r] = row_at(r, d, a.dn), x[1][r] = row_at(r, d + 32, a.dn);
+#pragma unroll
+        for (int r = 0; r < AB_EACH; r++) {
+            qsm[warp + r * AB_WARPS][d] = x[0][r];
+            if (d + 32 < a.dn) qsm[warp + r * AB_WARPS][d + 32] = x[1][r];
+        }
+    }
     const int row = a.R + a.dr;
-    if (blockIdx.x == h * nc)      // the rotated parts, with the head's first CTA
-#pragma unroll 4
-        for (int r = warp; r < rows; r += AB_WARPS)
+    if (blockIdx.x == h * nc) {     // the rotated parts, with the head's first CTA
+        uint16_t x[2][AB_EACH];
 #pragma unroll
-            for (int d = 0; d < 64; d += 32)
-                if (d + lane < a.dr) {
-                    const uint16_t x = q[(b0 + r) * a.qs + a.dn + d + lane];
-                    a.qa[((int64_t)(b0 + r) * a.H + h) * row + a.R + d + lane] = T == F16 ? f16_to_f32_hw(x) : bf16_to_f32(x);
-                }
+        for (int r = 0; r < AB_EACH; r++) x[0][r] = row_at(r, a.dn + lane, a.dn + a.dr), x[1][r] = row_at(r, a.dn + lane + 32, a.dn + a.dr);
+#pragma unroll
+        for (int r = 0; r < AB_EACH; r++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                if (warp + r * AB_WARPS < rows && lane + 32 * e < a.dr)
+                    a.qa[((int64_t)(b0 + warp + r * AB_WARPS) * a.H + h) * row + a.R + lane + 32 * e] = T == F16 ? f16_to_f32_hw(x[e][r]) : bf16_to_f32(x[e][r]);
+    }
     __syncthreads();
     if (r0 >= a.R) return;
     float acc[2][8][4] = {};
-    for (int d0 = 0; d0 < a.dn; d0 += 64)
+    // one step of 16 dims, not unrolled: code that runs once is fetched slower than it runs
+#pragma unroll 1
+    for (int d = 0; d < a.dn; d += 16) {
+        const uint4 v[4] = {pre[0][0], pre[0][1], pre[0][2], pre[0][3]};
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            const int d = d0 + 16 * s;
-            if (d >= a.dn) break;
-            uint32_t v[4][4];
+        for (int i = 0; i + 1 < AB_AHEAD; i++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[k][0] = pre[s][k].x, v[k][1] = pre[s][k].y, v[k][2] = pre[s][k].z, v[k][3] = pre[s][k].w;
-            fetch(pre[s], d + 64);
-            uint32_t f[2][4];
+            for (int k = 0; k < 4; k++) pre[i][k] = pre[i + 1][k];
+        fetch(pre[AB_AHEAD - 1], d + 16 * AB_AHEAD);
+        uint32_t f[2][4];
 #pragma unroll
-            for (int m = 0; m < 2; m++)
+        for (int m = 0; m < 2; m++)
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    f[m][k] = *reinterpret_cast<const uint32_t *>(&qsm[16 * m + g + 8 * (k & 1)][d + 2 * t + 8 * (k >> 1)]);
+            for (int k = 0; k < 4; k++)
+                f[m][k] = *reinterpret_cast<const uint32_t *>(&qsm[16 * m + g + 8 * (k & 1)][d + 2 * t + 8 * (k >> 1)]);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++) {
+            const uint32_t x[4] = {(&v[0].x)[i], (&v[1].x)[i], (&v[2].x)[i], (&v[3].x)[i]};
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t p0 = __byte_perm(v[0][i], v[1][i], e ? 0x7632 : 0x5410), p1 = __byte_perm(v[2][i], v[3][i], e ? 0x7632 : 0x5410);
+            for (int e = 0; e < 2; e++) {
+                const uint32_t p0 = __byte_perm(x[0], x[1], e ? 0x7632 : 0x5410), p1 = __byte_perm(x[2], x[3], e ? 0x7632 : 0x5410);
 #pragma unroll
-                    for (int m = 0; m < 2; m++) mma16<T>(acc[m][2 * i + e], f[m][0], f[m][1], f[m][2], f[m][3], p0, p1);
-                }
+                for (int m = 0; m < 2; m++) mma16<T>(acc[m][2 * i + e], f[m][0], f[m][1], f[m][2], f[m][3], p0, p1);
+            }
         }
+    }
     // column n of product i is latent dim 8 n + i
 #pragma unroll
     for (int m = 0; m < 2; m++)
@@ -328,46 +340,43 @@ __device__ __forceinline__ void expand16(uint32_t at, int rw, int q, const uint4
                      : "memory");
 }
 
-// Query rows of a run as the S product's first operand: eight lanes a head.
+// Query rows of a run as the S product's first operand: eight lanes a head, all of its loads before their use.
 template <int OT>
 __device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint32_t dst, int segs, const Run &r, int h0, int nh, int lt) {
     const int c8 = lt & 7, W = a.R + a.dr;
+#pragma unroll 1
     for (int h = lt >> 3; h < LH; h += LD_THREADS / 8) {
-        const float *src = a.qa + ((int64_t)r.b * a.H + h0 + h) * W;
-        float fac = a.sc2;
-        float up = 1.0f;
-        auto piece = [&](int s, float x[8]) {
-            const int e = s * 64 + c8 * 8;
-            if (h < nh && e < W) {
-                const float4 u = __ldcg(reinterpret_cast<const float4 *>(src + e)), v = __ldcg(reinterpret_cast<const float4 *>(src + e) + 1);
-                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-            } else {
+        const float4 *src = reinterpret_cast<const float4 *>(a.qa + ((int64_t)r.b * a.H + h0 + h) * W) + 2 * c8;
+        float4 x[9][2];
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = 0.0f;
-            }
-        };
+        for (int s = 0; s < 9; s++) {
+            const bool on = h < nh && s * 64 + c8 * 8 < W;
+            x[s][0] = on ? __ldcg(src + 16 * s) : make_float4(0, 0, 0, 0);
+            x[s][1] = on ? __ldcg(src + 16 * s + 1) : make_float4(0, 0, 0, 0);
+        }
+        float fac = a.sc2, up = 1.0f;
         if constexpr (OT == F16) {
             float m = 0.0f;
-            for (int s = 0; s < segs; s++) {
-                float x[8];
-                piece(s, x);
 #pragma unroll
-                for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
-            }
+            for (int s = 0; s < 9; s++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(x[s][i].x), fabsf(x[s][i].y)), fmaxf(fabsf(x[s][i].z), fabsf(x[s][i].w))));
 #pragma unroll
             for (int o = 4; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             const int k = f16_lift(m);
             up = pow2i(k), fac = __fmul_rn(fac, pow2i(-k));
         }
         if (c8 == 0) y.fac[h] = fac;
-        for (int s = 0; s < segs; s++) {
-            float x[8];
-            piece(s, x);
+#pragma unroll
+        for (int s = 0; s < 9; s++) {
+            if (s >= segs) break;
             uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float u = __fmul_rn(x[2 * i], up), v = __fmul_rn(x[2 * i + 1], up);
-                o[i] = take_pair<OT>(u, v);
+            for (int i = 0; i < 2; i++) {
+                float4 v = x[s][i];
+                v.x = __fmul_rn(v.x, up), v.y = __fmul_rn(v.y, up), v.z = __fmul_rn(v.z, up), v.w = __fmul_rn(v.w, up);
+                o[2 * i] = take_pair<OT>(v.x, v.y), o[2 * i + 1] = take_pair<OT>(v.z, v.w);
             }
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + s * SEG + h * 128 + ((c8 ^ (h & 7)) << 4)), "r"(o[0]),
                          "r"(o[1]), "r"(o[2]), "r"(o[3])
@@ -568,22 +577,24 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
         // where this lane's rows of 8 x 8 blocks go in P: lanes 0-7 block j, rows g; 8-15 rows g + 8; 16-31 block j + 1
         const int prow = 16 * warp + (lane & 15), pcol = lane >> 4;
         int k = 0;
-        bool ok = true, up = false;
+        bool ok = true, up = false, dry = true;
         while (!up && walk.next(r)) {
             float ref[2] = {-kv_inf(), -kv_inf()}, sum[2] = {}, fac[2] = {};
-            for (int i = 0; i < r.tiles; i++, k++) {
+            // One dry step while the first loads are on their way, on whatever tensor memory holds and with nothing kept: it
+            // brings the code near (code that runs for the first time is fetched slower than it runs).
+            for (int i = dry ? -1 : 0; i < r.tiles; i++, k++) {
                 const int buf = k & 1;
                 // a wait that fails shows at the next barrier of the four warps, where all of them give up
-                ok = core_wait(y, &y.sfull[buf], (k >> 1) & 1, a.err) && ok;
+                if (!dry) ok = core_wait(y, &y.sfull[buf], (k >> 1) & 1, a.err) && ok;
                 __syncwarp();
                 tc_after();
                 if (i == 0) fac[0] = y.fac[hd[0]], fac[1] = y.fac[hd[1]];
                 float v[8][4];
                 tm_ld_rows16(tm + lanes + buf * 64, v);
                 tc_before();
-                arrive(&y.sfree[buf]);
-                const int live = r.n - (r.u + i) * LT;
-                const uint32_t d0 = y.dead[buf][0], d1 = y.dead[buf][1];
+                if (!dry) arrive(&y.sfree[buf]);
+                const int live = dry ? LT : r.n - (r.u + i) * LT;
+                const uint32_t d0 = dry ? 0 : y.dead[buf][0], d1 = dry ? 0 : y.dead[buf][1];
                 float mx[2] = {-kv_inf(), -kv_inf()}, fade[2] = {1.0f, 1.0f};
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -644,7 +655,7 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                 if (k >= 1) ok = core_wait(y, &y.done[buf ^ 1], ((k - 1) >> 1) & 1, a.err) && ok;
                 __syncwarp();
                 if (16 * warp < cols) {
-                    const uint32_t p0 = smem_u32(pb) + prow * 128, p1 = smem_u32(kvb) + buf * segs * SEG + (segs - 1) * SEG + prow * 128;
+                    const uint32_t p0 = smem_u32(pb) + prow * 128, p1 = dry ? p0 : smem_u32(kvb) + buf * segs * SEG + (segs - 1) * SEG + prow * 128;
 #pragma unroll
                     for (int j = 0; j < 8; j += 2)
 #pragma unroll
@@ -656,6 +667,11 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                                          "r"(m0), "r"(m1), "r"(m2), "r"(m3)
                                          : "memory");
                         }
+                }
+                if (dry) {
+                    dry = false, k--;
+                    ref[0] = ref[1] = -kv_inf(), sum[0] = sum[1] = 0.0f;
+                    continue;
                 }
                 if (tid == 0) y.dead[buf][0] = y.dead[buf][1] = 0;
                 fence_proxy_async();
@@ -671,19 +687,26 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
             const int64_t piece = (int64_t)blockIdx.x * 2 + slot;
             float *o0 = whole ? a.qa + ((int64_t)r.b * a.H + h0) * W : a.o + piece * a.hp * a.R;
             const int pitch = whole ? W : a.R;
-            // the next 16 columns are read while these are stored
+            // columns of 16 heads at a time, the next ones read while these are stored
             float o[2][16];
-            const int all = pieces * cols;
             tm_ld16(tm_o + lanes, o[0]);
-#pragma unroll 2
-            for (int c = 0, z = 0; c < all; c += 16, z ^= 1) {
-                tm_wait_ld();
-                if (c + 16 < all) tm_ld16(tm_o + lanes + c + 16, o[z ^ 1]);
-                const int hc = c % cols, d = c / cols * 128 + 32 * warp + lane;
-                float *at = o0 + (int64_t)hc * pitch + d;
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 16) {
+                float *at = o0 + (int64_t)c * pitch + 32 * warp + lane;
 #pragma unroll
-                for (int j = 0; j < 16; j++)
-                    if (hc + j < nh) at[(int64_t)j * pitch] = o[z][j];
+                for (int blk = 0; blk < 4; blk++) {
+                    if (blk >= pieces) break;
+                    tm_wait_ld();
+                    if (blk + 1 < pieces) tm_ld16(tm_o + lanes + (blk + 1) * cols + c, o[(blk + 1) & 1]);
+                    else if (c + 16 < cols) tm_ld16(tm_o + lanes + c + 16, o[(blk + 1) & 1]);
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (c + j < nh) at[(int64_t)j * pitch + blk * 128] = o[blk & 1][j];
+                }
+                if (pieces & 1) {     // the columns after an odd number of blocks were read into the other half
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[0][j] = o[1][j];
+                }
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -692,10 +715,6 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                 if (t != 0 || hd[e] >= nh) continue;
                 if (whole) o0[(int64_t)hd[e] * W + a.R] = ref[e], o0[(int64_t)hd[e] * W + a.R + 1] = sum[e];
                 else a.ml[piece * a.hp + hd[e]] = make_float2(ref[e], sum[e]);
-            }
-            if (tid == 0 && r.u == 0) {
-                const int64_t upto = walk.cur - r.tiles + r.nu;
-                a.desc[(int64_t)r.b * a.passes + pass] = make_int4(cta, slot, (int)((upto * ctas - 1) / total), whole ? 0 : 1);
             }
             tc_before();
         }
@@ -711,20 +730,18 @@ constexpr int EX_WARPS = 8, EX_ROWS = 8;
 struct ExpandShared {
     uint4 ops[2][16][32];                // [term][32-dim step][lane]
     float join[EX_WARPS][512];
-    float wgt[EX_WARPS][ATTN_SMS], red[16][16 * EX_ROWS];
+    float2 ml[EX_WARPS];
+    float red[16][16 * EX_ROWS];
+    int64_t sums[EX_WARPS][2];
 };
 
-// A CTA a head and eight sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as two
-// terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o.
+// A CTA a head and up to eight sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as
+// two terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o.
 template <int T>
-__global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid_constant__ LatentArgs a) {
-    extern __shared__ __align__(16) uint8_t raw[];
-    ExpandShared &y = *reinterpret_cast<ExpandShared *>(raw);
-    auto &ops = y.ops;
-    auto &wgt = y.wgt;
-    auto &join = y.join;
-    const int h = blockIdx.x, b0 = blockIdx.y * EX_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rows = min(EX_ROWS, a.c.n_seqs - b0), pass = h / a.hp, hc = h - pass * a.hp, W = a.R + a.dr, steps = a.R / 32;
+__global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid_constant__ LatentArgs a, int ex_rows, int grid) {
+    __shared__ __align__(16) ExpandShared y;
+    const int h = blockIdx.x, b0 = blockIdx.y * ex_rows, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rows = min(ex_rows, a.c.n_seqs - b0), pass = h / a.hp, hc = h - pass * a.hp, W = a.R + a.dr, steps = a.R / 32;
     // warps over (16 value rows, part of the latent dims): ksplit parts where there are fewer row tiles than warps
     const int mt = a.dv / 16, ksplit = max(1, EX_WARPS / mt), items = mt * ksplit;
     const uint16_t *w = static_cast<const uint16_t *>(a.w) + ((int64_t)h * (a.dn + a.dv) + a.dn + g) * a.R + 8 * t;
@@ -735,111 +752,106 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid
         v[0] = __ldg(reinterpret_cast<const uint4 *>(p)), v[1] = __ldg(reinterpret_cast<const uint4 *>(p + 8 * (int64_t)a.R));
     };
     uint4 pre[8][2];      // the first 256 dims of the warp's first part, under way before the core has ended
+    const int p0 = first(warp), p1 = last(warp);
 #pragma unroll
-    for (int s = 0; s < 8; s++)
-        if (first(warp) + s < last(warp)) fetch(warp, first(warp) + s, pre[s]);
-    for (int i = threadIdx.x; i < 2 * 16 * 32; i += 32 * EX_WARPS) (&ops[0][0][0])[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    pdl_wait();
-
+    for (int s = 0; s < 8; s++) {
+        pre[s][0] = pre[s][1] = make_uint4(0, 0, 0, 0);
+        if (p0 + s < p1) fetch(warp, p0 + s, pre[s]);
+    }
+    for (int i = threadIdx.x; i < 2 * 16 * 32; i += 32 * EX_WARPS) (&y.ops[0][0][0])[i] = make_uint4(0, 0, 0, 0);
+    // the warp's row and its pieces, from the lengths
     int wpr = EX_WARPS;                                  // warps a row
     while (wpr * rows > EX_WARPS) wpr >>= 1;
-    const int row = warp / wpr, part = warp % wpr;
-    const bool work = row < rows;
-    float inv = 0.0f;
-    if (work) {
-        const int b = b0 + row, n = a.lens[b];
-        const int64_t cap = table_capacity(a.c);
-        float o[4][4] = {};
-        if (*a.err || n > cap) {
-            inv = kv_nan();
-        } else if (n > 0) {
-            const int4 ds = a.desc[(int64_t)b * a.passes + pass];
+    const int row = warp / wpr, part = warp % wpr, b = b0 + min(row, rows - 1);
+    int64_t before, all;
+    unit_sums<32 * EX_WARPS>(a.c, a.lens, LT, b0, y.sums, before, all);
+    for (int i = b0; i < b; i++) before += units_of(a.c, a.lens, i, LT);
+    const int n = a.lens[b], nu = units_of(a.c, a.lens, b, LT);
+    Span sp = {};
+    if (nu) sp = span_of(before, nu, all, grid);
+    // Twice in an SM's first CTA: the first round, on whatever the scratch holds, brings the code near while the core still
+    // runs (code that runs once is fetched slower than it runs); only the second stores.
+#pragma unroll 1
+    for (int round = blockIdx.y * gridDim.x + blockIdx.x < ATTN_SMS ? 0 : 1; round < 2; round++) {
+        if (round) pdl_wait();
+        __syncthreads();
+        if (row < rows) {
+            Joined<16> o;
             const float *whole = a.qa + ((int64_t)b * a.H + h) * W;
-            const int count = ds.w ? ds.z - ds.x + 1 : 1;
-            auto piece = [&](int i) { return ((int64_t)((ds.x + i) * a.passes + pass) * 2 + (i == 0 ? ds.y : 0)) * a.hp + hc; };
-            float mx = -kv_inf(), l = 0.0f;
-            for (int i = lane; i < count; i += 32) mx = fmaxf(mx, ds.w ? a.ml[piece(i)].x : whole[a.R]);
-            for (int s = 16; s >= 1; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-            for (int i = lane; i < count; i += 32) {
-                const float2 x = ds.w ? a.ml[piece(i)] : make_float2(whole[a.R], whole[a.R + 1]);
-                const float f = exp2_fast(__fsub_rn(x.x, mx == -kv_inf() ? 0.0f : mx));
-                wgt[warp][i] = f;
-                l = __fmaf_rn(f, x.y, l);
-            }
-            for (int s = 16; s >= 1; s >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, s));
-            __syncwarp();
-            inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-#pragma unroll 4
-            for (int i = part; i < count; i += wpr) {
-                const float *src = ds.w ? a.o + piece(i) * a.R : whole;
-                const float f = wgt[warp][i];
+            const int count = !nu ? 0 : sp.split() ? sp.last - sp.first + 1 : 1;
+#pragma unroll 2
+            for (int i = part; i < (round ? count : min(count, 2 * wpr)); i += wpr) {
+                const int64_t at = ((int64_t)((sp.first + i) * a.passes + pass) * 2 + (i == 0 ? sp.slot : 0)) * a.hp + hc;
+                const float *src = sp.split() ? a.o + at * a.R : whole;
+                const float2 ml = sp.split() ? __ldcg(a.ml + at) : make_float2(__ldcg(whole + a.R), __ldcg(whole + a.R + 1));
+                float x[16] = {};
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                     if (k < a.R / 128) {
-                        const float4 x = *reinterpret_cast<const float4 *>(src + 128 * k + 4 * lane);
-                        o[k][0] = __fmaf_rn(f, x.x, o[k][0]), o[k][1] = __fmaf_rn(f, x.y, o[k][1]);
-                        o[k][2] = __fmaf_rn(f, x.z, o[k][2]), o[k][3] = __fmaf_rn(f, x.w, o[k][3]);
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + 128 * k + 4 * lane));
+                        x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
                     }
+                o.add(ml, x);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                *reinterpret_cast<float4 *>(&y.join[warp][128 * k + 4 * lane]) = make_float4(o.o[4 * k], o.o[4 * k + 1], o.o[4 * k + 2], o.o[4 * k + 3]);
+            if (lane == 0) y.ml[warp] = make_float2(o.m, o.l);
+        }
+        __syncthreads();
+        // the row's warps together, eight dims a lane; nothing, too long a row and a failed wait as the entry point says
+        if (row < rows) {
+            const bool bad = n > table_capacity(a.c) || *reinterpret_cast<volatile int *>(a.err);
+            for (int c = lane + 32 * part; c < a.R / 8; c += 32 * wpr) {
+                Joined<8> o;
+                for (int p = 0; p < wpr; p++) o.add(y.ml[warp - part + p], &y.join[warp - part + p][8 * c]);
+                const float inv = bad ? kv_nan() : __fdiv_rn(1.0f, o.l);
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = !bad && o.l == 0.0f ? 0.0f : __fmul_rn(o.o[i], inv);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    uint4 v;
+                    v.x = take_pair<T>(x[0], x[1]), v.y = take_pair<T>(x[2], x[3]), v.z = take_pair<T>(x[4], x[5]), v.w = take_pair<T>(x[6], x[7]);
+                    y.ops[k][c >> 2][row * 4 + (c & 3)] = v;
+                }
             }
         }
+        __syncthreads();
+        for (int item = warp; item < items; item += EX_WARPS) {
+            float acc[4] = {};
+            auto step = [&](int s, const uint4 v[2]) {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (k < a.R / 128) *reinterpret_cast<float4 *>(&join[warp][128 * k + 4 * lane]) = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
-    }
-    __syncthreads();
-    // eight dims a lane of the row's first warp, over its warps' sums
-    if (work && part == 0)
-        for (int c = lane; c < a.R / 8; c += 32) {
-            float x[8];
+                for (int k = 1; k >= 0; k--) {
+                    const uint4 x = y.ops[k][s][lane];
+                    mma16<T>(acc, v[0].x, v[1].x, v[0].y, v[1].y, x.x, x.y);
+                    mma16<T>(acc, v[0].z, v[1].z, v[0].w, v[1].w, x.z, x.w);
+                }
+            };
+            int s = first(item);
+            const int end = last(item);
+            if (item == warp) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = join[warp][8 * c + i];
-            for (int p = 1; p < wpr; p++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = __fadd_rn(x[i], join[warp + p][8 * c + i]);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = inv == 0.0f ? 0.0f : __fmul_rn(x[i], inv);
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                uint4 v;
-                v.x = take_pair<T>(x[0], x[1]), v.y = take_pair<T>(x[2], x[3]), v.z = take_pair<T>(x[4], x[5]), v.w = take_pair<T>(x[6], x[7]);
-                ops[k][c >> 2][row * 4 + (c & 3)] = v;
+                for (int i = 0; i < 8; i++)
+                    if (s + i < end) step(s + i, pre[i]);
+                s += 8;
             }
-        }
-    __syncthreads();
-    float (&red)[16][16 * EX_ROWS] = y.red;
-    for (int item = warp; item < items; item += EX_WARPS) {
-        float acc[4] = {};
-        auto step = [&](int s, const uint4 v[2]) {
-#pragma unroll
-            for (int k = 1; k >= 0; k--) {
-                const uint4 x = ops[k][s][lane];
-                mma16<T>(acc, v[0].x, v[1].x, v[0].y, v[1].y, x.x, x.y);
-                mma16<T>(acc, v[0].z, v[1].z, v[0].w, v[1].w, x.z, x.w);
-            }
-        };
-        int s = first(item);
-        if (item == warp) {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (s + i < last(item)) step(s + i, pre[i]);
-            s += 8;
-        }
 #pragma unroll 4
-        for (; s < last(item); s++) {
-            uint4 v[2];
-            fetch(item, s, v);
-            step(s, v);
+            for (; s < end; s++) {
+                uint4 v[2];
+                fetch(item, s, v);
+                step(s, v);
+            }
+            y.red[item][g * EX_ROWS + 2 * t] = acc[0], y.red[item][g * EX_ROWS + 2 * t + 1] = acc[1];
+            y.red[item][(g + 8) * EX_ROWS + 2 * t] = acc[2], y.red[item][(g + 8) * EX_ROWS + 2 * t + 1] = acc[3];
         }
-        red[item][g * EX_ROWS + 2 * t] = acc[0], red[item][g * EX_ROWS + 2 * t + 1] = acc[1];
-        red[item][(g + 8) * EX_ROWS + 2 * t] = acc[2], red[item][(g + 8) * EX_ROWS + 2 * t + 1] = acc[3];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
-        const int rw = i / a.dv, j = i - rw * a.dv;
-        float x = red[j >> 4][(j & 15) * EX_ROWS + rw];
-        for (int k = 1; k < ksplit; k++) x = __fadd_rn(x, red[k * mt + (j >> 4)][(j & 15) * EX_ROWS + rw]);
-        io_store(a.out, T, (b0 + rw) * a.os + h * a.oh + j, x);
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
+            const int rw = i / a.dv, j = i - rw * a.dv;
+            float x = y.red[j >> 4][(j & 15) * EX_ROWS + rw];
+            for (int k = 1; k < ksplit; k++) x = __fadd_rn(x, y.red[k * mt + (j >> 4)][(j & 15) * EX_ROWS + rw]);
+            if (round) io_store(a.out, T, (b0 + rw) * a.os + h * a.oh + j, x);
+        }
     }
 }
 
@@ -847,7 +859,7 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid
 
 struct Plan {
     int passes, hp, grid, segs;
-    size_t qa, o, ml, desc, bytes, smem;
+    size_t qa, o, ml, bytes, smem;
 };
 
 Plan plan_of(const hxb_kv_cache *c, int H, int R) {
@@ -860,8 +872,7 @@ Plan plan_of(const hxb_kv_cache *c, int H, int R) {
     p.qa = up((size_t)c->n_seqs * H * c->head_dim * sizeof(float));
     p.o = (size_t)p.grid * 2 * p.hp * R * sizeof(float);
     p.ml = (size_t)p.grid * 2 * p.hp * sizeof(float2);
-    p.desc = (size_t)c->n_seqs * p.passes * sizeof(int4);
-    p.bytes = p.qa + p.o + p.ml + p.desc + 16;
+    p.bytes = p.qa + p.o + p.ml + 16;
     p.smem = 1024 + (size_t)(3 * p.segs + 1) * SEG + sizeof(CoreShared);
     return p;
 }
@@ -870,14 +881,15 @@ template <int CACHE, int T>
 cudaError_t launch(const LatentArgs &a, const Plan &p, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(k_latent_core<CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(k_latent_expand<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ExpandShared));
-    if (e != cudaSuccess) return e;
     const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS), B = a.c.n_seqs;
     e = launch_pdl(false, k_latent_absorb<T>, dim3(a.H * nc, (B + AB_ROWS - 1) / AB_ROWS), dim3(32 * AB_WARPS), 0, s, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a);
     if (e != cudaSuccess) return e;
-    return launch_pdl(true, k_latent_expand<T>, dim3(a.H, (B + EX_ROWS - 1) / EX_ROWS), dim3(32 * EX_WARPS), sizeof(ExpandShared), s, a);
+    // eight sequences share a read of the value rows; fewer a CTA where that would leave SMs without one
+    int rows = EX_ROWS;
+    while (rows > 1 && a.H * ((B + rows - 1) / rows) < 2 * ATTN_SMS) rows /= 2;
+    return launch_pdl(true, k_latent_expand<T>, dim3(a.H, (B + rows - 1) / rows), dim3(32 * EX_WARPS), 0, s, a, rows, p.grid / p.passes);
 }
 
 }  // namespace
@@ -919,7 +931,6 @@ extern "C" HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_
     a.qa = reinterpret_cast<float *>(at), at += p.qa;
     a.o = reinterpret_cast<float *>(at), at += p.o;
     a.ml = reinterpret_cast<float2 *>(at), at += p.ml;
-    a.desc = reinterpret_cast<int4 *>(at), at += p.desc;
     a.err = reinterpret_cast<int *>(at);
     a.lens = lens, a.q = q, a.w = w, a.out = out, a.qs = q_stride, a.qh = q_head_stride, a.os = out_stride, a.oh = out_head_stride;
     a.H = n_heads, a.R = rank, a.dr = dr, a.dn = nope, a.dv = v_dim, a.passes = p.passes, a.hp = p.hp;
