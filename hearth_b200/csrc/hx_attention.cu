@@ -69,32 +69,39 @@ int kv_view(const hxb_kv_cache *c, const char *who, bool latent, KvView *o) {
 
 namespace {
 
-constexpr int ROW_THREADS = 256;
-// Eight-element items a CTA of the row kernels (rotation, cache write and read) takes: a few per thread, so
-// that each has several loads in flight, while single tokens still spread over many CTAs.
-constexpr int ROW_ITEMS = 1024;
+// The row kernels (rotation, cache write and read) work on items of eight values; a thread has ROW_AHEAD of them in flight,
+// a CTA takes whole tokens up to ROW_ITEMS items (one token at least).
+constexpr int ROW_THREADS = 256, ROW_AHEAD = 4, ROW_ITEMS = ROW_THREADS * ROW_AHEAD;
 
 // ------------------------------------------------------------------------------------------- rotary tables
 
 struct FreqArg {
     double turns[512];   // inv_freq / (2 pi)
+    float fhi, flo;      // the factor in two terms
 };
 
-// cs[i][j] = factor * (cos, sin)(2 pi frac(p * turns_j)). The product and its fractional part are formed in 64
-// bits (far positions keep their phase); the f32 part of the fraction goes through sincospif and the rest, below
-// 2^-25 of a turn, enters to first order. 16 bytes written a thread.
-__global__ void __launch_bounds__(256) k_rope_table(const __grid_constant__ FreqArg f, int half, double factor,
-                                                    int64_t pos0, int64_t n_pos, float2 *__restrict__ cs) {
-    const int64_t n = n_pos * half;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t p = i / half;
-        const int j = (int)(i - p * half);
-        const double t = (double)(pos0 + p) * f.turns[j];
+constexpr int TABLE_ITEMS = 4096;   // values of a CTA, at least a row
+
+// cs[i][j] = factor * (cos, sin)(2 pi frac(p * turns_j)). The product and its fractional part are formed in 64 bits (far
+// positions keep their phase); the f32 part of the fraction goes through sincospif and the rest, below 2^-25 of a turn,
+// enters to first order. Written once, 8 bytes an angle; what bounds it is the arithmetic, some 60 instructions an angle.
+__global__ void __launch_bounds__(256) k_rope_table(const __grid_constant__ FreqArg f, int half, FastDiv by_half, int rows, int64_t pos0,
+                                                    int64_t n_pos, float2 *__restrict__ cs) {
+    __shared__ double turns[512];      // lanes of a warp want different ones, which the parameter bank serves one by one
+    for (int j = threadIdx.x; j < half; j += 256) turns[j] = f.turns[j];
+    __syncthreads();
+    const int64_t r0 = (int64_t)blockIdx.x * rows;
+    const int n = (int)min((int64_t)rows, n_pos - r0) * half;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int p = (int)by_half.div(i), j = i - p * half;
+        const double t = (double)(pos0 + r0 + p) * turns[j];
         const double r = 2.0 * (t - rint(t));      // half turns, in [-1, 1], exact after the product
         const float hi = (float)r, lo = (float)(r - (double)hi) * 3.14159265358979f;
         float s, c;
         sincospif(hi, &s, &c);
-        cs[i] = make_float2((float)(factor * (double)__fmaf_rn(-lo, s, c)), (float)(factor * (double)__fmaf_rn(lo, c, s)));
+        const float cc = __fmaf_rn(-lo, s, c), ss = __fmaf_rn(lo, c, s);
+        cs[r0 * half + i] = make_float2(__fmaf_rn(cc, f.fhi, cc * f.flo), __fmaf_rn(ss, f.fhi, ss * f.flo));
     }
 }
 
@@ -118,63 +125,71 @@ struct RopeArgs {
     const void *x;
     void *y;
     int64_t T, xs, xh, ys, yh;
-    int H, hd, units, tpc, in_place, vec;
-    FastDiv per_tok, per_head;
+    int H, hd, tpc, in_place;
+    int n_rot, n_copy;            // items of a head that are rotated, and copied
+    FastDiv rot_tok, rot_head, copy_tok, copy_head;
 };
 
-// Items own what they read and write, so y may be x. vec: an item is a chunk of eight (halves: the pair of
-// chunks j, j + half; then the chunks that are not rotated); otherwise one pair or one copied value.
-template <class TX, class TY>
+// Items own what they read and write, so y may be x. VEC: an item is a chunk of eight values (halves: the pair of chunks
+// j, j + half), else one pair or one copied value. A CTA takes its tokens' rotated items first, then the copied ones;
+// HBM bounds it.
+template <class TX, class TY, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS) k_rope(const __grid_constant__ RopeArgs a) {
     const int64_t t0 = (int64_t)blockIdx.x * a.tpc;
     const int nt = (int)min((int64_t)a.tpc, a.T - t0);
-    const int per = a.H * a.units, rot = 2 * a.r.half;
+    const int per = a.H * a.n_rot, rot = 2 * a.r.half;
+#pragma unroll 2
     for (int i = threadIdx.x; i < nt * per; i += ROW_THREADS) {
-        const int tl = (int)a.per_tok.div(i), u0 = i - tl * per;
-        const int h = (int)a.per_head.div(u0), u = u0 - h * a.units;
+        const int tl = (int)a.rot_tok.div(i), u0 = i - tl * per;
+        const int h = (int)a.rot_head.div(u0), u = u0 - h * a.n_rot;
         const int64_t t = t0 + tl;
-        const TX *x = static_cast<const TX *>(a.x) + t * a.xs + h * a.xh;
-        TY *y = static_cast<TY *>(a.y) + t * a.ys + h * a.yh;
-        const int n_rot = a.vec ? (a.r.style == 0 ? a.r.half / 8 : rot / 8) : a.r.half;
-        if (u >= n_rot) {   // not rotated
-            if (a.in_place) continue;
-            int e = (u - n_rot) * (a.vec ? 8 : 1);
-            if (e >= a.r.off) e += rot;
-            if (a.vec) {
-                float v[8];
-                load8(x + e, v, true);
-                store8(y + e, v, true);
-            } else {
-                y[e] = from_f32<TY>(to_f32(x[e]));
-            }
-            continue;
-        }
+        const TX *x = static_cast<const TX *>(a.x) + t * a.xs + h * a.xh + a.r.off;
+        TY *y = static_cast<TY *>(a.y) + t * a.ys + h * a.yh + a.r.off;
         const int p = a.pos[t];
         const bool ok = p >= 0 && p < a.r.n_pos;
         const float *cs = a.r.cs + (ok ? (int64_t)p : 0) * rot;
-        if (!a.vec) {
-            const int ia = a.r.off + (a.r.style == 0 ? u : 2 * u), ib = a.r.style == 0 ? ia + a.r.half : ia + 1;
+        const float bad = ok ? 0.0f : kv_nan();
+        if constexpr (!VEC) {
+            const int ia = a.r.style == 0 ? u : 2 * u, ib = a.r.style == 0 ? ia + a.r.half : ia + 1;
             float va = to_f32(x[ia]), vb = to_f32(x[ib]);
-            rotate(va, vb, ok ? cs[2 * u] : kv_nan(), ok ? cs[2 * u + 1] : kv_nan());
+            rotate(va, vb, ok ? cs[2 * u] : bad, ok ? cs[2 * u + 1] : bad);
             y[ia] = from_f32<TY>(va);
             y[ib] = from_f32<TY>(vb);
         } else if (a.r.style == 0) {
             float va[8], vb[8], c[16];
-            load8(x + a.r.off + 8 * u, va, true);
-            load8(x + a.r.off + a.r.half + 8 * u, vb, true);
-            load8(cs + 16 * u, c, ok);
-            load8(cs + 16 * u + 8, c + 8, ok);
+            load8(x + 8 * u, va, true);
+            load8(x + a.r.half + 8 * u, vb, true);
+            load8(cs + 16 * u, c, true);
+            load8(cs + 16 * u + 8, c + 8, true);
 #pragma unroll
-            for (int j = 0; j < 8; j++) rotate(va[j], vb[j], ok ? c[2 * j] : kv_nan(), ok ? c[2 * j + 1] : kv_nan());
-            store8(y + a.r.off + 8 * u, va, true);
-            store8(y + a.r.off + a.r.half + 8 * u, vb, true);
+            for (int j = 0; j < 8; j++) rotate(va[j], vb[j], ok ? c[2 * j] : bad, ok ? c[2 * j + 1] : bad);
+            store8(y + 8 * u, va, true);
+            store8(y + a.r.half + 8 * u, vb, true);
         } else {
             float v[8], c[8];
-            load8(x + a.r.off + 8 * u, v, true);
+            load8(x + 8 * u, v, true);
             load8(cs + 8 * u, c, true);
 #pragma unroll
-            for (int j = 0; j < 4; j++) rotate(v[2 * j], v[2 * j + 1], ok ? c[2 * j] : kv_nan(), ok ? c[2 * j + 1] : kv_nan());
-            store8(y + a.r.off + 8 * u, v, true);
+            for (int j = 0; j < 4; j++) rotate(v[2 * j], v[2 * j + 1], ok ? c[2 * j] : bad, ok ? c[2 * j + 1] : bad);
+            store8(y + 8 * u, v, true);
+        }
+    }
+    if (a.in_place || !a.n_copy) return;
+    const int cper = a.H * a.n_copy;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nt * cper; i += ROW_THREADS) {
+        const int tl = (int)a.copy_tok.div(i), u0 = i - tl * cper;
+        const int h = (int)a.copy_head.div(u0);
+        int e = (u0 - h * a.n_copy) * (VEC ? 8 : 1);
+        if (e >= a.r.off) e += rot;
+        const TX *x = static_cast<const TX *>(a.x) + (t0 + tl) * a.xs + h * a.xh + e;
+        TY *y = static_cast<TY *>(a.y) + (t0 + tl) * a.ys + h * a.yh + e;
+        if constexpr (VEC) {
+            float v[8];
+            load8(x, v, true);
+            store8(y, v, true);
+        } else {
+            *y = from_f32<TY>(to_f32(*x));
         }
     }
 }
@@ -188,24 +203,9 @@ struct RowArgs {
     void *x[2];              // k, v: rows read by a write, written by a read
     int64_t T, xs[2], xh[2];
     int sides, tpc, vec, rvec;
+    int step, parts;         // tokens side by side in a CTA, passes of its threads over a token
     FastDiv per_tok, per_side, per_head;
 };
-
-// Sequence of row t and its position; false for padding rows.
-__device__ __forceinline__ bool row_place(const RowArgs &a, int64_t t, int &b, int &pos) {
-    int lo = 0, hi = a.c.n_seqs;   // the last b with start[b] <= t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.start[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const int s0 = a.start[lo];
-    if (t < s0 || t >= a.start[lo + 1]) return false;
-    b = lo;
-    const int64_t p = (int64_t)a.pos0[lo] + (t - s0);
-    pos = p < 0 || p > 0x7fffffff ? -1 : (int)p;
-    return true;
-}
 
 // The rotated values of elements e .. e + 7 of a key row (its pairs may lie in another chunk, so they are read
 // again there; the cache never overlaps the row).
@@ -251,94 +251,184 @@ __device__ __forceinline__ void rotated8(const RowArgs &a, const TX *row, int e,
     }
 }
 
+// Rows of the CTA's tokens, found once per token: the pool row of head 0 (-1: no row, -2: padding) and the position.
+struct Places {
+    int64_t row[ROW_ITEMS];
+    int pos[ROW_ITEMS];
+};
+// Three rounds of loads: all of start at once (the sequence of the CTA's first token is the last that starts at or before
+// it; the tokens are consecutive, so the others' follow by steps), the sequence's words, the page.
+__device__ __forceinline__ void find_places(const RowArgs &a, int64_t t0, int nt, Places &p) {
+    const int B = a.c.n_seqs;
+    int b0 = -1;
+    for (int i0 = 0; i0 < B; i0 += ROW_THREADS) {
+        const int i = i0 + threadIdx.x, n = __syncthreads_count(i < B && a.start[i] <= t0);
+        b0 += n;
+        if (n < ROW_THREADS) break;
+    }
+    for (int i = threadIdx.x; i < nt; i += ROW_THREADS) {
+        const int64_t t = t0 + i;
+        int b = max(b0, 0);
+        int lo = a.start[b], hi = a.start[b + 1];
+        while (t >= hi && b + 1 < B) b++, lo = hi, hi = a.start[b + 1];
+        int64_t row = -2;
+        int pos = -1;
+        if (t >= lo && t < hi) {
+            const int64_t at = (int64_t)a.pos0[b] + (t - lo);
+            pos = at < 0 || at > 0x7fffffff ? -1 : (int)at;
+            row = kv_row(a.c, b, pos);
+        }
+        p.row[i] = row, p.pos[i] = pos;
+    }
+    __syncthreads();
+}
+
+// What a thread of a row kernel does: eight values of one head's key or value, the same ones of ROW_AHEAD tokens of the
+// CTA (every `step`-th from `first` on), so that its addresses are formed once.
+struct Share {
+    int first, side, h, e;
+    bool on;
+};
+__device__ __forceinline__ Share share_at(const RowArgs &a, int part) {
+    Share s;
+    const int per = (int)a.per_tok.d;
+    s.first = part ? 0 : (int)a.per_tok.div(threadIdx.x);      // more parts than one: a token at a time takes all threads
+    int u = threadIdx.x - s.first * per + part * ROW_THREADS;
+    s.on = s.first < a.step && u < per;
+    s.side = (int)a.per_side.div(u);
+    u -= s.side * (int)a.per_side.d;
+    s.h = (int)a.per_head.div(u), s.e = (u - s.h * (int)a.per_head.d) * 8;
+    return s;
+}
+
+// HBM bounds both kernels: a thread's rows are on their way before the places are known (write), or all at once after
+// that (read).
 template <class TX, int CACHE>
 __global__ void __launch_bounds__(ROW_THREADS) k_kv_write(const __grid_constant__ RowArgs a) {
+    __shared__ Places pl;
     const int64_t t0 = (int64_t)blockIdx.x * a.tpc;
     const int nt = (int)min((int64_t)a.tpc, a.T - t0);
-    const int per = (int)a.per_tok.d, side_n = (int)a.per_side.d, head_n = (int)a.per_head.d;
-    for (int i = threadIdx.x; i < nt * per; i += ROW_THREADS) {
-        const int tl = (int)a.per_tok.div(i);
-        int u = i - tl * per;
-        const int side = (int)a.per_side.div(u);
-        u -= side * side_n;
-        const int h = (int)a.per_head.div(u), e = (u - h * head_n) * 8;
-        const int64_t t = t0 + tl;
-        int b, pos;
-        if (!row_place(a, t, b, pos)) continue;
-        const int64_t row0 = kv_row(a.c, b, pos);
-        if (row0 < 0) continue;
-        const int64_t row = row0 + ((int64_t)h << a.c.pt_log2);
-        const TX *x = static_cast<const TX *>(a.x[side]) + t * a.xs[side] + h * a.xh[side];
-        float v[8];
-        load8(x + e, v, a.vec);
-        if (side == 0 && a.r.half) rotated8(a, x, e, pos, v);
+    for (int part = 0; part < a.parts; part++) {
+        const Share s = share_at(a, part);
+        const int64_t xs = s.side ? a.xs[1] : a.xs[0];
+        const TX *x = static_cast<const TX *>(s.side ? a.x[1] : a.x[0]) + (t0 + s.first) * xs + s.h * (s.side ? a.xh[1] : a.xh[0]);
+        float v[ROW_AHEAD][8];
+#pragma unroll
+        for (int k = 0; k < ROW_AHEAD; k++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[k][j] = 0.0f;
+            if (s.on && s.first + k * a.step < nt) load8(x + k * a.step * xs + s.e, v[k], a.vec);
+        }
+        if (part == 0) find_places(a, t0, nt, pl);
+        if (s.side == 0 && a.r.half)
+#pragma unroll
+            for (int k = 0; k < ROW_AHEAD; k++) {
+                const int tl = s.first + k * a.step;
+                if (s.on && tl < nt && pl.row[tl] >= 0) rotated8(a, x + k * a.step * xs, s.e, pl.pos[tl], v[k]);
+            }
+        float d = 0.0f, inv = 0.0f;      // Q8: lane j of a block's eight has the scale of token j % 4 and its inverse
         if constexpr (CACHE == Q8) {
-            // eight lanes hold a block: a CTA's items of one head are a multiple of eight, in lane order
-            const uint32_t grp = 0xffu << (threadIdx.x & 24);
-            float amax = 0.0f;
-            bool bad = false;
+            // Eight lanes hold a block: a head's pieces are a multiple of eight, in lane order. The largest magnitude as bits, so
+            // that NaN and infinities come out on top; two divisions a thread for its four tokens.
+            uint32_t amax[ROW_AHEAD];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                amax = fmaxf(amax, fabsf(v[j]));
-                bad = bad || !(fabsf(v[j]) < kv_inf());
+            for (int k = 0; k < ROW_AHEAD; k++) {
+                amax[k] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) amax[k] = max(amax[k], __float_as_uint(v[k][j]) & 0x7fffffffu);
+#pragma unroll
+                for (int w = 4; w >= 1; w >>= 1) amax[k] = max(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], w));
             }
+            static_assert(ROW_AHEAD == 4, "a lane's share of the scales");
+            const uint32_t m01 = threadIdx.x & 1 ? amax[1] : amax[0], m23 = threadIdx.x & 1 ? amax[3] : amax[2];
+            const uint32_t m = threadIdx.x & 2 ? m23 : m01;
+            d = __fdiv_rn(__uint_as_float(m), 127.0f);
+            inv = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            if (m >= 0x7f800000u) d = inv = kv_nan();
+        }
+        uint8_t *pool = static_cast<uint8_t *>(s.side ? a.c.v : a.c.k);
+        float *scales = (s.side ? a.c.vs : a.c.ks) + s.e / KV_BLOCK;
+        const int64_t head = (int64_t)s.h << a.c.pt_log2;
 #pragma unroll
-            for (int s = 4; s >= 1; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(grp, amax, s));
-            bad = (__ballot_sync(grp, bad) & grp) != 0;
-            const float d = __fdiv_rn(amax, 127.0f);
-            const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-            uint32_t q[2] = {0, 0};
+        for (int k = 0; k < ROW_AHEAD; k++) {
+            const float dk = CACHE == Q8 ? __shfl_sync(0xffffffffu, d, (threadIdx.x & 24) + k) : 0.0f;
+            const float ik = CACHE == Q8 ? __shfl_sync(0xffffffffu, inv, (threadIdx.x & 24) + k) : 0.0f;
+            const int tl = s.first + k * a.step;
+            if (!s.on || tl >= nt || pl.row[tl] < 0) continue;
+            const int64_t row = pl.row[tl] + head;
+            if constexpr (CACHE == Q8) {
+                uint32_t q[8];
+                if (fabsf(ik) < kv_inf()) {      // |x * inv| < 127.5: the sum's low byte is the rounded code
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float s = __fmul_rn(v[j], id);
-                if (s != s) s = 0.0f;
-                s = fminf(fmaxf(s, -127.0f), 127.0f);
-                q[j >> 2] |= ((uint32_t)__float2int_rn(s) & 0xffu) << (8 * (j & 3));
+                    for (int j = 0; j < 8; j++) q[j] = __float_as_uint(__fadd_rn(__fmul_rn(v[k][j], ik), 12582912.0f));
+                } else {                         // 1 / scale past f32's range (or no scale): 0 and the ends
+#pragma unroll
+                    for (int j = 0; j < 8; j++) q[j] = v[k][j] > 0.0f ? 127u : v[k][j] < 0.0f ? 129u : 0u;
+                }
+                auto pack = [](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                    return __byte_perm(__byte_perm(a0, a1, 0x0040), __byte_perm(a2, a3, 0x0040), 0x5410);
+                };
+                *reinterpret_cast<uint2 *>(pool + row * a.c.hd + s.e) = make_uint2(pack(q[0], q[1], q[2], q[3]), pack(q[4], q[5], q[6], q[7]));
+                if (s.e % KV_BLOCK == 0) scales[row * (a.c.hd / KV_BLOCK)] = dk;
+            } else if constexpr (CACHE == F16) {
+                store8(reinterpret_cast<__half *>(pool) + row * a.c.hd + s.e, v[k], true);
+            } else {
+                store8(reinterpret_cast<__nv_bfloat16 *>(pool) + row * a.c.hd + s.e, v[k], true);
             }
-            int8_t *pool = static_cast<int8_t *>(side ? a.c.v : a.c.k);
-            *reinterpret_cast<uint2 *>(pool + row * a.c.hd + e) = make_uint2(q[0], q[1]);
-            if (e % KV_BLOCK == 0) (side ? a.c.vs : a.c.ks)[row * (a.c.hd / KV_BLOCK) + e / KV_BLOCK] = bad ? kv_nan() : d;
-        } else if constexpr (CACHE == F16) {
-            store8(static_cast<__half *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
-        } else {
-            store8(static_cast<__nv_bfloat16 *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
         }
     }
 }
 
 template <class TY, int CACHE>
 __global__ void __launch_bounds__(ROW_THREADS) k_kv_read(const __grid_constant__ RowArgs a) {
+    __shared__ Places pl;
     const int64_t t0 = (int64_t)blockIdx.x * a.tpc;
     const int nt = (int)min((int64_t)a.tpc, a.T - t0);
-    const int per = (int)a.per_tok.d, side_n = (int)a.per_side.d, head_n = (int)a.per_head.d;
-    for (int i = threadIdx.x; i < nt * per; i += ROW_THREADS) {
-        const int tl = (int)a.per_tok.div(i);
-        int u = i - tl * per;
-        const int side = (int)a.per_side.div(u);
-        u -= side * side_n;
-        const int h = (int)a.per_head.div(u), e = (u - h * head_n) * 8;
-        const int64_t t = t0 + tl;
-        int b, pos;
-        if (!row_place(a, t, b, pos)) continue;
-        const int64_t row0 = kv_row(a.c, b, pos);
-        const int64_t row = row0 + ((int64_t)h << a.c.pt_log2);
-        TY *y = static_cast<TY *>(a.x[side]) + t * a.xs[side] + h * a.xh[side];
-        float v[8];
-        if (row0 < 0) {
+    find_places(a, t0, nt, pl);
+    for (int part = 0; part < a.parts; part++) {
+        const Share s = share_at(a, part);
+        if (!s.on) continue;
+        const uint8_t *pool = static_cast<const uint8_t *>(s.side ? a.c.v : a.c.k);
+        const float *scales = (s.side ? a.c.vs : a.c.ks) + s.e / KV_BLOCK;
+        const int64_t head = (int64_t)s.h << a.c.pt_log2;
+        uint4 raw[ROW_AHEAD];
+        float d[ROW_AHEAD];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = kv_nan();
-        } else if constexpr (CACHE == Q8) {
-            const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(side ? a.c.v : a.c.k) + row * a.c.hd + e);
-            const float d = (side ? a.c.vs : a.c.ks)[row * (a.c.hd / KV_BLOCK) + e / KV_BLOCK];
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                v[j] = __fmul_rn((float)(int8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3))), d);
-        } else if constexpr (CACHE == F16) {
-            load8(static_cast<const __half *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
-        } else {
-            load8(static_cast<const __nv_bfloat16 *>(side ? a.c.v : a.c.k) + row * a.c.hd + e, v, true);
+        for (int k = 0; k < ROW_AHEAD; k++) {
+            const int tl = s.first + k * a.step;
+            raw[k] = make_uint4(0, 0, 0, 0), d[k] = kv_nan();
+            if (tl >= nt || pl.row[tl] < 0) continue;
+            const int64_t row = pl.row[tl] + head;
+            if constexpr (CACHE == Q8) {
+                const uint2 q = *reinterpret_cast<const uint2 *>(pool + row * a.c.hd + s.e);
+                raw[k].x = q.x, raw[k].y = q.y;
+                d[k] = scales[row * (a.c.hd / KV_BLOCK)];
+            } else {
+                raw[k] = *reinterpret_cast<const uint4 *>(pool + (row * a.c.hd + s.e) * 2);
+            }
         }
-        store8(y + e, v, a.vec);
+        const int64_t xs = s.side ? a.xs[1] : a.xs[0];
+        TY *y = static_cast<TY *>(s.side ? a.x[1] : a.x[0]) + (t0 + s.first) * xs + s.h * (s.side ? a.xh[1] : a.xh[0]) + s.e;
+#pragma unroll
+        for (int k = 0; k < ROW_AHEAD; k++) {
+            const int tl = s.first + k * a.step;
+            if (tl >= nt || pl.row[tl] == -2) continue;
+            float v[8];
+            if constexpr (CACHE == Q8) {
+                codes4(raw[k].x, v);
+                codes4(raw[k].y, v + 4);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = __fmul_rn(v[j], d[k]);
+            } else {
+                const bool none = pl.row[tl] < 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint32_t w = (&raw[k].x)[j >> 1], h = j & 1 ? w >> 16 : w & 0xffffu;
+                    v[j] = none ? kv_nan() : CACHE == F16 ? f16_to_f32_hw(h) : bf16_to_f32(h);
+                }
+            }
+            store8(y + k * a.step * xs, v, a.vec);
+        }
     }
 }
 
@@ -377,12 +467,17 @@ bool rows_overlap(int64_t T, int64_t ts, int H, int64_t hs, int n) {
     return !(ts >= (H - 1) * hs + n || (hs >= (T - 1) * ts + n && ts >= n));
 }
 
-template <class TX>
-cudaError_t rope_to(const RopeArgs &a, int y_dtype, int grid, cudaStream_t s) {
-    if (y_dtype == F32) k_rope<TX, float><<<grid, ROW_THREADS, 0, s>>>(a);
-    else if (y_dtype == F16) k_rope<TX, __half><<<grid, ROW_THREADS, 0, s>>>(a);
-    else k_rope<TX, __nv_bfloat16><<<grid, ROW_THREADS, 0, s>>>(a);
-    return cudaSuccess;
+template <class TX, bool VEC>
+void rope_to(const RopeArgs &a, int y_dtype, int grid, cudaStream_t s) {
+    if (y_dtype == F32) k_rope<TX, float, VEC><<<grid, ROW_THREADS, 0, s>>>(a);
+    else if (y_dtype == F16) k_rope<TX, __half, VEC><<<grid, ROW_THREADS, 0, s>>>(a);
+    else k_rope<TX, __nv_bfloat16, VEC><<<grid, ROW_THREADS, 0, s>>>(a);
+}
+template <bool VEC>
+void rope_from(const RopeArgs &a, int x_dtype, int y_dtype, int grid, cudaStream_t s) {
+    if (x_dtype == F32) rope_to<float, VEC>(a, y_dtype, grid, s);
+    else if (x_dtype == F16) rope_to<__half, VEC>(a, y_dtype, grid, s);
+    else rope_to<__nv_bfloat16, VEC>(a, y_dtype, grid, s);
 }
 
 template <class T>
@@ -424,7 +519,8 @@ int kv_rows(const char *who, const hxb_kv_cache *c, const int32_t *start, const 
     a.rvec = rope && rope_vec(a.r);
     const int per_head = c->head_dim / 8, per_side = per_head * c->n_kv_heads, per = per_side * a.sides;
     a.per_head = FastDiv(per_head), a.per_side = FastDiv(per_side), a.per_tok = FastDiv(per);
-    a.tpc = std::max(1, ROW_ITEMS / per);
+    a.step = std::max(1, ROW_THREADS / per), a.parts = (per + ROW_THREADS - 1) / ROW_THREADS;
+    a.tpc = a.step * ROW_AHEAD;      // one round: more of them a CTA measured slower (nothing in flight between rounds)
     const int64_t grid = (T + a.tpc - 1) / a.tpc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == F32) rows_launch<float>(a, c->dtype, write, (int)grid, s);
@@ -482,10 +578,10 @@ extern "C" HXB_API int hxb_rope_table_dev(const double *inv_freq, int rope_dim, 
         if (!std::isfinite(inv_freq[j])) return attn_fail(HXB_E_ARG, "rope_table: frequency %d is not finite", j);
         f.turns[j] = inv_freq[j] / (2 * 3.14159265358979323846);
     }
-    const int64_t n = n_pos * (rope_dim / 2);
-    const int grid = (int)std::min<int64_t>((n + 255) / 256, 148 * 16);
-    k_rope_table<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(f, rope_dim / 2, attn_factor, pos0, n_pos,
-                                                                      reinterpret_cast<float2 *>(cs));
+    f.fhi = (float)attn_factor, f.flo = (float)(attn_factor - f.fhi);
+    const int half = rope_dim / 2, rows = std::max(1, TABLE_ITEMS / half);
+    k_rope_table<<<(int)((n_pos + rows - 1) / rows), 256, 0, static_cast<cudaStream_t>(stream)>>>(f, half, FastDiv(half), rows, pos0, n_pos,
+                                                                                               reinterpret_cast<float2 *>(cs));
     return attn_launched("rope_table") ? HXB_OK : HXB_E_DEVICE;
 }
 
@@ -510,17 +606,18 @@ extern "C" HXB_API int hxb_rope_dev(const hxb_rope *r, const int32_t *pos, int64
         return attn_fail(HXB_E_ARG, "rope: in place needs one type and one set of strides");
     a.pos = pos, a.x = x, a.y = y, a.T = T, a.xs = x_stride, a.xh = x_head_stride, a.ys = y_stride, a.yh = y_head_stride;
     a.H = n_heads, a.hd = head_dim;
-    a.vec = head_dim % 8 == 0 && rope_vec(a.r) && (2 * a.r.half) % 8 == 0 && vec_rows(x, x_dtype, T, x_stride, n_heads, x_head_stride) &&
-            vec_rows(y, y_dtype, T, y_stride, n_heads, y_head_stride);
     const int rot = 2 * a.r.half;
-    a.units = a.vec ? (a.r.style == 0 ? a.r.half / 8 : rot / 8) + (head_dim - rot) / 8 : a.r.half + head_dim - rot;
-    a.per_head = FastDiv(a.units), a.per_tok = FastDiv(a.units * n_heads);
-    a.tpc = std::max(1, ROW_ITEMS / (a.units * n_heads));
+    const bool vec = head_dim % 8 == 0 && rope_vec(a.r) && rot % 8 == 0 && vec_rows(x, x_dtype, T, x_stride, n_heads, x_head_stride) &&
+                     vec_rows(y, y_dtype, T, y_stride, n_heads, y_head_stride);
+    a.n_rot = !vec ? a.r.half : a.r.style == 0 ? a.r.half / 8 : rot / 8;
+    a.n_copy = (head_dim - rot) / (vec ? 8 : 1);
+    a.rot_head = FastDiv(a.n_rot), a.rot_tok = FastDiv(a.n_rot * n_heads);
+    a.copy_head = FastDiv(std::max(1, a.n_copy)), a.copy_tok = FastDiv(std::max(1, a.n_copy * n_heads));
+    a.tpc = std::max(1, ROW_ITEMS / ((a.n_rot + a.n_copy) * n_heads));
     const int grid = (int)((T + a.tpc - 1) / a.tpc);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (x_dtype == F32) rope_to<float>(a, y_dtype, grid, s);
-    else if (x_dtype == F16) rope_to<__half>(a, y_dtype, grid, s);
-    else rope_to<__nv_bfloat16>(a, y_dtype, grid, s);
+    if (vec) rope_from<true>(a, x_dtype, y_dtype, grid, s);
+    else rope_from<false>(a, x_dtype, y_dtype, grid, s);
     return attn_launched("rope") ? HXB_OK : HXB_E_DEVICE;
 }
 

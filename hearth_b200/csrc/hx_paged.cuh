@@ -62,6 +62,16 @@ __device__ __forceinline__ void store8(T *p, const float x[8], bool vec) {
     }
 }
 
+// The four signed bytes of w as floats, exactly: 2^23 + (byte + 128) assembled as bits, less 2^23 + 128 (an int-to-float
+// conversion runs at a quarter of the rate).
+__device__ __forceinline__ void codes4(uint32_t w, float o[4]) {
+    w ^= 0x80808080u;
+    o[0] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540)) - 8388736.0f;
+    o[1] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7541)) - 8388736.0f;
+    o[2] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7542)) - 8388736.0f;
+    o[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7543)) - 8388736.0f;
+}
+
 // i / d for 32-bit i by one multiply: exact for i < 2^31 and 1 <= d < 2^31 (round-up magic number with
 // s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1).
 struct FastDiv {
