@@ -21,11 +21,14 @@
 // of 8. The next tile's keys are on their way while the softmax and the values are worked on, and so on in turn:
 // 8 KB a warp, 12 warps an SM.
 //
-// Bits. Matrix operands have the cache's type (Q8: bf16, which holds the codes exactly, with the scales
-// applied in f32). Queries of more bits are split into terms (bf16: 3 for f32, 2 for f16; f16: 2 for f32,
+// Bits. Matrix operands have the cache's type (Q8: f16, which holds the codes exactly; the scales are applied in f32, a
+// value's to its weight). Queries of more bits are split into terms (bf16: 3 for f32, 2 for f16; f16: 2 for f32,
 // after a power of two that puts the head's largest value at 2^13), and weights into 2 terms (bf16 for f32
 // outputs: 3), since one rounding of each weight to the operand's type would be as large as the output's own.
-// f16 weights carry 2^14, so that those down to 2^-38 of the largest count.
+// f16 weights carry 2^14, so that those down to 2^-38 of the largest count; Q8 ones are taken relative to the power of
+// two of the largest value scale so far. Q8 keys of 16-bit queries go in as 1152 + code, the form the bytes have under f16's
+// exponent, and the sums start at -1152 times the query's: the products stay exact, and what the larger sums lose
+// is below 2^-18 of the score's terms.
 #include "hx_attn.cuh"
 
 #include <algorithm>
@@ -67,13 +70,15 @@ __device__ __forceinline__ uint32_t trans8x8(uint32_t x) {
     return y;
 }
 
-// Signed bytes 0, 1 (HI: 2, 3) of w as a bf16 pair, exactly: byte b is (128 + (b & 127)) - (128 + (b & 128)), and
-// 0x43 over a byte below 128 is the bf16 of 128 + it, over 0x80 of 256.
+// Bytes 0, 1 (HI: 2, 3) of codes as an f16 pair: a byte with its sign bit flipped under 0x64 is 1152 + code.
 template <bool HI>
-__device__ __forceinline__ uint32_t codes2(uint32_t w) {
-    const uint32_t x = __byte_perm(w, 0x43434343u, HI ? 0x4342 : 0x4140);
-    const uint32_t a = x & 0xff7fff7fu, b = x & 0xff80ff80u;
-    const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a), reinterpret_cast<const __nv_bfloat162 &>(b));
+__device__ __forceinline__ uint32_t lifted2(uint32_t flipped) {
+    return __byte_perm(flipped, 0x64646464u, HI ? 0x4342 : 0x4140);
+}
+template <bool HI>
+__device__ __forceinline__ uint32_t codes2(uint32_t flipped) {
+    const uint32_t x = lifted2<HI>(flipped), off = 0x64806480u;
+    const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(off));
     return reinterpret_cast<const uint32_t &>(r);
 }
 
@@ -91,13 +96,14 @@ template <int CACHE, int NTQ, int NTP, int NJ, int NHT>
 __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(const __grid_constant__ SplitArgs a) {
     using Sh = SplitShape<CACHE, NTQ, NTP, NJ, NHT>;
     constexpr int NS = Sh::NS, UNIT = Sh::UNIT, COLS = Sh::COLS;
-    constexpr float POFF = CACHE == F16 ? 14.0f : 0.0f;
-    constexpr int OT = CACHE == F16 ? F16 : BF16;   // the operands' type
+    constexpr int OT = CACHE == BF16 ? BF16 : F16;   // the operands' type
+    constexpr float POFF = OT == F16 ? 14.0f : 0.0f;
+    constexpr bool LIFTED = CACHE == Q8 && NTQ == 1;
     extern __shared__ __align__(16) uint8_t smem[];
     uint4 *qs = reinterpret_cast<uint4 *>(smem);                    // [term][column tile][32-dim step][lane]
     float *mrg = reinterpret_cast<float *>(smem + Sh::Q_BYTES);     // [warp][column][OROW]
     __shared__ int64_t scan[AD_WARPS];
-    __shared__ float wm[AD_WARPS][COLS], wl[AD_WARPS][COLS], qfac[COLS];
+    __shared__ float wm[AD_WARPS][COLS], wl[AD_WARPS][COLS], qfac[COLS], qsum[NJ][COLS];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.D, chunks = D / 8, n_pairs = a.c.Hkv * a.passes;
@@ -137,21 +143,51 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
             return (((int64_t)pg * a.c.Hkv + kvh) << a.c.pt_log2) + ((tok + rel) & ((1 << a.c.pt_log2) - 1));
         };
 
-        constexpr int KW = CACHE == Q8 ? NJ : 2 * NJ;
+        constexpr int KW = CACHE == Q8 ? NJ : 2 * NJ, ES = CACHE == Q8 ? 1 : 2;
         uint4 kr[NS][2][KW];
         float ks[NS][2][CACHE == Q8 ? NJ : 1], vs[NS][2][CACHE == Q8 ? NJ : 1];
         uint32_t vr[NS][4][NJ][CACHE == Q8 ? 2 : 4];
         bool dead[NS][2];     // a position in range without a row
+        // A tile with all its positions in whole pages and heads of 64 NJ dims needs no checks: one address a row block. Rows of a
+        // page lie D elements apart; *_lane is where a lane reads in them.
+        const bool whole_d = D == 64 * NJ && a.c.pt_log2 >= 4;
+        const uint32_t k_lane = (g * D) * ES + 16 * t, v_lane = (2 * t * D) * ES + g * (8 * ES);
+        auto plain_tile = [&](const int *pg, int i) {
+            const int tok = (u + i) * UNIT + warp * 16 * NS;
+            bool ok = whole_d && tok + 16 * NS <= n;
+#pragma unroll
+            for (int s = 0; s < NS; s++) ok = ok && (uint32_t)pg[s] < (uint64_t)a.c.n_pages;
+            return ok;
+        };
+        auto block_at = [&](int page, int tok) { return (((int64_t)page * a.c.Hkv + kvh) << a.c.pt_log2) + (tok & ((1 << a.c.pt_log2) - 1)); };
 
-        auto load_k = [&](const int *pg, int i) {
+        auto load_k = [&](const int *pg, int i, bool plain) {
 #pragma unroll
             for (int s = 0; s < NS; s++) {
                 const int tok = (u + i) * UNIT + (warp * NS + s) * 16;
+                if (plain) {
+                    const int64_t row = block_at(pg[s], tok);
+                    const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * (D * ES) + k_lane;
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        dead[s][r] = false;
+#pragma unroll
+                        for (int j = 0; j < KW; j++) kr[s][r][j] = __ldg(reinterpret_cast<const uint4 *>(p + r * 8 * 64 * NJ * ES) + 4 * j);
+                    }
+                    if constexpr (CACHE == Q8) {
+                        const float *kp = a.c.ks + (row + g) * NJ, *vp = a.c.vs + (row + g) * NJ;
+#pragma unroll
+                        for (int r = 0; r < 2; r++)
+#pragma unroll
+                            for (int j = 0; j < NJ; j++) ks[s][r][j] = __ldg(kp + r * 8 * NJ + j), vs[s][r][j] = __ldg(vp + r * 8 * NJ + j);
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     const int64_t row = row_at(pg[s], tok, g + 8 * r);
                     dead[s][r] = row < 0 && tok + g + 8 * r < n;
-                    const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * D * (CACHE == Q8 ? 1 : 2);
+                    const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * D * ES;
 #pragma unroll
                     for (int j = 0; j < KW; j++) {
                         const bool on = row >= 0 && (CACHE == Q8 ? 64 * j < D : 4 * j + t < chunks);
@@ -168,22 +204,24 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                 }
             }
         };
-        auto load_v = [&](const int *pg, int i) {
+        auto load_v = [&](const int *pg, int i, bool plain) {
 #pragma unroll
             for (int s = 0; s < NS; s++) {
                 const int tok = (u + i) * UNIT + (warp * NS + s) * 16;
+                const uint8_t *base = static_cast<const uint8_t *>(a.c.v) + (plain ? block_at(pg[s], tok) * (D * ES) + v_lane : 0);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int64_t row = row_at(pg[s], tok, 2 * t + (r & 1) + 8 * (r >> 1));
-                    const uint8_t *p = static_cast<const uint8_t *>(a.c.v) + row * D * (CACHE == Q8 ? 1 : 2);
+                    const int rel = (r & 1) + 8 * (r >> 1);
+                    const int64_t row = plain ? 0 : row_at(pg[s], tok, 2 * t + rel);
+                    const uint8_t *p = plain ? base + rel * 64 * NJ * ES : static_cast<const uint8_t *>(a.c.v) + row * D * ES + g * (8 * ES);
 #pragma unroll
                     for (int j = 0; j < NJ; j++) {
-                        const bool on = row >= 0 && g + 8 * j < chunks;
+                        const bool on = plain || (row >= 0 && g + 8 * j < chunks);
                         if constexpr (CACHE == Q8) {
-                            const uint2 x = on ? __ldg(reinterpret_cast<const uint2 *>(p) + g + 8 * j) : make_uint2(0, 0);
+                            const uint2 x = on ? __ldg(reinterpret_cast<const uint2 *>(p) + 8 * j) : make_uint2(0, 0);
                             vr[s][r][j][0] = x.x, vr[s][r][j][1] = x.y;
                         } else {
-                            const uint4 x = on ? __ldg(reinterpret_cast<const uint4 *>(p) + g + 8 * j) : make_uint4(0, 0, 0, 0);
+                            const uint4 x = on ? __ldg(reinterpret_cast<const uint4 *>(p) + 8 * j) : make_uint4(0, 0, 0, 0);
                             vr[s][r][j][0] = x.x, vr[s][r][j][1] = x.y, vr[s][r][j][2] = x.z, vr[s][r][j][3] = x.w;
                         }
                     }
@@ -192,8 +230,9 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
         };
 
         int pg[2] = {page_of(0), page2_of(0)}, pg_next[2];
-        load_k(pg, 0);
-        load_v(pg, 0);
+        bool plain = plain_tile(pg, 0);
+        if (plain) load_k(pg, 0, true), load_v(pg, 0, true);
+        else load_k(pg, 0, false), load_v(pg, 0, false);
         pg_next[0] = page_of(1), pg_next[1] = page2_of(1);
 
         // queries into shared memory as the products' column operands: a warp a head, a lane eight dims
@@ -205,7 +244,7 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                 for (int i = 0; i < 8; i++) x[i] = io_load(a.q, a.dtype, at + i);
             }
             float fac = a.sc2;
-            if constexpr (CACHE == F16) {
+            if constexpr (OT == F16) {
                 float m = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
@@ -218,6 +257,11 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
             }
             if (lane == 0) qfac[h] = fac;
             if (lane < 8 * NJ) {
+                float sum = 0.0f;
+                if constexpr (LIFTED) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sum += x[i];
+                }
                 const int step = CACHE == Q8 ? 2 * (lane >> 3) + (lane & 1) : lane >> 2, tt = CACHE == Q8 ? (lane & 7) >> 1 : lane & 3;
 #pragma unroll
                 for (int k = 0; k < NTQ; k++) {
@@ -226,10 +270,25 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                     w.z = take_pair<OT>(x[4], x[5]), w.w = take_pair<OT>(x[6], x[7]);
                     qs[((k * NHT + (h >> 3)) * 2 * NJ + step) * 32 + (h & 7) * 4 + tt] = w;
                 }
+                if constexpr (LIFTED) {      // what the operands, rounded, add up to over a block
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sum -= x[i];
+                    const uint32_t eight = 0xffu << (lane & 24);
+#pragma unroll
+                    for (int o = 1; o <= 4; o <<= 1) sum += __shfl_xor_sync(eight, sum, o);
+                    if ((lane & 7) == 0) qsum[lane >> 3][h] = -1152.0f * sum;
+                }
             }
         }
         __syncthreads();
-        float fac[NHT][2];
+        float fac[NHT][2], bias[LIFTED ? NJ : 1][NHT][2] = {};
+        int ve[CACHE == Q8 ? NJ : 1] = {};      // exponents of the largest value scales so far
+        if constexpr (LIFTED) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int c = 0; c < NHT; c++) bias[j][c][0] = qsum[j][8 * c + 2 * t], bias[j][c][1] = qsum[j][8 * c + 2 * t + 1];
+        }
 #pragma unroll
         for (int c = 0; c < NHT; c++) fac[c][0] = qfac[8 * c + 2 * t], fac[c][1] = qfac[8 * c + 2 * t + 1];
 
@@ -250,13 +309,14 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                     if constexpr (CACHE == Q8) {
 #pragma unroll
                         for (int j = 0; j < NJ; j++) {
-                            float p[4] = {};
+                            float p[4] = {bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1], bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1]};
                             const uint32_t w0[4] = {kr[z][0][j].x, kr[z][0][j].y, kr[z][0][j].z, kr[z][0][j].w};
                             const uint32_t w1[4] = {kr[z][1][j].x, kr[z][1][j].y, kr[z][1][j].z, kr[z][1][j].w};
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const uint32_t a0 = codes2<false>(w0[e]), a1 = codes2<false>(w1[e]);
-                                const uint32_t a2 = codes2<true>(w0[e]), a3 = codes2<true>(w1[e]);
+                                const uint32_t f0 = w0[e] ^ 0x80808080u, f1 = w1[e] ^ 0x80808080u;
+                                const uint32_t a0 = LIFTED ? lifted2<false>(f0) : codes2<false>(f0), a1 = LIFTED ? lifted2<false>(f1) : codes2<false>(f1);
+                                const uint32_t a2 = LIFTED ? lifted2<true>(f0) : codes2<true>(f0), a3 = LIFTED ? lifted2<true>(f1) : codes2<true>(f1);
 #pragma unroll
                                 for (int k = NTQ - 1; k >= 0; k--) {
                                     const uint4 q = qs[((k * NHT + c) * 2 * NJ + 2 * j + (e >> 1)) * 32 + lane];
@@ -286,20 +346,43 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                 for (int c = 0; c < NHT; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float x = __fmul_rn(s[z][c][e], fac[c][e & 1]);
-                        s[z][c][e] = dead[z][e >> 1] ? kv_nan() : tok + 16 * z + g + 8 * (e >> 1) < n ? x : -kv_inf();
+                        s[z][c][e] = __fmul_rn(s[z][c][e], fac[c][e & 1]);
+                        if (!plain) s[z][c][e] = dead[z][e >> 1] ? kv_nan() : tok + 16 * z + g + 8 * (e >> 1) < n ? s[z][c][e] : -kv_inf();
                     }
-            float pv[NS][2][CACHE == Q8 ? NJ : 1];   // the values' scales of this tile
+            float pv[NS][2][CACHE == Q8 ? NJ : 1];   // the values' scales of this tile, below 2 by the power of two that O carries
             if constexpr (CACHE == Q8) {
 #pragma unroll
-                for (int z = 0; z < NS; z++)
+                for (int j = 0; j < NJ; j++) {
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int r = 0; r < 2; r++)
+                    for (int z = 0; z < NS; z++)
 #pragma unroll
-                        for (int j = 0; j < NJ; j++) pv[z][r][j] = vs[z][r][j];
+                        for (int r = 0; r < 2; r++) {
+                            const uint32_t bits = __float_as_uint(vs[z][r][j]);
+                            top = max(top, bits < 0x7f800000u ? bits : 0u);
+                        }
+                    const int e = (int)(__reduce_max_sync(0xffffffffu, top) >> 23);
+                    if (e > ve[j]) {      // the same in every lane
+                        const float f = ve[j] == 0 ? 0.0f : exp2_fast((float)(ve[j] - e));
+#pragma unroll
+                        for (int c = 0; c < NHT; c++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+#pragma unroll
+                                for (int x = 0; x < 4; x++) o[c][j][k][x] = __fmul_rn(o[c][j][k][x], f);
+                        ve[j] = e;
+                    }
+                    const float inv = __uint_as_float((uint32_t)max(254 - ve[j], 1) << 23);
+#pragma unroll
+                    for (int z = 0; z < NS; z++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) pv[z][r][j] = ve[j] == 0 ? vs[z][r][j] : __fmul_rn(vs[z][r][j], inv);
+                }
             }
             const int pgv[2] = {pg_next[0], pg_next[1]};
-            if (i + 1 < nseg) load_k(pg_next, i + 1);
+            const bool next_plain = i + 1 < nseg && plain_tile(pg_next, i + 1);
+            if (next_plain) load_k(pg_next, i + 1, true);
+            else if (i + 1 < nseg) load_k(pg_next, i + 1, false);
             pg_next[0] = page_of(i + 2), pg_next[1] = page2_of(i + 2);
 
             // running maximum and sum
@@ -312,13 +395,13 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                     for (int z = 0; z < NS; z++) x = fmaxf(x, fmaxf(s[z][c][e], s[z][c][e + 2]));
 #pragma unroll
                     for (int w = 4; w <= 16; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-                    const float base = x == -kv_inf() ? 0.0f : x;
+                    const float base = x == -kv_inf() ? 0.0f : x, shift = __fsub_rn(base, POFF);
                     const float fade = exp2_fast(__fsub_rn(m[c][e], base));
                     l[c][e] = __fmul_rn(l[c][e], fade);
 #pragma unroll
                     for (int z = 0; z < NS; z++) {
-                        s[z][c][e] = exp2_fast(__fadd_rn(__fsub_rn(s[z][c][e], base), POFF));
-                        s[z][c][e + 2] = exp2_fast(__fadd_rn(__fsub_rn(s[z][c][e + 2], base), POFF));
+                        s[z][c][e] = exp2_fast(__fsub_rn(s[z][c][e], shift));
+                        s[z][c][e + 2] = exp2_fast(__fsub_rn(s[z][c][e + 2], shift));
                         l[c][e] = __fadd_rn(l[c][e], __fadd_rn(s[z][c][e], s[z][c][e + 2]));
                     }
                     m[c][e] = x;
@@ -355,8 +438,8 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                     for (int k = 0; k < 4; k++) {
                         uint32_t a0, a1, a2, a3;
                         if constexpr (CACHE == Q8) {
-                            const uint32_t w0 = __byte_perm(vr[z][0][j][k >> 1], vr[z][1][j][k >> 1], k & 1 ? 0x7362 : 0x5140);
-                            const uint32_t w1 = __byte_perm(vr[z][2][j][k >> 1], vr[z][3][j][k >> 1], k & 1 ? 0x7362 : 0x5140);
+                            const uint32_t w0 = __byte_perm(vr[z][0][j][k >> 1], vr[z][1][j][k >> 1], k & 1 ? 0x7362 : 0x5140) ^ 0x80808080u;
+                            const uint32_t w1 = __byte_perm(vr[z][2][j][k >> 1], vr[z][3][j][k >> 1], k & 1 ? 0x7362 : 0x5140) ^ 0x80808080u;
                             a0 = codes2<false>(w0), a1 = codes2<true>(w0), a2 = codes2<false>(w1), a3 = codes2<true>(w1);
                         } else {
                             a0 = __byte_perm(vr[z][0][j][k], vr[z][1][j][k], 0x5410), a1 = __byte_perm(vr[z][0][j][k], vr[z][1][j][k], 0x7632);
@@ -369,7 +452,9 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                                 mma16<OT>(o[c][j][k], a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
                     }
             }
-            if (i + 1 < nseg) load_v(pgv, i + 1);
+            if (next_plain) load_v(pgv, i + 1, true);
+            else if (i + 1 < nseg) load_v(pgv, i + 1, false);
+            plain = next_plain;
         }
 
         // the warps' pieces into one
@@ -395,9 +480,14 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
 #pragma unroll
                 for (int j = 0; j < NJ; j++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        *reinterpret_cast<float2 *>(dst + 64 * j + 8 * g + 2 * k) =
-                            make_float2(__fmul_rn(o[c][j][k][e], fade), __fmul_rn(o[c][j][k][e + 2], fade));
+                    for (int k = 0; k < 4; k++) {
+                        float x0 = __fmul_rn(o[c][j][k][e], fade), x1 = __fmul_rn(o[c][j][k][e + 2], fade);
+                        if constexpr (CACHE == Q8) {
+                            const float f = ve[j] == 0 ? 1.0f : __uint_as_float((uint32_t)ve[j] << 23);
+                            x0 = __fmul_rn(x0, f), x1 = __fmul_rn(x1, f);
+                        }
+                        *reinterpret_cast<float2 *>(dst + 64 * j + 8 * g + 2 * k) = make_float2(x0, x1);
+                    }
             }
         __syncthreads();
         const bool whole = nseg == nu;
@@ -532,7 +622,7 @@ cudaError_t split(const SplitArgs &a, int ctas, cudaStream_t s) {
     while (heads < Sh::COLS && 2 * heads * (a.D / 4) <= JOIN_THREADS &&
            (int64_t)pairs * (std::min(a.group, Sh::COLS) / (2 * heads)) * a.c.n_seqs >= 2 * ATTN_SMS)
         heads *= 2;
-    const JoinArgs j = {Sh::COLS, Sh::UNIT, ctas, heads, CACHE == F16 ? 14.0f : 0.0f};
+    const JoinArgs j = {Sh::COLS, Sh::UNIT, ctas, heads, CACHE == BF16 ? 0.0f : 14.0f};
     const cudaError_t e = launch_pdl(false, k, dim3(ctas), dim3(AD_THREADS), Sh::SMEM, s, a);
     if (e != cudaSuccess) return e;
     return launch_pdl(true, k_attn_join, dim3(pairs * ((Sh::COLS + heads - 1) / heads), a.c.n_seqs), dim3(JOIN_THREADS), 0, s, a, j);
@@ -598,7 +688,7 @@ extern "C" HXB_API int hxb_attn_decode_dev(const hxb_kv_cache *c, const int32_t 
     if (c->dtype == F16) e = dtype == F32 ? split_shape<F16, 2, 2>(a, p, s) : split_shape<F16, 1, 2>(a, p, s);
     else if (c->dtype == BF16)
         e = dtype == F32 ? split_shape<BF16, 3, 3>(a, p, s) : dtype == F16 ? split_shape<BF16, 2, 2>(a, p, s) : split_shape<BF16, 1, 2>(a, p, s);
-    else e = dtype == F32 ? split_shape<Q8, 3, 3>(a, p, s) : dtype == F16 ? split_shape<Q8, 2, 2>(a, p, s) : split_shape<Q8, 1, 2>(a, p, s);
+    else e = dtype == F32 ? split_shape<Q8, 2, 2>(a, p, s) : split_shape<Q8, 1, 2>(a, p, s);
     if (e != cudaSuccess) return attn_fail(HXB_E_DEVICE, "%s: %s", who, cudaGetErrorString(e));
     return HXB_OK;
 }
