@@ -39,6 +39,21 @@ __device__ __forceinline__ int units_of(const KvView &c, const int32_t *lens, in
     return n <= 0 || n > table_capacity(c) ? 0 : (int)(((int64_t)n + unit - 1) / unit);
 }
 
+// N units in `ctas` shares that differ by at most one: the first N % ctas have one more.
+struct Shares {
+    int64_t each;
+    int more;
+    __device__ __forceinline__ Shares(int64_t total, int ctas) {
+        if (total <= 0xffffffffll) each = (uint32_t)total / (uint32_t)ctas, more = (int)((uint32_t)total % (uint32_t)ctas);
+        else each = total / ctas, more = (int)(total % ctas);
+    }
+    __device__ __forceinline__ int64_t start(int cta) const { return cta * each + min(cta, more); }
+    __device__ __forceinline__ int of(int64_t unit) const {      // the share a unit is in
+        const int64_t big = more * (each + 1);
+        return (int)(unit < big ? unit / (each + 1) : more + (unit - big) / each);
+    }
+};
+
 // The share [cur, end) of CTA `cta` of `grid` in the N = n_pairs * sum_b units_of(b) units, laid out sequence by
 // sequence, pair by pair: the sequence of unit cur and the sum of the units of the sequences before it. False
 // without a share. ctas: the CTAs that have one (the first min(grid, N)). Every thread of the CTA calls it;
@@ -69,7 +84,10 @@ __device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, i
     ctas = (int)min((int64_t)grid, total);
     const int64_t start = base + upto - mine;             // units of the sequences before my chunk
     cur = end = 0;
-    if (total) cur = cta * total / ctas, end = (cta + 1) * total / ctas;
+    if (total) {
+        const Shares sh(total, ctas);
+        cur = sh.start(cta), end = sh.start(cta + 1);
+    }
     const bool none = cta >= ctas;
     // the chunk that holds unit cur: the last one that starts at or before it
     const int chunk = __syncthreads_count(start * n_pairs <= cur) - 1;
@@ -92,11 +110,10 @@ struct Span {
     __device__ __forceinline__ bool split() const { return first != last; }
 };
 __device__ __forceinline__ Span span_of(int64_t unit0, int nu, int64_t total, int grid) {
-    const int64_t ctas = min((int64_t)grid, total);
+    const Shares sh(total, (int)min((int64_t)grid, total));
     Span s;
-    // unit u is in the CTA c with c total / ctas <= u < (c + 1) total / ctas
-    s.first = (int)(((unit0 + 1) * ctas - 1) / total), s.last = (int)(((unit0 + nu) * ctas - 1) / total);
-    s.slot = unit0 == s.first * total / ctas ? 0 : 1;
+    s.first = sh.of(unit0), s.last = sh.of(unit0 + nu - 1);
+    s.slot = unit0 == sh.start(s.first) ? 0 : 1;
     return s;
 }
 // Units of the sequences before b, and of all: the same sums my_units forms. Every thread of the CTA calls it.

@@ -7,19 +7,18 @@
 // instructions (mma.sync m16n8k16; at 8 heads a kv head its rate is far above the reads', and the
 // fifth-generation unit's 128-row tiles would be 1/16 full).
 //
-// Split. A unit is 64 (Q8: 128) positions of one kv head of one sequence. The grid is as many CTAs as fit
+// Split. A unit is 64 positions of one kv head of one sequence. The grid is as many CTAs as fit
 // the GPU at once, and CTA c takes units [c N / G, (c + 1) N / G) of all N, in the order (sequence, kv head,
 // position), with N summed from the lengths on the device: the shares are equal whatever the lengths are, and a
 // captured graph follows them. A CTA that does all of a (sequence, kv head) writes its output; otherwise it
 // leaves (maximum, sum, output) in the scratch and the join kernel adds the pieces in order.
 //
-// A warp takes 16 (Q8: 32) positions of a unit. Keys and values go from HBM to registers in the order the
+// A warp takes 16 positions of a unit. Keys and values go from HBM to registers in the order the
 // matrix instructions want, without a stop in shared memory: S^T = K Q^T takes a 16-byte piece of a key row
 // per lane as two steps' operands (the same permutation of the head's dims on both sides leaves the
 // dot as it is); P^T is the accumulator transposed by movmatrix; O^T = V^T P^T takes 16-byte pieces of four
 // value rows per lane, paired by byte permutes. With heads as the 8 columns nothing is padded for groups
-// of 8. The next tile's keys are on their way while the softmax and the values are worked on, and so on in turn:
-// 8 KB a warp, 12 warps an SM.
+// of 8. The next tile's rows are on their way while one is worked on: up to 8 KB a warp, 12 warps an SM.
 //
 // Bits. Matrix operands have the cache's type (Q8: f16, which holds the codes exactly; the scales are applied in f32, a
 // value's to its weight). Queries of more bits are split into terms (bf16: 3 for f32, 2 for f16; f16: 2 for f32,
@@ -39,8 +38,10 @@ namespace {
 constexpr int AD_WARPS = 4, AD_THREADS = 32 * AD_WARPS;
 
 constexpr int ad_nj(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : 4; }   // blocks of 64 dims, padded
-// Resident CTAs an SM by registers: at 128 dims and one column tile 12 warps with 168 registers each.
-constexpr int ad_ctas(int nj, int nht) { return nj * nht <= 2 ? 3 : 2; }
+// Resident CTAs an SM by registers. 16-bit rows of 128 dims: 12 warps with 168 registers each, 8 KB a warp under way (16 with
+// 128 measured 68 % of the copy rate instead of 90 %). Q8 rows are half as long and cost more instructions a byte: 16
+// warps (52 us on 48 sequences of up to 6011; 12: 63, 20: 81).
+constexpr int ad_ctas(int cache, int nj, int nht) { return nj * nht <= 2 ? (cache == Q8 ? 4 : 3) : 2; }
 
 // What the join needs beside SplitArgs.
 struct JoinArgs {
@@ -84,8 +85,7 @@ __device__ __forceinline__ uint32_t codes2(uint32_t flipped) {
 
 template <int CACHE, int NTQ, int NTP, int NJ, int NHT>
 struct SplitShape {
-    static constexpr int NS = CACHE == Q8 && NJ <= 2 ? 2 : 1;      // 16-position tiles a warp takes at once
-    static constexpr int UNIT = AD_WARPS * 16 * NS;
+    static constexpr int UNIT = AD_WARPS * 16;
     static constexpr int COLS = 8 * NHT;
     static constexpr int OROW = 64 * NJ + 4;                       // floats between heads in the merge buffer
     static constexpr size_t Q_BYTES = (size_t)NTQ * NHT * 2 * NJ * 32 * 16;
@@ -93,9 +93,9 @@ struct SplitShape {
 };
 
 template <int CACHE, int NTQ, int NTP, int NJ, int NHT>
-__global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(const __grid_constant__ SplitArgs a) {
+__global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_split(const __grid_constant__ SplitArgs a) {
     using Sh = SplitShape<CACHE, NTQ, NTP, NJ, NHT>;
-    constexpr int NS = Sh::NS, UNIT = Sh::UNIT, COLS = Sh::COLS;
+    constexpr int UNIT = Sh::UNIT, COLS = Sh::COLS;
     constexpr int OT = CACHE == BF16 ? BF16 : F16;   // the operands' type
     constexpr float POFF = OT == F16 ? 14.0f : 0.0f;
     constexpr bool LIFTED = CACHE == Q8 && NTQ == 1;
@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
     if (!my_units<AD_THREADS>(a.c, a.lens, UNIT, n_pairs, blockIdx.x, gridDim.x, scan, b, acc, cur, end, total, ctas)) return;
     const int64_t first_unit = cur;
     int nu = units_of(a.c, a.lens, b, UNIT);
-    int pi = (int)((cur - acc * n_pairs) / nu), u = (int)((cur - acc * n_pairs) % nu);
+    const int64_t into = cur - acc * n_pairs;
+    int pi = into <= 0xffffffffll ? (int)((uint32_t)into / (uint32_t)nu) : (int)(into / nu), u = (int)(into - (int64_t)pi * nu);
 
     while (cur < end) {
         const int n = a.lens[b];
@@ -124,18 +125,12 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
         const int kvh = pi / a.passes, h0 = kvh * a.group + (pi - kvh * a.passes) * COLS;
         const int nh = min(COLS, (kvh + 1) * a.group - h0);
 
-        // pages of the warp's tiles, one tile ahead of their rows
+        // pages of the warp's tiles, asked for a tile ahead of their rows: one, or a lane's own where pages are under 16
         auto page_of = [&](int i) {
-            const int tok = (u + i) * UNIT + warp * 16 * NS + (a.c.pt_log2 >= 4 ? 0 : (lane & 15));
+            const int tok = (u + i) * UNIT + warp * 16 + (a.c.pt_log2 >= 4 ? 0 : (lane & 15));
             return i < nseg && tok < n ? a.c.table[(int64_t)b * a.c.table_stride + (tok >> a.c.pt_log2)] : -1;
         };
-        // Second tile of a pair (NS 2): its own page where pages are smaller than 32 or tiles of 16 differ.
-        auto page2_of = [&](int i) {
-            if constexpr (NS == 1) return -1;
-            const int tok = (u + i) * UNIT + warp * 16 * NS + 16 + (a.c.pt_log2 >= 4 ? 0 : (lane & 15));
-            return i < nseg && tok < n ? a.c.table[(int64_t)b * a.c.table_stride + (tok >> a.c.pt_log2)] : -1;
-        };
-        // row of position tok (relative to the pool's first row of this head), -1: none
+        // row of position tok + rel of this kv head, -1: none
         auto row_at = [&](int page, int tok, int rel) -> int64_t {
             int pg = page;
             if (a.c.pt_log2 < 4) pg = __shfl_sync(0xffffffffu, page, rel);
@@ -144,96 +139,86 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
         };
 
         constexpr int KW = CACHE == Q8 ? NJ : 2 * NJ, ES = CACHE == Q8 ? 1 : 2;
-        uint4 kr[NS][2][KW];
-        float ks[NS][2][CACHE == Q8 ? NJ : 1], vs[NS][2][CACHE == Q8 ? NJ : 1];
-        uint32_t vr[NS][4][NJ][CACHE == Q8 ? 2 : 4];
-        bool dead[NS][2];     // a position in range without a row
-        // A tile with all its positions in whole pages and heads of 64 NJ dims needs no checks: one address a row block. Rows of a
+        uint4 kr[2][KW];
+        float ks[2][CACHE == Q8 ? NJ : 1], vs[2][CACHE == Q8 ? NJ : 1];
+        uint32_t vr[4][NJ][CACHE == Q8 ? 2 : 4];
+        bool dead[2];     // a position in range without a row
+        // A tile with all its positions in one page and heads of 64 NJ dims needs no checks: one address a row block. Rows of a
         // page lie D elements apart; *_lane is where a lane reads in them.
         const bool whole_d = D == 64 * NJ && a.c.pt_log2 >= 4;
         const uint32_t k_lane = (g * D) * ES + 16 * t, v_lane = (2 * t * D) * ES + g * (8 * ES);
-        auto plain_tile = [&](const int *pg, int i) {
-            const int tok = (u + i) * UNIT + warp * 16 * NS;
-            bool ok = whole_d && tok + 16 * NS <= n;
-#pragma unroll
-            for (int s = 0; s < NS; s++) ok = ok && (uint32_t)pg[s] < (uint64_t)a.c.n_pages;
-            return ok;
+        auto plain_tile = [&](int pg, int i) {
+            return whole_d && (u + i) * UNIT + warp * 16 + 16 <= n && (uint32_t)pg < (uint64_t)a.c.n_pages;
         };
         auto block_at = [&](int page, int tok) { return (((int64_t)page * a.c.Hkv + kvh) << a.c.pt_log2) + (tok & ((1 << a.c.pt_log2) - 1)); };
 
-        auto load_k = [&](const int *pg, int i, bool plain) {
-#pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const int tok = (u + i) * UNIT + (warp * NS + s) * 16;
-                if (plain) {
-                    const int64_t row = block_at(pg[s], tok);
-                    const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * (D * ES) + k_lane;
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        dead[s][r] = false;
-#pragma unroll
-                        for (int j = 0; j < KW; j++) kr[s][r][j] = __ldg(reinterpret_cast<const uint4 *>(p + r * 8 * 64 * NJ * ES) + 4 * j);
-                    }
-                    if constexpr (CACHE == Q8) {
-                        const float *kp = a.c.ks + (row + g) * NJ, *vp = a.c.vs + (row + g) * NJ;
-#pragma unroll
-                        for (int r = 0; r < 2; r++)
-#pragma unroll
-                            for (int j = 0; j < NJ; j++) ks[s][r][j] = __ldg(kp + r * 8 * NJ + j), vs[s][r][j] = __ldg(vp + r * 8 * NJ + j);
-                    }
-                    continue;
-                }
+        auto load_k = [&](int pg, int i, bool plain) {
+            const int tok = (u + i) * UNIT + warp * 16;
+            if (plain) {
+                const int64_t row = block_at(pg, tok);
+                const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * (D * ES) + k_lane;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const int64_t row = row_at(pg[s], tok, g + 8 * r);
-                    dead[s][r] = row < 0 && tok + g + 8 * r < n;
-                    const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * D * ES;
+                    dead[r] = false;
 #pragma unroll
-                    for (int j = 0; j < KW; j++) {
-                        const bool on = row >= 0 && (CACHE == Q8 ? 64 * j < D : 4 * j + t < chunks);
-                        kr[s][r][j] = on ? __ldg(reinterpret_cast<const uint4 *>(p) + 4 * j + t) : make_uint4(0, 0, 0, 0);
-                    }
-                    if constexpr (CACHE == Q8) {
+                    for (int j = 0; j < KW; j++) kr[r][j] = __ldg(reinterpret_cast<const uint4 *>(p + r * 8 * 64 * NJ * ES) + 4 * j);
+                }
+                if constexpr (CACHE == Q8) {
+                    const float *kp = a.c.ks + (row + g) * NJ, *vp = a.c.vs + (row + g) * NJ;
 #pragma unroll
-                        for (int j = 0; j < NJ; j++) {
-                            const bool on = row >= 0 && 64 * j < D;
-                            ks[s][r][j] = on ? __ldg(a.c.ks + row * (D / KV_BLOCK) + j) : 0.0f;
-                            vs[s][r][j] = on ? __ldg(a.c.vs + row * (D / KV_BLOCK) + j) : 0.0f;
-                        }
+                    for (int r = 0; r < 2; r++)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) ks[r][j] = __ldg(kp + r * 8 * NJ + j), vs[r][j] = __ldg(vp + r * 8 * NJ + j);
+                }
+                return;
+            }
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int64_t row = row_at(pg, tok, g + 8 * r);
+                dead[r] = row < 0 && tok + g + 8 * r < n;
+                const uint8_t *p = static_cast<const uint8_t *>(a.c.k) + row * D * ES;
+#pragma unroll
+                for (int j = 0; j < KW; j++) {
+                    const bool on = row >= 0 && (CACHE == Q8 ? 64 * j < D : 4 * j + t < chunks);
+                    kr[r][j] = on ? __ldg(reinterpret_cast<const uint4 *>(p) + 4 * j + t) : make_uint4(0, 0, 0, 0);
+                }
+                if constexpr (CACHE == Q8) {
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) {
+                        const bool on = row >= 0 && 64 * j < D;
+                        ks[r][j] = on ? __ldg(a.c.ks + row * (D / KV_BLOCK) + j) : 0.0f;
+                        vs[r][j] = on ? __ldg(a.c.vs + row * (D / KV_BLOCK) + j) : 0.0f;
                     }
                 }
             }
         };
-        auto load_v = [&](const int *pg, int i, bool plain) {
+        auto load_v = [&](int pg, int i, bool plain) {
+            const int tok = (u + i) * UNIT + warp * 16;
+            const uint8_t *base = static_cast<const uint8_t *>(a.c.v) + (plain ? block_at(pg, tok) * (D * ES) + v_lane : 0);
 #pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const int tok = (u + i) * UNIT + (warp * NS + s) * 16;
-                const uint8_t *base = static_cast<const uint8_t *>(a.c.v) + (plain ? block_at(pg[s], tok) * (D * ES) + v_lane : 0);
+            for (int r = 0; r < 4; r++) {
+                const int rel = (r & 1) + 8 * (r >> 1);
+                const int64_t row = plain ? 0 : row_at(pg, tok, 2 * t + rel);
+                const uint8_t *p = plain ? base + rel * 64 * NJ * ES : static_cast<const uint8_t *>(a.c.v) + row * D * ES + g * (8 * ES);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int rel = (r & 1) + 8 * (r >> 1);
-                    const int64_t row = plain ? 0 : row_at(pg[s], tok, 2 * t + rel);
-                    const uint8_t *p = plain ? base + rel * 64 * NJ * ES : static_cast<const uint8_t *>(a.c.v) + row * D * ES + g * (8 * ES);
-#pragma unroll
-                    for (int j = 0; j < NJ; j++) {
-                        const bool on = plain || (row >= 0 && g + 8 * j < chunks);
-                        if constexpr (CACHE == Q8) {
-                            const uint2 x = on ? __ldg(reinterpret_cast<const uint2 *>(p) + 8 * j) : make_uint2(0, 0);
-                            vr[s][r][j][0] = x.x, vr[s][r][j][1] = x.y;
-                        } else {
-                            const uint4 x = on ? __ldg(reinterpret_cast<const uint4 *>(p) + 8 * j) : make_uint4(0, 0, 0, 0);
-                            vr[s][r][j][0] = x.x, vr[s][r][j][1] = x.y, vr[s][r][j][2] = x.z, vr[s][r][j][3] = x.w;
-                        }
+                for (int j = 0; j < NJ; j++) {
+                    const bool on = plain || (row >= 0 && g + 8 * j < chunks);
+                    if constexpr (CACHE == Q8) {
+                        const uint2 x = on ? __ldg(reinterpret_cast<const uint2 *>(p) + 8 * j) : make_uint2(0, 0);
+                        vr[r][j][0] = x.x, vr[r][j][1] = x.y;
+                    } else {
+                        const uint4 x = on ? __ldg(reinterpret_cast<const uint4 *>(p) + 8 * j) : make_uint4(0, 0, 0, 0);
+                        vr[r][j][0] = x.x, vr[r][j][1] = x.y, vr[r][j][2] = x.z, vr[r][j][3] = x.w;
                     }
                 }
             }
         };
 
-        int pg[2] = {page_of(0), page2_of(0)}, pg_next[2];
+        int pg = page_of(0), pg_next;
         bool plain = plain_tile(pg, 0);
         if (plain) load_k(pg, 0, true), load_v(pg, 0, true);
         else load_k(pg, 0, false), load_v(pg, 0, false);
-        pg_next[0] = page_of(1), pg_next[1] = page2_of(1);
+        pg_next = page_of(1);
 
         // queries into shared memory as the products' column operands: a warp a head, a lane eight dims
         for (int h = warp; h < COLS; h += AD_WARPS) {
@@ -297,70 +282,66 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
 #pragma unroll
         for (int c = 0; c < NHT; c++) m[c][0] = m[c][1] = -kv_inf(), l[c][0] = l[c][1] = 0.0f;
 
+        // The next tile's keys are asked for once this one's scores are formed, its values after this one's.
         for (int i = 0; i < nseg; i++) {
-            const int tok = (u + i) * UNIT + warp * 16 * NS;
-            float s[NS][NHT][4];
+            const int tok = (u + i) * UNIT + warp * 16, pgv = pg_next;
+            const bool more = i + 1 < nseg, next_plain = more && plain_tile(pg_next, i + 1);
             // S^T = K Q^T
+            float s[NHT][4];
 #pragma unroll
-            for (int z = 0; z < NS; z++)
+            for (int c = 0; c < NHT; c++) {
+                s[c][0] = s[c][1] = s[c][2] = s[c][3] = 0.0f;
+                if constexpr (CACHE == Q8) {
 #pragma unroll
-                for (int c = 0; c < NHT; c++) {
-                    s[z][c][0] = s[z][c][1] = s[z][c][2] = s[z][c][3] = 0.0f;
-                    if constexpr (CACHE == Q8) {
+                    for (int j = 0; j < NJ; j++) {
+                        float p[4] = {bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1], bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1]};
+                        const uint32_t w0[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w};
+                        const uint32_t w1[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
 #pragma unroll
-                        for (int j = 0; j < NJ; j++) {
-                            float p[4] = {bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1], bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1]};
-                            const uint32_t w0[4] = {kr[z][0][j].x, kr[z][0][j].y, kr[z][0][j].z, kr[z][0][j].w};
-                            const uint32_t w1[4] = {kr[z][1][j].x, kr[z][1][j].y, kr[z][1][j].z, kr[z][1][j].w};
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const uint32_t f0 = w0[e] ^ 0x80808080u, f1 = w1[e] ^ 0x80808080u;
-                                const uint32_t a0 = LIFTED ? lifted2<false>(f0) : codes2<false>(f0), a1 = LIFTED ? lifted2<false>(f1) : codes2<false>(f1);
-                                const uint32_t a2 = LIFTED ? lifted2<true>(f0) : codes2<true>(f0), a3 = LIFTED ? lifted2<true>(f1) : codes2<true>(f1);
-#pragma unroll
-                                for (int k = NTQ - 1; k >= 0; k--) {
-                                    const uint4 q = qs[((k * NHT + c) * 2 * NJ + 2 * j + (e >> 1)) * 32 + lane];
-                                    mma16<OT>(p, a0, a1, a2, a3, e & 1 ? q.z : q.x, e & 1 ? q.w : q.y);
-                                }
-                            }
-                            s[z][c][0] = __fmaf_rn(p[0], ks[z][0][j], s[z][c][0]);
-                            s[z][c][1] = __fmaf_rn(p[1], ks[z][0][j], s[z][c][1]);
-                            s[z][c][2] = __fmaf_rn(p[2], ks[z][1][j], s[z][c][2]);
-                            s[z][c][3] = __fmaf_rn(p[3], ks[z][1][j], s[z][c][3]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 2 * NJ; j++)
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t f0 = w0[e] ^ 0x80808080u, f1 = w1[e] ^ 0x80808080u;
+                            const uint32_t a0 = LIFTED ? lifted2<false>(f0) : codes2<false>(f0), a1 = LIFTED ? lifted2<false>(f1) : codes2<false>(f1);
+                            const uint32_t a2 = LIFTED ? lifted2<true>(f0) : codes2<true>(f0), a3 = LIFTED ? lifted2<true>(f1) : codes2<true>(f1);
 #pragma unroll
                             for (int k = NTQ - 1; k >= 0; k--) {
-                                const uint4 q = qs[((k * NHT + c) * 2 * NJ + j) * 32 + lane];
-                                mma16<OT>(s[z][c], kr[z][0][j].x, kr[z][1][j].x, kr[z][0][j].y, kr[z][1][j].y, q.x, q.y);
-                                mma16<OT>(s[z][c], kr[z][0][j].z, kr[z][1][j].z, kr[z][0][j].w, kr[z][1][j].w, q.z, q.w);
+                                const uint4 q = qs[((k * NHT + c) * 2 * NJ + 2 * j + (e >> 1)) * 32 + lane];
+                                mma16<OT>(p, a0, a1, a2, a3, e & 1 ? q.z : q.x, e & 1 ? q.w : q.y);
                             }
+                        }
+                        s[c][0] = __fmaf_rn(p[0], ks[0][j], s[c][0]);
+                        s[c][1] = __fmaf_rn(p[1], ks[0][j], s[c][1]);
+                        s[c][2] = __fmaf_rn(p[2], ks[1][j], s[c][2]);
+                        s[c][3] = __fmaf_rn(p[3], ks[1][j], s[c][3]);
                     }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2 * NJ; j++)
+#pragma unroll
+                        for (int k = NTQ - 1; k >= 0; k--) {
+                            const uint4 q = qs[((k * NHT + c) * 2 * NJ + j) * 32 + lane];
+                            mma16<OT>(s[c], kr[0][j].x, kr[1][j].x, kr[0][j].y, kr[1][j].y, q.x, q.y);
+                            mma16<OT>(s[c], kr[0][j].z, kr[1][j].z, kr[0][j].w, kr[1][j].w, q.z, q.w);
+                        }
                 }
+            }
             // scores in the log2 domain; positions past the end have no weight, one without a row has no value
 #pragma unroll
-            for (int z = 0; z < NS; z++)
+            for (int c = 0; c < NHT; c++)
 #pragma unroll
-                for (int c = 0; c < NHT; c++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        s[z][c][e] = __fmul_rn(s[z][c][e], fac[c][e & 1]);
-                        if (!plain) s[z][c][e] = dead[z][e >> 1] ? kv_nan() : tok + 16 * z + g + 8 * (e >> 1) < n ? s[z][c][e] : -kv_inf();
-                    }
-            float pv[NS][2][CACHE == Q8 ? NJ : 1];   // the values' scales of this tile, below 2 by the power of two that O carries
+                for (int e = 0; e < 4; e++) {
+                    s[c][e] = __fmul_rn(s[c][e], fac[c][e & 1]);
+                    if (!plain) s[c][e] = dead[e >> 1] ? kv_nan() : tok + g + 8 * (e >> 1) < n ? s[c][e] : -kv_inf();
+                }
+            float pv[2][CACHE == Q8 ? NJ : 1];   // the values' scales of this tile, below 2 by the power of two that O carries
             if constexpr (CACHE == Q8) {
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
                     uint32_t top = 0;
 #pragma unroll
-                    for (int z = 0; z < NS; z++)
-#pragma unroll
-                        for (int r = 0; r < 2; r++) {
-                            const uint32_t bits = __float_as_uint(vs[z][r][j]);
-                            top = max(top, bits < 0x7f800000u ? bits : 0u);
-                        }
+                    for (int r = 0; r < 2; r++) {
+                        const uint32_t bits = __float_as_uint(vs[r][j]);
+                        top = max(top, bits < 0x7f800000u ? bits : 0u);
+                    }
                     const int e = (int)(__reduce_max_sync(0xffffffffu, top) >> 23);
                     if (e > ve[j]) {      // the same in every lane
                         const float f = ve[j] == 0 ? 0.0f : exp2_fast((float)(ve[j] - e));
@@ -374,36 +355,26 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                     }
                     const float inv = __uint_as_float((uint32_t)max(254 - ve[j], 1) << 23);
 #pragma unroll
-                    for (int z = 0; z < NS; z++)
-#pragma unroll
-                        for (int r = 0; r < 2; r++) pv[z][r][j] = ve[j] == 0 ? vs[z][r][j] : __fmul_rn(vs[z][r][j], inv);
+                    for (int r = 0; r < 2; r++) pv[r][j] = ve[j] == 0 ? vs[r][j] : __fmul_rn(vs[r][j], inv);
                 }
             }
-            const int pgv[2] = {pg_next[0], pg_next[1]};
-            const bool next_plain = i + 1 < nseg && plain_tile(pg_next, i + 1);
-            if (next_plain) load_k(pg_next, i + 1, true);
-            else if (i + 1 < nseg) load_k(pg_next, i + 1, false);
-            pg_next[0] = page_of(i + 2), pg_next[1] = page2_of(i + 2);
+            if (next_plain) load_k(pgv, i + 1, true);
+            else if (more) load_k(pgv, i + 1, false);
+            pg_next = page_of(i + 2);
 
-            // running maximum and sum
+            // running maximum and sum; the earlier sums fade together
 #pragma unroll
             for (int c = 0; c < NHT; c++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float x = m[c][e];
-#pragma unroll
-                    for (int z = 0; z < NS; z++) x = fmaxf(x, fmaxf(s[z][c][e], s[z][c][e + 2]));
+                    float x = fmaxf(m[c][e], fmaxf(s[c][e], s[c][e + 2]));
 #pragma unroll
                     for (int w = 4; w <= 16; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
                     const float base = x == -kv_inf() ? 0.0f : x, shift = __fsub_rn(base, POFF);
                     const float fade = exp2_fast(__fsub_rn(m[c][e], base));
-                    l[c][e] = __fmul_rn(l[c][e], fade);
-#pragma unroll
-                    for (int z = 0; z < NS; z++) {
-                        s[z][c][e] = exp2_fast(__fsub_rn(s[z][c][e], shift));
-                        s[z][c][e + 2] = exp2_fast(__fsub_rn(s[z][c][e + 2], shift));
-                        l[c][e] = __fadd_rn(l[c][e], __fadd_rn(s[z][c][e], s[z][c][e + 2]));
-                    }
+                    s[c][e] = exp2_fast(__fsub_rn(s[c][e], shift));
+                    s[c][e + 2] = exp2_fast(__fsub_rn(s[c][e + 2], shift));
+                    l[c][e] = __fmaf_rn(l[c][e], fade, __fadd_rn(s[c][e], s[c][e + 2]));
                     m[c][e] = x;
                     if (!__all_sync(0xffffffffu, fade == 1.0f)) {
 #pragma unroll
@@ -414,46 +385,43 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(NJ, NHT)) k_attn_split(con
                 }
 
             // O^T += V^T P^T
+            uint32_t bp[NHT][CACHE == Q8 ? NJ : 1][NTP][2];
 #pragma unroll
-            for (int z = 0; z < NS; z++) {
-                uint32_t bp[NHT][CACHE == Q8 ? NJ : 1][NTP][2];
+            for (int c = 0; c < NHT; c++)
 #pragma unroll
-                for (int c = 0; c < NHT; c++)
-#pragma unroll
-                    for (int j = 0; j < (CACHE == Q8 ? NJ : 1); j++) {
-                        float x[4] = {s[z][c][0], s[z][c][1], s[z][c][2], s[z][c][3]};
-                        if constexpr (CACHE == Q8) {
-                            x[0] = __fmul_rn(x[0], pv[z][0][j]), x[1] = __fmul_rn(x[1], pv[z][0][j]);
-                            x[2] = __fmul_rn(x[2], pv[z][1][j]), x[3] = __fmul_rn(x[3], pv[z][1][j]);
-                        }
-#pragma unroll
-                        for (int k = 0; k < NTP; k++) {
-                            bp[c][j][k][0] = trans8x8(take_pair<OT>(x[0], x[1]));
-                            bp[c][j][k][1] = trans8x8(take_pair<OT>(x[2], x[3]));
-                        }
+                for (int j = 0; j < (CACHE == Q8 ? NJ : 1); j++) {
+                    float x[4] = {s[c][0], s[c][1], s[c][2], s[c][3]};
+                    if constexpr (CACHE == Q8) {
+                        x[0] = __fmul_rn(x[0], pv[0][j]), x[1] = __fmul_rn(x[1], pv[0][j]);
+                        x[2] = __fmul_rn(x[2], pv[1][j]), x[3] = __fmul_rn(x[3], pv[1][j]);
                     }
 #pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint32_t a0, a1, a2, a3;
-                        if constexpr (CACHE == Q8) {
-                            const uint32_t w0 = __byte_perm(vr[z][0][j][k >> 1], vr[z][1][j][k >> 1], k & 1 ? 0x7362 : 0x5140) ^ 0x80808080u;
-                            const uint32_t w1 = __byte_perm(vr[z][2][j][k >> 1], vr[z][3][j][k >> 1], k & 1 ? 0x7362 : 0x5140) ^ 0x80808080u;
-                            a0 = codes2<false>(w0), a1 = codes2<true>(w0), a2 = codes2<false>(w1), a3 = codes2<true>(w1);
-                        } else {
-                            a0 = __byte_perm(vr[z][0][j][k], vr[z][1][j][k], 0x5410), a1 = __byte_perm(vr[z][0][j][k], vr[z][1][j][k], 0x7632);
-                            a2 = __byte_perm(vr[z][2][j][k], vr[z][3][j][k], 0x5410), a3 = __byte_perm(vr[z][2][j][k], vr[z][3][j][k], 0x7632);
-                        }
-#pragma unroll
-                        for (int c = 0; c < NHT; c++)
-#pragma unroll
-                            for (int x = NTP - 1; x >= 0; x--)
-                                mma16<OT>(o[c][j][k], a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
+                    for (int k = 0; k < NTP; k++) {
+                        bp[c][j][k][0] = trans8x8(take_pair<OT>(x[0], x[1]));
+                        bp[c][j][k][1] = trans8x8(take_pair<OT>(x[2], x[3]));
                     }
-            }
+                }
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t a0, a1, a2, a3;
+                    if constexpr (CACHE == Q8) {
+                        const uint32_t w0 = __byte_perm(vr[0][j][k >> 1], vr[1][j][k >> 1], k & 1 ? 0x7362 : 0x5140) ^ 0x80808080u;
+                        const uint32_t w1 = __byte_perm(vr[2][j][k >> 1], vr[3][j][k >> 1], k & 1 ? 0x7362 : 0x5140) ^ 0x80808080u;
+                        a0 = codes2<false>(w0), a1 = codes2<true>(w0), a2 = codes2<false>(w1), a3 = codes2<true>(w1);
+                    } else {
+                        a0 = __byte_perm(vr[0][j][k], vr[1][j][k], 0x5410), a1 = __byte_perm(vr[0][j][k], vr[1][j][k], 0x7632);
+                        a2 = __byte_perm(vr[2][j][k], vr[3][j][k], 0x5410), a3 = __byte_perm(vr[2][j][k], vr[3][j][k], 0x7632);
+                    }
+#pragma unroll
+                    for (int c = 0; c < NHT; c++)
+#pragma unroll
+                        for (int x = NTP - 1; x >= 0; x--)
+                            mma16<OT>(o[c][j][k], a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
+                }
             if (next_plain) load_v(pgv, i + 1, true);
-            else if (i + 1 < nseg) load_v(pgv, i + 1, false);
+            else if (more) load_v(pgv, i + 1, false);
             plain = next_plain;
         }
 
@@ -604,9 +572,10 @@ Plan plan_of(const hxb_kv_cache *c, int H) {
     // 16 columns halve the reads of groups over 8; at 256 dims their sums do not fit the registers
     p.nht = group > 8 && p.nj <= 2 ? 2 : 1;
     p.passes = (group + 8 * p.nht - 1) / (8 * p.nht);
-    p.ctas = ATTN_SMS * ad_ctas(p.nj, p.nht);
-    p.ml = (size_t)p.ctas * 2 * 8 * p.nht * sizeof(float2);
-    p.o = (size_t)p.ctas * 2 * 8 * p.nht * c->head_dim * sizeof(float);
+    p.ctas = ATTN_SMS * ad_ctas(c->dtype, p.nj, p.nht);
+    const int most = ATTN_SMS * std::max(ad_ctas(Q8, p.nj, p.nht), ad_ctas(BF16, p.nj, p.nht));      // one size for every type
+    p.ml = (size_t)most * 2 * 8 * p.nht * sizeof(float2);
+    p.o = (size_t)most * 2 * 8 * p.nht * c->head_dim * sizeof(float);
     p.bytes = p.ml + p.o;
     return p;
 }

@@ -321,23 +321,29 @@ struct RawRows {
         d = on ? __ldg(a.c.ks + row * segs + s) : 0.0f;
     }
 };
-// 16 codes times d as f16, into pieces 2 q and 2 q + 1 of a block row.
-__device__ __forceinline__ void expand16(uint32_t at, int rw, int q, const uint4 &code, float d) {
-    const uint32_t in[4] = {code.x ^ 0x80808080u, code.y ^ 0x80808080u, code.z ^ 0x80808080u, code.w ^ 0x80808080u};
-    uint32_t o[8];
+// 32 codes times d as f16, into four 16-byte pieces of a block row, in packed f32 pairs.
+__device__ __forceinline__ void expand32(uint32_t at, int rw, int half, const RawRows &r) {
+    const uint64_t d2 = (uint64_t)__float_as_uint(r.d) << 32 | __float_as_uint(r.d);
+    const uint64_t off = (uint64_t)__float_as_uint(-8388736.0f) << 32 | __float_as_uint(-8388736.0f);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        // 2^23 + (code + 128) as a float's bits
-        const float lo = __uint_as_float(__byte_perm(in[e >> 1], 0x4b000000u, e & 1 ? 0x7542 : 0x7540)) - 8388736.0f;
-        const float hi = __uint_as_float(__byte_perm(in[e >> 1], 0x4b000000u, e & 1 ? 0x7543 : 0x7541)) - 8388736.0f;
-        const __half2 h = __floats2half2_rn(__fmul_rn(lo, d), __fmul_rn(hi, d));
-        o[e] = reinterpret_cast<const uint32_t &>(h);
-    }
+    for (int c = 0; c < 4; c++) {      // eight codes a piece
+        const uint4 &w4 = r.code[c >> 1];
+        uint32_t o[4];
 #pragma unroll
-    for (int c = 0; c < 2; c++)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + rw * 128 + (((2 * q + c) ^ (rw & 7)) << 4)), "r"(o[4 * c]),
-                     "r"(o[4 * c + 1]), "r"(o[4 * c + 2]), "r"(o[4 * c + 3])
+        for (int e = 0; e < 4; e++) {
+            const uint32_t w = (c & 1 ? (e < 2 ? w4.z : w4.w) : (e < 2 ? w4.x : w4.y)) ^ 0x80808080u;
+            // 2^23 + (code + 128) as a float's bits, twice
+            const uint32_t lo = __byte_perm(w, 0x4b000000u, e & 1 ? 0x7542 : 0x7540), hi = __byte_perm(w, 0x4b000000u, e & 1 ? 0x7543 : 0x7541);
+            uint64_t x = (uint64_t)hi << 32 | lo;
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(off));
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(d2));
+            const __half2 h = __floats2half2_rn(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
+            o[e] = reinterpret_cast<const uint32_t &>(h);
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + rw * 128 + (((4 * half + c) ^ (rw & 7)) << 4)), "r"(o[0]),
+                     "r"(o[1]), "r"(o[2]), "r"(o[3])
                      : "memory");
+    }
 }
 
 // Query rows of a run as the S product's first operand: eight lanes a head, all of its loads before their use.
@@ -445,24 +451,27 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                 const int k = k0 + i;
                 rows.find(a, r, i, lt);
                 if constexpr (CACHE == Q8) {
-                    RawRows raw[5];
+                    // three block columns ahead of the one at work; rolled, since the unrolled code was fetched slower than it ran
+                    RawRows raw[3];
 #pragma unroll
-                    for (int s = 0; s < 5; s++) raw[s].fetch(a, rows.row[0], s, segs, lt);
+                    for (int s = 0; s < 3; s++) raw[s].fetch(a, rows.row[0], s, segs, lt);
                     if (k >= 2) ok = wait(&y.freed[buf], ((k >> 1) - 1) & 1);
-                    if (!ok) break;
                     bool all = k < 2;
+#pragma unroll 1
+                    for (int s0 = 0; ok && s0 < segs; s0 += 3)
 #pragma unroll
-                    for (int s = 0; s < 9; s++) {
-                        if (s < segs) {
+                        for (int e = 0; e < 3; e++) {
+                            const int s = s0 + e;
+                            if (s >= segs) break;
                             if (s >= 2 * half && !all) {
                                 ok = wait(&y.done[buf], ((k >> 1) - 1) & 1), all = true;
                                 if (!ok) break;
                             }
-                            expand16(dst + s * SEG, lt >> 1, 2 * (lt & 1), raw[s % 5].code[0], raw[s % 5].d);
-                            expand16(dst + s * SEG, lt >> 1, 2 * (lt & 1) + 1, raw[s % 5].code[1], raw[s % 5].d);
+                            const RawRows now = raw[e];
+                            raw[e].fetch(a, rows.row[0], s + 3, segs, lt);
+                            expand32(dst + s * SEG, lt >> 1, lt & 1, now);
                         }
-                        if (s < 4) raw[s % 5].fetch(a, rows.row[0], s + 5, segs, lt);
-                    }
+                    if (!ok) break;
                 } else {
                     const int c8 = lt & 7, tail = a.dr / 8;
                     auto copy = [&](int s0, int s1) {
