@@ -40,9 +40,12 @@ namespace {
 constexpr int LT = 64;                  // positions a tile
 constexpr int LH = 64;                  // heads a CTA (rows of S)
 constexpr int SEG = LT * 128;           // 64 dims of 64 rows: a 128-byte swizzled block column
-constexpr int LD_WARPS = 4, LD_THREADS = 32 * LD_WARPS;      // loading warps a tile buffer
-constexpr int SCORE_WARP = 4, VALUE_WARP = 5, LD_WARP0 = 6;
-constexpr int CORE_WARPS = LD_WARP0 + 2 * LD_WARPS, CORE_THREADS = 32 * CORE_WARPS;
+constexpr int SCORE_WARP = 4, LD_WARP0 = 6, LD_WARPS = 8;       // 0-3 softmax, 4 scores, 5 values, the others load
+constexpr int CORE_WARPS = LD_WARP0 + LD_WARPS, CORE_THREADS = 32 * CORE_WARPS;
+// 16-bit rows: four loading warps for each of the two tile buffers, so that one in flight never waits for the other. Q8: all
+// eight for one tile after the other: expanding a tile takes four warps as long as both tiles' products.
+template <int CACHE> constexpr int LD_GROUPS = CACHE == Q8 ? 1 : 2;
+template <int CACHE> constexpr int LD_THREADS = 32 * LD_WARPS / LD_GROUPS<CACHE>;
 constexpr float REF_SLACK = 7.0f;
 
 struct LatentArgs {
@@ -284,13 +287,13 @@ struct Walk {
     }
 };
 
-// A loading thread's rows of a tile. 16-bit rows: eight lanes a 128-byte block row, 16 rows at once; Q8: two lanes a row.
+// A loading thread's rows of a tile. 16-bit rows: eight lanes a 128-byte block row, 16 rows at once; Q8: four lanes a row.
 template <int CACHE>
 struct TileRows {
     static constexpr int N = CACHE == Q8 ? 1 : 4;
     int64_t row[N];
     uint32_t dead;      // positions in range that have no row
-    static __device__ __forceinline__ int at(int lt, int k) { return CACHE == Q8 ? lt >> 1 : (lt >> 3) + 16 * k; }
+    static __device__ __forceinline__ int at(int lt, int k) { return CACHE == Q8 ? lt >> 2 : (lt >> 3) + 16 * k; }
     __device__ __forceinline__ void find(const LatentArgs &a, const Run &r, int tile, int lt) {
         dead = 0;
 #pragma unroll
@@ -302,36 +305,36 @@ struct TileRows {
     }
     // marks them for the softmax (bit position of the tile)
     __device__ __forceinline__ void mark(CoreShared &y, int buf, int lt) const {
-        if (!dead || (lt & (CACHE == Q8 ? 1 : 7))) return;
+        if (!dead || (lt & (CACHE == Q8 ? 3 : 7))) return;
 #pragma unroll
         for (int k = 0; k < N; k++)
             if (dead >> k & 1) atomicOr(&y.dead[buf][at(lt, k) >> 5], 1u << (at(lt, k) & 31));
     }
 };
 
-// Raw Q8 codes of half a block column, and the scales: asked for a step ahead of their use.
+// Sixteen Q8 codes of a block and their scale. The loads are volatile so that they stay where they are written: ahead of
+// the wait for the buffer.
 struct RawRows {
-    uint4 code[2];
+    uint4 code;
     float d;
     __device__ __forceinline__ void fetch(const LatentArgs &a, int64_t row, int s, int segs, int lt) {
-        const bool on = row >= 0 && s < segs;
-        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(a.c.k) + row * a.c.hd + s * 64) + 2 * (lt & 1);
-        code[0] = on ? __ldg(p) : make_uint4(0, 0, 0, 0);
-        code[1] = on ? __ldg(p + 1) : make_uint4(0, 0, 0, 0);
-        d = on ? __ldg(a.c.ks + row * segs + s) : 0.0f;
+        code = make_uint4(0, 0, 0, 0), d = 0.0f;
+        if (row < 0 || s >= segs) return;
+        const int8_t *p = static_cast<const int8_t *>(a.c.k) + row * a.c.hd + s * 64 + 16 * (lt & 3);
+        asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(code.x), "=r"(code.y), "=r"(code.z), "=r"(code.w) : "l"(p));
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(d) : "l"(a.c.ks + row * segs + s));
     }
 };
-// 32 codes times d as f16, into four 16-byte pieces of a block row, in packed f32 pairs.
-__device__ __forceinline__ void expand32(uint32_t at, int rw, int half, const RawRows &r) {
+// The codes times d as f16, into pieces 2 q and 2 q + 1 of a block row, in packed f32 pairs.
+__device__ __forceinline__ void expand16(uint32_t at, int rw, int q, const RawRows &r) {
     const uint64_t d2 = (uint64_t)__float_as_uint(r.d) << 32 | __float_as_uint(r.d);
     const uint64_t off = (uint64_t)__float_as_uint(-8388736.0f) << 32 | __float_as_uint(-8388736.0f);
 #pragma unroll
-    for (int c = 0; c < 4; c++) {      // eight codes a piece
-        const uint4 &w4 = r.code[c >> 1];
+    for (int c = 0; c < 2; c++) {
         uint32_t o[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const uint32_t w = (c & 1 ? (e < 2 ? w4.z : w4.w) : (e < 2 ? w4.x : w4.y)) ^ 0x80808080u;
+            const uint32_t w = (c ? (e < 2 ? r.code.z : r.code.w) : (e < 2 ? r.code.x : r.code.y)) ^ 0x80808080u;
             // 2^23 + (code + 128) as a float's bits, twice
             const uint32_t lo = __byte_perm(w, 0x4b000000u, e & 1 ? 0x7542 : 0x7540), hi = __byte_perm(w, 0x4b000000u, e & 1 ? 0x7543 : 0x7541);
             uint64_t x = (uint64_t)hi << 32 | lo;
@@ -340,18 +343,18 @@ __device__ __forceinline__ void expand32(uint32_t at, int rw, int half, const Ra
             const __half2 h = __floats2half2_rn(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
             o[e] = reinterpret_cast<const uint32_t &>(h);
         }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + rw * 128 + (((4 * half + c) ^ (rw & 7)) << 4)), "r"(o[0]),
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + rw * 128 + (((2 * q + c) ^ (rw & 7)) << 4)), "r"(o[0]),
                      "r"(o[1]), "r"(o[2]), "r"(o[3])
                      : "memory");
     }
 }
 
 // Query rows of a run as the S product's first operand: eight lanes a head, all of its loads before their use.
-template <int OT>
+template <int OT, int THREADS>
 __device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint32_t dst, int segs, const Run &r, int h0, int nh, int lt) {
     const int c8 = lt & 7, W = a.R + a.dr;
 #pragma unroll 1
-    for (int h = lt >> 3; h < LH; h += LD_THREADS / 8) {
+    for (int h = lt >> 3; h < LH; h += THREADS / 8) {
         const float4 *src = reinterpret_cast<const float4 *>(a.qa + ((int64_t)r.b * a.H + h0 + h) * W) + 2 * c8;
         float4 x[9][2];
 #pragma unroll
@@ -415,7 +418,7 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
     }
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&y.full[i], LD_THREADS);
+            mbar_init(&y.full[i], LD_THREADS<CACHE>);
             mbar_init(&y.freed[i], 1);
             mbar_init(&y.sfull[i], 1);
             mbar_init(&y.sfree[i], 128);
@@ -439,26 +442,28 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
 
     const int pieces = a.R / 128, half = (pieces + 1) / 2;      // blocks of 128 dims; those freed first
     if (warp >= LD_WARP0) {
-        // ---- loading: the first four warps the even tiles, the others the odd ones
-        const int buf = (warp - LD_WARP0) / LD_WARPS, lt = tid - 32 * (LD_WARP0 + buf * LD_WARPS);
-        const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
+        // ---- loading: a group takes every GROUPS-th tile
+        constexpr int GROUPS = LD_GROUPS<CACHE>, THREADS = LD_THREADS<CACHE>;
+        const int group = (tid - 32 * LD_WARP0) / THREADS, lt = (tid - 32 * LD_WARP0) % THREADS;
         TileRows<CACHE> rows;
         auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, core_wait(y, bar, parity, a.err)); };
         bool ok = true, waited = false;
         int k0 = 0;      // tiles before this run
         while (ok && walk.next(r)) {
-            for (int i = (k0 ^ buf) & 1; ok && i < r.tiles; i += 2) {
-                const int k = k0 + i;
+            for (int i = GROUPS == 1 ? 0 : (k0 ^ group) & 1; ok && i < r.tiles; i += GROUPS) {
+                const int k = k0 + i, buf = k & 1;
+                const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
                 rows.find(a, r, i, lt);
                 if constexpr (CACHE == Q8) {
-                    // three block columns ahead of the one at work; rolled, since the unrolled code was fetched slower than it ran
-                    RawRows raw[3];
+                    // all of a tile's codes into registers while the tiles before are at work; then three block columns at a time,
+                    // the registers moved down in between (unrolled to nine the code was fetched slower than it ran)
+                    RawRows raw[9];
 #pragma unroll
-                    for (int s = 0; s < 3; s++) raw[s].fetch(a, rows.row[0], s, segs, lt);
+                    for (int s = 0; s < 9; s++) raw[s].fetch(a, rows.row[0], s, segs, lt);
                     if (k >= 2) ok = wait(&y.freed[buf], ((k >> 1) - 1) & 1);
                     bool all = k < 2;
 #pragma unroll 1
-                    for (int s0 = 0; ok && s0 < segs; s0 += 3)
+                    for (int s0 = 0; ok && s0 < segs; s0 += 3) {
 #pragma unroll
                         for (int e = 0; e < 3; e++) {
                             const int s = s0 + e;
@@ -467,10 +472,11 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                                 ok = wait(&y.done[buf], ((k >> 1) - 1) & 1), all = true;
                                 if (!ok) break;
                             }
-                            const RawRows now = raw[e];
-                            raw[e].fetch(a, rows.row[0], s + 3, segs, lt);
-                            expand32(dst + s * SEG, lt >> 1, lt & 1, now);
+                            expand16(dst + s * SEG, lt >> 2, lt & 3, raw[e]);
                         }
+#pragma unroll
+                        for (int e = 0; e < 6; e++) raw[e] = raw[e + 3];
+                    }
                     if (!ok) break;
                 } else {
                     const int c8 = lt & 7, tail = a.dr / 8;
@@ -499,7 +505,7 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                     if (!waited) pdl_wait(), waited = true;
                     if (k >= 1) ok = wait(&y.done[buf ^ 1], ((k - 1) >> 1) & 1);
                     if (!ok) break;
-                    load_q<OT>(a, y, smem_u32(qb), segs, r, h0, nh, lt);
+                    load_q<OT, THREADS>(a, y, smem_u32(qb), segs, r, h0, nh, lt);
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_proxy_async();
