@@ -50,7 +50,9 @@ struct Shares {
     __device__ __forceinline__ int64_t start(int cta) const { return cta * each + min(cta, more); }
     __device__ __forceinline__ int of(int64_t unit) const {      // the share a unit is in
         const int64_t big = more * (each + 1);
-        return (int)(unit < big ? unit / (each + 1) : more + (unit - big) / each);
+        const int64_t n = unit < big ? unit : unit - big, d = unit < big ? each + 1 : each;
+        const int q = ((n | d) >> 32) == 0 ? (int)((uint32_t)n / (uint32_t)d) : (int)(n / d);
+        return unit < big ? q : more + q;
     }
 };
 

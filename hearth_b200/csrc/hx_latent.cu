@@ -740,21 +740,25 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
 
 // ------------------------------------------------------------------------------------------- expand
 
-constexpr int EX_WARPS = 8, EX_ROWS = 8;
+constexpr int EX_WARPS = 16, EX_ROWS = 16;
 
 struct ExpandShared {
-    uint4 ops[2][16][32];                // [term][32-dim step][lane]
-    float join[EX_WARPS][512];
+    uint32_t ops[2][16][2][32][4];       // [term][32-dim step][eight rows][lane]
+    union {
+        float join[EX_WARPS][512];
+        float red[16][16 * EX_ROWS];
+    };
     float2 ml[EX_WARPS];
-    float red[16][16 * EX_ROWS];
+    uint32_t over;                       // sequences longer than their table
     int64_t sums[EX_WARPS][2];
 };
 
-// A CTA a head and up to eight sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as
+// A CTA a head and up to sixteen sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as
 // two terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o.
 template <int T>
-__global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid_constant__ LatentArgs a, int ex_rows, int grid) {
-    __shared__ __align__(16) ExpandShared y;
+__global__ void __launch_bounds__(32 * EX_WARPS, 1) k_latent_expand(const __grid_constant__ LatentArgs a, int ex_rows, int grid) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    ExpandShared &y = *reinterpret_cast<ExpandShared *>(raw);
     const int h = blockIdx.x, b0 = blockIdx.y * ex_rows, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rows = min(ex_rows, a.c.n_seqs - b0), pass = h / a.hp, hc = h - pass * a.hp, W = a.R + a.dr, steps = a.R / 32;
     // warps over (16 value rows, part of the latent dims): ksplit parts where there are fewer row tiles than warps
@@ -766,14 +770,14 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid
         const uint16_t *p = w + (int64_t)(item % mt) * 16 * a.R + s * 32;
         v[0] = __ldg(reinterpret_cast<const uint4 *>(p)), v[1] = __ldg(reinterpret_cast<const uint4 *>(p + 8 * (int64_t)a.R));
     };
-    uint4 pre[8][2];      // the first 256 dims of the warp's first part, under way before the core has ended
-    const int p0 = first(warp), p1 = last(warp);
-#pragma unroll
-    for (int s = 0; s < 8; s++) {
-        pre[s][0] = pre[s][1] = make_uint4(0, 0, 0, 0);
-        if (p0 + s < p1) fetch(warp, p0 + s, pre[s]);
+    // the head's value rows on their way to L2 before the core has ended
+    for (int i = threadIdx.x; i < a.dv * (a.R / 64); i += 32 * EX_WARPS)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t *>(a.w) + ((int64_t)h * (a.dn + a.dv) + a.dn) * a.R + (int64_t)i * 64));
+    for (int i = threadIdx.x; i < 2 * 16 * 2 * 32; i += 32 * EX_WARPS) reinterpret_cast<uint4 *>(&y.ops)[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < 32) {
+        const uint32_t over = __ballot_sync(0xffffffffu, lane < rows && a.lens[b0 + min(lane, rows - 1)] > table_capacity(a.c));
+        if (lane == 0) y.over = over;
     }
-    for (int i = threadIdx.x; i < 2 * 16 * 32; i += 32 * EX_WARPS) (&y.ops[0][0][0])[i] = make_uint4(0, 0, 0, 0);
     // the warp's row and its pieces, from the lengths
     int wpr = EX_WARPS;                                  // warps a row
     while (wpr * rows > EX_WARPS) wpr >>= 1;
@@ -784,18 +788,18 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid
     const int n = a.lens[b], nu = units_of(a.c, a.lens, b, LT);
     Span sp = {};
     if (nu) sp = span_of(before, nu, all, grid);
-    // Twice in an SM's first CTA: the first round, on whatever the scratch holds, brings the code near while the core still
-    // runs (code that runs once is fetched slower than it runs); only the second stores.
+    // Twice in an SM's first CTA where the core leaves SMs free: the first round, on whatever the scratch holds, brings the code
+    // near while the core still runs (code that runs once is fetched slower than it runs); only the second stores.
 #pragma unroll 1
-    for (int round = blockIdx.y * gridDim.x + blockIdx.x < ATTN_SMS ? 0 : 1; round < 2; round++) {
+    for (int round = all < grid && blockIdx.y * gridDim.x + blockIdx.x < ATTN_SMS ? 0 : 1; round < 2; round++) {
         if (round) pdl_wait();
         __syncthreads();
         if (row < rows) {
             Joined<16> o;
             const float *whole = a.qa + ((int64_t)b * a.H + h) * W;
             const int count = !nu ? 0 : sp.split() ? sp.last - sp.first + 1 : 1;
-#pragma unroll 2
-            for (int i = part; i < (round ? count : min(count, 2 * wpr)); i += wpr) {
+#pragma unroll 4
+            for (int i = part; i < (round ? count : min(count, 4 * wpr)); i += wpr) {
                 const int64_t at = ((int64_t)((sp.first + i) * a.passes + pass) * 2 + (i == 0 ? sp.slot : 0)) * a.hp + hc;
                 const float *src = sp.split() ? a.o + at * a.R : whole;
                 const float2 ml = sp.split() ? __ldcg(a.ml + at) : make_float2(__ldcg(whole + a.R), __ldcg(whole + a.R + 1));
@@ -814,51 +818,49 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 2) k_latent_expand(const __grid
             if (lane == 0) y.ml[warp] = make_float2(o.m, o.l);
         }
         __syncthreads();
-        // the row's warps together, eight dims a lane; nothing, too long a row and a failed wait as the entry point says
-        if (row < rows) {
-            const bool bad = n > table_capacity(a.c) || *reinterpret_cast<volatile int *>(a.err);
-            for (int c = lane + 32 * part; c < a.R / 8; c += 32 * wpr) {
-                Joined<8> o;
-                for (int p = 0; p < wpr; p++) o.add(y.ml[warp - part + p], &y.join[warp - part + p][8 * c]);
-                const float inv = bad ? kv_nan() : __fdiv_rn(1.0f, o.l);
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = !bad && o.l == 0.0f ? 0.0f : __fmul_rn(o.o[i], inv);
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    uint4 v;
-                    v.x = take_pair<T>(x[0], x[1]), v.y = take_pair<T>(x[2], x[3]), v.z = take_pair<T>(x[4], x[5]), v.w = take_pair<T>(x[6], x[7]);
-                    y.ops[k][c >> 2][row * 4 + (c & 3)] = v;
-                }
+        // a row's warps together, two dims a thread; nothing, too long a row and a failed wait as the entry point says
+        const bool failed = *reinterpret_cast<volatile int *>(a.err);
+        for (int i = threadIdx.x; i < rows * (a.R / 2); i += 32 * EX_WARPS) {
+            const int rw = i / (a.R / 2), d = 2 * (i - rw * (a.R / 2));
+            Joined<2> o;
+            if (wpr == 1) {
+                o.l = y.ml[rw].y, o.o[0] = y.join[rw][d], o.o[1] = y.join[rw][d + 1];
+            } else {
+#pragma unroll 2
+                for (int p = rw * wpr; p < (rw + 1) * wpr; p++) o.add(y.ml[p], &y.join[p][d]);
             }
+            const bool bad = failed || (y.over >> rw & 1);
+            const float inv = bad ? kv_nan() : o.l == 0.0f ? 0.0f : __fdiv_rn(1.0f, o.l);
+            float x0 = bad || o.l != 0.0f ? __fmul_rn(o.o[0], inv) : 0.0f, x1 = bad || o.l != 0.0f ? __fmul_rn(o.o[1], inv) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; k++) y.ops[k][d >> 5][rw >> 3][(rw & 7) * 4 + ((d >> 3) & 3)][(d >> 1) & 3] = take_pair<T>(x0, x1);
         }
         __syncthreads();
         for (int item = warp; item < items; item += EX_WARPS) {
-            float acc[4] = {};
+            float acc[2][4] = {};
             auto step = [&](int s, const uint4 v[2]) {
 #pragma unroll
-                for (int k = 1; k >= 0; k--) {
-                    const uint4 x = y.ops[k][s][lane];
-                    mma16<T>(acc, v[0].x, v[1].x, v[0].y, v[1].y, x.x, x.y);
-                    mma16<T>(acc, v[0].z, v[1].z, v[0].w, v[1].w, x.z, x.w);
+                for (int c = 0; c < 2; c++) {
+                    if (8 * c >= rows) break;
+#pragma unroll
+                    for (int k = 1; k >= 0; k--) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(y.ops[k][s][c][lane]);
+                        mma16<T>(acc[c], v[0].x, v[1].x, v[0].y, v[1].y, x.x, x.y);
+                        mma16<T>(acc[c], v[0].z, v[1].z, v[0].w, v[1].w, x.z, x.w);
+                    }
                 }
             };
-            int s = first(item);
             const int end = last(item);
-            if (item == warp) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (s + i < end) step(s + i, pre[i]);
-                s += 8;
-            }
-#pragma unroll 4
-            for (; s < end; s++) {
+#pragma unroll 8
+            for (int s = first(item); s < end; s++) {
                 uint4 v[2];
                 fetch(item, s, v);
                 step(s, v);
             }
-            y.red[item][g * EX_ROWS + 2 * t] = acc[0], y.red[item][g * EX_ROWS + 2 * t + 1] = acc[1];
-            y.red[item][(g + 8) * EX_ROWS + 2 * t] = acc[2], y.red[item][(g + 8) * EX_ROWS + 2 * t + 1] = acc[3];
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) y.red[item][(g + 8 * (e >> 1)) * EX_ROWS + 8 * c + 2 * t + (e & 1)] = acc[c][e];
         }
         __syncthreads();
         for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
@@ -896,15 +898,17 @@ template <int CACHE, int T>
 cudaError_t launch(const LatentArgs &a, const Plan &p, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(k_latent_core<CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
     if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(k_latent_expand<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ExpandShared));
+    if (e != cudaSuccess) return e;
     const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS), B = a.c.n_seqs;
     e = launch_pdl(false, k_latent_absorb<T>, dim3(a.H * nc, (B + AB_ROWS - 1) / AB_ROWS), dim3(32 * AB_WARPS), 0, s, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a);
     if (e != cudaSuccess) return e;
-    // eight sequences share a read of the value rows; fewer a CTA where that would leave SMs without one
+    // sixteen sequences share a read of the value rows; fewer a CTA where that would leave SMs without one
     int rows = EX_ROWS;
-    while (rows > 1 && a.H * ((B + rows - 1) / rows) < 2 * ATTN_SMS) rows /= 2;
-    return launch_pdl(true, k_latent_expand<T>, dim3(a.H, (B + rows - 1) / rows), dim3(32 * EX_WARPS), 0, s, a, rows, p.grid / p.passes);
+    while (rows > 1 && 4 * a.H * ((B + rows - 1) / rows) < 3 * ATTN_SMS) rows /= 2;
+    return launch_pdl(true, k_latent_expand<T>, dim3(a.H, (B + rows - 1) / rows), dim3(32 * EX_WARPS), sizeof(ExpandShared), s, a, rows, p.grid / p.passes);
 }
 
 }  // namespace
