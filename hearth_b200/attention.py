@@ -11,8 +11,9 @@ one new token a sequence over it, for programs that keep their own decoder aroun
 Caches are plain tensors: k_cache, v_cache [n_pages, n_kv_heads, page_tokens, head_dim] in float16, bfloat16 or,
 quantised in blocks of 64, int8 with k_scale, v_scale [n_pages, n_kv_heads, page_tokens, head_dim / 64] float32.
 table [n_seqs, max_pages] int32 names the pages of each sequence (an expanded row is one table for all). Work is
-enqueued on `stream` (default: torch's current stream of the tensors' device) without waiting; a wrong argument
-raises ValueError before anything is enqueued.
+enqueued on `stream` (default: torch's current stream of the tensors' device) without waiting, and what a call allocates
+(outputs that are not given, scratch) belongs to that stream; tensors passed in have to live until the stream is done with
+them. A wrong argument raises ValueError before anything is enqueued.
 """
 from __future__ import annotations
 
@@ -73,6 +74,8 @@ class _on:
         for t in tensors:
             if t is not None and t.device != dev:
                 _bad("tensors must be on one CUDA device")
+        if getattr(stream, "device", dev) != dev:
+            _bad(f"stream is on {stream.device}, the tensors are on {dev}")
         self.guard = None if cuda.current_device() == dev.index else cuda.device(dev)
         self.dev, self.user = dev, stream
         self.ptr = (_torch()[3](dev.index) or _CUDA_STREAM_LEGACY) if stream is None else _stream(stream)
@@ -86,17 +89,24 @@ class _on:
         if self.guard is not None:
             self.guard.__exit__(*a)
 
-    def scratch(self, given, n):
-        """n bytes for work on the call's stream."""
-        torch = _torch()[0]
-        if given is not None:
-            if given.dtype != torch.uint8 or not given.is_contiguous() or given.numel() < n:
-                _bad(f"workspace must be a contiguous uint8 tensor of at least {n} bytes")
-            return given
-        t = torch.empty(n, dtype=torch.uint8, device=self.dev)
+    def new(self, like, shape, dtype):
+        """A new contiguous tensor beside `like`, in the memory of the call's stream."""
+        cuda = _torch()[0].cuda
         if self.user is not None:
-            t.record_stream(self.user if hasattr(self.user, "cuda_stream") else torch.cuda.ExternalStream(int(self.user), self.dev))
-        return t
+            with cuda.stream(self.user if hasattr(self.user, "cuda_stream") else cuda.ExternalStream(int(self.user), self.dev)):
+                return like.new_empty(shape, dtype=dtype)
+        if like.dtype == dtype and like.shape == shape and like.is_contiguous():
+            return _torch()[0].empty_like(like)
+        return like.new_empty(shape, dtype=dtype)
+
+    def scratch(self, like, given, n):
+        """n bytes for work on the call's stream."""
+        uint8 = _torch()[0].uint8
+        if given is None:
+            return self.new(like, (n,), uint8)
+        if given.dtype != uint8 or not given.is_contiguous() or given.numel() < n:
+            _bad(f"workspace must be a contiguous uint8 tensor of at least {n} bytes")
+        return given
 
 
 def _done(rc, name):
@@ -144,13 +154,6 @@ def _rope(cs, interleaved, offset):
     return Rope(cs.data_ptr(), cs.shape[0], 2 * cs.shape[1], offset, int(bool(interleaved)))
 
 
-def _like(t, shape, dtype):
-    """A new contiguous tensor beside t."""
-    if t.is_contiguous() and t.dtype == dtype and t.shape == shape:
-        return _torch()[0].empty_like(t)
-    return t.new_empty(shape, dtype=dtype)
-
-
 def _io(t, what):
     d = _torch()[1].get(t.dtype)
     if d is None:
@@ -181,9 +184,10 @@ def rope_table(freqs, n_pos: int, *, first: int = 0, factor: float = 1.0, out=No
     if n_pos < 0:
         _bad("n_pos must not be negative")
     if out is None:
-        out = torch.empty((n_pos, f.size, 2), dtype=torch.float32, device="cuda" if device is None else device)
-        if stream is not None and hasattr(stream, "cuda_stream"):
-            out.record_stream(stream)
+        if device is None:
+            device = stream.device if hasattr(stream, "device") else "cuda"
+        beside = torch.empty(0, dtype=torch.float32, device=device)
+        out = _on(stream, beside).new(beside, (n_pos, f.size, 2), torch.float32)
     if out.dtype != torch.float32 or out.shape != (n_pos, f.size, 2) or not out.is_contiguous():
         _bad("out must be a contiguous float32 [n_pos, len(freqs), 2] tensor")
     with _on(stream, out) as s:
@@ -197,13 +201,14 @@ def rope(x, pos, cs, *, interleaved: bool = False, offset: int = 0, out=None, st
     xp, xs, xh, shape = _rows(x, "x")
     T, H, D = shape
     r, p = _rope(cs, interleaved, offset), _ints(pos, "pos", T)
+    on = _on(stream, x, pos, cs, out)
     if out is None:
-        out = _like(x, shape, x.dtype)
+        out = on.new(x, shape, x.dtype)
     yp, ys, yh, yshape = _rows(out, "out")
     if yshape != shape:
         _bad("out must have x's shape")
     dx, dy = _io(x, "x"), _io(out, "out")
-    with _on(stream, x, pos, cs, out) as s:
+    with on as s:
         _done(lib().hxb_rope_dev(C.byref(r), p, T, H, D, xp, dx, xs, xh, yp, dy, ys, yh, s), "hxb_rope_dev")
     return out
 
@@ -278,16 +283,16 @@ def decode_attention(q, k_cache, v_cache, table, lens, *, scale: float, k_scale=
     torch = _torch()[0]
     on = _on(stream, q, k_cache, v_cache, table, lens, k_scale, v_scale, out, lse, workspace)
     if out is None:
-        out = _like(q, shape, q.dtype)
+        out = on.new(q, shape, q.dtype)
     op, os, oh, oshape = _rows(out, "out")
     if oshape != shape or out.dtype != q.dtype:
         _bad("out must be like q")
     if lse is None and return_lse:
-        lse = _like(q, (B, H), torch.float32)
+        lse = on.new(q, (B, H), torch.float32)
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
         _bad("lse must be a contiguous float32 [n_seqs, heads] tensor")
     with on as s:
-        ws = on.scratch(workspace, _workspace(B, c.n_kv_heads, D, H, 0))
+        ws = on.scratch(q, workspace, _workspace(B, c.n_kv_heads, D, H, 0))
         _done(lib().hxb_attn_decode_dev(C.byref(c), lp, qp, qs, qh, H, dt, scale, op, os, oh, None if lse is None else lse.data_ptr(),
                                         ws.data_ptr(), ws.numel(), s), "hxb_attn_decode_dev")
     return (out, lse) if return_lse else out
@@ -311,12 +316,12 @@ def latent_attention(q, w, c_cache, table, lens, *, scale: float, c_scale=None, 
     lp, dt = _ints(lens, "lens", B), _io(q, "q")
     on = _on(stream, q, w, c_cache, table, lens, c_scale, out, workspace)
     if out is None:
-        out = _like(q, (B, H, vd), q.dtype)
+        out = on.new(q, (B, H, vd), q.dtype)
     op, os, oh, oshape = _rows(out, "out")
     if oshape != (B, H, vd) or out.dtype != q.dtype:
         _bad(f"out must be [{B}, {H}, {vd}] in q's type")
     with on as s:
-        ws = on.scratch(workspace, _workspace(B, 1, c.head_dim, H, R))
+        ws = on.scratch(q, workspace, _workspace(B, 1, c.head_dim, H, R))
         _done(lib().hxb_latent_decode_dev(C.byref(c), lp, qp, qs, qh, w.data_ptr(), H, R, nope, vd, dt, scale, op, os, oh,
                                           ws.data_ptr(), ws.numel(), s), "hxb_latent_decode_dev")
     return out

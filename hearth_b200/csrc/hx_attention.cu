@@ -45,7 +45,7 @@ int kv_view(const hxb_kv_cache *c, const char *who, bool latent, KvView *o) {
     if (c->page_tokens < 1 || c->page_tokens > 1024 || (c->page_tokens & (c->page_tokens - 1)))
         return attn_fail(HXB_E_ARG, "%s: page_tokens %d (a power of two up to 1024)", who, c->page_tokens);
     if (c->n_pages < 0 || c->n_pages > 0x7fffffff || c->table_pages < 0 || c->n_seqs < 0 || c->table_stride < 0 ||
-        (int64_t)c->table_pages * c->page_tokens > 0x7fffffff)
+        (int64_t)c->table_pages * c->page_tokens > 0x7fffff00)   // positions fit an int with a tile to spare
         return attn_fail(HXB_E_ARG, "%s: bad page counts", who);
     if (c->table_stride && c->table_stride < c->table_pages)
         return attn_fail(HXB_E_ARG, "%s: table rows overlap (stride %lld, %d pages)", who, (long long)c->table_stride,

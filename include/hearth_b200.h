@@ -104,7 +104,9 @@ HXB_API int hxb_matmul_noalloc(int dtype, const void *W, int64_t n_rows, int64_t
  * HXB_E_UNSUPPORTED (a shape the kernels do not take) with a message, before anything is enqueued.
  * Values on the device that break one (a page id outside the pool, a position outside a table)
  * never cause an access: what they would have given reads as NaN, what they would have written is
- * left out. */
+ * left out. Slots that hold no position of a sequence may hold anything, NaN included. Attention takes
+ * the rows of its positions and its queries to be finite: an infinity or NaN among them gives that
+ * head a NaN or infinite output, or leaves the position without weight. */
 
 /* Rotary frequencies (host arithmetic in 64 bits): inv_freq[j], j < rope_dim / 2, and the factor for
  * the table's values. scaling: HXB_ROPE_NONE theta^(-2j / rope_dim); HXB_ROPE_LINEAR the same / factor;

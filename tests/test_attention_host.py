@@ -88,7 +88,8 @@ BAD_CACHE = [(dict(dtype=0), UNSUP), (dict(dtype=4), UNSUP), (dict(n_kv_heads=0)
              (dict(page_tokens=2048), ARG), (dict(page_tokens=0), ARG), (dict(n_pages=-1), ARG), (dict(k=0), ARG),
              (dict(k=P + 8), ARG), (dict(v=P + 2), ARG), (dict(table=0), ARG), (dict(table_stride=1), ARG), (dict(table_pages=-1), ARG),
              (dict(n_seqs=-1), ARG), (dict(dtype=3), ARG), (dict(k_scale=P), ARG), (dict(v=0), ARG),
-             (dict(table_pages=1 << 28, table_stride=1 << 28), ARG)]
+             (dict(table_pages=1 << 28, table_stride=1 << 28), ARG),
+             (dict(page_tokens=1, table_pages=0x7fffffff, table_stride=0x7fffffff), ARG)]
 
 
 @pytest.mark.parametrize("kw,code", BAD_CACHE)

@@ -658,3 +658,68 @@ def test_two_streams_and_two_graphs_at_once(gpu):
                 G.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_calls_on_another_stream_allocate_there(gpu):
+    """Outputs and scratch that a call makes itself are usable on the stream it was given, with no other synchronisation."""
+    g = gen(50)
+    (kp, _), (vp, _) = (f := filled(g, [500, 77], 2, 16, 64, "bf16"))[0]
+    q = randn(g, 2, 8, 64, dtype=torch.bfloat16).cuda()
+    args = (q, kp.cuda(), vp.cuda(), f[1].cuda(), torch.tensor([500, 77], dtype=torch.int32).cuda())
+    cs = hb.rope_table(hb.rope_freqs(64, 1e4)[0], 100)
+    pos = torch.tensor([3, 99], dtype=torch.int32).cuda()
+    want = hb.decode_attention(*args, scale=0.1, return_lse=True), hb.rope(q, pos, cs)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for stream in (s, s.cuda_stream):
+        junk = torch.full((1 << 24,), float("nan")).cuda()      # work on the current stream whose memory is freed at once
+        del junk
+        got = hb.decode_attention(*args, scale=0.1, return_lse=True, stream=stream)
+        rot = hb.rope(q, pos, cs, stream=stream)
+        table = hb.rope_table(hb.rope_freqs(64, 1e4)[0], 100, stream=stream)
+        s.synchronize()
+        assert torch.equal(got[0], want[0][0]) and torch.equal(got[1], want[0][1]) and torch.equal(rot, want[1]) and torch.equal(table, cs)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+def test_latent_attention_captured(gpu, cache):
+    """One captured call follows new queries, rows, lengths and pages in the same buffers; the scratch is used again and again."""
+    g = gen(51)
+    pools, table, (rows,) = filled(g, [150, 70, 9], 1, 16, 320, cache, sides=1)
+    cp, cs = (cu(t) for t in pools[0])
+    w, td = randn(g, 8, 64, 256, dtype=torch.bfloat16, scale=0.06).cuda(), table.cuda()
+    q, lens = torch.zeros(3, 8, 96, dtype=torch.bfloat16).cuda(), torch.zeros(3, dtype=torch.int32).cuda()
+    hb.latent_attention(q, w, cp, td, lens, scale=0.1, c_scale=cs)
+    G = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(G):
+        out = hb.latent_attention(q, w, cp, td, lens, scale=0.1, c_scale=cs)
+    for i, ls in enumerate([[150, 70, 9], [1, 0, 2], [64, 65, 1], [149, 70, 0], [0, 0, 0]]):
+        q.copy_(randn(g, 3, 8, 96, dtype=torch.bfloat16))
+        lens.copy_(torch.tensor(ls, dtype=torch.int32))
+        G.replay()
+        assert torch.equal(out, hb.latent_attention(q, w, cp, td, lens, scale=0.1, c_scale=cs)), i
+        for b, n in enumerate(ls):
+            if n == 0:
+                assert (out[b] == 0).all()
+                continue
+            qc = q[b].cpu().double()
+            qa = torch.cat([torch.einsum("hd,hdr->hr", qc[:, :32], w.cpu()[:, :32].double()), qc[:, 32:]], -1)
+            o, _, _, _ = attend(qa, rows[b][:n], rows[b][:n, :, :256], 0.1)
+            want = torch.einsum("hr,hvr->hv", o, w.cpu()[:, 32:].double())
+            assert (out[b].cpu().double() - want).norm() <= 4 * half_step(torch.bfloat16) * want.norm()
+
+
+def test_workspace_sizes(gpu):
+    """The sizes the size functions give are enough, and no fewer bytes are taken."""
+    g = gen(52)
+    for cache in ("bf16", "q8"):
+        (kp, ks), (vp, vs) = (f := filled(g, [40], 2, 16, 64, cache))[0]
+        args = (randn(g, 1, 8, 64, dtype=torch.bfloat16).cuda(), kp.cuda(), vp.cuda(), f[1].cuda(), torch.tensor([40], dtype=torch.int32).cuda())
+        n = hb.attention_workspace(1, 8, 2, 64)
+        kw = dict(scale=0.1, k_scale=cu(ks), v_scale=cu(vs))
+        a = hb.decode_attention(*args, workspace=torch.zeros(n, dtype=torch.uint8).cuda(), **kw)
+        assert torch.equal(a, hb.decode_attention(*args, **kw))
+        with pytest.raises(ValueError):
+            hb.decode_attention(*args, workspace=torch.zeros(n - 16, dtype=torch.uint8).cuda(), **kw)
+    assert hb.latent_workspace(4, 16, 512, 64) > 4 * 16 * 576 * 4
