@@ -611,6 +611,7 @@ int attn_check_io(const char *who, int B, int H, const void *q, int64_t qs, int6
     const size_t size = dtype == F32 ? 4 : 2;
     auto off = [](const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
     if (!q || !out || !lens) return attn_fail(HXB_E_ARG, "%s: null pointer", who);
+    if (q == out) return attn_fail(HXB_E_ARG, "%s: not in place (out is q)", who);
     if (off(q, size) || off(out, size) || off(lens, 4)) return attn_fail(HXB_E_ARG, "%s: pointer not aligned to its elements", who);
     if (qs < 0 || qh < 0 || os < 0 || (H > 1 && oh < od) || (B > 1 && os < (int64_t)(H - 1) * oh + od))
         return attn_fail(HXB_E_ARG, "%s: bad strides", who);

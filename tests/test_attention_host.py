@@ -155,7 +155,7 @@ def test_rope_table_refusals():
 
 def test_attention_refusals():
     L = hb.lib()
-    ok = dict(c=cache(), lens=P, q=P, qs=256, qh=64, H=4, dt=2, scale=1.0, out=P, os=256, oh=64, lse=None, ws=P, n=1 << 30)
+    ok = dict(c=cache(), lens=P, q=P, qs=256, qh=64, H=4, dt=2, scale=1.0, out=P + (1 << 20), os=256, oh=64, lse=None, ws=P, n=1 << 30)
 
     def call(**kw):
         d = dict(ok, **kw)
@@ -164,7 +164,8 @@ def test_attention_refusals():
     assert call(c=cache(n_seqs=0)) == 0
     assert call(c=cache(head_dim=72)) == UNSUP and call(c=cache(head_dim=512)) == UNSUP
     for kw in (dict(H=3), dict(H=0), dict(dt=3), dict(lens=0), dict(q=0), dict(out=0), dict(ws=0), dict(ws=P + 8), dict(n=0), dict(oh=32),
-               dict(os=128), dict(qs=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=P + 1), dict(lse=P + 2)):
+               dict(os=128), dict(qs=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=P + 1), dict(lse=P + 2), dict(out=P),
+               dict(c=cache(n_seqs=65536))):
         assert call(**kw) == ARG, kw
     assert L.hxb_attn_decode_workspace(C.byref(ok["c"]), 4) > 0
 
@@ -172,7 +173,7 @@ def test_attention_refusals():
 def test_latent_refusals():
     L = hb.lib()
     lat = lambda **kw: cache(**dict(dict(n_kv_heads=1, head_dim=576, v=0), **kw))  # noqa: E731
-    ok = dict(c=lat(), lens=P, q=P, qs=4 * 192, qh=192, w=P, H=4, R=512, dn=128, dv=128, dt=2, scale=1.0, out=P, os=512, oh=128, ws=P,
+    ok = dict(c=lat(), lens=P, q=P, qs=4 * 192, qh=192, w=P, H=4, R=512, dn=128, dv=128, dt=2, scale=1.0, out=P + (1 << 20), os=512, oh=128, ws=P,
               n=1 << 30)
 
     def call(**kw):
@@ -183,7 +184,7 @@ def test_latent_refusals():
     for kw in (dict(R=500), dict(R=64), dict(R=384), dict(R=576), dict(dn=8), dict(dv=100), dict(dv=512), dict(c=lat(head_dim=520))):
         assert call(**kw) == UNSUP, kw
     for kw in (dict(c=lat(v=P)), dict(c=lat(n_kv_heads=2)), dict(c=lat(dtype=1)), dict(dt=0), dict(H=0), dict(H=512), dict(w=0),
-               dict(w=P + 2), dict(ws=0), dict(n=16), dict(lens=0), dict(oh=64)):
+               dict(w=P + 2), dict(ws=0), dict(n=16), dict(lens=0), dict(oh=64), dict(out=P), dict(c=lat(n_seqs=65536))):
         assert call(**kw) == ARG, kw
     assert L.hxb_latent_decode_workspace(C.byref(ok["c"]), 4, 512) > 0
 

@@ -723,3 +723,173 @@ def test_workspace_sizes(gpu):
         with pytest.raises(ValueError):
             hb.decode_attention(*args, workspace=torch.zeros(n - 16, dtype=torch.uint8).cuda(), **kw)
     assert hb.latent_workspace(4, 16, 512, 64) > 4 * 16 * 576 * 4
+
+
+# ----------------------------------------------------------------------------------------- the edges of the calls
+
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+def test_offsets_past_32_bits(gpu, cache):
+    """Pages at the far end of a pool of more than 2^31 elements: the same bits as from its first pages."""
+    g = gen(60)
+    pt, D, lens = 64, 128, [300, 129, 64]
+    n_pages = (1 << 31) // (pt * D) + 40
+    dt = torch.int8 if cache == "q8" else torch.bfloat16
+    kp, vp = (torch.empty(n_pages, 1, pt, D, dtype=dt, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(n_pages, 1, pt, D // 64, device="cuda") if cache == "q8" else None for _ in range(2))
+    near = torch.tensor([[0, 3, 1, 2, 4], [5, 7, 6, -1, -1], [8, -1, -1, -1, -1]], dtype=torch.int32)
+    far = torch.where(near >= 0, n_pages - 1 - near, near)
+    k, v = (randn(g, sum(lens), 1, D).cuda() for _ in range(2))
+    q = randn(g, 3, 8, D, dtype=torch.bfloat16).cuda()
+    start = torch.tensor([0, 300, 429, 493], dtype=torch.int32).cuda()
+    zero, n = torch.zeros(3, dtype=torch.int32).cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    got = []
+    for table in (near.cuda(), far.cuda()):
+        hb.kv_write(k, v, kp, vp, table, start, zero, k_scale=ks, v_scale=vs)
+        ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+        hb.kv_read(kp, vp, table, start, zero, ko, vo, k_scale=ks, v_scale=vs)
+        got.append((ko, vo, *hb.decode_attention(q, kp, vp, table, n, scale=0.09, k_scale=ks, v_scale=vs, return_lse=True)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+    assert (got[1][0] - k).abs().max() <= (k.abs().max() / 127 if cache == "q8" else half_step(torch.bfloat16) * k.abs().max())
+    del kp, vp
+    w = randn(g, 4, 64, 128, dtype=torch.bfloat16, scale=0.08).cuda()
+    n_pages = (1 << 31) // (pt * 192) + 40
+    cp = torch.empty(n_pages, 1, pt, 192, dtype=dt, device="cuda")
+    cs = torch.empty(n_pages, 1, pt, 3, device="cuda") if cache == "q8" else None
+    far = torch.where(near >= 0, n_pages - 1 - near, near)
+    c, ql = randn(g, sum(lens), 1, 192).cuda(), randn(g, 3, 4, 32 + 64, dtype=torch.bfloat16).cuda()
+    got = []
+    for table in (near.cuda(), far.cuda()):
+        hb.kv_write(c, None, cp, None, table, start, zero, k_scale=cs)
+        got.append(hb.latent_attention(ql, w, cp, table, n, scale=0.1, c_scale=cs))
+    assert torch.equal(*got) and torch.isfinite(got[0]).all()
+
+
+def test_rows_of_many_sequences(gpu):
+    """More sequences than a CTA's threads, most of them without a row, padding at both ends; the table of one page each."""
+    g = gen(61)
+    B, pt = 1500, 4
+    count = torch.randint(-3, 4, (B,), generator=g).clamp(min=0)
+    start = torch.cat([torch.zeros(1, dtype=torch.int64), count.cumsum(0)]) + 5
+    T = int(start[-1]) + 7
+    pages = torch.randperm(B, generator=g).to(torch.int32)
+    x = randn(g, T, 1, 64)
+    cp = torch.full((B, 1, pt, 64), 9.0, dtype=torch.bfloat16)
+    want = cp.clone()
+    for b in range(B):
+        for i in range(int(count[b])):
+            want[pages[b], 0, i] = x[int(start[b]) + i, 0].to(torch.bfloat16)
+    dev, st, p0 = cp.cuda(), start.to(torch.int32).cuda(), torch.zeros(B, dtype=torch.int32).cuda()
+    hb.kv_write(x.cuda(), None, dev, None, pages[:, None].cuda(), st, p0)
+    assert torch.equal(dev.cpu(), want)
+    out = torch.full((T, 1, 64), 3.0).cuda()
+    hb.kv_read(dev, None, pages[:, None].cuda(), st, p0, out, None)
+    ref = torch.full((T, 1, 64), 3.0)
+    ref[5:T - 7] = x[5:T - 7].to(torch.bfloat16).float()
+    assert torch.equal(out.cpu(), ref)
+
+
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+def test_lengths_out_of_range(gpu, cache):
+    """Negative lengths are empty, ones past the table give NaN, whatever else is in the batch; a table without pages."""
+    g = gen(62)
+    lens = [40, -7, 33, 40, -2 ** 31, 2 ** 31 - 1]
+    pools, table, _ = filled(g, [40] * 6, 1, 8, 192, cache)
+    (kp, ks), (vp, vs) = ((cu(a), cu(b)) for a, b in pools)
+    t, n = table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    t4 = t[:, :4]                                       # rows of 32 positions only: 33 and 40 are past them
+    q = randn(g, 6, 4, 192, dtype=torch.bfloat16).cuda()
+    w = randn(g, 4, 48 + 16, 128, dtype=torch.bfloat16, scale=0.1).cuda()
+    ql = randn(g, 6, 4, 48 + 64, dtype=torch.bfloat16).cuda()
+    att = lambda tb, ln: hb.decode_attention(q, kp, vp, tb, ln, scale=0.1, k_scale=ks, v_scale=vs, return_lse=True)  # noqa: E731
+    lat = lambda tb, ln: hb.latent_attention(ql, w, kp, tb, ln, scale=0.1, c_scale=ks)  # noqa: E731
+    for b in range(6):
+        alone = torch.zeros(6, dtype=torch.int32).cuda()
+        alone[b] = lens[b]
+        assert torch.equal(att(t, n)[0][b].view(torch.int16), att(t, alone)[0][b].view(torch.int16)) or lens[b] > 0
+    out, lse = att(t, n)
+    lo = lat(t, n)
+    assert torch.isfinite(out[[0, 2, 3]]).all() and torch.isfinite(lse[[0, 2, 3]]).all() and torch.isfinite(lo[[0, 2, 3]]).all()
+    assert (out[[1, 4]] == 0).all() and (lse[[1, 4]] == -math.inf).all() and (lo[[1, 4]] == 0).all()
+    assert torch.isnan(out[5]).all() and torch.isnan(lse[5]).all() and torch.isnan(lo[5]).all()
+    out, lse = att(t4, n)
+    lo = lat(t4, n)
+    assert torch.isnan(out[[0, 2, 3, 5]]).all() and torch.isnan(lo[[0, 2, 3, 5]]).all() and (out[[1, 4]] == 0).all() and (lo[[1, 4]] == 0).all()
+    t0 = torch.empty(6, 0, dtype=torch.int32).cuda()
+    out, lse = att(t0, n)
+    lo = lat(t0, n)
+    assert torch.isnan(out[[0, 2, 3, 5]]).all() and torch.isnan(lo[[0, 2, 3, 5]]).all() and (out[[1, 4]] == 0).all() and (lo[[1, 4]] == 0).all()
+
+
+@pytest.mark.parametrize("cache,R,H", [("bf16", 128, 16), ("q8", 512, 64), ("bf16", 512, 130), ("f16", 256, 8)])
+def test_latent_calls_in_a_row_and_side_by_side(gpu, cache, R, H):
+    """Many calls without a wait in between, one scratch, other queries and lengths each time; then on two streams at once."""
+    g = gen(63)
+    W, pt, B = R + 64, 64, 7
+    pages = 40
+    if cache == "q8":
+        cp, cs = torch.randint(-127, 128, (pages, 1, pt, W), generator=g).to(torch.int8), torch.rand((pages, 1, pt, W // 64), generator=g) / 64
+        x = torch.bfloat16
+    else:
+        cp, cs, x = randn(g, pages, 1, pt, W, dtype=F[cache]), None, F[cache]
+    cp, cs = cp.cuda(), cu(cs)
+    w = randn(g, H, 64 + 64, R, dtype=x, scale=R ** -0.5).cuda()
+    table = torch.randint(0, pages, (B, 60), generator=g, dtype=torch.int32).cuda()
+    lens = [torch.tensor(v, dtype=torch.int32).cuda() for v in
+            ([3000, 1, 0, 64, 65, 700, 128], [0, 0, 0, 0, 0, 0, 3], [3840] * 7, [64] * 7, [1, 2, 3, 4, 5, 6, 3840], [0] * 7)]
+    qs = [randn(g, B, H, 64 + 64, dtype=x).cuda() for _ in range(6)]
+    call = lambda i, **kw: hb.latent_attention(qs[i % 6], w, cp, table, lens[(i + i // 6) % 6], scale=0.09, c_scale=cs, **kw)  # noqa: E731
+    want = []
+    for i in range(36):
+        want.append(call(i))
+        torch.cuda.synchronize()
+        assert torch.isfinite(want[-1]).all()
+    ws = torch.empty(hb.latent_workspace(B, H, R, 64), dtype=torch.uint8, device="cuda")
+    outs = [torch.empty_like(want[0]) for _ in range(36)]
+    for _ in range(3):
+        for o in outs:
+            o.fill_(9.0)
+        for i in range(36):
+            call(i, workspace=ws, out=outs[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [call(i, stream=(a, b)[i % 2]) for i in range(36)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_attention_calls_in_a_row(gpu):
+    """Many calls without a wait in between on one scratch, from one CTA's work to all."""
+    g = gen(64)
+    kp, vp = (randn(g, 60, 2, 32, 128, dtype=torch.bfloat16).cuda() for _ in range(2))
+    table = torch.randint(0, 60, (5, 100), generator=g, dtype=torch.int32).cuda()
+    lens = [torch.tensor(v, dtype=torch.int32).cuda() for v in ([3200] * 5, [0, 1, 0, 0, 0], [3000, 17, 64, 65, 0], [0] * 5, [1, 2, 3, 4, 5])]
+    q = [randn(g, 5, 16, 128, dtype=torch.bfloat16).cuda() for _ in range(4)]
+    ws = torch.empty(hb.attention_workspace(5, 16, 2, 128), dtype=torch.uint8, device="cuda")
+    want = []
+    for i in range(20):
+        want.append(hb.decode_attention(q[i % 4], kp, vp, table, lens[i % 5], scale=0.09))
+        torch.cuda.synchronize()
+    for _ in range(5):
+        got = [hb.decode_attention(q[i % 4], kp, vp, table, lens[i % 5], scale=0.09, workspace=ws) for i in range(20)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_that_are_refused(gpu):
+    """Outputs that are the queries themselves, more sequences than a launch takes, a stream of nowhere."""
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    i32 = torch.int32
+    kc = z(2, 1, 16, 64)
+    q = z(2, 4, 64)
+    with pytest.raises(ValueError, match="in place"):
+        hb.decode_attention(q, kc, kc, z(2, 1, dtype=i32), z(2, dtype=i32), scale=1.0, out=q)
+    with pytest.raises(ValueError, match="65535"):
+        hb.decode_attention(z(65536, 1, 64), kc, kc, z(65536, 1, dtype=i32), z(65536, dtype=i32), scale=1.0)
+    cl = z(1, 1, 16, 192)
+    ql = z(2, 4, 32 + 64)
+    with pytest.raises(ValueError, match="in place"):
+        hb.latent_attention(ql, z(4, 32 + 96, 128), cl, z(2, 1, dtype=i32), z(2, dtype=i32), scale=1.0, out=ql)
+    with pytest.raises(ValueError, match="65535"):
+        hb.latent_attention(z(65536, 1, 32 + 64), z(1, 48, 128), cl, z(65536, 1, dtype=i32), z(65536, dtype=i32), scale=1.0)
