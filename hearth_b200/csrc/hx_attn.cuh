@@ -56,18 +56,25 @@ struct Shares {
     }
 };
 
-// The share [cur, end) of CTA `cta` of `grid` in the N = n_pairs * sum_b units_of(b) units, laid out sequence by
+// What a (sequence, pair) counts in the division: its units, and before them `extra` that stand for the beginning and the end of
+// a CTA's piece of it (queries, sums out), so that a CTA with several pieces gets fewer units.
+__device__ __forceinline__ int work_of(const KvView &c, const int32_t *lens, int b, int unit, int extra) {
+    const int nu = units_of(c, lens, b, unit);
+    return nu ? nu + extra : 0;
+}
+
+// The share [cur, end) of CTA `cta` of `grid` in the N = n_pairs * sum_b work_of(b) units, laid out sequence by
 // sequence, pair by pair: the sequence of unit cur and the sum of the units of the sequences before it. False
 // without a share. ctas: the CTAs that have one (the first min(grid, N)). Every thread of the CTA calls it;
 // scan: one word a warp.
 template <int THREADS>
-__device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, int unit, int n_pairs, int cta, int grid,
+__device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, int unit, int extra, int n_pairs, int cta, int grid,
                                          int64_t *scan, int &b, int64_t &before, int64_t &cur, int64_t &end,
                                          int64_t &total, int &ctas) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = c.n_seqs;
     const int per = (B + THREADS - 1) / THREADS;
     int64_t mine = 0;
-    for (int i = tid * per; i < min(B, (tid + 1) * per); i++) mine += units_of(c, lens, i, unit);
+    for (int i = tid * per; i < min(B, (tid + 1) * per); i++) mine += work_of(c, lens, i, unit, extra);
     int64_t upto = mine;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -98,34 +105,34 @@ __device__ __forceinline__ bool my_units(const KvView &c, const int32_t *lens, i
     if (none) return false;
     b = chunk * per, before = scan[0];
     for (;;) {
-        const int nu = units_of(c, lens, b, unit);
-        if ((before + nu) * n_pairs > cur) break;
-        before += nu, b++;
+        const int nw = work_of(c, lens, b, unit, extra);
+        if ((before + nw) * n_pairs > cur) break;
+        before += nw, b++;
     }
     return true;
 }
 
-// Where a (sequence, pair)'s work went, from the lengths alone: CTAs first .. last, each with one piece, in slot 0 but
-// for the first CTA where the pair is not what it began with. One CTA: it wrote the result itself.
+// Where a (sequence, pair)'s work [unit0, unit0 + extra + nu) went, from the lengths alone: CTAs first .. last, each with one
+// piece, in slot 0 but for the first CTA where the pair is not what it began with. One CTA: it wrote the result itself.
 struct Span {
     int first, last, slot;
     __device__ __forceinline__ bool split() const { return first != last; }
 };
-__device__ __forceinline__ Span span_of(int64_t unit0, int nu, int64_t total, int grid) {
+__device__ __forceinline__ Span span_of(int64_t unit0, int extra, int nu, int64_t total, int grid) {
     const Shares sh(total, (int)min((int64_t)grid, total));
     Span s;
-    s.first = sh.of(unit0), s.last = sh.of(unit0 + nu - 1);
-    s.slot = unit0 == sh.start(s.first) ? 0 : 1;
+    s.first = sh.of(unit0 + extra), s.last = sh.of(unit0 + extra + nu - 1);
+    s.slot = sh.start(s.first) >= unit0 ? 0 : 1;
     return s;
 }
-// Units of the sequences before b, and of all: the same sums my_units forms. Every thread of the CTA calls it.
+// The work of the sequences before b, and of all: the same sums my_units forms. Every thread of the CTA calls it.
 template <int THREADS>
-__device__ __forceinline__ void unit_sums(const KvView &c, const int32_t *lens, int unit, int b, int64_t (*scratch)[2], int64_t &before, int64_t &all) {
+__device__ __forceinline__ void work_sums(const KvView &c, const int32_t *lens, int unit, int extra, int b, int64_t (*scratch)[2], int64_t &before, int64_t &all) {
     before = all = 0;
     for (int i = threadIdx.x; i < c.n_seqs; i += THREADS) {
-        const int nu = units_of(c, lens, i, unit);
-        all += nu;
-        if (i < b) before += nu;
+        const int nw = work_of(c, lens, i, unit, extra);
+        all += nw;
+        if (i < b) before += nw;
     }
 #pragma unroll
     for (int s = 16; s >= 1; s >>= 1) all += __shfl_xor_sync(0xffffffffu, all, s), before += __shfl_xor_sync(0xffffffffu, before, s);
