@@ -87,60 +87,63 @@ __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_co
 #pragma unroll
     for (int i = 0; i < AB_AHEAD; i++) fetch(pre[i], 16 * i);
     const uint16_t *q = static_cast<const uint16_t *>(a.q) + h * a.qh;
-    constexpr int AB_EACH = AB_ROWS / AB_WARPS;      // rows a warp stages: all its loads of 64 values before their stores
+    constexpr int AB_EACH = AB_ROWS / AB_WARPS;      // rows a warp stages: all its loads before their stores
     auto row_at = [&](int r, int d, int lim) -> uint16_t {
         return warp + r * AB_WARPS < rows && d < lim ? __ldg(q + (b0 + warp + r * AB_WARPS) * a.qs + d) : 0;
     };
-#pragma unroll 1
-    for (int d = lane; d < a.dn; d += 64) {
-        uint16_t x[2][AB_EACH];
-#pragma unroll
-        for (int r = 0; r < AB_EACH; r++) x[0][r] = row_at(r, d, a.dn), x[1][r] = row_at(r, d + 32, a.dn);
-#pragma unroll
-        for (int r = 0; r < AB_EACH; r++) {
-            qsm[warp + r * AB_WARPS][d] = x[0][r];
-            if (d + 32 < a.dn) qsm[warp + r * AB_WARPS][d + 32] = x[1][r];
-        }
-    }
     const int row = a.R + a.dr;
-    if (blockIdx.x == h * nc) {     // the rotated parts, with the head's first CTA
-        uint16_t x[2][AB_EACH];
+    const bool rot = blockIdx.x == h * nc;      // the rotated parts, with the head's first CTA
+    uint16_t xr[2][AB_EACH];
 #pragma unroll
-        for (int r = 0; r < AB_EACH; r++) x[0][r] = row_at(r, a.dn + lane, a.dn + a.dr), x[1][r] = row_at(r, a.dn + lane + 32, a.dn + a.dr);
+    for (int r = 0; r < AB_EACH; r++) xr[0][r] = rot ? row_at(r, a.dn + lane, a.dn + a.dr) : 0, xr[1][r] = rot ? row_at(r, a.dn + lane + 32, a.dn + a.dr) : 0;
+#pragma unroll 1
+    for (int d = lane; d < a.dn; d += 128) {
+        uint16_t x[4][AB_EACH];
+#pragma unroll
+        for (int r = 0; r < AB_EACH; r++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e][r] = row_at(r, d + 32 * e, a.dn);
+#pragma unroll
+        for (int r = 0; r < AB_EACH; r++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (d + 32 * e < a.dn) qsm[warp + r * AB_WARPS][d + 32 * e] = x[e][r];
+    }
+    if (rot) {
 #pragma unroll
         for (int r = 0; r < AB_EACH; r++)
 #pragma unroll
             for (int e = 0; e < 2; e++)
                 if (warp + r * AB_WARPS < rows && lane + 32 * e < a.dr)
-                    a.qa[((int64_t)(b0 + warp + r * AB_WARPS) * a.H + h) * row + a.R + lane + 32 * e] = T == F16 ? f16_to_f32_hw(x[e][r]) : bf16_to_f32(x[e][r]);
+                    a.qa[((int64_t)(b0 + warp + r * AB_WARPS) * a.H + h) * row + a.R + lane + 32 * e] = T == F16 ? f16_to_f32_hw(xr[e][r]) : bf16_to_f32(xr[e][r]);
     }
     __syncthreads();
     if (r0 >= a.R) return;
     float acc[2][8][4] = {};
-    // one step of 16 dims, not unrolled: code that runs once is fetched slower than it runs
+    // AB_AHEAD steps of 16 dims, each with registers of its own (moving a load's registers on would wait for it)
 #pragma unroll 1
-    for (int d = 0; d < a.dn; d += 16) {
-        const uint4 v[4] = {pre[0][0], pre[0][1], pre[0][2], pre[0][3]};
+    for (int d0 = 0; d0 < a.dn; d0 += 16 * AB_AHEAD) {
 #pragma unroll
-        for (int i = 0; i + 1 < AB_AHEAD; i++)
+        for (int j = 0; j < AB_AHEAD; j++) {
+            const int d = d0 + 16 * j;
+            if (d >= a.dn) break;
+            uint32_t f[2][4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) pre[i][k] = pre[i + 1][k];
-        fetch(pre[AB_AHEAD - 1], d + 16 * AB_AHEAD);
-        uint32_t f[2][4];
+            for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+                for (int k = 0; k < 4; k++)
+                    f[m][k] = *reinterpret_cast<const uint32_t *>(&qsm[16 * m + g + 8 * (k & 1)][d + 2 * t + 8 * (k >> 1)]);
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                f[m][k] = *reinterpret_cast<const uint32_t *>(&qsm[16 * m + g + 8 * (k & 1)][d + 2 * t + 8 * (k >> 1)]);
+            for (int i = 0; i < 4; i++) {
+                const uint32_t x[4] = {(&pre[j][0].x)[i], (&pre[j][1].x)[i], (&pre[j][2].x)[i], (&pre[j][3].x)[i]};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t x[4] = {(&v[0].x)[i], (&v[1].x)[i], (&v[2].x)[i], (&v[3].x)[i]};
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t p0 = __byte_perm(x[0], x[1], e ? 0x7632 : 0x5410), p1 = __byte_perm(x[2], x[3], e ? 0x7632 : 0x5410);
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const uint32_t p0 = __byte_perm(x[0], x[1], e ? 0x7632 : 0x5410), p1 = __byte_perm(x[2], x[3], e ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int m = 0; m < 2; m++) mma16<T>(acc[m][2 * i + e], f[m][0], f[m][1], f[m][2], f[m][3], p0, p1);
+                    for (int m = 0; m < 2; m++) mma16<T>(acc[m][2 * i + e], f[m][0], f[m][1], f[m][2], f[m][3], p0, p1);
+                }
             }
+            fetch(pre[j], d + 16 * AB_AHEAD);
         }
     }
     // column n of product i is latent dim 8 n + i
@@ -746,7 +749,7 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
 
 // ------------------------------------------------------------------------------------------- expand
 
-constexpr int EX_WARPS = 16, EX_ROWS = 16;
+constexpr int EX_WARPS = 16, EX_ROWS = 16, EX_KEPT = 8;
 
 struct ExpandShared {
     uint32_t ops[2][16][2][32][4];       // [term][32-dim step][eight rows][lane]
@@ -755,6 +758,8 @@ struct ExpandShared {
         float red[16][16 * EX_ROWS];
     };
     float2 ml[EX_WARPS];
+    float fac[EX_WARPS];                 // a piece's factor in its row's o
+    uint4 w[EX_KEPT][2][32 * EX_WARPS];  // the threads' first weights
     uint32_t over;                       // sequences longer than their table
     int64_t sums[EX_WARPS][2];
 };
@@ -771,14 +776,14 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 1) k_latent_expand(const __grid
     const int mt = a.dv / 16, ksplit = max(1, EX_WARPS / mt), items = mt * ksplit;
     const uint16_t *w = static_cast<const uint16_t *>(a.w) + ((int64_t)h * (a.dn + a.dv) + a.dn + g) * a.R + 8 * t;
     auto first = [&](int item) { return item / mt * steps / ksplit; };
-    auto last = [&](int item) { return item < items ? (item / mt + 1) * steps / ksplit : 0; };
-    auto fetch = [&](int item, int s, uint4 v[2]) {
-        const uint16_t *p = w + (int64_t)(item % mt) * 16 * a.R + s * 32;
-        v[0] = __ldg(reinterpret_cast<const uint4 *>(p)), v[1] = __ldg(reinterpret_cast<const uint4 *>(p + 8 * (int64_t)a.R));
-    };
-    // the head's value rows on their way to L2 before the core has ended
-    for (int i = threadIdx.x; i < a.dv * (a.R / 64); i += 32 * EX_WARPS)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t *>(a.w) + ((int64_t)h * (a.dn + a.dv) + a.dn) * a.R + (int64_t)i * 64));
+    auto last = [&](int item) { return item < items ? (item / mt + 1) * steps / ksplit : 0; };      // none for a warp without an item
+    auto at = [&](int item, int s, int k) { return w + (int64_t)(item % mt) * 16 * a.R + s * 32 + k * 8 * (int64_t)a.R; };
+    // A warp has one item at most. Its first weights come into shared memory (places of its own) before the core has ended: an SM
+    // takes 128 KB from L2 in about 5000 cycles.
+    const int s_first = first(warp), s_end = last(warp);
+#pragma unroll
+    for (int i = 0; i < EX_KEPT; i++)
+        if (s_first + i < s_end) cp16(smem_u32(&y.w[i][0][threadIdx.x]), at(warp, s_first + i, 0), true), cp16(smem_u32(&y.w[i][1][threadIdx.x]), at(warp, s_first + i, 1), true);
     for (int i = threadIdx.x; i < 2 * 16 * 2 * 32; i += 32 * EX_WARPS) reinterpret_cast<uint4 *>(&y.ops)[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x < 32) {
         const uint32_t over = __ballot_sync(0xffffffffu, lane < rows && a.lens[b0 + min(lane, rows - 1)] > table_capacity(a.c));
@@ -818,57 +823,81 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 1) k_latent_expand(const __grid
                     }
                 o.add(ml, x);
             }
+            // nothing, too long a row and a failed wait as the entry point says
+            const bool bad = *reinterpret_cast<volatile int *>(a.err) || (y.over >> row & 1);
+            if (wpr == 1) {     // the row is whole
+                const float inv = bad ? kv_nan() : o.l == 0.0f ? 0.0f : __fdiv_rn(1.0f, o.l);
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                *reinterpret_cast<float4 *>(&y.join[warp][128 * k + 4 * lane]) = make_float4(o.o[4 * k], o.o[4 * k + 1], o.o[4 * k + 2], o.o[4 * k + 3]);
-            if (lane == 0) y.ml[warp] = make_float2(o.m, o.l);
-        }
-        __syncthreads();
-        // a row's warps together, two dims a thread; nothing, too long a row and a failed wait as the entry point says
-        const bool failed = *reinterpret_cast<volatile int *>(a.err);
-        for (int i = threadIdx.x; i < rows * (a.R / 2); i += 32 * EX_WARPS) {
-            const int rw = i / (a.R / 2), d = 2 * (i - rw * (a.R / 2));
-            Joined<2> o;
-            if (wpr == 1) {
-                o.l = y.ml[rw].y, o.o[0] = y.join[rw][d], o.o[1] = y.join[rw][d + 1];
+                for (int k = 0; k < 4; k++) {
+                    if (k >= a.R / 128) break;
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = bad || o.l != 0.0f ? __fmul_rn(o.o[4 * k + e], inv) : 0.0f;
+#pragma unroll
+                    for (int term = 0; term < 2; term++) {
+                        uint2 p;
+                        p.x = take_pair<T>(x[0], x[1]), p.y = take_pair<T>(x[2], x[3]);
+                        *reinterpret_cast<uint2 *>(&y.ops[term][4 * k + (lane >> 3)][row >> 3][(row & 7) * 4 + ((lane >> 1) & 3)][2 * (lane & 1)]) = p;
+                    }
+                }
             } else {
-#pragma unroll 2
-                for (int p = rw * wpr; p < (rw + 1) * wpr; p++) o.add(y.ml[p], &y.join[p][d]);
-            }
-            const bool bad = failed || (y.over >> rw & 1);
-            const float inv = bad ? kv_nan() : o.l == 0.0f ? 0.0f : __fdiv_rn(1.0f, o.l);
-            float x0 = bad || o.l != 0.0f ? __fmul_rn(o.o[0], inv) : 0.0f, x1 = bad || o.l != 0.0f ? __fmul_rn(o.o[1], inv) : 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2; k++) y.ops[k][d >> 5][rw >> 3][(rw & 7) * 4 + ((d >> 3) & 3)][(d >> 1) & 3] = take_pair<T>(x0, x1);
+                for (int k = 0; k < 4; k++)
+                    *reinterpret_cast<float4 *>(&y.join[warp][128 * k + 4 * lane]) = make_float4(o.o[4 * k], o.o[4 * k + 1], o.o[4 * k + 2], o.o[4 * k + 3]);
+                if (lane == 0) y.ml[warp] = make_float2(o.m, bad ? kv_nan() : o.l);
+            }
+        }
+        if (wpr > 1) {     // a row's warps together, two dims a thread
+            __syncthreads();
+            if (threadIdx.x < rows * wpr) {
+                const int p0 = threadIdx.x / wpr * wpr;
+                float m = -kv_inf(), l = 0.0f;
+                for (int p = p0; p < p0 + wpr; p++) m = fmaxf(m, y.ml[p].x);
+                const float base = m == -kv_inf() ? 0.0f : m;
+                for (int p = p0; p < p0 + wpr; p++) l = __fmaf_rn(y.ml[p].y, exp2_fast(__fsub_rn(y.ml[p].x, base)), l);
+                y.fac[threadIdx.x] = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(__fsub_rn(y.ml[threadIdx.x].x, base)), l);
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < rows * (a.R / 2); i += 32 * EX_WARPS) {
+                const int rw = i / (a.R / 2), d = 2 * (i - rw * (a.R / 2));
+                float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll 4
+                for (int p = rw * wpr; p < (rw + 1) * wpr; p++) {
+                    const float2 v = *reinterpret_cast<const float2 *>(&y.join[p][d]);
+                    x0 = __fmaf_rn(v.x, y.fac[p], x0), x1 = __fmaf_rn(v.y, y.fac[p], x1);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; k++) y.ops[k][d >> 5][rw >> 3][(rw & 7) * 4 + ((d >> 3) & 3)][(d >> 1) & 3] = take_pair<T>(x0, x1);
+            }
         }
         __syncthreads();
-        for (int item = warp; item < items; item += EX_WARPS) {
+        if (warp < items) {
             float acc[2][4] = {};
-            auto step = [&](int s, const uint4 v[2]) {
+            auto step = [&](int s, const uint4 &v0, const uint4 &v1) {
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     if (8 * c >= rows) break;
 #pragma unroll
                     for (int k = 1; k >= 0; k--) {
                         const uint4 x = *reinterpret_cast<const uint4 *>(y.ops[k][s][c][lane]);
-                        mma16<T>(acc[c], v[0].x, v[1].x, v[0].y, v[1].y, x.x, x.y);
-                        mma16<T>(acc[c], v[0].z, v[1].z, v[0].w, v[1].w, x.z, x.w);
+                        mma16<T>(acc[c], v0.x, v1.x, v0.y, v1.y, x.x, x.y);
+                        mma16<T>(acc[c], v0.z, v1.z, v0.w, v1.w, x.z, x.w);
                     }
                 }
             };
-            const int end = last(item);
-#pragma unroll 8
-            for (int s = first(item); s < end; s++) {
-                uint4 v[2];
-                fetch(item, s, v);
-                step(s, v);
-            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 4
+            for (int i = 0; i < EX_KEPT; i++)
+                if (s_first + i < s_end) step(s_first + i, y.w[i][0][threadIdx.x], y.w[i][1][threadIdx.x]);
+#pragma unroll 4
+            for (int s = s_first + EX_KEPT; s < s_end; s++) step(s, __ldg(reinterpret_cast<const uint4 *>(at(warp, s, 0))), __ldg(reinterpret_cast<const uint4 *>(at(warp, s, 1))));
 #pragma unroll
             for (int c = 0; c < 2; c++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) y.red[item][(g + 8 * (e >> 1)) * EX_ROWS + 8 * c + 2 * t + (e & 1)] = acc[c][e];
+                for (int e = 0; e < 4; e++) y.red[warp][(g + 8 * (e >> 1)) * EX_ROWS + 8 * c + 2 * t + (e & 1)] = acc[c][e];
         }
         __syncthreads();
+#pragma unroll 4
         for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
             const int rw = i / a.dv, j = i - rw * a.dv;
             float x = y.red[j >> 4][(j & 15) * EX_ROWS + rw];
