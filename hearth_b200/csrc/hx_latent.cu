@@ -454,21 +454,24 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
         // ---- loading: a group takes every GROUPS-th tile
         constexpr int GROUPS = LD_GROUPS<CACHE>, THREADS = LD_THREADS<CACHE>;
         const int group = (tid - 32 * LD_WARP0) / THREADS, lt = (tid - 32 * LD_WARP0) % THREADS;
-        TileRows<CACHE> rows;
+        TileRows<CACHE> rows, next;
         auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, core_wait(y, bar, parity, a.err)); };
         bool ok = true, waited = false;
         int k0 = 0;      // tiles before this run
         while (ok && walk.next(r)) {
-            for (int i = GROUPS == 1 ? 0 : (k0 ^ group) & 1; ok && i < r.tiles; i += GROUPS) {
+            const int i0 = GROUPS == 1 ? 0 : (k0 ^ group) & 1;
+            if (i0 < r.tiles) next.find(a, r, i0, lt);
+            for (int i = i0; ok && i < r.tiles; i += GROUPS) {
                 const int k = k0 + i, buf = k & 1;
                 const uint32_t dst = smem_u32(kvb) + buf * segs * SEG;
-                rows.find(a, r, i, lt);
+                rows = next;
                 if constexpr (CACHE == Q8) {
                     // all of a tile's codes into registers while the tiles before are at work; then three block columns at a time,
                     // the registers moved down in between (unrolled to nine the code was fetched slower than it ran)
                     RawRows raw[9];
 #pragma unroll
                     for (int s = 0; s < 9; s++) raw[s].fetch(a, rows.row[0], s, segs, lt);
+                    if (i + GROUPS < r.tiles) next.find(a, r, i + GROUPS, lt);      // the next tile's places, ahead too
                     if (k >= 2) ok = wait(&y.freed[buf], ((k >> 1) - 1) & 1);
                     bool all = k < 2;
 #pragma unroll 1
@@ -508,6 +511,7 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
                     if (k >= 2) ok = wait(&y.done[buf], ((k >> 1) - 1) & 1);
                     if (!ok) break;
                     copy(2 * half, segs);
+                    if (i + GROUPS < r.tiles) next.find(a, r, i + GROUPS, lt);
                 }
                 rows.mark(y, buf, lt);
                 if (i == 0) {     // the first tile's warps bring the queries, once the last run's products are done
