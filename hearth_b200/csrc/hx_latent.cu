@@ -56,7 +56,9 @@ struct LatentArgs {
     const int32_t *lens;
     const void *q, *w;
     void *out;
-    float *qa;              // [n_seqs][H][R + dr]; a head whose work one CTA did leaves its o, maximum and sum here
+    // [n_seqs][H][R + dr] f32; for a bf16 cache the products' bf16 operands in the first half of each row. A head whose work
+    // one CTA did leaves its o, maximum and sum here.
+    float *qa;
     float2 *ml;             // [CTAs][2][hp]
     float *o;               // [CTAs][2][hp][R]
     int *err;
@@ -69,7 +71,7 @@ struct LatentArgs {
 
 constexpr int AB_WARPS = 4, AB_ROWS = 32, AB_AHEAD = 4;
 
-template <int T>
+template <int T, bool ROUND>
 __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_constant__ LatentArgs a) {
     __shared__ uint16_t qsm[AB_ROWS][256 + 8];
     const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS);
@@ -114,8 +116,12 @@ __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_co
         for (int r = 0; r < AB_EACH; r++)
 #pragma unroll
             for (int e = 0; e < 2; e++)
-                if (warp + r * AB_WARPS < rows && lane + 32 * e < a.dr)
-                    a.qa[((int64_t)(b0 + warp + r * AB_WARPS) * a.H + h) * row + a.R + lane + 32 * e] = T == F16 ? f16_to_f32_hw(xr[e][r]) : bf16_to_f32(xr[e][r]);
+                if (warp + r * AB_WARPS < rows && lane + 32 * e < a.dr) {
+                    float *dst = a.qa + ((int64_t)(b0 + warp + r * AB_WARPS) * a.H + h) * row;
+                    const int d = a.R + lane + 32 * e;
+                    if constexpr (ROUND) reinterpret_cast<uint16_t *>(dst)[d] = xr[e][r];
+                    else dst[d] = T == F16 ? f16_to_f32_hw(xr[e][r]) : bf16_to_f32(xr[e][r]);
+                }
     }
     __syncthreads();
     if (r0 >= a.R) return;
@@ -153,12 +159,23 @@ __global__ void __launch_bounds__(32 * AB_WARPS) k_latent_absorb(const __grid_co
         for (int e = 0; e < 2; e++) {
             const int r = 16 * m + g + 8 * e;
             if (r >= rows) continue;
-            float *dst = a.qa + ((int64_t)(b0 + r) * a.H + h) * row + r0 + 16 * t;
+            float *dst = a.qa + ((int64_t)(b0 + r) * a.H + h) * row;
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+            for (int n = 0; n < 2; n++) {
+                if constexpr (ROUND) {
+                    uint32_t o[4];
 #pragma unroll
-                for (int i = 0; i < 8; i += 4)
-                    *reinterpret_cast<float4 *>(dst + 8 * n + i) = make_float4(acc[m][i][2 * e + n], acc[m][i + 1][2 * e + n], acc[m][i + 2][2 * e + n], acc[m][i + 3][2 * e + n]);
+                    for (int i = 0; i < 4; i++) {
+                        float x = acc[m][2 * i][2 * e + n], y = acc[m][2 * i + 1][2 * e + n];
+                        o[i] = take_pair<T>(x, y);
+                    }
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(dst) + r0 + 16 * t + 8 * n) = make_uint4(o[0], o[1], o[2], o[3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4)
+                        *reinterpret_cast<float4 *>(dst + r0 + 16 * t + 8 * n + i) = make_float4(acc[m][i][2 * e + n], acc[m][i + 1][2 * e + n], acc[m][i + 2][2 * e + n], acc[m][i + 3][2 * e + n]);
+                }
+            }
         }
 }
 
@@ -358,10 +375,23 @@ __device__ __forceinline__ void expand16(uint32_t at, int rw, int q, const RawRo
     }
 }
 
-// Query rows of a run as the S product's first operand: eight lanes a head, all of its loads before their use.
+// Query rows of a run as the S product's first operand: eight lanes a head. bf16: copies that the caller waits for (from f32 rows it
+// took 7700 cycles, most of them between two round trips to L2). f16: a power of two a head, from f32.
 template <int OT, int THREADS>
 __device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint32_t dst, int segs, const Run &r, int h0, int nh, int lt) {
     const int c8 = lt & 7, W = a.R + a.dr;
+    if constexpr (OT == BF16) {
+#pragma unroll 2
+        for (int h = lt >> 3; h < LH; h += THREADS / 8) {
+            const uint16_t *src = reinterpret_cast<const uint16_t *>(a.qa + ((int64_t)r.b * a.H + h0 + min(h, nh - 1)) * W) + 8 * c8;
+            for (int s = 0; s < segs; s++) {
+                const bool on = h < nh && s * 64 + c8 * 8 < W;
+                cp16(dst + s * SEG + h * 128 + ((c8 ^ (h & 7)) << 4), on ? src + s * 64 : src, on);
+            }
+            if (c8 == 0) y.fac[h] = a.sc2;
+        }
+        return;
+    }
 #pragma unroll 1
     for (int h = lt >> 3; h < LH; h += THREADS / 8) {
         const float4 *src = reinterpret_cast<const float4 *>(a.qa + ((int64_t)r.b * a.H + h0 + h) * W) + 2 * c8;
@@ -714,22 +744,24 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
             const int slot = r.b == b0 ? 0 : 1, W = a.R + a.dr;
             const int64_t piece = (int64_t)blockIdx.x * 2 + slot;
             float *o0 = whole ? a.qa + ((int64_t)r.b * a.H + h0) * W : a.o + piece * a.hp * a.R;
-            const int pitch = whole ? W : a.R;
+            const int64_t pitch = whole ? W : a.R;
             // columns of 16 heads at a time, the next ones read while these are stored
             float o[2][16];
             tm_ld16(tm_o + lanes, o[0]);
 #pragma unroll 1
             for (int c = 0; c < cols; c += 16) {
                 float *at = o0 + (int64_t)c * pitch + 32 * warp + lane;
+                const bool all = c + 16 <= nh;
 #pragma unroll
                 for (int blk = 0; blk < 4; blk++) {
                     if (blk >= pieces) break;
                     tm_wait_ld();
                     if (blk + 1 < pieces) tm_ld16(tm_o + lanes + (blk + 1) * cols + c, o[(blk + 1) & 1]);
                     else if (c + 16 < cols) tm_ld16(tm_o + lanes + c + 16, o[(blk + 1) & 1]);
+                    float *p = at + blk * 128;
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        if (c + j < nh) at[(int64_t)j * pitch + blk * 128] = o[blk & 1][j];
+                    for (int j = 0; j < 16; j++, p += pitch)
+                        if (all || c + j < nh) *p = o[blk & 1][j];
                 }
                 if (pieces & 1) {     // the columns after an odd number of blocks were read into the other half
 #pragma unroll
@@ -940,7 +972,7 @@ cudaError_t launch(const LatentArgs &a, const Plan &p, cudaStream_t s) {
     e = cudaFuncSetAttribute(k_latent_expand<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ExpandShared));
     if (e != cudaSuccess) return e;
     const int nc = (a.R + 64 * AB_WARPS - 1) / (64 * AB_WARPS), B = a.c.n_seqs;
-    e = launch_pdl(false, k_latent_absorb<T>, dim3(a.H * nc, (B + AB_ROWS - 1) / AB_ROWS), dim3(32 * AB_WARPS), 0, s, a);
+    e = launch_pdl(false, k_latent_absorb<T, CACHE == BF16>, dim3(a.H * nc, (B + AB_ROWS - 1) / AB_ROWS), dim3(32 * AB_WARPS), 0, s, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(true, k_latent_core<CACHE>, dim3(p.grid), dim3(CORE_THREADS), p.smem, s, a);
     if (e != cudaSuccess) return e;
