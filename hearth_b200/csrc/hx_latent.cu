@@ -2,8 +2,9 @@
 // engine/src/model.c:739-787 in another order of summation), in three launches chained by programmatic
 // dependent launch:
 //
-//   k_latent_absorb  qa[b][h] = [sum_d q[d] w[h][d] | q's rotated part], f32 into the scratch; mma.sync, a
-//                    warp 64 latent dims of a head for 32 sequences, weights straight into registers.
+//   k_latent_absorb  qa[b][h] = [sum_d q[d] w[h][d] | q's rotated part] into the scratch (f32; for a bf16 cache rounded to the
+//                    products' operands); mma.sync, a warp 64 latent dims of a head for 32 sequences, weights straight
+//                    into registers.
 //   k_latent_core    softmax(scale qa C^T) C over the pages, on the fifth-generation tensor cores.
 //   k_latent_expand  joins the core's pieces and multiplies by w's value rows.
 //
@@ -19,10 +20,18 @@
 //
 // With O transposed its 4 x 64 columns and two S buffers take 384 of the 512 tensor-memory columns at 64 heads (O
 // itself, 64 rows high, would leave half of the lanes empty), and the tile in shared memory is used twice. Shared
-// memory: Q 72 KB, two tiles of 72 KB, P 8 KB. Warps 0-3 softmax, 4 issues the MMAs, 5-12 load, four for each of
-// the two tiles, so that the one in flight never waits for the one at work. Rows are fetched by 16-byte
-// asynchronous copies rather than tensor maps: they take any page size, and rows past the end arrive as zeros
-// (an unused slot may hold NaN, and 0 x NaN would reach every sum).
+// memory: Q 72 KB, two tiles of 72 KB, P 8 KB. Warps 0-3 softmax, 4 issues the scores' products, 5 the values', 6-13 load:
+// 16-bit rows four warps for each of the two tiles, so that the one in flight never waits for the one at work. Rows
+// are fetched by 16-byte asynchronous copies: they take any page size, and rows past the end arrive as zeros
+// (an unused slot may hold NaN, and 0 x NaN would reach every sum); tensor-map boxes of 64 x 64 took longer.
+//
+// Measured (64 heads, 512 + 64 values a row, 128 + 128 a head): 32 sequences of up to 8191, bf16: 87 us, 204 MB of
+// rows and 17 MB of weights, 2.5 TB/s; one of 1531: 26 us; 4 Q8 sequences of up to 65536 with 16 heads: 61 us. Of the 87 us
+// absorb takes 7, the core 68 after it and expand 11 after that. A tile of the core takes some 4500 cycles
+// (72 KB: 16 bytes a cycle and SM, the copy rate is 23): its buffer waits for scores (1500), softmax (1900) and half of
+// the values' products (1300) before the next rows (3000 to 4000) may follow, and there is room for two buffers. Asking for
+// the next rows in L2 ahead made it slower (106 us for 99), Q8 codes asked for over a tile's end too (73 us for 66:
+// the proxy fence waits for loads under way).
 //
 // ref is the running maximum, moved only when a score passes it by 2^7 (O^T is then rescaled in tensor memory):
 // the weights relative to it stay below 2^7 (f16 operands: 2^15, lifted by 2^8), and most tiles skip the rescale.
@@ -69,6 +78,8 @@ struct LatentArgs {
 
 // ------------------------------------------------------------------------------------------- absorb
 
+// Weights from HBM bound it (8.4 MB at 64 heads of 128 + 512, 1.3 us), in practice the round trips of a CTA: queries, then two
+// batches of weights; 6.8 us for 32 sequences, 5.5 for one.
 constexpr int AB_WARPS = 4, AB_ROWS = 32, AB_AHEAD = 4;
 
 template <int T, bool ROUND>
@@ -801,7 +812,9 @@ struct ExpandShared {
 };
 
 // A CTA a head and up to sixteen sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as
-// two terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o.
+// two terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o. Reads from L2 bound it:
+// 128 KB of weights a head (before the core has ended where its SM is free) and 2 KB a piece. 11 us after the core
+// with 32 sequences of 64 heads, 5 with one.
 template <int T>
 __global__ void __launch_bounds__(32 * EX_WARPS, 1) k_latent_expand(const __grid_constant__ LatentArgs a, int ex_rows, int grid) {
     extern __shared__ __align__(16) uint8_t raw[];
