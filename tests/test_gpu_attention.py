@@ -893,3 +893,26 @@ def test_calls_that_are_refused(gpu):
         hb.latent_attention(ql, z(4, 32 + 96, 128), cl, z(2, 1, dtype=i32), z(2, dtype=i32), scale=1.0, out=ql)
     with pytest.raises(ValueError, match="65535"):
         hb.latent_attention(z(65536, 1, 32 + 64), z(1, 48, 128), cl, z(65536, 1, dtype=i32), z(65536, dtype=i32), scale=1.0)
+
+
+@pytest.mark.parametrize("cache", ["bf16", "f16", "q8"])
+@pytest.mark.parametrize("H", [4, 128])
+def test_latent_batch_with_rows_out_of_range(gpu, cache, H):
+    """Sequences that cannot be read between ones that can, with few heads (a sequence's pieces joined by several warps) and
+    many (a warp a sequence): zeros, NaN, and the others as without them."""
+    g = gen(65)
+    lens = [40, -3, 33, 10 ** 6, 64, 0, 1, 130, 65, 17, 200, 5, 129]
+    x = "f16" if cache == "f16" else "bf16"
+    pools, table, (rows,) = filled(g, [max(0, min(n, 200)) for n in lens], 1, 16, 320, cache, sides=1)
+    table[7, 4] = 10 ** 6                                    # no such page
+    cp, cs = (cu(t) for t in pools[0])
+    q, w = randn(g, 13, H, 64 + 64, dtype=F[x]), randn(g, H, 64 + 128, 256, dtype=F[x], scale=0.06)
+    out = hb.latent_attention(q.cuda(), w.cuda(), cp, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scale=0.09, c_scale=cs).cpu()
+    assert (out[[1, 5]] == 0).all() and torch.isnan(out[[3, 7]]).all()
+    for b in (0, 2, 4, 6, 8, 9, 10, 11, 12):
+        qd, wd = q[b].double(), w.double()
+        qa = torch.cat([torch.einsum("hd,hdr->hr", qd[:, :64], wd[:, :64]), qd[:, 64:]], -1)
+        o, _, _, _ = attend(qa, rows[b], rows[b][..., :256], 0.09)
+        want = torch.einsum("hr,hvr->hv", o, wd[:, 64:])
+        # in the 2-norm at most the half steps of the queries, the weights and the output as operands together
+        assert (out[b].double() - want).norm() <= 4 * half_step(torch.bfloat16 if cache == "q8" else F[x]) * want.norm(), b
