@@ -84,8 +84,9 @@ constexpr int TABLE_ITEMS = 4096;   // values of a CTA, at least a row
 
 // cs[i][j] = factor * (cos, sin)(2 pi frac(p * turns_j)). The product and its fractional part are formed in 64 bits (far
 // positions keep their phase); the f32 part of the fraction goes through sincospif and the rest, below 2^-25 of a turn,
-// enters to first order. Written once, 8 bytes an angle; what bounds it is the arithmetic, some 60 instructions an angle:
-// 131072 positions of 64 angles in 25 us, 2.7 TB/s.
+// enters to first order. Written once, 8 bytes an angle; the writes bound it: 131072 positions of 64 angles in 24.6 us, 2.7 TB/s
+// (four times as many 3.3, the write half of the copy rate). Phases as 64-bit integers with shorter polynomials, and 16-byte
+// stores, took the same time to a hundredth.
 __global__ void __launch_bounds__(256) k_rope_table(const __grid_constant__ FreqArg f, int half, FastDiv by_half, int rows, int64_t pos0,
                                                     int64_t n_pos, float2 *__restrict__ cs) {
     __shared__ double turns[512];      // lanes of a warp want different ones, which the parameter bank serves one by one

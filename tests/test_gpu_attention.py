@@ -916,3 +916,15 @@ def test_latent_batch_with_rows_out_of_range(gpu, cache, H):
         want = torch.einsum("hr,hvr->hv", o, wd[:, 64:])
         # in the 2-norm at most the half steps of the queries, the weights and the output as operands together
         assert (out[b].double() - want).norm() <= 4 * half_step(torch.bfloat16 if cache == "q8" else F[x]) * want.norm(), b
+
+
+def test_rope_table_of_any_frequencies(gpu):
+    """Frequencies of more than a turn, tiny, negative and zero ones, at positions of either sign."""
+    f = torch.tensor([0.0, 1.0, -1.0, 6.5, -300.25, 1e-7, -1e-7, 1e-12, 2 * math.pi, 3e-3, 0.5, 1e4], dtype=torch.float64)
+    for first in (-2 ** 31 + 1, -5, 0, 2 ** 31 - 40):
+        got = hb.rope_table(f.numpy(), 40, first=first).cpu().double()
+        ang = torch.arange(first, first + 40, dtype=torch.float64)[:, None] * f
+        want = torch.stack([ang.cos(), ang.sin()], -1)
+        # 2 ulp of the value (4 half steps), and the 64-bit phase: angle * 2^-52, each side's
+        tol = 4 * W * want.abs() + (ang.abs() * 2.0 ** -51)[..., None] + 2.0 ** -40
+        assert (got - want).abs().le(tol).all(), (first, ((got - want).abs() / tol).max())
