@@ -26,7 +26,7 @@
 // (an unused slot may hold NaN, and 0 x NaN would reach every sum); tensor-map boxes of 64 x 64 took longer.
 //
 // Measured (64 heads, 512 + 64 values a row, 128 + 128 a head): 32 sequences of up to 8191, bf16: 87 us, 204 MB of
-// rows and 17 MB of weights, 2.5 TB/s; one of 1531: 26 us; 4 Q8 sequences of up to 65536 with 16 heads: 61 us. Of the 87 us
+// rows and 17 MB of weights, 2.5 TB/s; one of 1531: 26 us; 4 Q8 sequences of up to 65536 with 16 heads: 63 us. Of the 87 us
 // absorb takes 7, the core 68 after it and expand 11 after that. A tile of the core takes some 4500 cycles
 // (72 KB: 16 bytes a cycle and SM, the copy rate is 23): its buffer waits for scores (1500), softmax (1900) and half of
 // the values' products (1300) before the next rows (3000 to 4000) may follow, and there is room for two buffers. Asking for
