@@ -301,7 +301,8 @@ def _places(s):
 def _codes(x):
     """The Q8 codes and scales of blocks of 64 (the activation blocks' rule)."""
     blk = x.view(*x.shape[:-1], x.shape[-1] // 64, 64)
-    d = blk.abs().amax(-1) / 127.0
+    # by a tensor: a Python number on the right becomes a product with the rounded 1 / 127 on a GPU, a scale in twenty off by an ulp
+    d = blk.abs().amax(-1) / torch.full((), 127.0, device=x.device)
     inv = torch.where(d != 0, 1.0 / d, torch.zeros_like(d))
     return (blk * inv[..., None]).clamp(-127, 127).round().to(torch.int8).view(x.shape), d
 
