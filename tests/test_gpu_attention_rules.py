@@ -1,0 +1,54 @@
+"""What the attention operators' entry points promise, on the GPU: the quantiser's rule in every form of it, the bits that
+weights and rows carry into the matrix products, far rotary positions, and batches with sequences that cannot be read.
+
+Bounds are those of tests/test_gpu_attention.py with, for a weight, what the kernels carry of it: u is half a step of an
+element type; two bf16 terms leave 2^-16 of a value (each 2^-8), three 2^-24, two f16 terms 2^-22, one f16 term 2^-11."""
+import math
+from fractions import Fraction
+
+import numpy as np
+import pytest
+import torch
+
+import hearth_b200 as hb
+from tests.attn_util import F, attend, gen, half_step, put, pool, randn, table_of
+from tests.test_gpu_attention import cu, filled
+
+gpu_only = pytest.mark.gpu
+W = 2.0 ** -24
+
+
+def carried(cache, x):
+    """What a decode weight loses as the matrix operands the kernel carries it in."""
+    if cache == "bf16":
+        return half_step(torch.bfloat16) ** (3 if x == "f32" else 2)
+    return half_step(torch.float16) ** 2
+
+
+def check_out(got, want, vabs, big, n, x, up, D):
+    """An attention output's bound. Below 2^-14 the values of f16 are 2^-24 apart, so that rounding to it is off by up to 2^-25
+    whatever the value's own size."""
+    ds = (D + 16) * W * big[:, None]
+    tol = half_step(F[x]) * want.abs() + (2.0 ** -25 if x == "f16" else 1e-30) + (2 * ds + up + 2.0 ** -21 + n * W) * vabs
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), (err / tol).max()
+
+
+# ----------------------------------------------------------------------------------------- the quantiser's rule
+
+@gpu_only
+@pytest.mark.parametrize("x", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rot", [0, 64])
+def test_cache_rows_equal_their_plain_form(gpu, x, rot):
+    """Rows of every type through a Q8 cache and back as f32: the calls' outputs, those of the plain form that the operators are
+    measured against, and the rule in 64 bits are equal bit for bit (rows of few bits land on half a code often)."""
+    from perf import operators as P
+    case = dict(op="kv", B=3, n_new=700, Hkv=2, D=128, pt=16, cache="q8", x=x, y="f32", rot=rot, off=0, inter=False, past=40, latent=False)
+    want = [t.float() for t in P.exact(case, 5)]
+    try:
+        for own in (False, True):
+            P.own = own
+            for got, ref in zip(P.run(P.prepare(case, 5)), want):
+                assert torch.equal(got, ref), (own, (got != ref).sum())
+    finally:
+        P.own = False
