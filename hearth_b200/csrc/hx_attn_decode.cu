@@ -21,7 +21,7 @@
 // of 8. The next tile's rows are on their way while one is worked on: up to 8 KB a warp, 12 warps an SM.
 //
 // Measured: one bf16 sequence of 262147, 32 heads over 4 of 128: 96 us, 5.6 TB/s, 87 % of the copy rate (the split kernel
-// alone 96 %); 48 Q8 sequences of up to 6011: 60 us, 3.1 TB/s, where a CTA has several pieces, each with its own queries, first
+// alone 96 %); 48 Q8 sequences of up to 6011: 58.6 us, 3.1 TB/s, where a CTA has several pieces, each with its own queries, first
 // loads and sums (some 12 us a call together), and half of the issue slots go to codes and weights; one f16 sequence of 777
 // with 16 heads: 13 us on the GPU, 22 with the call.
 //
@@ -30,9 +30,9 @@
 // after a power of two that puts the head's largest value at 2^13), and weights into 2 terms (bf16 for f32
 // outputs: 3), since one rounding of each weight to the operand's type would be as large as the output's own.
 // f16 weights carry 2^14, so that those down to 2^-38 of the largest count; Q8 ones are taken relative to the power of
-// two of the largest value scale so far. Q8 keys of 16-bit queries go in as 1152 + code, the form the bytes have under f16's
-// exponent, and the sums start at -1152 times the query's: the products stay exact, and what the larger sums lose
-// is below 2^-18 of the score's terms.
+// two of the largest value scale so far. Q8 keys go in as the codes themselves, one packed subtraction a pair from the form the
+// bytes have under f16's exponent (1152 + code): taking 1152 times the query off the sums instead loses up to 2^-12
+// of the score's terms where one large key channel leaves the others of its block codes of a few steps.
 #include "hx_attn.cuh"
 
 #include <algorithm>
@@ -79,14 +79,10 @@ __device__ __forceinline__ uint32_t trans8x8(uint32_t x) {
     return y;
 }
 
-// Bytes 0, 1 (HI: 2, 3) of codes as an f16 pair: a byte with its sign bit flipped under 0x64 is 1152 + code.
-template <bool HI>
-__device__ __forceinline__ uint32_t lifted2(uint32_t flipped) {
-    return __byte_perm(flipped, 0x64646464u, HI ? 0x4342 : 0x4140);
-}
+// Bytes 0, 1 (HI: 2, 3) of codes as an f16 pair: a byte with its sign bit flipped under 0x64 is 1152 + code, less 1152.
 template <bool HI>
 __device__ __forceinline__ uint32_t codes2(uint32_t flipped) {
-    const uint32_t x = lifted2<HI>(flipped), off = 0x64806480u;
+    const uint32_t x = __byte_perm(flipped, 0x64646464u, HI ? 0x4342 : 0x4140), off = 0x64806480u;
     const __half2 r = __hsub2(reinterpret_cast<const __half2 &>(x), reinterpret_cast<const __half2 &>(off));
     return reinterpret_cast<const uint32_t &>(r);
 }
@@ -106,12 +102,11 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_sp
     constexpr int UNIT = Sh::UNIT, COLS = Sh::COLS;
     constexpr int OT = CACHE == BF16 ? BF16 : F16;   // the operands' type
     constexpr float POFF = OT == F16 ? 14.0f : 0.0f;
-    constexpr bool LIFTED = CACHE == Q8 && NTQ == 1;
     extern __shared__ __align__(16) uint8_t smem[];
     uint4 *qs = reinterpret_cast<uint4 *>(smem);                    // [term][column tile][32-dim step][lane]
     float *mrg = reinterpret_cast<float *>(smem + Sh::Q_BYTES);     // [warp][column][OROW]
     __shared__ int64_t scan[AD_WARPS];
-    __shared__ float wm[AD_WARPS][COLS], wl[AD_WARPS][COLS], qfac[COLS], qsum[NJ][COLS];
+    __shared__ float wm[AD_WARPS][COLS], wl[AD_WARPS][COLS], qfac[COLS];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int D = a.D, chunks = D / 8, n_pairs = a.c.Hkv * a.passes;
@@ -256,11 +251,6 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_sp
             }
             if (lane == 0) qfac[h] = fac;
             if (lane < 8 * NJ) {
-                float sum = 0.0f;
-                if constexpr (LIFTED) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sum += x[i];
-                }
                 const int step = CACHE == Q8 ? 2 * (lane >> 3) + (lane & 1) : lane >> 2, tt = CACHE == Q8 ? (lane & 7) >> 1 : lane & 3;
 #pragma unroll
                 for (int k = 0; k < NTQ; k++) {
@@ -269,25 +259,11 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_sp
                     w.z = take_pair<OT>(x[4], x[5]), w.w = take_pair<OT>(x[6], x[7]);
                     qs[((k * NHT + (h >> 3)) * 2 * NJ + step) * 32 + (h & 7) * 4 + tt] = w;
                 }
-                if constexpr (LIFTED) {      // what the operands, rounded, add up to over a block
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sum -= x[i];
-                    const uint32_t eight = 0xffu << (lane & 24);
-#pragma unroll
-                    for (int o = 1; o <= 4; o <<= 1) sum += __shfl_xor_sync(eight, sum, o);
-                    if ((lane & 7) == 0) qsum[lane >> 3][h] = -1152.0f * sum;
-                }
             }
         }
         __syncthreads();
-        float fac[NHT][2], bias[LIFTED ? NJ : 1][NHT][2] = {};
+        float fac[NHT][2];
         int ve[CACHE == Q8 ? NJ : 1] = {};      // exponents of the largest value scales so far
-        if constexpr (LIFTED) {
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-                for (int c = 0; c < NHT; c++) bias[j][c][0] = qsum[j][8 * c + 2 * t], bias[j][c][1] = qsum[j][8 * c + 2 * t + 1];
-        }
 #pragma unroll
         for (int c = 0; c < NHT; c++) fac[c][0] = qfac[8 * c + 2 * t], fac[c][1] = qfac[8 * c + 2 * t + 1];
 
@@ -308,14 +284,13 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_sp
                 if constexpr (CACHE == Q8) {
 #pragma unroll
                     for (int j = 0; j < NJ; j++) {
-                        float p[4] = {bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1], bias[LIFTED ? j : 0][c][0], bias[LIFTED ? j : 0][c][1]};
+                        float p[4] = {};
                         const uint32_t w0[4] = {kr[0][j].x, kr[0][j].y, kr[0][j].z, kr[0][j].w};
                         const uint32_t w1[4] = {kr[1][j].x, kr[1][j].y, kr[1][j].z, kr[1][j].w};
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const uint32_t f0 = w0[e] ^ 0x80808080u, f1 = w1[e] ^ 0x80808080u;
-                            const uint32_t a0 = LIFTED ? lifted2<false>(f0) : codes2<false>(f0), a1 = LIFTED ? lifted2<false>(f1) : codes2<false>(f1);
-                            const uint32_t a2 = LIFTED ? lifted2<true>(f0) : codes2<true>(f0), a3 = LIFTED ? lifted2<true>(f1) : codes2<true>(f1);
+                            const uint32_t a0 = codes2<false>(f0), a1 = codes2<false>(f1), a2 = codes2<true>(f0), a3 = codes2<true>(f1);
 #pragma unroll
                             for (int k = NTQ - 1; k >= 0; k--) {
                                 const uint4 q = qs[((k * NHT + c) * 2 * NJ + 2 * j + (e >> 1)) * 32 + lane];

@@ -52,3 +52,35 @@ def test_cache_rows_equal_their_plain_form(gpu, x, rot):
                 assert torch.equal(got, ref), (own, (got != ref).sum())
     finally:
         P.own = False
+
+
+# ----------------------------------------------------------------------------------------- the bits of the products
+
+def check_lse(got, want, big, n, D):
+    assert ((got.double() - want).abs() <= (D + 16) * W * big + 2.0 ** -20 + n * W + 2 * W * want.abs()).all(), (got.double() - want).abs().max()
+
+
+@gpu_only
+@pytest.mark.parametrize("x", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("H,Hkv", [(8, 1), (4, 4), (32, 2)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_q8_keys_with_a_large_channel(gpu, x, H, Hkv, D):
+    """One large key and value channel a block, which sets the block's scale, so that the other codes are 0 to 2; queries of one
+    sign and scores of 20 to 50, whose terms hold no cancellation: the sums may lose a few f32 roundings of them."""
+    g = gen(70)
+    n, pt = 200, 16
+    table, total = table_of(g, [n], pt)
+    (kp, ks), (vp, vs) = (pool(g, total, Hkv, pt, D, "q8") for _ in range(2))
+    step = 1.0 / 16
+    k, v = ((torch.randint(0, 3, (n, Hkv, D), generator=g) * step).double() for _ in range(2))
+    k[:, :, 5::64] = v[:, :, 17::64] = 127 * step
+    krows, vrows = (torch.stack([put(p, s, table, 0, i, pt, r[i]) for i in range(n)]) for p, s, r in ((kp, ks, k), (vp, vs, v)))
+    q = (0.5 + torch.rand((1, H, D), generator=g)).to(F[x])
+    q[..., 5::64] = 0.01
+    scale = 32.0 / (D * step)
+    out, lse = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.tensor([n], dtype=torch.int32).cuda(), scale=scale,
+                                   k_scale=ks.cuda(), v_scale=vs.cuda(), return_lse=True)
+    want, wl, vabs, big = attend(q[0].double(), krows, vrows, scale)
+    assert 20 < big.min() and big.max() < 50
+    check_lse(lse[0].cpu(), wl, big, n, D)
+    check_out(out[0].cpu(), want, vabs, big, n, x, carried("q8", x), D)
