@@ -76,20 +76,21 @@ constexpr int ROW_THREADS = 256, ROW_AHEAD = 4, ROW_ITEMS = ROW_THREADS * ROW_AH
 // ------------------------------------------------------------------------------------------- rotary tables
 
 struct FreqArg {
-    double turns[512];   // inv_freq / (2 pi)
+    double2 turns[512];  // inv_freq / (2 pi) in two terms
     float fhi, flo;      // the factor in two terms
 };
 
 constexpr int TABLE_ITEMS = 4096;   // values of a CTA, at least a row
 
-// cs[i][j] = factor * (cos, sin)(2 pi frac(p * turns_j)). The product and its fractional part are formed in 64 bits (far
-// positions keep their phase); the f32 part of the fraction goes through sincospif and the rest, below 2^-25 of a turn,
-// enters to first order. Written once, 8 bytes an angle; the writes bound it: 131072 positions of 64 angles in 24.6 us, 2.7 TB/s
-// (four times as many 3.3, the write half of the copy rate). Phases as 64-bit integers with shorter polynomials, and 16-byte
-// stores, took the same time to a hundredth.
+// cs[i][j] = factor * (cos, sin)(2 pi frac(p * turns_j)). The product and its fractional part are formed in 64 bits, with what the
+// quotient and the product lose there added to the fraction (without it a frequency of 1 near position 2^31 is off by
+// 2^-22); the f32 part of the fraction goes through sincospif and the rest, below 2^-25 of a half turn,
+// enters to first order. 131072 positions of 64 angles, 67 MB written once: 24.6 us, 2.7 TB/s. A copy without sincospif takes 18.6 us,
+// one without the 64-bit fraction 18.5, one without either 18.6, and a fill with a constant 12.3: arithmetic and writes
+// each hold up the other.
 __global__ void __launch_bounds__(256) k_rope_table(const __grid_constant__ FreqArg f, int half, FastDiv by_half, int rows, int64_t pos0,
                                                     int64_t n_pos, float2 *__restrict__ cs) {
-    __shared__ double turns[512];      // lanes of a warp want different ones, which the parameter bank serves one by one
+    __shared__ double2 turns[512];     // lanes of a warp want different ones, which the parameter bank serves one by one
     for (int j = threadIdx.x; j < half; j += 256) turns[j] = f.turns[j];
     __syncthreads();
     const int64_t r0 = (int64_t)blockIdx.x * rows;
@@ -97,8 +98,8 @@ __global__ void __launch_bounds__(256) k_rope_table(const __grid_constant__ Freq
 #pragma unroll 2
     for (int i = threadIdx.x; i < n; i += 256) {
         const int p = (int)by_half.div(i), j = i - p * half;
-        const double t = (double)(pos0 + r0 + p) * turns[j];
-        const double r = 2.0 * (t - rint(t));      // half turns, in [-1, 1], exact after the product
+        const double x = (double)(pos0 + r0 + p), t = x * turns[j].x;
+        const double r = 2.0 * ((t - rint(t)) + __fma_rn(x, turns[j].y, __fma_rn(x, turns[j].x, -t)));      // half turns, in [-1, 1] or just past it
         const float hi = (float)r, lo = (float)(r - (double)hi) * 3.14159265358979f;
         float s, c;
         sincospif(hi, &s, &c);
@@ -578,9 +579,11 @@ extern "C" HXB_API int hxb_rope_table_dev(const double *inv_freq, int rope_dim, 
     if (n_pos == 0) return HXB_OK;
     if (!cs || !aligned(cs, 8)) return attn_fail(HXB_E_ARG, "rope_table: the table must be 8-byte aligned");
     FreqArg f;
+    const double turn = 2 * 3.14159265358979323846, turn_rest = 2.4492935982947064e-16;      // 2 pi in two terms
     for (int j = 0; j < rope_dim / 2; j++) {
         if (!std::isfinite(inv_freq[j])) return attn_fail(HXB_E_ARG, "rope_table: frequency %d is not finite", j);
-        f.turns[j] = inv_freq[j] / (2 * 3.14159265358979323846);
+        const double t = inv_freq[j] / turn;
+        f.turns[j] = make_double2(t, (std::fma(-t, turn, inv_freq[j]) - t * turn_rest) / turn);
     }
     f.fhi = (float)attn_factor, f.flo = (float)(attn_factor - f.fhi);
     const int half = rope_dim / 2, rows = std::max(1, TABLE_ITEMS / half);

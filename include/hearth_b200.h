@@ -117,7 +117,8 @@ enum { HXB_ROPE_NONE = 0, HXB_ROPE_LINEAR = 1, HXB_ROPE_NTK = 2, HXB_ROPE_YARN =
 HXB_API int hxb_rope_freqs(int rope_dim, double theta, int scaling, double factor, int original, double beta_fast,
                            double beta_slow, double *inv_freq, double *attn_factor);
 /* cs [n_pos][rope_dim / 2][2] = attn_factor * (cos, sin)(p * inv_freq[j]) for p = pos0 + i, |p| < 2^31. inv_freq
- * is a host array. The angle is reduced in 64 bits, so far positions lose nothing (within 2 ulp of f32). */
+ * is a host array. The angle is reduced with twice 64 bits, so that far positions lose nothing: a value is within
+ * 2^-22 of itself (2 ulp of f32) and 2^-44 of attn_factor, for |p * inv_freq| < 2^52. */
 HXB_API int hxb_rope_table_dev(const double *inv_freq, int rope_dim, double attn_factor, int64_t pos0, int64_t n_pos,
                                float *cs, void *stream);
 

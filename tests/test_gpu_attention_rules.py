@@ -84,3 +84,51 @@ def test_q8_keys_with_a_large_channel(gpu, x, H, Hkv, D):
     assert 20 < big.min() and big.max() < 50
     check_lse(lse[0].cpu(), wl, big, n, D)
     check_out(out[0].cpu(), want, vabs, big, n, x, carried("q8", x), D)
+
+
+# ----------------------------------------------------------------------------------------- far rotary positions
+
+def _pi():
+    """pi * 2^220 by Machin's formula."""
+    def atan_inv(m):
+        total, term, k = 0, (1 << 260) // m, 0
+        while term:
+            total += (-1) ** k * (term // (2 * k + 1))
+            term //= m * m
+            k += 1
+        return total
+    return (16 * atan_inv(5) - 4 * atan_inv(239)) >> 40
+
+
+def exact_table(freqs, first, n):
+    """cos and sin of p * f with the angle reduced as a fraction: [n, len(freqs), 2]."""
+    quarter, out = _pi() // 2, np.empty((n, len(freqs), 2))
+    for j, f in enumerate(freqs):
+        num, den = Fraction(float(f)).as_integer_ratio()
+        for i in range(n):
+            a = ((first + i) * num << 220) // den
+            k = (2 * a + quarter) // (2 * quarter)
+            r = (a - k * quarter) / (1 << 220)
+            c, s = math.cos(r), math.sin(r)
+            out[i, j] = ((c, s), (-s, c), (-c, -s), (s, -c))[k % 4]
+    return torch.from_numpy(out)
+
+
+def test_exact_table():
+    f = [1.0, 0.731, -3e-5, 0.0]
+    a = torch.arange(-3, 40, dtype=torch.float64)[:, None] * torch.tensor(f, dtype=torch.float64)
+    assert (exact_table(f, -3, 43) - torch.stack([a.cos(), a.sin()], -1)).abs().max() < 1e-14
+
+
+@gpu_only
+@pytest.mark.parametrize("first", [2 ** 31 - 400, -2 ** 31 + 1, 10 ** 9 + 7, 131072, 0])
+@pytest.mark.parametrize("scaling,factor", [("none", 1.0), ("yarn", 7.3)])
+def test_rope_table_at_far_positions(gpu, first, scaling, factor):
+    """The phase loses nothing at any position: against angles reduced as fractions, 2^-22 of the value (an ulp of sincospif and
+    two roundings) and 2^-44 of the factor (the fraction's rest to first order)."""
+    f, a = hb.rope_freqs(64, 1e4, scaling=scaling, factor=factor)
+    f = np.concatenate([f, [1.0, -1.0, 6.5, 300.25, math.pi, 2 * math.pi, 1e-7]])
+    got = hb.rope_table(f, 400, first=first, factor=a).cpu().double()
+    want = exact_table(f, first, 400) * a
+    err, tol = (got - want).abs(), 2.0 ** -22 * want.abs() + a * 2.0 ** -44
+    assert (err <= tol).all(), ((err / tol).max(), (err > tol).sum())
