@@ -86,6 +86,148 @@ def test_q8_keys_with_a_large_channel(gpu, x, H, Hkv, D):
     check_out(out[0].cpu(), want, vabs, big, n, x, carried("q8", x), D)
 
 
+T_OPPOSITE = [s * 2.0 ** -e for e in range(12) for s in (1.0, 1.25, 1.625)]      # exact in every type
+
+
+def opposite_rows(g, D, cache):
+    """Two positions with opposite values, and keys that are one value each: out = tanh(t) v, where nothing of the weights' own
+    size is left, so that what a weight loses shows."""
+    table, total = table_of(g, [2], 16)
+    (kp, ks), (vp, vs) = (pool(g, total, 1, 16, D, cache) for _ in range(2))
+    k = torch.zeros(1, D, dtype=torch.float64)
+    k[0, 0] = 1.0
+    v = randn(g, 1, D).double()
+    krows, vrows = (torch.stack([put(p, s, table, 0, i, 16, r * (1 - 2 * i)) for i in range(2)]) for p, s, r in ((kp, ks, k), (vp, vs, v)))
+    return kp, ks, vp, vs, table, krows, vrows
+
+
+@gpu_only
+@pytest.mark.parametrize("x", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+def test_decode_weights_carry_their_terms(gpu, cache, x):
+    D, B = 64, len(T_OPPOSITE)
+    kp, ks, vp, vs, table, krows, vrows = opposite_rows(gen(71), D, cache)
+    q = torch.zeros(B, 2, D, dtype=F[x])
+    q[:, 0, 0], q[:, 1, 0] = torch.tensor(T_OPPOSITE, dtype=F[x]), -torch.tensor(T_OPPOSITE, dtype=F[x])
+    out = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda().expand(B, -1), torch.full((B,), 2, dtype=torch.int32).cuda(), scale=1.0,
+                              k_scale=cu(ks), v_scale=cu(vs)).cpu()
+    for b in range(B):
+        want, _, vabs, big = attend(q[b].double(), krows, vrows, 1.0)
+        check_out(out[b], want, vabs, big, 2, x, carried(cache, x), D)
+
+
+@pytest.mark.parametrize("x", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+def test_a_term_less_is_seen(cache, x):
+    """The bounds of the test above, with a term less planted in the oracle's weights: outside them."""
+    D, op = 64, torch.bfloat16 if cache == "bf16" else torch.float16
+    _, _, _, _, _, krows, vrows = opposite_rows(gen(71), D, cache)
+    seen = 0
+    for t in T_OPPOSITE:
+        q = torch.zeros(1, D, dtype=torch.float64)
+        q[0, 0] = t
+        want, _, vabs, big = attend(q, krows, vrows, 1.0)
+        s = krows[:, 0] @ q[0]
+        p = torch.exp(s - s.max())
+        w = p.float().to(op).double()
+        if cache == "bf16" and x == "f32":                # two terms of three
+            w = w + (p - w).float().to(op).double()
+        got = ((w[:, None] * vrows[:, 0]).sum(0) / p.sum()).float().to(F[x])
+        try:
+            check_out(got[None], want, vabs, big, 2, x, carried(cache, x), D)
+        except AssertionError:
+            seen += 1
+    assert seen >= 4, seen
+
+
+def latent_opposite(g, R, cache, x):
+    """The same for latent attention: latents c and -c, queries along c, value rows that pick the latent's own values."""
+    dr, dn, dv, pt = 64, 16, min(R, 256), 16
+    table, total = table_of(g, [2], pt)
+    cp, cs = pool(g, total, 1, pt, R + dr, cache)
+    c = torch.zeros(1, R + dr, dtype=torch.float64)
+    c[0, :R] = (0.5 + torch.rand(R, generator=g)).double() * (1 - 2 * torch.randint(0, 2, (R,), generator=g))
+    rows = torch.stack([put(cp, cs, table, 0, i, pt, c * (1 - 2 * i)) for i in range(2)])
+    w = torch.zeros(1, dn + dv, R, dtype=F[x])
+    w[0, 0] = (torch.sign(c[0, :R]) * (0.5 + torch.rand(R, generator=g))).to(F[x])
+    w[0, dn:] = torch.eye(dv, R)
+    q = torch.zeros(len(T_OPPOSITE), 1, dn + dr, dtype=F[x])
+    q[:, 0, 0] = torch.tensor(T_OPPOSITE, dtype=F[x])
+    return cp, cs, table, rows, w, q, dn, dv
+
+
+def latent_bound(rows, w, q, b, R, dn, dv, cache, x, scale):
+    """The 64-bit output and its bound: scores lose the queries' operands (and a Q8 row's, in f16), weights two bf16 terms or one
+    f16 term, o its two terms; opposite rows round alike, so a Q8 row's rounding is relative to the output."""
+    op = half_step(torch.bfloat16 if cache == "bf16" else torch.float16)
+    qa = torch.cat([q[b, :, :dn].double() @ w[0, :dn].double(), q[b, :, dn:].double()], -1)
+    o, _, vabs, big = attend(qa, rows, rows[..., :R], scale)
+    ds = ((2 if cache == "q8" else 1) * op + (R + 96) * W) * big
+    lost = op ** 2 if cache == "bf16" else op
+    want, vabs = o[0, :dv], vabs[0, :dv]
+    # 2^-25: half the distance of f16's values below 2^-14, 2^-24
+    return want, (2.0 ** -25 if x == "f16" else 0.0) + (half_step(F[x]) + (op if cache == "q8" else 0.0) + 2.0 ** -15) * want.abs() + (2 * ds + lost + 2.0 ** -21 + (R + 16) * W) * vabs
+
+
+@gpu_only
+@pytest.mark.parametrize("cache,x", [("bf16", "bf16"), ("f16", "f16"), ("q8", "f16"), ("q8", "bf16")])
+@pytest.mark.parametrize("R", [128, 512])
+def test_latent_weights_and_rows_carry_their_terms(gpu, cache, x, R):
+    cp, cs, table, rows, w, q, dn, dv = latent_opposite(gen(72), R, cache, x)
+    B, scale = len(T_OPPOSITE), 1.0 / R
+    out = hb.latent_attention(q.cuda(), w.cuda(), cp.cuda(), table.cuda().expand(B, -1), torch.full((B,), 2, dtype=torch.int32).cuda(), scale=scale,
+                              c_scale=cu(cs)).cpu()
+    for b in range(B):
+        want, tol = latent_bound(rows, w, q, b, R, dn, dv, cache, x, scale)
+        err = (out[b, 0].double() - want).abs()
+        assert (err <= tol).all(), (T_OPPOSITE[b], (err / tol).max())
+
+
+@pytest.mark.parametrize("cache,x", [("bf16", "bf16"), ("f16", "f16"), ("q8", "f16")])
+def test_a_latent_term_less_is_seen(cache, x):
+    """The bounds of the test above with one bf16 term planted in the oracle's weights (for a Q8 cache, in the rows too)."""
+    R, scale, seen = 128, 1.0 / 128, 0
+    _, _, _, rows, w, q, dn, dv = latent_opposite(gen(72), R, cache, x)
+    bf = lambda t: t.float().to(torch.bfloat16).double()  # noqa: E731
+    for b in range(len(T_OPPOSITE)):
+        want, tol = latent_bound(rows, w, q, b, R, dn, dv, cache, x, scale)
+        r = bf(rows) if cache == "q8" else rows
+        qa = torch.cat([q[b, :, :dn].double() @ w[0, :dn].double(), q[b, :, dn:].double()], -1)
+        s = (r[:, 0] @ qa[0]) * scale
+        p = torch.exp(s - s.max())
+        got = ((bf(p)[:, None] * r[:, 0, :dv]).sum(0) / p.sum()).float().to(F[x]).double()
+        seen += bool(((got - want).abs() > tol).any())
+    assert seen >= 4, seen
+
+
+# ----------------------------------------------------------------------------------------- sequences out of range
+
+@gpu_only
+@pytest.mark.parametrize("cache", ["bf16", "f16", "q8"])
+@pytest.mark.parametrize("H,Hkv,D", [(8, 1, 64), (4, 4, 128), (40, 2, 64), (16, 2, 256)])
+def test_decode_batch_with_sequences_out_of_range(gpu, cache, H, Hkv, D):
+    """Negative, empty and too long sequences and one with a bad page between ones that can be read: zeros, NaN, and the
+    others' values."""
+    g = gen(73)
+    lens = [40, -7, 33, 2 ** 31 - 1, 64, 0, 1, 130, 65, 17, 200, 10 ** 6, 5, -2 ** 31, 129]
+    pools, table, (krows, vrows) = filled(g, [max(0, min(n, 200)) for n in lens], Hkv, 16, D, cache)
+    table[7, 4] = 10 ** 6                                    # no such page
+    (kp, ks), (vp, vs) = pools
+    q = randn(g, len(lens), H, D, dtype=torch.float16)
+    out, lse = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), scale=D ** -0.5,
+                                   k_scale=cu(ks), v_scale=cu(vs), return_lse=True)
+    out, lse = out.cpu(), lse.cpu()
+    for b, n in enumerate(lens):
+        if n <= 0:
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all()
+        elif n > 200 or b == 7:
+            assert torch.isnan(out[b]).all() and torch.isnan(lse[b]).all()
+        else:
+            want, wl, vabs, big = attend(q[b].double(), krows[b], vrows[b], D ** -0.5)
+            check_out(out[b], want, vabs, big, n, "f16", carried(cache, "f16"), D)
+            check_lse(lse[b], wl, big, n, D)
+
+
 # ----------------------------------------------------------------------------------------- far rotary positions
 
 def _pi():
