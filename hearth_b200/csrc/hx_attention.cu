@@ -502,14 +502,14 @@ int kv_rows(const char *who, const hxb_kv_cache *c, const int32_t *start, const 
             int64_t ks, int64_t kh, void *v, int64_t vs, int64_t vh, int dtype, const hxb_rope *rope, bool write,
             void *stream) {
     RowArgs a = {};
-    const bool latent = c && !c->v;
+    if (c && c->n_pages && !c->v && v) return attn_fail(HXB_E_ARG, "%s: v rows for a cache without v", who);
+    const bool latent = c && !c->v && !v && (c->n_pages || c->n_kv_heads == 1);      // a pool of no pages has no pointers
     int rc = kv_view(c, who, latent, &a.c);
     if (rc != HXB_OK) return rc;
     if (T < 0 || T > 0x7fffffff || !io_dtype(dtype)) return attn_fail(HXB_E_ARG, "%s: bad row count or dtype", who);
     if (rope && !rope_view(rope, c->head_dim, who, &a.r, &rc)) return rc;
     if (T == 0 || c->n_seqs == 0) return HXB_OK;
     if (!start || !pos0 || !k || (!latent && !v)) return attn_fail(HXB_E_ARG, "%s: null pointer", who);
-    if (latent && v) return attn_fail(HXB_E_ARG, "%s: v rows for a cache without v", who);
     if (!aligned(start, 4) || !aligned(pos0, 4) || !aligned(k, elem_size(dtype)) || !aligned(v, elem_size(dtype)))
         return attn_fail(HXB_E_ARG, "%s: pointer not aligned to its elements", who);
     if (ks < 0 || kh < 0 || (!latent && (vs < 0 || vh < 0)) ||

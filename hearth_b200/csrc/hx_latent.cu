@@ -1035,6 +1035,7 @@ extern "C" HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_
     a.o = reinterpret_cast<float *>(at), at += p.o;
     a.ml = reinterpret_cast<float2 *>(at), at += p.ml;
     a.err = reinterpret_cast<int *>(at);
+    if (!a.c.k) a.c.k = ws;      // a pool of no pages: copies of no bytes still name an address
     a.lens = lens, a.q = q, a.w = w, a.out = out, a.qs = q_stride, a.qh = q_head_stride, a.os = out_stride, a.oh = out_head_stride;
     a.H = n_heads, a.R = rank, a.dr = dr, a.dn = nope, a.dv = v_dim, a.passes = p.passes, a.hp = p.hp;
     a.sc2 = scale * 1.44269504088896f;

@@ -225,3 +225,16 @@ def test_python_calls_refuse_before_device_work():
             f()
             pytest.fail(f"call {i} was accepted")
     assert f32 is torch.float32
+
+
+def test_empty_pools_need_no_pointers():
+    """A pool of no pages (its tensors have no memory) is taken by every call, with keys and values and latent."""
+    L = hb.lib()
+    for heads in (1, 2):
+        c = cache(n_kv_heads=heads, n_pages=0, k=0, v=0)
+        for v in (P, None):
+            assert L.hxb_kv_write_dev(C.byref(c), P, P, 0, P, 128, 64, v, 128, 64, 2, None, None) == 0, hb.last_error()
+            assert L.hxb_kv_read_dev(C.byref(c), P, P, 0, P, 128, 64, v, 128, 64, 2, None) == 0, hb.last_error()
+    c = cache(v=0)
+    assert L.hxb_kv_write_dev(C.byref(c), P, P, 5, P, 128, 64, P, 128, 64, 2, None, None) == ARG and "without v" in hb.last_error()
+    assert L.hxb_kv_write_dev(C.byref(c), P, P, 5, P, 128, 64, None, 0, 0, 2, None, None) == ARG

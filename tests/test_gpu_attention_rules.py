@@ -228,6 +228,29 @@ def test_decode_batch_with_sequences_out_of_range(gpu, cache, H, Hkv, D):
             check_lse(lse[b], wl, big, n, D)
 
 
+@gpu_only
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+def test_pools_without_pages(gpu, cache):
+    """No position has a page: nothing is written, rows read back and outputs are NaN, empty sequences stay zeros."""
+    dt, x = (torch.int8 if cache == "q8" else torch.bfloat16), torch.bfloat16
+    kp, vp = (torch.empty(0, 2, 16, 64, dtype=dt, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(0, 2, 16, 1, device="cuda") if cache == "q8" else None for _ in range(2))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    table, start, pos0 = torch.zeros(2, 4, dtype=torch.int32).cuda(), i32(0, 3, 5), i32(0, 7)
+    k = randn(gen(74), 5, 2, 64, dtype=x).cuda()
+    hb.kv_write(k, k, kp, vp, table, start, pos0, k_scale=ks, v_scale=vs)
+    ko, vo = torch.zeros_like(k), torch.zeros_like(k)
+    hb.kv_read(kp, vp, table, start, pos0, ko, vo, k_scale=ks, v_scale=vs)
+    assert torch.isnan(ko).all() and torch.isnan(vo).all()
+    out = hb.decode_attention(k[:2].expand(2, 2, 64).contiguous(), kp, vp, table, i32(30, 0), scale=0.1, k_scale=ks, v_scale=vs)
+    assert torch.isnan(out[0]).all() and (out[1] == 0).all()
+    cp = torch.empty(0, 1, 16, 192, dtype=dt, device="cuda")
+    cs = torch.empty(0, 1, 16, 3, device="cuda") if cache == "q8" else None
+    q, w = randn(gen(75), 2, 4, 32 + 64, dtype=x).cuda(), randn(gen(76), 4, 32 + 16, 128, dtype=x).cuda()
+    out = hb.latent_attention(q, w, cp, table, i32(30, 0), scale=0.1, c_scale=cs)
+    assert torch.isnan(out[0]).all() and (out[1] == 0).all()
+
+
 # ----------------------------------------------------------------------------------------- far rotary positions
 
 def _pi():
