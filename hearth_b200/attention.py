@@ -151,6 +151,8 @@ def _cache(k, v, table, k_scale, v_scale):
 def _rope(cs, interleaved, offset):
     if cs.dtype != _torch()[0].float32 or cs.dim() != 3 or cs.shape[2] != 2 or not cs.is_contiguous():
         _bad("cs must be a contiguous float32 [positions, rope_dim / 2, 2] table")
+    if not 0 <= offset < 1 << 31:      # C's int would wrap
+        _bad(f"offset must not be negative or past a head, got {offset}")
     return Rope(cs.data_ptr(), cs.shape[0], 2 * cs.shape[1], offset, int(bool(interleaved)))
 
 
@@ -169,6 +171,8 @@ def rope_freqs(rope_dim: int, theta: float, *, scaling: str = "none", factor: fl
         _bad(f"scaling must be one of {sorted(_SCALINGS)}, got {scaling!r}")
     if not 2 <= rope_dim <= 1024 or rope_dim % 2:
         _bad(f"rope_dim must be even, 2 to 1024, got {rope_dim}")
+    if not -1 << 31 <= original < 1 << 31:      # C's int would wrap
+        _bad(f"original must be a count of positions, got {original}")
     f, a = np.empty(rope_dim // 2, np.float64), C.c_double()
     _done(lib().hxb_rope_freqs(rope_dim, theta, _SCALINGS[scaling], factor, original, beta_fast, beta_slow, f.ctypes.data,
                                C.byref(a)), "hxb_rope_freqs")
@@ -183,6 +187,8 @@ def rope_table(freqs, n_pos: int, *, first: int = 0, factor: float = 1.0, out=No
         _bad("freqs must be a vector")
     if n_pos < 0:
         _bad("n_pos must not be negative")
+    if not -1 << 31 < first < 1 << 31 or n_pos > (1 << 31) - max(first, 0):
+        _bad(f"positions must lie below 2^31, got {n_pos} from {first} on")
     if out is None:
         if device is None:
             device = stream.device if hasattr(stream, "device") else "cuda"

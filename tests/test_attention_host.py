@@ -238,3 +238,13 @@ def test_empty_pools_need_no_pointers():
     c = cache(v=0)
     assert L.hxb_kv_write_dev(C.byref(c), P, P, 5, P, 128, 64, P, 128, 64, 2, None, None) == ARG and "without v" in hb.last_error()
     assert L.hxb_kv_write_dev(C.byref(c), P, P, 5, P, 128, 64, None, 0, 0, 2, None, None) == ARG
+
+
+def test_numbers_that_c_would_wrap_are_refused():
+    x, cs, pos = torch.zeros(5, 2, 64), torch.zeros(10, 32, 2), torch.zeros(5, dtype=torch.int32)
+    for f, msg in ((lambda: hb.rope(x, pos, cs, offset=1 << 32), "offset"), (lambda: hb.rope(x, pos, cs, offset=-1 << 32), "offset"),
+                   (lambda: hb.rope_freqs(64, 1e4, scaling="yarn", factor=2.0, original=(1 << 32) + 4096), "original"),
+                   (lambda: hb.rope_table([1.0], 4, first=1 << 64), "positions"), (lambda: hb.rope_table([1.0], 4, first=-1 << 31), "positions"),
+                   (lambda: hb.rope_table([1.0], 1 << 40), "positions"), (lambda: hb.rope_table([1.0], 3, first=(1 << 31) - 2), "positions")):
+        with pytest.raises(ValueError, match=msg):
+            f()
