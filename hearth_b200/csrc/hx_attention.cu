@@ -553,7 +553,7 @@ extern "C" HXB_API int hxb_rope_freqs(int rope_dim, double theta, int scaling, d
     if (scaling == HXB_ROPE_YARN) {
         if (original < 1 || !(beta_fast > beta_slow) || !(beta_slow > 0) || !std::isfinite(beta_fast))
             return attn_fail(HXB_E_ARG, "rope_freqs: bad original, beta_fast or beta_slow");
-        // the j at which a frequency makes beta turns over the original positions
+        // the j at which a frequency makes beta turns over the original positions (hi not above 0: none makes beta_slow)
         lo = std::floor(rope_dim * std::log(original / (beta_fast * 2 * pi)) / (2 * std::log(theta)));
         hi = std::ceil(rope_dim * std::log(original / (beta_slow * 2 * pi)) / (2 * std::log(theta)));
         lo = std::max(lo, 0.0);
@@ -564,7 +564,7 @@ extern "C" HXB_API int hxb_rope_freqs(int rope_dim, double theta, int scaling, d
         const double f = std::pow(base, -2.0 * j / rope_dim);
         double keep = 1.0;
         if (scaling == HXB_ROPE_LINEAR) keep = 0.0;
-        if (scaling == HXB_ROPE_YARN) keep = 1.0 - std::min(std::max((j - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+        if (scaling == HXB_ROPE_YARN) keep = hi <= 0 ? 0.0 : 1.0 - std::min(std::max((j - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
         inv_freq[j] = f * keep + (scaling == HXB_ROPE_NONE || scaling == HXB_ROPE_NTK ? 0.0 : f / factor * (1.0 - keep));
     }
     *attn_factor = scaling == HXB_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;

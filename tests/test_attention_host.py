@@ -248,3 +248,12 @@ def test_numbers_that_c_would_wrap_are_refused():
                    (lambda: hb.rope_table([1.0], 1 << 40), "positions"), (lambda: hb.rope_table([1.0], 3, first=(1 << 31) - 2), "positions")):
         with pytest.raises(ValueError, match=msg):
             f()
+
+
+@pytest.mark.parametrize("original,slow", [(1, 1.0), (6, 1.0), (100, 20.0), (4096, 700.0)])
+def test_rope_freqs_yarn_where_no_frequency_turns(original, slow):
+    """Where even the first frequency makes beta_slow turns or fewer over the original positions, all are divided."""
+    assert original / (2 * math.pi) <= slow
+    f, _ = hb.rope_freqs(64, 1e4)
+    g, _ = hb.rope_freqs(64, 1e4, scaling="yarn", factor=8.0, original=original, beta_fast=32 * slow, beta_slow=slow)
+    np.testing.assert_allclose(g, f / 8, rtol=1e-14)
