@@ -576,6 +576,7 @@ extern "C" HXB_API int hxb_rope_table_dev(const double *inv_freq, int rope_dim, 
     if (rope_dim < 2 || rope_dim % 2 || rope_dim > 1024 || !inv_freq || n_pos < 0 || pos0 <= -(1ll << 31) ||
         pos0 >= (1ll << 31) || n_pos > (1ll << 31) - std::max<int64_t>(pos0, 0))
         return attn_fail(HXB_E_ARG, "rope_table: bad rope_dim, positions or frequencies");
+    if (!std::isfinite((float)attn_factor)) return attn_fail(HXB_E_ARG, "rope_table: factor %g is not finite in f32", attn_factor);
     if (n_pos == 0) return HXB_OK;
     if (!cs || !aligned(cs, 8)) return attn_fail(HXB_E_ARG, "rope_table: the table must be 8-byte aligned");
     FreqArg f;

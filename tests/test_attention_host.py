@@ -257,3 +257,9 @@ def test_rope_freqs_yarn_where_no_frequency_turns(original, slow):
     f, _ = hb.rope_freqs(64, 1e4)
     g, _ = hb.rope_freqs(64, 1e4, scaling="yarn", factor=8.0, original=original, beta_fast=32 * slow, beta_slow=slow)
     np.testing.assert_allclose(g, f / 8, rtol=1e-14)
+
+
+@pytest.mark.parametrize("factor", [float("nan"), float("inf"), 1e39])
+def test_rope_table_refuses_factors(factor):
+    f = (C.c_double * 2)(1.0, 0.5)
+    assert hb.lib().hxb_rope_table_dev(f, 4, factor, 0, 10, P, None) == ARG and "factor" in hb.last_error()
