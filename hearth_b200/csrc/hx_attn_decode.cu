@@ -20,10 +20,10 @@
 // value rows per lane, paired by byte permutes. With heads as the 8 columns nothing is padded for groups
 // of 8. The next tile's rows are on their way while one is worked on: up to 8 KB a warp, 12 warps an SM.
 //
-// Measured: one bf16 sequence of 262147, 32 heads over 4 of 128: 96 us, 5.6 TB/s, 87 % of the copy rate (the split kernel
-// alone 96 %); 48 Q8 sequences of up to 6011: 58.6 us, 3.1 TB/s, where a CTA has several pieces, each with its own queries, first
+// Measured: one bf16 sequence of 262147, 32 heads over 4 of 128: 95 us, 5.6 TB/s, 87 % of the copy rate (the split kernel
+// alone 96 %); 48 Q8 sequences of up to 6011: 58.4 us, 3.2 TB/s, where a CTA has several pieces, each with its own queries, first
 // loads and sums (some 12 us a call together), and half of the issue slots go to codes and weights; one f16 sequence of 777
-// with 16 heads: 13 us on the GPU, 22 with the call.
+// with 16 heads: 12 us on the GPU, 22 with the call.
 //
 // Bits. Matrix operands have the cache's type (Q8: f16, which holds the codes exactly; the scales are applied in f32, a
 // value's to its weight). Queries of more bits are split into terms (bf16: 3 for f32, 2 for f16; f16: 2 for f32,
@@ -41,14 +41,15 @@ namespace hx {
 namespace {
 
 constexpr int AD_WARPS = 4, AD_THREADS = 32 * AD_WARPS;
-// Units a piece's beginning and end count for in the division: 48 Q8 sequences of up to 6011: 64.1 us with 0, 62.2, 60.2 and 60.6
+// Units a piece's beginning and end count for in the division: 48 Q8 sequences of up to 6011: 61.5 us with 0, 60.1, 58.5 and 59.4
 // with 1 to 3.
 constexpr int AD_EXTRA = 2;
 
 constexpr int ad_nj(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : 4; }   // blocks of 64 dims, padded
 // Resident CTAs an SM by registers. 16-bit rows of 128 dims: 12 warps with 168 registers each, 8 KB a warp under way (16 with
 // 128 measured 68 % of the copy rate instead of 90 %). Q8 rows are half as long and cost more instructions a byte: 16
-// warps (52 us on 48 sequences of up to 6011; 12: 63, 20: 81).
+// warps (58.5 us a call on 48 sequences of up to 6011; 12: 61.4, 20: 87), whose 128 registers spill 16 bytes of stores and 24
+// of loads at 128 dims (44 and 72 for f32 queries; no other instance spills).
 constexpr int ad_ctas(int cache, int nj, int nht) { return nj * nht <= 2 ? (cache == Q8 ? 4 : 3) : 2; }
 
 // What the join needs beside SplitArgs.
@@ -502,42 +503,35 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constan
         return;
     }
     const int count = sp.last - sp.first + 1;
-    // Twice in an SM's first CTA: the first round, on whatever the scratch holds, brings the code near while the split kernel
-    // still runs (code that runs once is fetched slower than it runs); only the second stores.
-#pragma unroll 1
-    for (int round = blockIdx.y * gridDim.x + blockIdx.x < ATTN_SMS ? 0 : 1; round < 2; round++) {
-        if (round) pdl_wait();
-        __syncthreads();
-        Joined<4> mine;
-        if (live)
+    pdl_wait();
+    Joined<4> mine;
+    if (live)
 #pragma unroll 8
-            for (int i = gr; i < (round ? count : min(count, 8 * groups)); i += groups) {
-                const int64_t at = ((int64_t)(sp.first + i) * 2 + (i == 0 ? sp.slot : 0)) * j.cols + col;
-                const float2 ml = __ldcg(a.ml + at);
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.o + at * D) + qd);
+        for (int i = gr; i < count; i += groups) {
+            const int64_t at = ((int64_t)(sp.first + i) * 2 + (i == 0 ? sp.slot : 0)) * j.cols + col;
+            const float2 ml = __ldcg(a.ml + at);
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.o + at * D) + qd);
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            mine.add(ml, v);
+        }
+    if (groups > 1) {
+        part[tid] = make_float4(mine.o[0], mine.o[1], mine.o[2], mine.o[3]), part_ml[tid] = make_float2(mine.m, mine.l);
+        __syncthreads();
+        if (gr == 0)
+#pragma unroll 1
+            for (int k = 1; k < min(groups, count); k++) {
+                const float4 x = part[k * each + tid];
                 const float v[4] = {x.x, x.y, x.z, x.w};
-                mine.add(ml, v);
+                mine.add(part_ml[k * each + tid], v);
             }
-        if (groups > 1) {
-            part[tid] = make_float4(mine.o[0], mine.o[1], mine.o[2], mine.o[3]), part_ml[tid] = make_float2(mine.m, mine.l);
-            __syncthreads();
-            if (gr == 0)
-#pragma unroll 1
-                for (int k = 1; k < min(groups, count); k++) {
-                    const float4 x = part[k * each + tid];
-                    const float v[4] = {x.x, x.y, x.z, x.w};
-                    mine.add(part_ml[k * each + tid], v);
-                }
-        }
-        if (round && live && gr == 0) {
-#pragma unroll 1
-            for (int k = 0; k < 4; k++) {
-                io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + 4 * qd + k, mine.l == 0.0f ? 0.0f : __fdiv_rn(mine.o[0], mine.l));
-                mine.o[0] = mine.o[1], mine.o[1] = mine.o[2], mine.o[2] = mine.o[3];
-            }
-            if (qd == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = lse_of(mine.m, mine.l, j.off);
-        }
     }
+    if (!live || gr) return;
+#pragma unroll 1
+    for (int k = 0; k < 4; k++) {
+        io_store(a.out, a.dtype, b * a.os + (int64_t)h * a.oh + 4 * qd + k, mine.l == 0.0f ? 0.0f : __fdiv_rn(mine.o[0], mine.l));
+        mine.o[0] = mine.o[1], mine.o[1] = mine.o[2], mine.o[2] = mine.o[3];
+    }
+    if (qd == 0 && a.lse) a.lse[(int64_t)b * a.H + h] = lse_of(mine.m, mine.l, j.off);
 }
 
 // ------------------------------------------------------------------------------------------- host side

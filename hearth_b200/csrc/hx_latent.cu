@@ -25,9 +25,9 @@
 // are fetched by 16-byte asynchronous copies: they take any page size, and rows past the end arrive as zeros
 // (an unused slot may hold NaN, and 0 x NaN would reach every sum); tensor-map boxes of 64 x 64 took longer.
 //
-// Measured (64 heads, 512 + 64 values a row, 128 + 128 a head): 32 sequences of up to 8191, bf16: 87 us, 204 MB of
-// rows and 17 MB of weights, 2.5 TB/s; one of 1531: 26 us; 4 Q8 sequences of up to 65536 with 16 heads: 63 us. Of the 87 us
-// absorb takes 7, the core 68 after it and expand 11 after that. A tile of the core takes some 4500 cycles
+// Measured (64 heads, 512 + 64 values a row, 128 + 128 a head): 32 sequences of up to 8191, bf16: 86 us, 204 MB of
+// rows and 17 MB of weights, 2.6 TB/s; one of 1531: 26 us; 4 Q8 sequences of up to 65536 with 16 heads: 62 us. Of the 86 us
+// absorb takes 7, the core 68 after it and expand 10 after that. A tile of the core takes some 4500 cycles
 // (72 KB: 16 bytes a cycle and SM, the copy rate is 23): its buffer waits for scores (1500), softmax (1900) and half of
 // the values' products (1300) before the next rows (3000 to 4000) may follow, and there is room for two buffers. Asking for
 // the next rows in L2 ahead made it slower (106 us for 99), Q8 codes asked for over a tile's end too (73 us for 66:
@@ -650,7 +650,9 @@ __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_co
         while (!up && walk.next(r)) {
             float ref[2] = {-kv_inf(), -kv_inf()}, sum[2] = {}, fac[2] = {};
             // One dry step while the first loads are on their way, on whatever tensor memory holds and with nothing kept: it
-            // brings the code near (code that runs for the first time is fetched slower than it runs).
+            // brings the code near (code that runs for the first time is fetched slower than it runs): one sequence of 1531 in 24.0 us
+            // of GPU time, 24.7 without it, 4 Q8 ones of up to 65536 in 62.7 and 64.5. The same in the kernels that join cost more
+            // than it gave (0.5 to 1.6 us).
             for (int i = dry ? -1 : 0; i < r.tiles; i++, k++) {
                 const int buf = k & 1;
                 // a wait that fails shows at the next barrier of the four warps, where all of them give up
@@ -813,8 +815,8 @@ struct ExpandShared {
 
 // A CTA a head and up to sixteen sequences. Warps first join the pieces (weights 2^(m_i - max m), in a fixed order) into o, as
 // two terms of the weights' type in shared memory; then each multiplies 16 value rows by (a part of) o. Reads from L2 bound it:
-// 128 KB of weights a head (before the core has ended where its SM is free) and 2 KB a piece. 11 us after the core
-// with 32 sequences of 64 heads, 5 with one.
+// 128 KB of weights a head (before the core has ended where its SM is free) and 2 KB a piece. 10 us after the core
+// with 32 sequences of 64 heads, 4 with one.
 template <int T>
 __global__ void __launch_bounds__(32 * EX_WARPS, 1) k_latent_expand(const __grid_constant__ LatentArgs a, int ex_rows, int grid) {
     extern __shared__ __align__(16) uint8_t raw[];
@@ -848,111 +850,106 @@ __global__ void __launch_bounds__(32 * EX_WARPS, 1) k_latent_expand(const __grid
     const int n = a.lens[b], nu = units_of(a.c, a.lens, b, LT);
     Span sp = {};
     if (nu) sp = span_of(before, CORE_EXTRA, nu, all, grid);
-    // Twice in an SM's first CTA where the core leaves SMs free: the first round, on whatever the scratch holds, brings the code
-    // near while the core still runs (code that runs once is fetched slower than it runs); only the second stores.
-#pragma unroll 1
-    for (int round = all < grid && blockIdx.y * gridDim.x + blockIdx.x < ATTN_SMS ? 0 : 1; round < 2; round++) {
-        if (round) pdl_wait();
-        __syncthreads();
-        if (row < rows) {
-            Joined<16> o;
-            const float *whole = a.qa + ((int64_t)b * a.H + h) * W;
-            const int count = !nu ? 0 : sp.split() ? sp.last - sp.first + 1 : 1;
+    pdl_wait();
+    __syncthreads();
+    if (row < rows) {
+        Joined<16> o;
+        const float *whole = a.qa + ((int64_t)b * a.H + h) * W;
+        const int count = !nu ? 0 : sp.split() ? sp.last - sp.first + 1 : 1;
 #pragma unroll 4
-            for (int i = part; i < (round ? count : min(count, 4 * wpr)); i += wpr) {
-                const int64_t at = ((int64_t)((sp.first + i) * a.passes + pass) * 2 + (i == 0 ? sp.slot : 0)) * a.hp + hc;
-                const float *src = sp.split() ? a.o + at * a.R : whole;
-                const float2 ml = sp.split() ? __ldcg(a.ml + at) : make_float2(__ldcg(whole + a.R), __ldcg(whole + a.R + 1));
-                float x[16] = {};
+        for (int i = part; i < count; i += wpr) {
+            const int64_t at = ((int64_t)((sp.first + i) * a.passes + pass) * 2 + (i == 0 ? sp.slot : 0)) * a.hp + hc;
+            const float *src = sp.split() ? a.o + at * a.R : whole;
+            const float2 ml = sp.split() ? __ldcg(a.ml + at) : make_float2(__ldcg(whole + a.R), __ldcg(whole + a.R + 1));
+            float x[16] = {};
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (k < a.R / 128) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + 128 * k + 4 * lane));
-                        x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
-                    }
-                o.add(ml, x);
-            }
-            // nothing, too long a row and a failed wait as the entry point says
-            const bool bad = *reinterpret_cast<volatile int *>(a.err) || (y.over >> row & 1);
-            if (wpr == 1) {     // the row is whole
-                const float inv = bad ? kv_nan() : o.l == 0.0f ? 0.0f : __fdiv_rn(1.0f, o.l);
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    if (k >= a.R / 128) break;
-                    float x[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = bad || o.l != 0.0f ? __fmul_rn(o.o[4 * k + e], inv) : 0.0f;
-#pragma unroll
-                    for (int term = 0; term < 2; term++) {
-                        uint2 p;
-                        p.x = take_pair<T>(x[0], x[1]), p.y = take_pair<T>(x[2], x[3]);
-                        *reinterpret_cast<uint2 *>(&y.ops[term][4 * k + (lane >> 3)][row >> 3][(row & 7) * 4 + ((lane >> 1) & 3)][2 * (lane & 1)]) = p;
-                    }
+            for (int k = 0; k < 4; k++)
+                if (k < a.R / 128) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + 128 * k + 4 * lane));
+                    x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
                 }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    *reinterpret_cast<float4 *>(&y.join[warp][128 * k + 4 * lane]) = make_float4(o.o[4 * k], o.o[4 * k + 1], o.o[4 * k + 2], o.o[4 * k + 3]);
-                if (lane == 0) y.ml[warp] = make_float2(o.m, bad ? kv_nan() : o.l);
-            }
+            o.add(ml, x);
         }
-        if (wpr > 1) {     // a row's warps together, two dims a thread
-            __syncthreads();
-            if (threadIdx.x < rows * wpr) {
-                const int p0 = threadIdx.x / wpr * wpr;
-                float m = -kv_inf(), l = 0.0f;
-                for (int p = p0; p < p0 + wpr; p++) m = fmaxf(m, y.ml[p].x);
-                const float base = m == -kv_inf() ? 0.0f : m;
-                for (int p = p0; p < p0 + wpr; p++) l = __fmaf_rn(y.ml[p].y, exp2_fast(__fsub_rn(y.ml[p].x, base)), l);
-                y.fac[threadIdx.x] = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(__fsub_rn(y.ml[threadIdx.x].x, base)), l);
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < rows * (a.R / 2); i += 32 * EX_WARPS) {
-                const int rw = i / (a.R / 2), d = 2 * (i - rw * (a.R / 2));
-                float x0 = 0.0f, x1 = 0.0f;
-#pragma unroll 4
-                for (int p = rw * wpr; p < (rw + 1) * wpr; p++) {
-                    const float2 v = *reinterpret_cast<const float2 *>(&y.join[p][d]);
-                    x0 = __fmaf_rn(v.x, y.fac[p], x0), x1 = __fmaf_rn(v.y, y.fac[p], x1);
-                }
+        // nothing, too long a row and a failed wait as the entry point says
+        const bool bad = *reinterpret_cast<volatile int *>(a.err) || (y.over >> row & 1);
+        if (wpr == 1) {     // the row is whole
+            const float inv = bad ? kv_nan() : o.l == 0.0f ? 0.0f : __fdiv_rn(1.0f, o.l);
 #pragma unroll
-                for (int k = 0; k < 2; k++) y.ops[k][d >> 5][rw >> 3][(rw & 7) * 4 + ((d >> 3) & 3)][(d >> 1) & 3] = take_pair<T>(x0, x1);
+            for (int k = 0; k < 4; k++) {
+                if (k >= a.R / 128) break;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = bad || o.l != 0.0f ? __fmul_rn(o.o[4 * k + e], inv) : 0.0f;
+#pragma unroll
+                for (int term = 0; term < 2; term++) {
+                    uint2 p;
+                    p.x = take_pair<T>(x[0], x[1]), p.y = take_pair<T>(x[2], x[3]);
+                    *reinterpret_cast<uint2 *>(&y.ops[term][4 * k + (lane >> 3)][row >> 3][(row & 7) * 4 + ((lane >> 1) & 3)][2 * (lane & 1)]) = p;
+                }
             }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                *reinterpret_cast<float4 *>(&y.join[warp][128 * k + 4 * lane]) = make_float4(o.o[4 * k], o.o[4 * k + 1], o.o[4 * k + 2], o.o[4 * k + 3]);
+            if (lane == 0) y.ml[warp] = make_float2(o.m, bad ? kv_nan() : o.l);
+        }
+    }
+    if (wpr > 1) {     // a row's warps together, two dims a thread
+        __syncthreads();
+        if (threadIdx.x < rows * wpr) {
+            const int p0 = threadIdx.x / wpr * wpr;
+            float m = -kv_inf(), l = 0.0f;
+            for (int p = p0; p < p0 + wpr; p++) m = fmaxf(m, y.ml[p].x);
+            const float base = m == -kv_inf() ? 0.0f : m;
+            for (int p = p0; p < p0 + wpr; p++) l = __fmaf_rn(y.ml[p].y, exp2_fast(__fsub_rn(y.ml[p].x, base)), l);
+            y.fac[threadIdx.x] = l == 0.0f ? 0.0f : __fdiv_rn(exp2_fast(__fsub_rn(y.ml[threadIdx.x].x, base)), l);
         }
         __syncthreads();
-        if (warp < items) {
-            float acc[2][4] = {};
-            auto step = [&](int s, const uint4 &v0, const uint4 &v1) {
+        for (int i = threadIdx.x; i < rows * (a.R / 2); i += 32 * EX_WARPS) {
+            const int rw = i / (a.R / 2), d = 2 * (i - rw * (a.R / 2));
+            float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll 4
+            for (int p = rw * wpr; p < (rw + 1) * wpr; p++) {
+                const float2 v = *reinterpret_cast<const float2 *>(&y.join[p][d]);
+                x0 = __fmaf_rn(v.x, y.fac[p], x0), x1 = __fmaf_rn(v.y, y.fac[p], x1);
+            }
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    if (8 * c >= rows) break;
+            for (int k = 0; k < 2; k++) y.ops[k][d >> 5][rw >> 3][(rw & 7) * 4 + ((d >> 3) & 3)][(d >> 1) & 3] = take_pair<T>(x0, x1);
+        }
+    }
+    __syncthreads();
+    if (warp < items) {
+        float acc[2][4] = {};
+        auto step = [&](int s, const uint4 &v0, const uint4 &v1) {
 #pragma unroll
-                    for (int k = 1; k >= 0; k--) {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(y.ops[k][s][c][lane]);
-                        mma16<T>(acc[c], v0.x, v1.x, v0.y, v1.y, x.x, x.y);
-                        mma16<T>(acc[c], v0.z, v1.z, v0.w, v1.w, x.z, x.w);
-                    }
+            for (int c = 0; c < 2; c++) {
+                if (8 * c >= rows) break;
+#pragma unroll
+                for (int k = 1; k >= 0; k--) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(y.ops[k][s][c][lane]);
+                    mma16<T>(acc[c], v0.x, v1.x, v0.y, v1.y, x.x, x.y);
+                    mma16<T>(acc[c], v0.z, v1.z, v0.w, v1.w, x.z, x.w);
                 }
-            };
-            asm volatile("cp.async.wait_all;" ::: "memory");
+            }
+        };
+        asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 4
-            for (int i = 0; i < EX_KEPT; i++)
-                if (s_first + i < s_end) step(s_first + i, y.w[i][0][threadIdx.x], y.w[i][1][threadIdx.x]);
+        for (int i = 0; i < EX_KEPT; i++)
+            if (s_first + i < s_end) step(s_first + i, y.w[i][0][threadIdx.x], y.w[i][1][threadIdx.x]);
 #pragma unroll 4
-            for (int s = s_first + EX_KEPT; s < s_end; s++) step(s, __ldg(reinterpret_cast<const uint4 *>(at(warp, s, 0))), __ldg(reinterpret_cast<const uint4 *>(at(warp, s, 1))));
+        for (int s = s_first + EX_KEPT; s < s_end; s++) step(s, __ldg(reinterpret_cast<const uint4 *>(at(warp, s, 0))), __ldg(reinterpret_cast<const uint4 *>(at(warp, s, 1))));
 #pragma unroll
-            for (int c = 0; c < 2; c++)
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) y.red[warp][(g + 8 * (e >> 1)) * EX_ROWS + 8 * c + 2 * t + (e & 1)] = acc[c][e];
-        }
-        __syncthreads();
+            for (int e = 0; e < 4; e++) y.red[warp][(g + 8 * (e >> 1)) * EX_ROWS + 8 * c + 2 * t + (e & 1)] = acc[c][e];
+    }
+    __syncthreads();
 #pragma unroll 4
-        for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
-            const int rw = i / a.dv, j = i - rw * a.dv;
-            float x = y.red[j >> 4][(j & 15) * EX_ROWS + rw];
-            for (int k = 1; k < ksplit; k++) x = __fadd_rn(x, y.red[k * mt + (j >> 4)][(j & 15) * EX_ROWS + rw]);
-            if (round) io_store(a.out, T, (b0 + rw) * a.os + h * a.oh + j, x);
-        }
+    for (int i = threadIdx.x; i < rows * a.dv; i += 32 * EX_WARPS) {
+        const int rw = i / a.dv, j = i - rw * a.dv;
+        float x = y.red[j >> 4][(j & 15) * EX_ROWS + rw];
+        for (int k = 1; k < ksplit; k++) x = __fadd_rn(x, y.red[k * mt + (j >> 4)][(j & 15) * EX_ROWS + rw]);
+        io_store(a.out, T, (b0 + rw) * a.os + h * a.oh + j, x);
     }
 }
 
