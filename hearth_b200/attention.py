@@ -13,7 +13,8 @@ quantised in blocks of 64, int8 with k_scale, v_scale [n_pages, n_kv_heads, page
 table [n_seqs, max_pages] int32 names the pages of each sequence (an expanded row is one table for all). Work is
 enqueued on `stream` (default: torch's current stream of the tensors' device) without waiting, and what a call allocates
 (outputs that are not given, scratch) belongs to that stream; tensors passed in have to live until the stream is done with
-them. A wrong argument raises ValueError before anything is enqueued.
+them. A wrong argument raises ValueError before anything is enqueued. The calls are made for inference: autograd does not see them,
+and what they return has no graph, whatever their arguments require.
 """
 from __future__ import annotations
 

@@ -171,10 +171,15 @@ HXB_API int hxb_kv_read_dev(const hxb_kv_cache *c, const int32_t *start, const i
 /* Attention of one new token a sequence over its cached positions 0 .. lens[b] - 1 (lens [n_seqs], device; the new
  * token's own row is in the cache): out[b][h] = sum_r p_r v_r, p = softmax(scale * q[b][h] . k_r), kv head
  * h / (n_heads / n_kv_heads); lse[b][h] (may be NULL) = ln sum_r exp(scale * q . k_r). A length of 0 or less
- * gives zeros and -inf, one past the table's table_pages * page_tokens NaN. At most 65535 sequences. q and out [n_seqs][n_heads][head_dim] of one element type; head_dim a multiple of 16 up
- * to 256. Several tokens of one sequence are several rows with a shared table row (table_stride 0, or equal
- * rows) and their own lengths. Scores, maxima, sums and outputs are f32 until the last rounding. The work is split over the
- * positions whatever the lengths are and joined in a fixed order: the same inputs give the same bits.
+ * gives zeros and -inf, one past the table's table_pages * page_tokens NaN. At most 65535 sequences. q and out
+ * [n_seqs][n_heads][head_dim] of one element type; head_dim a multiple of 16 up to 256. Several tokens of one
+ * sequence are several rows with a shared table row (table_stride 0, or equal rows) and their own lengths.
+ * Scores, maxima, sums and outputs are f32 until the last rounding. For the matrix instructions queries and weights
+ * are sums of 16-bit values: over an f16 or Q8 cache two f16 ones (they leave less than 2^-22 of a weight, or of a
+ * head's largest query value), over a bf16 cache two bf16 ones (2^-16), for f32 queries three. Over f16 and Q8 caches
+ * weights under 2^-38 of the largest count as zero, a Q8 one taken times its block's value scale in this.
+ * The work is split over the positions whatever the lengths are and joined in a fixed order: the same inputs give
+ * the same bits.
  * ws: device scratch of at least hxb_attn_decode_workspace(c, n_heads) bytes, 16-byte aligned, contents free
  * before and after; calls that may overlap on the GPU need one each. */
 HXB_API size_t hxb_attn_decode_workspace(const hxb_kv_cache *c, int n_heads);
@@ -193,7 +198,8 @@ HXB_API int hxb_attn_decode_dev(const hxb_kv_cache *c, const int32_t *lens, cons
  * the cache has it too, or is Q8. rank a multiple of 128 up to 512, head_dim - rank a multiple of 16 from 16
  * to 64, nope and v_dim multiples of 16 up to 256, n_heads up to 256; w contiguous, 16-byte aligned. For the matrix
  * instructions qa is rounded to the cache's type, and a Q8 cache's values and qa to f16, so values over 65504 count as
- * infinite there and ones under 2^-14 lose bits; scores, sums and o stay f32. */
+ * infinite there and ones under 2^-14 lose bits; weights go in as two bf16 values, or one f16 one over an f16 or Q8
+ * cache; scores, sums and o stay f32. */
 HXB_API size_t hxb_latent_decode_workspace(const hxb_kv_cache *c, int n_heads, int rank);
 HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_t *lens, const void *q, int64_t q_stride,
                                   int64_t q_head_stride, const void *w, int n_heads, int rank, int nope, int v_dim,
