@@ -33,6 +33,9 @@
 // two of the largest value scale so far. Q8 keys go in as the codes themselves, one packed subtraction a pair from the form the
 // bytes have under f16's exponent (1152 + code): taking 1152 times the query off the sums instead loses up to 2^-12
 // of the score's terms where one large key channel leaves the others of its block codes of a few steps.
+// The matrix instructions cut their sums off instead of rounding them, so that a long chain of them drifts: by 2^-18 over the
+// tiles of 262147 positions. 16-bit outputs round far above that; f32 ones (WIDE) take each tile's products, and each 32 dims of a
+// score, into a sum of their own and add those in f32.
 #include "hx_attn.cuh"
 
 #include <algorithm>
@@ -49,7 +52,7 @@ constexpr int ad_nj(int D) { return D <= 64 ? 1 : D <= 128 ? 2 : 4; }   // block
 // Resident CTAs an SM by registers. 16-bit rows of 128 dims: 12 warps with 168 registers each, 8 KB a warp under way (16 with
 // 128 measured 68 % of the copy rate instead of 90 %). Q8 rows are half as long and cost more instructions a byte: 16
 // warps (58.5 us a call on 48 sequences of up to 6011; 12: 61.4, 20: 87), whose 128 registers spill 16 bytes of stores and 24
-// of loads at 128 dims (44 and 72 for f32 queries; no other instance spills).
+// of loads at 128 dims (f32 queries at most 60 and 96, there and in four other instances, for 0 to 3 % of their time).
 constexpr int ad_ctas(int cache, int nj, int nht) { return nj * nht <= 2 ? (cache == Q8 ? 4 : 3) : 2; }
 
 // What the join needs beside SplitArgs.
@@ -103,6 +106,7 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_sp
     constexpr int UNIT = Sh::UNIT, COLS = Sh::COLS;
     constexpr int OT = CACHE == BF16 ? BF16 : F16;   // the operands' type
     constexpr float POFF = OT == F16 ? 14.0f : 0.0f;
+    constexpr bool WIDE = NTQ == (CACHE == BF16 ? 3 : 2);   // f32 queries and outputs: sums of products rounded to nearest, see above
     extern __shared__ __align__(16) uint8_t smem[];
     uint4 *qs = reinterpret_cast<uint4 *>(smem);                    // [term][column tile][32-dim step][lane]
     float *mrg = reinterpret_cast<float *>(smem + Sh::Q_BYTES);     // [warp][column][OROW]
@@ -304,14 +308,24 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_sp
                         s[c][3] = __fmaf_rn(p[3], ks[1][j], s[c][3]);
                     }
                 } else {
+                    float rest[4] = {};      // WIDE: the lower terms' products, too small for their truncation to matter
 #pragma unroll
-                    for (int j = 0; j < 2 * NJ; j++)
+                    for (int j = 0; j < 2 * NJ; j++) {
+                        float first[4] = {};
 #pragma unroll
                         for (int k = NTQ - 1; k >= 0; k--) {
                             const uint4 q = qs[((k * NHT + c) * 2 * NJ + j) * 32 + lane];
-                            mma16<OT>(s[c], kr[0][j].x, kr[1][j].x, kr[0][j].y, kr[1][j].y, q.x, q.y);
-                            mma16<OT>(s[c], kr[0][j].z, kr[1][j].z, kr[0][j].w, kr[1][j].w, q.z, q.w);
+                            float(&to)[4] = WIDE ? (k == 0 ? first : rest) : s[c];
+                            mma16<OT>(to, kr[0][j].x, kr[1][j].x, kr[0][j].y, kr[1][j].y, q.x, q.y);
+                            mma16<OT>(to, kr[0][j].z, kr[1][j].z, kr[0][j].w, kr[1][j].w, q.z, q.w);
                         }
+                        if constexpr (WIDE)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s[c][e] = __fadd_rn(s[c][e], first[e]);
+                    }
+                    if constexpr (WIDE)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[c][e] = __fadd_rn(s[c][e], rest[e]);
                 }
             }
             // scores in the log2 domain; positions past the end have no weight, one without a row has no value
@@ -405,10 +419,16 @@ __global__ void __launch_bounds__(AD_THREADS, ad_ctas(CACHE, NJ, NHT)) k_attn_sp
                         a2 = __byte_perm(vr[2][j][k], vr[3][j][k], 0x5410), a3 = __byte_perm(vr[2][j][k], vr[3][j][k], 0x7632);
                     }
 #pragma unroll
-                    for (int c = 0; c < NHT; c++)
+                    for (int c = 0; c < NHT; c++) {
+                        float tile[4] = {};
+                        float(&to)[4] = WIDE ? tile : o[c][j][k];
 #pragma unroll
                         for (int x = NTP - 1; x >= 0; x--)
-                            mma16<OT>(o[c][j][k], a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
+                            mma16<OT>(to, a0, a1, a2, a3, bp[c][CACHE == Q8 ? j : 0][x][0], bp[c][CACHE == Q8 ? j : 0][x][1]);
+                        if constexpr (WIDE)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[c][j][k][e] = __fadd_rn(o[c][j][k][e], tile[e]);
+                    }
                 }
             if (next_plain) load_v(pgv, i + 1, true);
             else if (more) load_v(pgv, i + 1, false);

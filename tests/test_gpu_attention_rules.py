@@ -200,6 +200,52 @@ def test_a_latent_term_less_is_seen(cache, x):
     assert seen >= 4, seen
 
 
+@gpu_only
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_f32_outputs_of_long_sums_do_not_drift(gpu, cache, D):
+    """Equal weights and positive values: the output is the values' mean, and its error that of the sums alone. A CTA's warp adds
+    its share of the tiles, t of them; the partial sums are half of the last one on average, so that their roundings are below t / 2
+    half steps of it, and a tile's own two or three products, the pieces of the warps and CTAs and the division 24 more."""
+    g = gen(77)
+    n, Hkv, pt = 200_003, 4, 64
+    pages = -(-n // pt)
+    kp = torch.zeros(pages, Hkv, pt, D, device="cuda", dtype=torch.int8 if cache == "q8" else F[cache])
+    if cache == "q8":
+        vp, ks, vs = torch.randint(64, 128, kp.shape, generator=g).to(torch.int8).cuda(), *(torch.ones(pages, Hkv, pt, D // 64).cuda() / 64 for _ in range(2))
+    else:
+        vp, ks, vs = (1 + torch.rand(kp.shape, generator=g)).to(F[cache]).cuda(), None, None
+    table = torch.randperm(pages, generator=g).to(torch.int32)[None].cuda()
+    q = randn(g, 1, Hkv, D).cuda()
+    out = hb.decode_attention(q, kp, vp, table, torch.tensor([n], dtype=torch.int32).cuda(), scale=0.1, k_scale=ks, v_scale=vs)[0]
+    rows = vp[table[0].long()].transpose(1, 2).reshape(-1, Hkv, D)[:n].double() / (64 if cache == "q8" else 1)
+    t = -(-pages * Hkv // (148 * 3)) + 3
+    err = ((out.double() - rows.mean(0)).abs() / rows.mean(0)).max()
+    assert err <= (t / 2 + 24) * W, err / W
+
+
+@gpu_only
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_f32_scores_of_long_rows_do_not_drift(gpu, cache, D):
+    """One position, positive keys and queries: lse is the score. Its 32 or 64 dims at a time are cut off by two products each and
+    added with one rounding of a partial sum that is half of the last one on average; scaling and ln 2 are six roundings more."""
+    g = gen(78)
+    B = 64
+    (kp, ks), (vp, vs) = (pool(g, B, 1, 16, D, cache) for _ in range(2))
+    table = torch.arange(B, dtype=torch.int32)[:, None]
+    k = (1 + torch.rand(B, 1, D, generator=g)).double()
+    rows = torch.stack([put(kp, ks, table, b, 0, 16, k[b]) for b in range(B)])
+    for b in range(B):
+        put(vp, vs, table, b, 0, 16, k[b])
+    q = 1 + torch.rand(B, 8, D, generator=g)
+    _, lse = hb.decode_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.ones(B, dtype=torch.int32).cuda(), scale=0.1, k_scale=cu(ks),
+                                 v_scale=cu(vs), return_lse=True)
+    want = torch.einsum("bhd,bd->bh", q.double(), rows[:, 0]) * float(np.float32(0.1))
+    err = ((lse.cpu().double() - want).abs() / want).max()
+    assert err <= (D / 32 / 2 + 4 + 6) * W, err / W
+
+
 # ----------------------------------------------------------------------------------------- sequences out of range
 
 @gpu_only
