@@ -37,8 +37,12 @@
 // the weights relative to it stay below 2^7 (f16 operands: 2^15, lifted by 2^8), and most tiles skip the rescale.
 //
 // Bits. Operands have the cache's type; Q8 rows are expanded to f16 (code x scale in f32, rounded once to 11 bits; bf16's 8
-// would add an error as large as the output's own). f16 queries are lifted by a power of two a head. bf16 weights
-// go in as two terms for the same reason, the second into the tile's rotated part, which S no longer needs.
+// would add an error as large as the output's own). f16 queries are lifted by a power of two a head. Weights
+// go in as two terms for the same reason, the second into the tile's rotated part, which S no longer needs (32 sequences of up to
+// 8191 in f16: 92.6 us, 89.7 with one term and an error of 1.5 times the plain form's instead of 1.3). Over a Q8 cache they have
+// one f16 term: the rows' rounding is what shows there with f16 outputs (0.0004 to the plain form's 0.0002 in 32 bits;
+// with a second term 0.0004 too, and 93.0 us for 88.6); with bf16 outputs neither does. Queries have one term: a second would
+// take 72 KB of shared memory from the second tile (bf16: error 0.0020 to 0.0023, the outputs' own rounding 0.0017).
 #include "hx_attn.cuh"
 
 #include <algorithm>
@@ -447,7 +451,7 @@ __device__ __forceinline__ void load_q(const LatentArgs &a, CoreShared &y, uint3
 template <int CACHE>
 __global__ void __launch_bounds__(CORE_THREADS, 1) k_latent_core(const __grid_constant__ LatentArgs a) {
     constexpr int OT = CACHE == BF16 ? BF16 : F16;
-    constexpr int NTP = OT == BF16 ? 2 : 1;
+    constexpr int NTP = CACHE == Q8 ? 1 : 2;
     constexpr float POFF = OT == F16 ? 8.0f : 0.0f;
     extern __shared__ uint8_t raw[];
     uint8_t *base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);

@@ -198,8 +198,8 @@ HXB_API int hxb_attn_decode_dev(const hxb_kv_cache *c, const int32_t *lens, cons
  * the cache has it too, or is Q8. rank a multiple of 128 up to 512, head_dim - rank a multiple of 16 from 16
  * to 64, nope and v_dim multiples of 16 up to 256, n_heads up to 256; w contiguous, 16-byte aligned. For the matrix
  * instructions qa is rounded to the cache's type, and a Q8 cache's values and qa to f16, so values over 65504 count as
- * infinite there and ones under 2^-14 lose bits; weights go in as two bf16 values, or one f16 one over an f16 or Q8
- * cache; scores, sums and o stay f32. */
+ * infinite there and ones under 2^-14 lose bits; weights go in as two values of the cache's type, over a Q8 cache as
+ * one f16 value; scores, sums and o stay f32. */
 HXB_API size_t hxb_latent_decode_workspace(const hxb_kv_cache *c, int n_heads, int rank);
 HXB_API int hxb_latent_decode_dev(const hxb_kv_cache *c, const int32_t *lens, const void *q, int64_t q_stride,
                                   int64_t q_head_stride, const void *w, int n_heads, int rank, int nope, int v_dim,

@@ -157,13 +157,13 @@ def latent_opposite(g, R, cache, x):
 
 
 def latent_bound(rows, w, q, b, R, dn, dv, cache, x, scale):
-    """The 64-bit output and its bound: scores lose the queries' operands (and a Q8 row's, in f16), weights two bf16 terms or one
-    f16 term, o its two terms; opposite rows round alike, so a Q8 row's rounding is relative to the output."""
+    """The 64-bit output and its bound: scores lose the queries' operands (and a Q8 row's, in f16), weights two terms or, over a
+    Q8 cache, one, o its two terms; opposite rows round alike, so a Q8 row's rounding is relative to the output."""
     op = half_step(torch.bfloat16 if cache == "bf16" else torch.float16)
     qa = torch.cat([q[b, :, :dn].double() @ w[0, :dn].double(), q[b, :, dn:].double()], -1)
     o, _, vabs, big = attend(qa, rows, rows[..., :R], scale)
     ds = ((2 if cache == "q8" else 1) * op + (R + 96) * W) * big
-    lost = op ** 2 if cache == "bf16" else op
+    lost = op if cache == "q8" else op ** 2
     want, vabs = o[0, :dv], vabs[0, :dv]
     # 2^-25: half the distance of f16's values below 2^-14, 2^-24
     return want, (2.0 ** -25 if x == "f16" else 0.0) + (half_step(F[x]) + (op if cache == "q8" else 0.0) + 2.0 ** -15) * want.abs() + (2 * ds + lost + 2.0 ** -21 + (R + 16) * W) * vabs
@@ -185,10 +185,11 @@ def test_latent_weights_and_rows_carry_their_terms(gpu, cache, x, R):
 
 @pytest.mark.parametrize("cache,x", [("bf16", "bf16"), ("f16", "f16"), ("q8", "f16")])
 def test_a_latent_term_less_is_seen(cache, x):
-    """The bounds of the test above with one bf16 term planted in the oracle's weights (for a Q8 cache, in the rows too)."""
+    """The bounds of the test above with a term less planted in the oracle's weights: one of the cache's type, for a Q8 cache one of
+    bf16, in the rows too."""
     R, scale, seen = 128, 1.0 / 128, 0
     _, _, _, rows, w, q, dn, dv = latent_opposite(gen(72), R, cache, x)
-    bf = lambda t: t.float().to(torch.bfloat16).double()  # noqa: E731
+    bf = lambda t: t.float().to(torch.float16 if cache == "f16" else torch.bfloat16).double()  # noqa: E731
     for b in range(len(T_OPPOSITE)):
         want, tol = latent_bound(rows, w, q, b, R, dn, dv, cache, x, scale)
         r = bf(rows) if cache == "q8" else rows
