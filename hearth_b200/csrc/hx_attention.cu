@@ -67,6 +67,16 @@ int kv_view(const hxb_kv_cache *c, const char *who, bool latent, KvView *o) {
     return HXB_OK;
 }
 
+// Whether rows [T][H][n] by these strides may overlap themselves; used for outputs.
+bool rows_overlap(int64_t T, int64_t ts, int H, int64_t hs, int n) {
+    if (T > 1 && ts < 1) return true;
+    if (H > 1 && hs < 1) return true;
+    if (H > 1 && hs < n) return true;
+    if (T <= 1) return false;
+    if (H <= 1) return ts < n;
+    return !(ts >= (H - 1) * hs + n || (hs >= (T - 1) * ts + n && ts >= n));
+}
+
 namespace {
 
 // The row kernels (rotation, cache write and read) work on items of eight values; a thread has ROW_AHEAD of them in flight,
@@ -460,16 +470,6 @@ bool vec_rows(const void *p, int dtype, int64_t T, int64_t ts, int H, int64_t hs
 
 bool rope_vec(const RopeView &r) {
     return aligned(r.cs, 16) && r.off % 8 == 0 && (r.style == 0 ? r.half % 8 == 0 : r.half % 4 == 0);
-}
-
-// Whether rows [T][H][n] by these strides may overlap themselves; used for outputs.
-bool rows_overlap(int64_t T, int64_t ts, int H, int64_t hs, int n) {
-    if (T > 1 && ts < 1) return true;
-    if (H > 1 && hs < 1) return true;
-    if (H > 1 && hs < n) return true;
-    if (T <= 1) return false;
-    if (H <= 1) return ts < n;
-    return !(ts >= (H - 1) * hs + n || (hs >= (T - 1) * ts + n && ts >= n));
 }
 
 template <class TX, bool VEC>

@@ -609,7 +609,7 @@ int attn_check_io(const char *who, int B, int H, const void *q, int64_t qs, int6
     if (!q || !out || !lens) return attn_fail(HXB_E_ARG, "%s: null pointer", who);
     if (q == out) return attn_fail(HXB_E_ARG, "%s: not in place (out is q)", who);
     if (off(q, size) || off(out, size) || off(lens, 4)) return attn_fail(HXB_E_ARG, "%s: pointer not aligned to its elements", who);
-    if (qs < 0 || qh < 0 || os < 0 || (H > 1 && oh < od) || (B > 1 && os < (int64_t)(H - 1) * oh + od))
+    if (qs < 0 || qh < 0 || os < 0 || oh < 0 || rows_overlap(B, os, H, oh, od))
         return attn_fail(HXB_E_ARG, "%s: bad strides", who);
     if (!(fabsf(scale) < INFINITY)) return attn_fail(HXB_E_ARG, "%s: scale is not finite", who);
     return HXB_OK;

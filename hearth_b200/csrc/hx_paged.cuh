@@ -109,6 +109,7 @@ int kv_view(const hxb_kv_cache *c, const char *who, bool latent, KvView *out);
 
 // The message hxb_last_error() returns, and the code back (hx_attention.cu).
 int attn_fail(int code, const char *fmt, ...);
+bool rows_overlap(int64_t T, int64_t ts, int H, int64_t hs, int n);
 bool attn_launched(const char *who);   // the last launch's status; sets the message
 
 }  // namespace hx

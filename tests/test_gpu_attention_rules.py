@@ -298,6 +298,28 @@ def test_pools_without_pages(gpu, cache):
     assert torch.isnan(out[0]).all() and (out[1] == 0).all()
 
 
+@gpu_only
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+def test_outputs_by_head(gpu, cache):
+    """Outputs whose tokens lie closer than their heads ([heads, tokens, dim] seen as [tokens, heads, dim]), with room between
+    them that keeps what it holds."""
+    g = gen(79)
+    lens = [40, 0, 70, 9, 1]
+    pools, table, _ = filled(g, lens, 2, 16, 192, cache)
+    (kp, ks), (vp, vs) = ((cu(a), cu(b)) for a, b in pools)
+    n, q = torch.tensor(lens, dtype=torch.int32).cuda(), randn(g, 5, 8, 192, dtype=torch.bfloat16).cuda()
+    by_head = lambda d: torch.full((8, 5, d + 8), 7.0, dtype=torch.bfloat16).cuda()  # noqa: E731
+    out = by_head(192)
+    hb.decode_attention(q, kp, vp, table.cuda(), n, scale=0.07, k_scale=ks, v_scale=vs, out=out.transpose(0, 1)[..., :192])
+    assert torch.equal(out.transpose(0, 1)[..., :192], hb.decode_attention(q, kp, vp, table.cuda(), n, scale=0.07, k_scale=ks, v_scale=vs))
+    assert (out[..., 192:] == 7.0).all()
+    cp, cs = kp[:, :1].contiguous(), None if ks is None else ks[:, :1].contiguous()
+    ql, w, out = randn(g, 5, 8, 32 + 64, dtype=torch.bfloat16).cuda(), randn(g, 8, 32 + 48, 128, dtype=torch.bfloat16, scale=0.1).cuda(), by_head(48)
+    hb.latent_attention(ql, w, cp, table.cuda(), n, scale=0.1, c_scale=cs, out=out.transpose(0, 1)[..., :48])
+    assert torch.equal(out.transpose(0, 1)[..., :48], hb.latent_attention(ql, w, cp, table.cuda(), n, scale=0.1, c_scale=cs))
+    assert (out[..., 48:] == 7.0).all()
+
+
 # ----------------------------------------------------------------------------------------- far rotary positions
 
 def _pi():
